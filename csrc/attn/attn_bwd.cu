@@ -1,0 +1,709 @@
+// Attention's backward pass on the 5th-generation tensor cores, with the probabilities computed
+// again from the forward's log-sum-exp (head_dim <= 128, GQA, causal or full, padded batches).
+//
+//   P  = exp(c Q K^T - L)  (0 where the mask leaves a pair out)
+//   dV = P^T dO                         summed over the query heads of a KV head
+//   dS = P * (dO V^T - rowsum(dO * O))
+//   dQ = c dS K,   dK = c dS^T Q
+//
+// Two kernels, so that no gradient is summed by atomics (the same result on every run):
+//   dK, dV  one CTA per 128 keys of a KV head walks the 64-query tiles of its query heads
+//   dQ      one CTA per 128 queries of a head walks the 64-key tiles
+// Both keep their rows (keys, or queries) in the MMA's 128 lanes and compute S and dP of a
+// 64-column tile from shared memory; the softmax threads turn a lane's 64 values into P and dS
+// and write them, as 16-bit pairs, over S and dP in tensor memory, from where they are the A
+// operand of the accumulating products. P and dS therefore never touch shared memory, and the
+// transposed form (S^T) needs no transposition. Rounding P and dS to 16 bits enters each
+// gradient at 2^-9 relative per term, independently; sums are fp32 in tensor memory.
+//
+// Tensor memory of the dK/dV kernel: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512
+// columns, all there are; this is what sets the 64-query tile. Two softmax warpgroups take the
+// two stages in turn, so that the tensor pipe works on one tile while the other is exponentiated.
+//
+// Seven products instead of the five of a single kernel is the price of the fixed summation
+// order (and of no fp32 dQ in memory).
+//
+// Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared
+// memory before a product contracts over them, so that whatever padding holds (NaN too) adds 0.
+//
+// Work split: where the key tiles x KV heads leave SMs idle, the query heads of a KV head are
+// divided among `nsplit` CTAs, which leave fp32 partials that a third kernel adds in order.
+#include <c10/cuda/CUDAGuard.h>
+#include "../common/om_host.h"
+#include "../common/om_ptx.cuh"
+
+namespace om {
+
+namespace fa_bw {
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NSTAGE = 4;
+template <int D>
+struct Cfg {
+  static constexpr int H = D / 64;               // 64-wide halves of the head dimension
+  static constexpr int BIG = 128 * 64 * 2;       // one half of 128 rows
+  static constexpr int SMALL = 64 * 64 * 2;      // one half of 64 rows
+  static constexpr int FIX_BYTES = 2 * H * BIG;  // the two resident operands (K, V or Q, dO)
+  static constexpr int ST_BYTES = 2 * H * SMALL; // the two streamed ones
+  static constexpr int STAT = 64 * 8;            // (-lse log2 e, delta) of 64 queries
+  static constexpr int STAT_OFF = FIX_BYTES + NSTAGE * ST_BYTES;
+  static constexpr int BAR_OFF = STAT_OFF + NSTAGE * STAT;
+  static constexpr int SMEM = BAR_OFF + 256 + 1024;
+};
+}  // namespace fa_bw
+
+struct AttnBwdArgs {
+  const float2* stat;   // [B, H, Tp] (-lse log2 e or -inf, delta)
+  const int* lens;      // optional [B] valid tokens
+  __nv_bfloat16 *dq, *dk, *dv;  // contiguous [B, T, H, D], [B, S, Hkv, D]
+  float* part;          // nsplit > 1: [nsplit][2][B, S, Hkv, D]
+  int B, T, S, H, Hkv, G, hd;
+  int Tp;               // T rounded up to 64
+  int causal, off;      // key j visible to query i when j <= i + off
+  int nsplit, gper;     // query heads of one CTA
+  float scale, scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// (-lse log2 e, rowsum(dO * O)) of every query row, laid out [B, H, Tp] for the kernels below.
+// Rows without a visible key (lse = -inf), beyond the length or beyond T get (-inf, 0): P = 0.
+// 16 lanes a row, 8 elements each.
+__global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16* __restrict__ o,
+                                                            const __nv_bfloat16* __restrict__ go,
+                                                            const float* __restrict__ lse, const int* lens,
+                                                            float2* __restrict__ stat, int B, int T, int Tp, int H,
+                                                            int hd, long long ob, long long ot, long long oh,
+                                                            long long gb, long long gt, long long gh) {
+  const int sub = threadIdx.x & 15;
+  const long long n = (long long)B * Tp * H;
+  for (long long i = (blockIdx.x * 256ll + threadIdx.x) >> 4; i < ((n + 1) & ~1ll); i += gridDim.x * 16ll) {
+    const int h = (int)(i % H);
+    const int t = (int)(i / H % Tp);
+    const int b = (int)(i / H / Tp);
+    float d = 0.f, l = -INFINITY;
+    const bool live = i < n && t < (lens ? min(lens[b], T) : T);
+    if (live) {
+      l = lse[((long long)b * T + t) * H + h];
+      if (sub * 8 < hd) {
+        float x[8], y[8];
+        unpack8(*reinterpret_cast<const uint4*>(o + b * ob + t * ot + h * oh + sub * 8), x);
+        unpack8(*reinterpret_cast<const uint4*>(go + b * gb + t * gt + h * gh + sub * 8), y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d += x[j] * y[j];
+      }
+    }
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    if (sub == 0 && i < n)
+      stat[((long long)b * H + h) * Tp + t] =
+          l == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-l * fa_bw::LOG2E, d);
+  }
+}
+
+// Clears rows [from, 64) of one streamed operand (H halves of 64 rows x 128 bytes).
+template <int HALVES>
+__device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
+  for (int i = lane; i < HALVES * (64 - from) * 8; i += 32) {
+    const int half = i / ((64 - from) * 8), in = i % ((64 - from) * 8);
+    sts128(smem_u32(p + half * fa_bw::Cfg<64>::SMALL + from * 128 + in * 16), make_uint4(0, 0, 0, 0));
+  }
+}
+
+// One lane's 64 columns of S and dP (tensor memory) -> P and dS, 16 bits, written over them.
+// COLQ: columns are queries (S^T): stat per column from shared memory; else one stat per lane.
+// Column j is visible when lo <= j < hi.
+template <bool COLQ>
+__device__ __forceinline__ void softmax_grad(uint32_t s_tmem, uint32_t dp_tmem, uint32_t stat_smem, float2 own,
+                                             float c2, int lo, int hi, bool masked, bool want_p) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t sv[32], dv[32];
+    tmem_ld_32x32b_x32(s_tmem + half * 32, sv);
+    tmem_ld_32x32b_x32(dp_tmem + half * 32, dv);
+    tc_wait_ld();
+    uint32_t pk[16], dk[16];
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      float2 a = own, b = own;
+      if constexpr (COLQ) {
+        const uint4 u = lds128(stat_smem + (half * 32 + j) * 8);
+        a = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+        b = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+      }
+      float p0 = fast_exp2(fmaf(__uint_as_float(sv[j]), c2, a.x));
+      float p1 = fast_exp2(fmaf(__uint_as_float(sv[j + 1]), c2, b.x));
+      float d0 = p0 * (__uint_as_float(dv[j]) - a.y);
+      float d1 = p1 * (__uint_as_float(dv[j + 1]) - b.y);
+      if (masked) {  // selected, not multiplied: what lies under a mask may be anything
+        const int c = half * 32 + j;
+        const bool v0 = c >= lo && c < hi, v1 = c + 1 >= lo && c + 1 < hi;
+        p0 = v0 ? p0 : 0.f;
+        d0 = v0 ? d0 : 0.f;
+        p1 = v1 ? p1 : 0.f;
+        d1 = v1 ? d1 : 0.f;
+      }
+      pk[j / 2] = pack_bf16x2(p0, p1);
+      dk[j / 2] = pack_bf16x2(d0, d1);
+    }
+    if (want_p) tmem_st_32x32b_x16(s_tmem + half * 16, pk);
+    tmem_st_32x32b_x16(dp_tmem + half * 16, dk);
+  }
+  tc_wait_st();
+}
+
+// 128 accumulator rows (lane = row) of D columns, times `f`, to global rows; rows >= `rows` are
+// not there. OUT is bf16 or fp32.
+template <int D, typename OUT>
+__device__ __forceinline__ void write_acc(uint32_t tmem, OUT* dst, bool live, bool zero, float f, int hd) {
+#pragma unroll 1
+  for (int q = 0; q < D / 32; ++q) {
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(tmem + q * 32, v);
+    tc_wait_ld();
+    if (!live) continue;
+    float x[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = zero ? 0.f : __uint_as_float(v[j]) * f;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      if (q * 32 + j >= hd) continue;  // hd is a multiple of 8
+      if constexpr (sizeof(OUT) == 2) {
+        *reinterpret_cast<uint4*>(dst + q * 32 + j) = pack8(x + j);
+      } else {
+        reinterpret_cast<float4*>(dst + q * 32 + j)[0] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        reinterpret_cast<float4*>(dst + q * 32 + j)[1] = make_float4(x[j + 4], x[j + 5], x[j + 6], x[j + 7]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ dK, dV
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    attn_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const AttnBwdArgs a) {
+  using C = fa_bw::Cfg<D>;
+  constexpr int NS = fa_bw::NSTAGE;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* full = kv_full + 1;     // [NS]
+  uint64_t* empty = full + NS;      // [NS]
+  uint64_t* land = empty + NS;      // a padded tile before its rows are cleared
+  uint64_t* s_full = land + 1;      // [2]
+  uint64_t* p_full = s_full + 2;    // [2]
+  uint64_t* acc_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // heaviest tiles (the first keys, under a causal mask) first
+  const int per = a.B * a.Hkv * a.nsplit;
+  const int kt = blockIdx.x / per;
+  int rest = blockIdx.x % per;
+  const int split = rest % a.nsplit;
+  rest /= a.nsplit;
+  const int kvh = rest % a.Hkv, b = rest / a.Hkv;
+  const int k0 = kt * 128;
+  const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
+  const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
+  const int g0 = split * a.gper, g1 = min(a.G, g0 + a.gper);
+  const int qt0 = a.causal ? max(0, k0 - a.off) / 64 : 0;
+  const int qt1 = (nq + 63) / 64;
+  const int nqt = k0 < nk ? max(0, qt1 - qt0) : 0;
+  const int total = nqt * max(0, g1 - g0);
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(land, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // dV [0, D), dK [128, 128 + D), stage s: S^T at 256 + 128 s, dP^T 64 on
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (the whole warp)
+    bool ok = true;
+    int it = 0, landed = 0;
+    if (total > 0 && lane == 0) {
+      mbar_arrive_expect_tx(kv_full, C::FIX_BYTES);
+      for (int h = 0; h < C::H; ++h)
+        for (int r = 0; r < 2; ++r) {
+          tma_load_4d(smem + h * C::BIG + r * C::SMALL, &tmK, kv_full, h * 64, kvh, k0 + r * 64, b);
+          tma_load_4d(smem + (C::H + h) * C::BIG + r * C::SMALL, &tmV, kv_full, h * 64, kvh, k0 + r * 64, b);
+        }
+    }
+    for (; it < total; ++it) {
+      const int s = it % NS;
+      const int head = kvh * a.G + g0 + it / nqt, q0 = (qt0 + it % nqt) * 64;
+      ok = mbar_wait(&empty[s], ((it / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
+      const bool pad = nq - q0 < 64 && nq < a.T;  // rows beyond T are zero already (the copy fills them)
+      uint64_t* bar = pad ? land : &full[s];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::ST_BYTES + C::STAT);
+        for (int h = 0; h < C::H; ++h) {
+          tma_load_4d(st + h * C::SMALL, &tmQ, bar, h * 64, head, q0, b);
+          tma_load_4d(st + (C::H + h) * C::SMALL, &tmG, bar, h * 64, head, q0, b);
+        }
+        bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + ((size_t)b * a.H + head) * a.Tp + q0, C::STAT, bar);
+      }
+      __syncwarp();
+      if (pad) {
+        ok = mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL);
+        ++landed;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        clear_rows<2 * C::H>(st, nq - q0, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+      }
+    }
+    if (!ok) {  // wait (bounded) for the loads that may still be in flight
+      for (int j = max(0, it - NS); j < it; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
+      mbar_wait(kv_full, 0, nullptr, 0);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (total > 0 && elect_one()) {
+      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
+      constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
+      const uint32_t k_addr = smem_u32(smem), v_addr = k_addr + C::H * C::BIG;
+      bool ok = mbar_wait(kv_full, 0, a.status, OM_ERR_WAIT_FULL);
+      for (int it = 0; it <= total && ok; ++it) {
+        if (it < total) {
+          const int s = it % NS;
+          if (!mbar_wait(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
+          const uint32_t g_addr = q_addr + C::H * C::SMALL;
+          const uint32_t d = tmem + 256 + (it & 1) * 128;
+          // stage it & 1 was last read by the products of tile it - 2, issued before: they run in order
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_f16(d, smem_desc_sw128(k_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(q_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_f16(d + 64, smem_desc_sw128(v_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(g_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+          tc_commit(&s_full[it & 1]);
+        }
+        if (it > 0) {
+          const int j = it - 1, s = j % NS;
+          if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
+          const uint32_t g_addr = q_addr + C::H * C::SMALL;
+          const uint32_t p = tmem + 256 + (j & 1) * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 16 queries a step
+            tc_mma_f16_ts(tmem, p + k * 8, smem_desc_sw128_mn(g_addr + k * 2048, C::SMALL, 1024), IDESC_A,
+                          j > 0 || k > 0);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc_mma_f16_ts(tmem + 128, p + 64 + k * 8, smem_desc_sw128_mn(q_addr + k * 2048, C::SMALL, 1024), IDESC_A,
+                          j > 0 || k > 0);
+          tc_commit(&empty[s]);
+        }
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax and output
+    const int wg = (warp - 4) >> 2;
+    const int t = threadIdx.x & 127;  // key row == TMEM lane
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int key = k0 + t;
+    bool ok = true;
+    for (int it = wg; it < total; it += 2) {
+      const int q0 = (qt0 + it % nqt) * 64;
+      ok = mbar_wait(&s_full[wg], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+      // every thread that waits for a tile's statistics waits for its load as well
+      ok = ok && mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const bool masked = k0 + 128 > nk || (a.causal && k0 + 127 > q0 + a.off);
+      const int lo = key >= nk ? 64 : (a.causal ? key - a.off - q0 : 0);
+      const uint32_t st = tmem + lanes + 256 + wg * 128;
+      softmax_grad<true>(st, st + 64, smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT), make_float2(0.f, 0.f),
+                         a.scale_log2, lo, 64, masked, true);
+      tc_fence_before();
+      mbar_arrive(&p_full[wg]);
+    }
+    if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+      // warpgroup 0 writes dV, warpgroup 1 writes dK
+      const bool live = key < a.S;
+      const size_t at = (((size_t)b * a.S + key) * a.Hkv + kvh) * a.hd;
+      const float f = wg ? a.scale : 1.f;
+      const uint32_t acc = tmem + lanes + wg * 128;
+      if (a.nsplit > 1) {
+        const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
+        write_acc<D>(acc, a.part + (split * 2 + wg) * plane + at, live, total == 0, f, a.hd);
+      } else {
+        write_acc<D>(acc, (wg ? a.dk : a.dv) + at, live, total == 0, f, a.hd);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds the query-head splits' fp32 partials in split order.
+__global__ void __launch_bounds__(256) attn_bwd_join_kernel(const float* __restrict__ part, int nsplit, long long n,
+                                                            __nv_bfloat16* __restrict__ dv,
+                                                            __nv_bfloat16* __restrict__ dk) {
+  for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < 2 * n; i += gridDim.x * 1024ll) {
+    const int k = i >= n;
+    const long long at = i - k * n;  // n is a multiple of 8
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < nsplit; ++j) {
+      const float4 p = *reinterpret_cast<const float4*>(part + (2 * j + k) * n + at);
+      s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+    }
+    uint2 o;
+    o.x = pack_bf16x2(s.x, s.y);
+    o.y = pack_bf16x2(s.z, s.w);
+    *reinterpret_cast<uint2*>((k ? dk : dv) + at) = o;
+  }
+}
+
+// ------------------------------------------------------------------ dQ
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    attn_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const AttnBwdArgs a) {
+  using C = fa_bw::Cfg<D>;
+  constexpr int NS = fa_bw::NSTAGE;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* full = q_full + 1;
+  uint64_t* empty = full + NS;
+  uint64_t* land = empty + NS;
+  uint64_t* s_full = land + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* acc_full = p_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // heaviest tiles (the last queries, under a causal mask) first; the heads of a KV head side by side
+  const int per = a.B * a.H;
+  const int tiles = (a.T + 127) / 128;
+  const int qt = tiles - 1 - blockIdx.x / per;
+  const int head = blockIdx.x % per % a.H, b = blockIdx.x % per / a.H;
+  const int kvh = head / a.G;
+  const int q0 = qt * 128;
+  const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
+  const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
+  const int last = min(nq, q0 + 128) - 1;  // last valid query of the tile
+  const int kend = last < q0 ? 0 : (a.causal ? min(nk, last + a.off + 1) : nk);
+  const int total = kend > 0 ? (kend + 63) / 64 : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(land, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;  // dQ [0, D), stage s: S at 128 + 128 s, dP 64 on
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer (the whole warp)
+    bool ok = true;
+    int it = 0, landed = 0;
+    if (total > 0 && lane == 0) {
+      mbar_arrive_expect_tx(q_full, C::FIX_BYTES);
+      for (int h = 0; h < C::H; ++h)
+        for (int r = 0; r < 2; ++r) {
+          tma_load_4d(smem + h * C::BIG + r * C::SMALL, &tmQ, q_full, h * 64, head, q0 + r * 64, b);
+          tma_load_4d(smem + (C::H + h) * C::BIG + r * C::SMALL, &tmG, q_full, h * 64, head, q0 + r * 64, b);
+        }
+    }
+    for (; it < total; ++it) {
+      const int s = it % NS, k0 = it * 64;
+      ok = mbar_wait(&empty[s], ((it / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
+      const bool pad = nk - k0 < 64 && nk < a.S;
+      uint64_t* bar = pad ? land : &full[s];
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, C::ST_BYTES);
+        for (int h = 0; h < C::H; ++h) {
+          tma_load_4d(st + h * C::SMALL, &tmK, bar, h * 64, kvh, k0, b);
+          tma_load_4d(st + (C::H + h) * C::SMALL, &tmV, bar, h * 64, kvh, k0, b);
+        }
+      }
+      __syncwarp();
+      if (pad) {
+        ok = mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL);
+        ++landed;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        clear_rows<2 * C::H>(st, nk - k0, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+      }
+    }
+    if (!ok) {
+      for (int j = max(0, it - NS); j < it; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
+      mbar_wait(q_full, 0, nullptr, 0);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (total > 0 && elect_one()) {
+      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
+      constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
+      const uint32_t q_addr = smem_u32(smem), g_addr = q_addr + C::H * C::BIG;
+      bool ok = mbar_wait(q_full, 0, a.status, OM_ERR_WAIT_FULL);
+      for (int it = 0; it <= total && ok; ++it) {
+        if (it < total) {
+          const int s = it % NS;
+          if (!mbar_wait(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t k_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
+          const uint32_t v_addr = k_addr + C::H * C::SMALL;
+          const uint32_t d = tmem + 128 + (it & 1) * 128;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_f16(d, smem_desc_sw128(q_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(k_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            tc_mma_f16(d + 64, smem_desc_sw128(g_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(v_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+          tc_commit(&s_full[it & 1]);
+        }
+        if (it > 0) {
+          const int j = it - 1, s = j % NS;
+          if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t k_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
+          const uint32_t p = tmem + 128 + (j & 1) * 128 + 64;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // 16 keys a step
+            tc_mma_f16_ts(tmem, p + k * 8, smem_desc_sw128_mn(k_addr + k * 2048, C::SMALL, 1024), IDESC_A,
+                          j > 0 || k > 0);
+          tc_commit(&empty[s]);
+        }
+      }
+      if (ok) tc_commit(acc_full);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax and output
+    const int wg = (warp - 4) >> 2;
+    const int t = threadIdx.x & 127;  // query row == TMEM lane
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const int q = q0 + t;
+    const bool row = q < nq;
+    float2 own = make_float2(-INFINITY, 0.f);
+    if (row) own = a.stat[((size_t)b * a.H + head) * a.Tp + q];
+    const bool empty_row = own.x == -INFINITY;  // padding, or no visible key: gradient 0
+    bool ok = true;
+    for (int it = wg; it < total; it += 2) {
+      const int k0 = it * 64;
+      ok = mbar_wait(&s_full[wg], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const bool masked = k0 + 64 > nk || (a.causal && k0 + 63 > q0 + a.off);
+      const int hi = min(nk - k0, a.causal ? q + a.off + 1 - k0 : 64);
+      const uint32_t st = tmem + lanes + 128 + wg * 128;
+      softmax_grad<false>(st, st + 64, 0, own, a.scale_log2, 0, hi, masked, false);
+      tc_fence_before();
+      mbar_arrive(&p_full[wg]);
+    }
+    if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok && wg == 0) {
+      tc_fence_after();
+      write_acc<D>(tmem + lanes, a.dq + (((size_t)b * a.T + q) * a.H + head) * a.hd, q < a.T,
+                   total == 0 || empty_row, a.scale, a.hd);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// [B, T, H, D] rows (D contiguous) as a 4-D map with boxes of 64 tokens x 64 elements
+static CUtensorMap map_bthd(const torch::Tensor& x) {
+  const uint64_t B = x.size(0), T = x.size(1), H = x.size(2), D = x.size(3);
+  CUtensorMap m;
+  cuuint64_t dims[4] = {D, H, T, B};
+  // the stride of a dimension of one element is never used: give it a legal value
+  const uint64_t sh = H > 1 ? x.stride(2) : D, st = T > 1 ? x.stride(1) : H * D, sb = B > 1 ? x.stride(0) : T * H * D;
+  cuuint64_t strides[3] = {sh * 2, st * 2, sb * 2};
+  cuuint32_t box[4] = {64, 1, 64, 1};
+  cuuint32_t es[4] = {1, 1, 1, 1};
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.data_ptr(), dims, strides, box, es,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "attention_bwd: cuTensorMapEncodeTiled failed: ", (int)r);
+  return m;
+}
+
+template <int D>
+static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CUtensorMap& g, const CUtensorMap& k,
+                            const CUtensorMap& v, cudaStream_t st) {
+  using C = fa_bw::Cfg<D>;
+  static std::atomic<bool> attr_set[64];
+  int dev;
+  OM_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!attr_set[dev].load()) {
+    OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_kv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_q_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    attr_set[dev].store(true);
+  }
+  const long long kv = (long long)((a.S + 127) / 128) * a.B * a.Hkv * a.nsplit;
+  const long long qb = (long long)((a.T + 127) / 128) * a.B * a.H;
+  TORCH_CHECK(kv < (1ll << 31) && qb < (1ll << 31), "attention_bwd: too many tiles");
+  if (kv) {
+    attn_bwd_kv_kernel<D><<<(unsigned)kv, 384, C::SMEM, st>>>(q, g, k, v, a);
+    OM_LAUNCH_CHECK();
+  }
+  if (a.nsplit > 1 && kv) {
+    const long long n = (long long)a.B * a.S * a.Hkv * a.hd;
+    const int blocks = (int)std::min<long long>((2 * n + 1023) / 1024, (long long)num_sms() * 8);
+    attn_bwd_join_kernel<<<blocks, 256, 0, st>>>(a.part, a.nsplit, n, a.dv, a.dk);
+    OM_LAUNCH_CHECK();
+  }
+  if (qb) {
+    attn_bwd_q_kernel<D><<<(unsigned)qb, 384, C::SMEM, st>>>(q, g, k, v, a);
+    OM_LAUNCH_CHECK();
+  }
+}
+
+}  // namespace om
+
+// q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D] bf16 (D contiguous, other strides multiples of 8),
+// lse fp32 [B, T, H] natural log, lens int32 [B] (T == S). dq, dk, dv contiguous.
+void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
+                      torch::Tensor dout, c10::optional<torch::Tensor> lens, double scale, bool causal,
+                      torch::Tensor dq, torch::Tensor dk, torch::Tensor dv, torch::Tensor status) {
+  auto rows = [&](const torch::Tensor& t, const char* name, at::IntArrayRef shape, bool dense) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.sizes() == shape,
+                "attention_bwd: ", name, " must be a bf16 CUDA tensor of shape ", shape);
+    bool ok = (t.stride(3) == 1 || t.size(3) == 1) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
+    if (t.numel()) TORCH_CHECK(ok && (!dense || t.is_contiguous()), "attention_bwd: layout of ", name);
+  };
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "attention_bwd: q [B, T, H, D], k / v [B, S, Hkv, D]");
+  const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), S = k.size(1), Hkv = k.size(2);
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention_bwd: head_dim must be a multiple of 8 up to 128 (got ", D,
+              ")");
+  TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "attention_bwd: query heads must be a multiple of KV heads");
+  rows(q, "q", {B, T, H, D}, false);
+  rows(k, "k", {B, S, Hkv, D}, false);
+  rows(v, "v", {B, S, Hkv, D}, false);
+  rows(out, "out", {B, T, H, D}, false);
+  rows(dout, "dout", {B, T, H, D}, false);
+  rows(dq, "dq", {B, T, H, D}, true);
+  rows(dk, "dk", {B, S, Hkv, D}, true);
+  rows(dv, "dv", {B, S, Hkv, D}, true);
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 3 &&
+                  lse.size(0) == B && lse.size(1) == T && lse.size(2) == H,
+              "attention_bwd: lse must be contiguous fp32 [B, T, H]");
+  om::AttnBwdArgs a{};
+  if (lens.has_value()) {
+    TORCH_CHECK(T == S, "attention_bwd: lens needs as many queries as keys");
+    TORCH_CHECK(lens->is_cuda() && lens->scalar_type() == at::kInt && lens->is_contiguous() && lens->dim() == 1 &&
+                    lens->size(0) == B,
+                "attention_bwd: lens must be int32 [B]");
+    a.lens = lens->data_ptr<int>();
+  }
+  TORCH_CHECK(T < (1 << 30) && S < (1 << 30), "attention_bwd: sequence too long");
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto st = at::cuda::getCurrentCUDAStream().stream();
+  if (B == 0 || T == 0 || S == 0) {
+    dq.zero_();
+    dk.zero_();
+    dv.zero_();
+    return;
+  }
+  auto ptr = [](const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); };
+  a.B = (int)B; a.T = (int)T; a.S = (int)S; a.H = (int)H; a.Hkv = (int)Hkv; a.G = (int)(H / Hkv); a.hd = (int)D;
+  a.Tp = (int)((T + 63) / 64 * 64);
+  a.causal = causal;
+  a.off = (int)(S - T);
+  a.scale = (float)scale;
+  a.scale_log2 = (float)(scale * 1.4426950408889634);
+  a.dq = ptr(dq);
+  a.dk = ptr(dk);
+  a.dv = ptr(dv);
+  a.status = status.data_ptr<int>();
+  auto stat = torch::empty({B * H * a.Tp, 2}, lse.options());
+  a.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
+  // query heads of a KV head are divided until the CTAs are twice the SMs (a causal mask makes
+  // them uneven) or each has one head
+  const int64_t base = (S + 127) / 128 * B * Hkv, want = 2 * om::num_sms();
+  a.nsplit = (int)std::min<int64_t>(a.G, std::max<int64_t>(1, want / base));
+  a.gper = (a.G + a.nsplit - 1) / a.nsplit;
+  a.nsplit = (a.G + a.gper - 1) / a.gper;
+  torch::Tensor part;
+  if (a.nsplit > 1) {
+    part = torch::empty({(int64_t)a.nsplit * 2 * B * S * Hkv * D}, lse.options());
+    a.part = part.data_ptr<float>();
+  }
+  const long long n = (long long)B * a.Tp * H;
+  const int blocks = (int)std::min<long long>((n + 15) / 16, (long long)om::num_sms() * 16);
+  om::attn_bwd_stat_kernel<<<blocks, 256, 0, st>>>(
+      ptr(out), ptr(dout), lse.data_ptr<float>(), a.lens, reinterpret_cast<float2*>(stat.data_ptr<float>()), a.B, a.T,
+      a.Tp, a.H, a.hd, out.stride(0), out.stride(1), out.stride(2), dout.stride(0), dout.stride(1), dout.stride(2));
+  OM_LAUNCH_CHECK();
+  const CUtensorMap mq = om::map_bthd(q), mg = om::map_bthd(dout), mk = om::map_bthd(k), mv = om::map_bthd(v);
+  if (D <= 64)
+    om::attn_bwd_launch<64>(a, mq, mg, mk, mv, st);
+  else
+    om::attn_bwd_launch<128>(a, mq, mg, mk, mv, st);
+}

@@ -79,6 +79,26 @@ void om_moe_permute(torch::Tensor x, torch::Tensor ids, torch::Tensor counts, to
 void om_moe_combine(torch::Tensor yp, torch::Tensor row_of, torch::Tensor wts, torch::Tensor out, bool add);
 void om_grouped_gemm(torch::Tensor x, torch::Tensor w, torch::Tensor offsets, torch::Tensor y, torch::Tensor status);
 
+void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
+                      torch::Tensor dout, c10::optional<torch::Tensor> lens, double scale, bool causal,
+                      torch::Tensor dq, torch::Tensor dk, torch::Tensor dv, torch::Tensor status);
+void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<torch::Tensor> gu,
+               torch::Tensor status);
+void om_swiglu_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor gu, torch::Tensor dh,
+                   c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status);
+void om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
+                    double scale, double smoothing, int64_t ignore, torch::Tensor loss, torch::Tensor lse,
+                    torch::Tensor status);
+void om_linear_xent_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
+                        double scale, double smoothing, int64_t ignore, torch::Tensor lse, torch::Tensor dloss,
+                        c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status);
+void om_norm_train(torch::Tensor x, c10::optional<torch::Tensor> delta, torch::Tensor w,
+                   c10::optional<torch::Tensor> b, bool layer, double eps, torch::Tensor y,
+                   c10::optional<torch::Tensor> h, torch::Tensor stats);
+void om_norm_train_bwd(torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats,
+                       c10::optional<torch::Tensor> dh, bool layer, torch::Tensor dx, torch::Tensor dw,
+                       c10::optional<torch::Tensor> db);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("launch_count", [] { return (int64_t)om::g_launches.load(); }, "kernel launches issued so far");
   m.doc() = "openmini_v1_b200 sm_100a kernels";
@@ -139,4 +159,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sp_wait", &om_sp_wait, "wait until every rank pushed its normed rows for this epoch");
   m.def("mla_workspace", &om_mla_workspace, "fp32 workspace floats of mla_decode");
   m.def("mla_decode", &om_mla_decode, "latent attention over a paged 576-wide latent cache (absorbed form)");
+  m.def("attention_bwd", &om_attention_bwd, "gradient of causal / full GQA attention from its log-sum-exp (tcgen05)");
+  m.def("swiglu", &om_swiglu, "silu(x Wg^T) * (x Wu^T) in one tcgen05 GEMM");
+  m.def("swiglu_bwd", &om_swiglu_bwd, "gradient of swiglu");
+  m.def("linear_xent", &om_linear_xent, "cross entropy of x W^T without the logits");
+  m.def("linear_xent_bwd", &om_linear_xent_bwd, "gradient of linear_xent, in pieces of the vocabulary");
+  m.def("norm_train", &om_norm_train, "(residual add +) RMSNorm / LayerNorm with row statistics");
+  m.def("norm_train_bwd", &om_norm_train_bwd, "gradient of norm_train with the weight gradient's reduction");
 }

@@ -5,7 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
-#include <torch/extension.h>
+#include <torch/types.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <atomic>
 #include <mutex>

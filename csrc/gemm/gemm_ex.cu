@@ -1,0 +1,103 @@
+// Plain products of the training operators on gemm_ex.cuh (dX = dY W, dW = dY^T X).
+#include "gemm_ex.h"
+
+namespace om {
+
+// Sums the fp32 planes of a split contraction in plane order and rounds once.
+__global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __restrict__ P, int splits, long long rows,
+                                                             int cols, int ldacc, __nv_bfloat16* __restrict__ out,
+                                                             long long ldo, int vec) {
+  const int nv = ldacc >> 2;
+  const long long plane = rows * ldacc;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * nv; i += gridDim.x * 256ll) {
+    const long long r = i / nv;
+    const int c = (int)(i - r * nv) * 4;
+    if (c >= cols) continue;
+    float4 a = *reinterpret_cast<const float4*>(P + r * ldacc + c);
+    for (int s = 1; s < splits; ++s) {
+      const float4 b = *reinterpret_cast<const float4*>(P + s * plane + r * ldacc + c);
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    __nv_bfloat16* o = out + r * ldo + c;
+    if (vec && c + 4 <= cols) {
+      uint2 w;
+      w.x = pack_bf16x2(a.x, a.y);
+      w.y = pack_bf16x2(a.z, a.w);
+      *reinterpret_cast<uint2*>(o) = w;
+    } else {
+      const float f[4] = {a.x, a.y, a.z, a.w};
+      for (int j = 0; j < 4 && c + j < cols; ++j) o[j] = __float2bfloat16_rn(f[j]);
+    }
+  }
+}
+
+GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
+  const int sms = num_sms();
+  const int64_t tr = ceil_div(rows, 128);
+  GxPlan p;
+  // 128 x 256 tiles feed the tensor cores best; half as wide ones where those would not fill the SMs
+  p.bn = cols <= 128 || tr * ceil_div(cols, 256) < sms ? 128 : 256;
+  const int64_t tiles = tr * ceil_div(cols, p.bn);
+  const int kb = ceil_div(K, 64);
+  // a split has to be worth its fp32 plane (written and read once): 8 steps of 64 at least
+  int s = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
+  const int per = ceil_div(kb, s);
+  p.splits = ceil_div(kb, per);
+  return p;
+}
+
+int64_t gx_acc_floats(const GxPlan& p, int64_t rows, int64_t cols, bool pieces) {
+  return p.splits > 1 || pieces ? (int64_t)p.splits * rows * ceil_div(cols, 32) * 32 : 0;
+}
+
+template <int BN>
+static void product_bn(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
+                       const EpiStore::Args& e, int* status, cudaStream_t st) {
+  GemmX g{};
+  g.rows = (int)rows;
+  g.cols = (int)cols;
+  g.num_kb = ceil_div(K, 64);
+  g.kb_per_split = ceil_div(g.num_kb, p.splits);
+  // a piece shorter than the planned one may have fewer splits: the planes it leaves out keep
+  // the sums of the pieces before it (the first piece is never shorter than the plan's K)
+  g.splits = ceil_div(g.num_kb, g.kb_per_split);
+  TORCH_CHECK(e.add || g.splits == p.splits, "gx_product: the first piece is shorter than planned");
+  g.tiles_r = ceil_div(rows, 128);
+  g.tiles_c = ceil_div(cols, BN);
+  g.b_step = BN;
+  g.b_second = BN / 2;
+  g.status = status;
+  const CUtensorMap ta = gx_map(a.p, a.mn, rows, K, a.ld, 128);
+  const CUtensorMap tb = gx_map(b.p, b.mn, cols, K, b.ld, BN / 2);
+  TORCH_CHECK(b.mn, "gx_product: B is MN-major");
+  if (a.mn)
+    gx_launch<BN, true, true, EpiStore>(ta, tb, g, e, st);
+  else
+    gx_launch<BN, false, true, EpiStore>(ta, tb, g, e, st);
+}
+
+void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
+                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st) {
+  EpiStore::Args e{};
+  e.out = out;
+  e.ldo = (int)ldo;
+  e.vec = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool direct = p.splits == 1 && first && last;
+  e.acc = direct ? nullptr : acc;
+  e.ldacc = ceil_div(cols, 32) * 32;
+  e.add = !first;
+  e.last = last && p.splits == 1;
+  if (p.bn == 128)
+    product_bn<128>(p, a, b, rows, cols, K, e, status, st);
+  else
+    product_bn<256>(p, a, b, rows, cols, K, e, status, st);
+  if (last && p.splits > 1) {
+    const long long work = (long long)rows * (e.ldacc / 4);
+    const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)num_sms() * 8);
+    planes_to_bf16_kernel<<<blocks, 256, 0, st>>>(acc, p.splits, rows, (int)cols, e.ldacc, out, ldo,
+                                                  ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0);
+    OM_LAUNCH_CHECK();
+  }
+}
+
+}  // namespace om

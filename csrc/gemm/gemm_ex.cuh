@@ -1,0 +1,249 @@
+// Persistent tcgen05 GEMM with a choice of operand layouts and a fused epilogue, for the
+// training operators:
+//
+//   D[r, c] = sum_k A(r, k) B(c, k)
+//
+// Each operand is either K-major (rows of contiguous k) or MN-major (rows of contiguous r or
+// c, one row per k), so a gradient product reads its operands as they lie in memory:
+//   dX = dY W      A = dY K-major,  B = W MN-major
+//   dW = dY^T X    A = dY MN-major, B = X MN-major
+// and no transposed copy is made. B is loaded as two halves of BN / 2 rows whose distance is
+// an argument: BN / 2 for one matrix, F for the two stacked projections of a gated block, so
+// gate and up columns of the same features meet in one accumulator tile.
+//
+// Roles as in gemm_tc.cuh (256 threads: TMA warp, MMA warp, TMEM warp, four epilogue warps),
+// two TMEM accumulators, so that the epilogue of tile i runs beside the products of tile i+1.
+// What bounds it: 128 x 256 tiles read 12 KB of shared memory per 16-deep MMA step (96 of its
+// 128 cycles), so the tensor pipe, not shared memory, is the limit for BN = 256; BN = 64 and
+// 128 are for grids that would otherwise leave SMs idle.
+//
+// Epi is a functor type with Args and
+//   static void tile(const GemmX&, const Args&, uint32_t tbase, int r, int tc, int sp)
+// called by every epilogue thread (accumulator row r, TMEM lane address tbase).
+#pragma once
+#include <cuda.h>
+#include "../common/om_ptx.cuh"
+
+namespace om {
+
+struct GemmX {
+  int rows, cols;    // extents of D (for a gated pair: cols = F)
+  int num_kb;        // 64-deep steps of the whole contraction
+  int splits, kb_per_split;
+  int tiles_r, tiles_c;
+  int b_step;        // rows of B per column tile (K-major B): BN, or BN / 2 for a gated pair
+  int b_second;      // distance of the second half's rows (K-major B): BN / 2, or F
+  int* status;
+};
+
+constexpr int GX_GROUP = 16;  // row tiles walked before the next column tile: 16 x 9 tiles in flight share L2 lines
+
+__device__ __forceinline__ void gx_coords(const GemmX& g, int u, int& tr, int& tc, int& sp) {
+  sp = u % g.splits;
+  const int t = u / g.splits;
+  const int per = GX_GROUP * g.tiles_c;
+  const int first = (t / per) * GX_GROUP;
+  const int n = min(GX_GROUP, g.tiles_r - first);
+  const int in = t % per;
+  tr = first + in % n;
+  tc = in / n;
+}
+
+// kind::f16, bf16 operands, fp32 accumulator; bit 15 / 16 select an MN-major A / B
+__host__ __device__ constexpr uint32_t idesc_bf16_x(int M, int N, bool amn, bool bmn) {
+  return idesc_bf16_f32(M, N) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
+}
+
+template <int BN>
+struct GemmXCfg {
+  static constexpr int BM = 128, BK = 64;
+  static constexpr int A_BYTES = BM * BK * 2;
+  static constexpr int B_BYTES = BN * BK * 2;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = (200 * 1024) / STAGE_BYTES > 8 ? 8 : (200 * 1024) / STAGE_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align slack*/ + 256;
+};
+
+template <int BN, bool AMN, bool BMN, class Epi>
+__global__ void __launch_bounds__(256, 1)
+    gemm_ex_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmX g,
+                   const typename Epi::Args e) {
+  using C = GemmXCfg<BN>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = g.tiles_r * g.tiles_c * g.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 128);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, C::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      int it = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        int tr, tc, sp;
+        gx_coords(g, u, tr, tc, sp);
+        const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, g.status, OM_ERR_WAIT_EMPTY)) { ok = false; break; }
+          uint8_t* a_dst = smem + s * C::STAGE_BYTES;
+          uint8_t* b_dst = a_dst + C::A_BYTES;
+          mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
+          if constexpr (AMN) {
+            tma_load_2d(a_dst, &tmA, &full[s], tr * 128, kb * 64);
+            tma_load_2d(a_dst + 8192, &tmA, &full[s], tr * 128 + 64, kb * 64);
+          } else {
+            tma_load_2d(a_dst, &tmA, &full[s], kb * 64, tr * 128);
+          }
+          if constexpr (BMN) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load_2d(b_dst + j * 8192, &tmB, &full[s], tc * BN + j * 64, kb * 64);
+          } else {
+            tma_load_2d(b_dst, &tmB, &full[s], kb * 64, tc * g.b_step);
+            tma_load_2d(b_dst + C::B_BYTES / 2, &tmB, &full[s], kb * 64, tc * g.b_step + g.b_second);
+          }
+        }
+      }
+      if (!ok)  // wait (bounded) for the loads that may still be in flight
+        for (int j = max(0, it - C::STAGES); j < it; ++j)
+          mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr, 0);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t IDESC = idesc_bf16_x(128, BN, AMN, BMN);
+      int it = 0, local = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++local) {
+        int tr, tc, sp;
+        gx_coords(g, u, tr, tc, sp);
+        const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+        const int acc = local & 1;
+        if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, g.status, OM_ERR_WAIT_ACCUM)) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&full[s], (it / C::STAGES) & 1, g.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::A_BYTES;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // 16 deep: 32 bytes of a K-major row, two 8-row atoms MN-major
+            const uint64_t ad = AMN ? smem_desc_sw128_mn(a_addr + k * 2048, 8192, 1024)
+                                    : smem_desc_sw128(a_addr + k * 32, 1024);
+            const uint64_t bd = BMN ? smem_desc_sw128_mn(b_addr + k * 2048, 8192, 1024)
+                                    : smem_desc_sw128(b_addr + k * 32, 1024);
+            tc_mma_f16(tmem + acc * BN, ad, bd, IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+          }
+          tc_commit(&empty[s]);
+        }
+        if (ok) tc_commit(&tfull[acc]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    int local = 0;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++local) {
+      int tr, tc, sp;
+      gx_coords(g, u, tr, tc, sp);
+      const int acc = local & 1;
+      if (!mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM)) break;
+      tc_fence_after();
+      Epi::template tile<BN>(g, e, tmem + ((uint32_t)(q * 32) << 16) + acc * BN, tr * 128 + q * 32 + lane, tc, sp);
+      tc_fence_before();
+      mbar_arrive(&tempty[acc]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// 32 fp32 of one accumulator row, columns c0 .. c0 + 31, to bf16. `n` of them exist.
+__device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const float (&f)[32], int n, bool vec) {
+  if (n >= 32 && vec) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) *reinterpret_cast<uint4*>(dst + j) = pack8(f + j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) dst[j] = __float2bfloat16_rn(f[j]);
+  }
+}
+
+// Plain result: bf16 rows, or fp32 sums that several launches (pieces of a long contraction)
+// and splits add up. A piece adds to what the launch before it left: no atomics, one order.
+struct EpiStore {
+  struct Args {
+    __nv_bfloat16* out;
+    int ldo, vec;
+    float* acc;        // [splits][rows][ldacc] fp32, ldacc a multiple of 32; null: straight to out
+    int ldacc;
+    int add, last;     // add: acc holds earlier pieces; last: write out instead of acc (splits == 1)
+  };
+  template <int BN>
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, uint32_t tbase, int r, int tc, int sp) {
+#pragma unroll 1
+    for (int cc = 0; cc < BN / 32; ++cc) {
+      const int c0 = tc * BN + cc * 32;
+      if (c0 >= g.cols) break;  // the same for the whole warp
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(tbase + cc * 32, v);
+      tc_wait_ld();
+      if (r >= g.rows) continue;
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+      if (e.acc != nullptr) {
+        float4* a = reinterpret_cast<float4*>(e.acc + ((size_t)sp * g.rows + r) * e.ldacc + c0);
+        if (e.add) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float4 o = a[j];
+            f[4 * j] += o.x; f[4 * j + 1] += o.y; f[4 * j + 2] += o.z; f[4 * j + 3] += o.w;
+          }
+        }
+        if (!e.last) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) a[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+          continue;
+        }
+      }
+      store_row32(e.out + (size_t)r * e.ldo + c0, f, g.cols - c0, e.vec);
+    }
+  }
+};
+
+}  // namespace om

@@ -1,0 +1,53 @@
+// Host side of gemm_ex.cuh: tensor maps, launch and the plain products of the training
+// operators.
+#pragma once
+#include "../common/om_host.h"
+#include "gemm_ex.cuh"
+
+namespace om {
+
+inline int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Operand of logical extent [rows, K]: K-major (`ld` elements between rows), or MN-major (`ld`
+// elements between k). A K-major box has `box` rows and 64 k, an MN-major one 64 x 64.
+inline CUtensorMap gx_map(const void* p, bool mn, uint64_t rows, uint64_t K, uint64_t ld, uint32_t box) {
+  return mn ? make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, rows, K, ld, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)
+            : make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, rows, ld, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int BN, bool AMN, bool BMN, class Epi>
+void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmX& g, const typename Epi::Args& e,
+               cudaStream_t st) {
+  using C = GemmXCfg<BN>;
+  static std::atomic<bool> attr_set[64];
+  int dev;
+  OM_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!attr_set[dev].load()) {
+    OM_CUDA_CHECK(cudaFuncSetAttribute(gemm_ex_kernel<BN, AMN, BMN, Epi>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
+    attr_set[dev].store(true);
+  }
+  const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
+  TORCH_CHECK(units < (1ll << 31), "gemm: too many tiles");
+  const int grid = (int)std::min<long long>(units, num_sms());
+  gemm_ex_kernel<BN, AMN, BMN, Epi><<<grid, 256, C::SMEM_BYTES, st>>>(ta, tb, g, e);
+  OM_LAUNCH_CHECK();
+}
+
+struct GxOperand {
+  const void* p;
+  bool mn;
+  int64_t ld;
+};
+
+// out[rows, cols] (+)= A . B over K, split over K where the tiles alone leave SMs idle.
+// `acc` (from gx_acc_floats) carries fp32 sums from piece to piece; first / last tell the piece's place.
+struct GxPlan {
+  int bn, splits;
+};
+GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K);
+int64_t gx_acc_floats(const GxPlan& p, int64_t rows, int64_t cols, bool pieces);
+void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
+                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st);
+
+}  // namespace om

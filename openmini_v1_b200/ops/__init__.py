@@ -17,7 +17,8 @@ from . import reference as ref
 __all__ = [
     "DeviceContext", "ctx", "linear", "rmsnorm", "layernorm", "silu_mul", "gelu", "softmax",
     "embedding", "rope_kv", "kv_write", "paged_attention", "sample", "repetition_penalty",
-    "check_status",
+    "check_status", "attention_bwd", "swiglu", "swiglu_bwd", "linear_xent", "linear_xent_bwd", "norm_train",
+    "norm_train_bwd",
 ]
 
 
@@ -278,3 +279,177 @@ def repetition_penalty(logits, prev, penalty):
         return ref.repetition_penalty(logits, prev, penalty)
     _native.C().repetition_penalty(logits, prev.to(torch.int32).contiguous(), penalty)
     return logits
+
+
+# ------------------------------------------------------------------ training operators
+# Scratch of these is allocated per call on the current stream (the caching allocator keeps
+# it), so calls on different streams never share any.
+
+def _rows(x):
+    """``x`` as [rows, K] whose rows a TMA copy can read: contiguous, 16-byte aligned."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(-1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _heads(x):
+    """``x`` [B, T, H, D] with D contiguous and every other stride a positive multiple of 8."""
+    if x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and (s % 8 or s <= 0)
+                                                    for n, s in zip(x.shape[:3], x.stride()[:3])):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _same_device(op, *tensors):
+    d = tensors[0].device
+    if any(t is not None and t.device != d for t in tensors):
+        raise ValueError(f"{op}: all tensors must be on {d}")
+
+
+def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
+    """Gradient (dq, dk, dv) of attention from what its forward kept: q, out, dout [B, T, H, D],
+    k, v [B, S, Hkv, D], ``lse`` fp32 [B, T, H] (natural log of the sum of exp of the scaled scores;
+    -inf for a row without a visible key, whose gradient is 0).
+
+    ``causal`` masks are aligned to the last key (query i sees keys <= i + S - T). ``lens`` int32 [B]
+    (T == S) is the number of valid tokens of right-padded sequences: padding takes no gradient,
+    whatever it holds. head_dim: a multiple of 8 up to 128."""
+    _same_device("attention_bwd", q, k, v, out, lse, dout, lens)
+    if not q.is_cuda:
+        return ref.attention_bwd(q, k, v, out, lse, dout, scale, causal, lens)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or out.shape != q.shape or dout.shape != q.shape:
+        raise ValueError("attention_bwd: q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D]")
+    q, k, v, out, dout = (_heads(t) for t in (q, k, v, out.to(q.dtype), dout.to(q.dtype)))
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    _native.C().attention_bwd(q, k, v, out, lse.contiguous(), dout,
+                              None if lens is None else lens.to(torch.int32).contiguous(), float(scale), bool(causal),
+                              dq, dk, dv, ctx(q.device).status)
+    return dq, dk, dv
+
+
+def swiglu(x, w, save=False):
+    """silu(x Wg^T) * (x Wu^T) of x [..., K] and w [2F, K] (gate rows first) -> [..., F]. With
+    ``save`` also the projections [rows, 2F] that :func:`swiglu_bwd` reads."""
+    _same_device("swiglu", x, w)
+    if not x.is_cuda:
+        return ref.swiglu(x, w, save)
+    if w.dim() != 2 or w.shape[0] % 2 or w.shape[1] != x.shape[-1]:
+        raise ValueError("swiglu: w must be [2F, K]")
+    x2, F = _rows(x), w.shape[0] // 2
+    h = torch.empty(x2.shape[0], F, dtype=x.dtype, device=x.device)
+    gu = torch.empty(x2.shape[0], 2 * F, dtype=x.dtype, device=x.device) if save else None
+    _native.C().swiglu(x2, _rows(w), h, gu, ctx(x.device).status)
+    h = h.view(*x.shape[:-1], F)
+    return (h, gu) if save else h
+
+
+def swiglu_bwd(x, w, gu, dh, need_dx=True, need_dw=True):
+    """Gradient (dx, dw) of :func:`swiglu` from its saved projections and dh [..., F]."""
+    _same_device("swiglu_bwd", x, w, gu, dh)
+    if not x.is_cuda:
+        return ref.swiglu_bwd(x, w, gu, dh, need_dx, need_dw)
+    x2 = _rows(x)
+    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
+    d2 = dh.to(x.dtype).reshape(-1, dh.shape[-1])
+    _native.C().swiglu_bwd(x2, _rows(w), gu, d2 if d2.stride(-1) == 1 else d2.contiguous(), dx, dw,
+                           ctx(x.device).status)
+    return dx.view(x.shape) if need_dx else None, dw
+
+
+def _xent_args(op, x, w, targets, smoothing, keep):
+    _same_device(op, x, w, targets, keep)
+    if w.dim() != 2 or w.shape[1] != x.shape[-1] or targets.shape != x.shape[:-1]:
+        raise ValueError(f"{op}: x [..., K], w [V, K], targets [...]")
+    if targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"{op}: targets must be integers")
+    if not 0.0 <= smoothing < 1.0:
+        raise ValueError(f"{op}: label smoothing must be in [0, 1)")
+    if keep is not None and smoothing:
+        raise ValueError(f"{op}: label smoothing over a keep mask is not defined")
+
+
+def linear_xent(x, w, targets, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None):
+    """Cross entropy of the logits scale * x w^T, which are never stored: (loss, lse) fp32 [...] of
+    x [..., K], w [V, K] and targets [...].
+
+    Rows whose target is ``ignore_index`` have loss 0. ``keep``: packed mask int32 [rows, ceil(V / 32)]
+    as :func:`sample` returns it; columns outside it have probability 0 (a target outside it has an
+    infinite loss, an empty row lse = -inf). Other targets outside [0, V) count as ignored and set
+    the device status."""
+    _xent_args("linear_xent", x, w, targets, smoothing, keep)
+    if not x.is_cuda:
+        return ref.linear_xent(x, w, targets, scale, smoothing, ignore_index, keep)
+    loss = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    lse = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    _native.C().linear_xent(_rows(x), _rows(w), targets.long().reshape(-1), keep, float(scale), float(smoothing),
+                            int(ignore_index), loss, lse, ctx(x.device).status)
+    return loss, lse
+
+
+def linear_xent_bwd(x, w, targets, lse, dloss, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None, need_dx=True,
+                    need_dw=True):
+    """Gradient (dx, dw) of :func:`linear_xent`; ``dloss`` fp32 [...] is the loss's gradient row by row."""
+    _xent_args("linear_xent_bwd", x, w, targets, smoothing, keep)
+    if not x.is_cuda:
+        return ref.linear_xent_bwd(x, w, targets, lse, dloss, scale, smoothing, ignore_index, keep, need_dx, need_dw)
+    x2 = _rows(x)
+    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
+    _native.C().linear_xent_bwd(x2, _rows(w), targets.long().reshape(-1), keep, float(scale), float(smoothing),
+                                int(ignore_index), lse.reshape(-1).contiguous(),
+                                dloss.float().reshape(-1).contiguous(), dx, dw, ctx(x.device).status)
+    return dx.view(x.shape) if need_dx else None, dw
+
+
+def _norm_kind(kind, b):
+    if kind not in ("rms", "layer"):
+        raise ValueError(f"norm kind {kind!r}: 'rms' or 'layer'")
+    if kind == "rms" and b is not None:
+        raise ValueError("RMSNorm takes no bias")
+    return kind == "layer"
+
+
+def norm_train(x, w, b=None, eps=1e-5, kind="rms", delta=None):
+    """(y, h, stats): y = norm(h) * w (+ b) with h = x (+ delta, rounded to x's type), and the rows'
+    fp32 (mean, 1 / std) that :func:`norm_train_bwd` reads. x bf16 (w, b bf16 or fp32) or fp32."""
+    layer = _norm_kind(kind, b)
+    _same_device("norm_train", x, w, b, delta)
+    if not x.is_cuda:
+        return ref.norm_train(x, w, b, eps, kind, delta)
+    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x2 if x2.stride(-1) == 1 else x2.contiguous()
+    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(x2.shape[0], 2, dtype=torch.float32, device=x.device)
+    h = d2 = None
+    if delta is not None:
+        if delta.shape != x.shape or delta.dtype != x.dtype:
+            raise ValueError("norm_train: delta must be like x")
+        d2 = delta.reshape(x2.shape)
+        d2 = d2 if d2.stride(-1) == 1 else d2.contiguous()
+        h = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
+    _native.C().norm_train(x2, d2, w.contiguous(), None if b is None else b.contiguous(), layer, float(eps), y, h,
+                           stats)
+    return y.view(x.shape), x if h is None else h.view(x.shape), stats
+
+
+def norm_train_bwd(dy, h, w, stats, kind="rms", bias=False, dh=None):
+    """(dx, dw, db) of :func:`norm_train`: ``dh`` is the gradient that h itself receives (the residual
+    stream's), added to dx; dw, db have w's type; db is None without ``bias``."""
+    layer = _norm_kind(kind, w if bias else None)
+    _same_device("norm_train_bwd", dy, h, w, stats, dh)
+    if not h.is_cuda:
+        return ref.norm_train_bwd(dy, h, w, stats, kind, bias, dh)
+
+    def rows(t):
+        t = t.to(h.dtype).reshape(-1, h.shape[-1])
+        return t if t.stride(-1) == 1 else t.contiguous()
+
+    h2 = rows(h)
+    dx = torch.empty(h2.shape, dtype=h.dtype, device=h.device)
+    dw = torch.empty(w.shape, dtype=w.dtype, device=h.device)
+    db = torch.empty(w.shape, dtype=w.dtype, device=h.device) if bias else None
+    _native.C().norm_train_bwd(rows(dy), h2, w.contiguous(), stats, None if dh is None else rows(dh), layer, dx, dw,
+                               db)
+    return dx.view(h.shape), dw, db

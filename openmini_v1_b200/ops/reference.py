@@ -286,3 +286,120 @@ def mla_decode(q, cache, block_tables, row_seq, row_ctx, scale):
         s = (q[r].float() @ rows_kv.t()) * scale
         out[r] = (torch.softmax(s, -1) @ rows_kv[:, :512]).to(q.dtype)
     return out
+
+
+# ------------------------------------------------------------------ training operators
+def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
+    """dq, dk, dv of softmax(scale q k^T) v from its log-sum-exp (see ops.attention_bwd)."""
+    B, T, H, D = q.shape
+    S, Hkv = k.shape[1], k.shape[2]
+    G = H // Hkv
+    dev = q.device
+    vis = torch.ones(1, T, S, dtype=torch.bool, device=dev)
+    if causal:
+        vis = vis.tril(S - T)
+    row = torch.ones(B, T, dtype=torch.bool, device=dev)
+    if lens is not None:
+        if T != S:
+            raise ValueError("attention_bwd: lens needs as many queries as keys")
+        row = torch.arange(T, device=dev)[None, :] < lens.to(dev)[:, None]
+        vis = vis & row[:, :, None] & row[:, None, :]
+    vis = vis[:, None]                                                             # [B or 1, 1, T, S]
+    clean = lambda x: x.float().masked_fill(~row[:, :, None, None], 0.0)           # noqa: E731
+    qf, gf, of = clean(q), clean(dout), clean(out)
+    kf = (clean(k) if T == S else k.float()).repeat_interleave(G, dim=2)
+    vf = (clean(v) if T == S else v.float()).repeat_interleave(G, dim=2)
+    s = torch.einsum("bqhd,bkhd->bhqk", qf, kf) * scale
+    l = lse.permute(0, 2, 1)[..., None]
+    p = torch.exp(s - torch.where(torch.isfinite(l), l, torch.zeros_like(l)))
+    p = p.masked_fill(~vis | torch.isneginf(l), 0.0)
+    dv = torch.einsum("bhqk,bqhd->bkhd", p, gf)
+    dp = torch.einsum("bqhd,bkhd->bhqk", gf, vf)
+    delta = (gf * of).sum(-1).permute(0, 2, 1)[..., None]
+    ds = (p * (dp - delta)).masked_fill(~vis, 0.0)
+    dq = torch.einsum("bhqk,bkhd->bqhd", ds, kf) * scale
+    dk = torch.einsum("bhqk,bqhd->bkhd", ds, qf) * scale
+    if G > 1:
+        dk = dk.view(B, S, Hkv, G, D).sum(3)
+        dv = dv.view(B, S, Hkv, G, D).sum(3)
+    return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
+
+
+def swiglu(x, w, save=False):
+    F = w.shape[0] // 2
+    z = x.float() @ w.float().t()
+    g, u = z[..., :F], z[..., F:]
+    h = (g / (1 + torch.exp(-g)) * u).to(x.dtype)
+    return (h, z.reshape(-1, 2 * F).to(x.dtype)) if save else h
+
+
+def swiglu_bwd(x, w, gu, dh, need_dx=True, need_dw=True):
+    F = w.shape[0] // 2
+    g, u = gu[:, :F].float(), gu[:, F:].float()
+    d = dh.reshape(-1, F).float()
+    s = 1 / (1 + torch.exp(-g))
+    dz = torch.cat([d * u * s * (1 + g * (1 - s)), d * g * s], dim=1)
+    dx = (dz @ w.float()).to(x.dtype).view(x.shape) if need_dx else None
+    dw = (dz.t() @ x.reshape(-1, x.shape[-1]).float()).to(w.dtype) if need_dw else None
+    return dx, dw
+
+
+def _xent_logits(x, w, targets, scale, ignore_index, keep):
+    V = w.shape[0]
+    z = (x.reshape(-1, x.shape[-1]).float() @ w.float().t()) * scale
+    if keep is not None:
+        bits = (keep[:, :, None] >> torch.arange(32, dtype=torch.int32, device=keep.device)) & 1
+        z = z.masked_fill(bits.reshape(keep.shape[0], -1)[:, :V] == 0, float("-inf"))
+    t = targets.reshape(-1).long()
+    valid = (t != ignore_index) & (t >= 0) & (t < V)
+    return z, t.clamp(0, V - 1)[:, None], valid
+
+
+def linear_xent(x, w, targets, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None):
+    z, at, valid = _xent_logits(x, w, targets, scale, ignore_index, keep)
+    lse = torch.logsumexp(z, -1)
+    zt = z.gather(1, at)[:, 0]
+    loss = torch.where(torch.isneginf(zt), torch.full_like(lse, float("inf")), lse - zt)
+    if smoothing:
+        loss = (1 - smoothing) * loss + smoothing * (lse - z.mean(-1))
+    loss = torch.where(valid, loss, torch.zeros_like(loss))
+    return loss.view(targets.shape), lse.view(targets.shape)
+
+
+def linear_xent_bwd(x, w, targets, lse, dloss, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None, need_dx=True,
+                    need_dw=True):
+    z, at, valid = _xent_logits(x, w, targets, scale, ignore_index, keep)
+    gone = torch.isneginf(z)
+    p = torch.exp(z - lse.reshape(-1, 1)) - smoothing / w.shape[0]
+    p = p.scatter_add(1, at, torch.full_like(z[:, :1], smoothing - 1.0)).masked_fill(gone, 0.0)
+    g = torch.where(valid, dloss.reshape(-1).float(), torch.zeros_like(z[:, 0]))[:, None] * scale
+    dz = torch.where(g == 0, torch.zeros_like(p), p * g)
+    dx = (dz @ w.float()).to(x.dtype).view(x.shape) if need_dx else None
+    dw = (dz.t() @ x.reshape(-1, x.shape[-1]).float()).to(w.dtype) if need_dw else None
+    return dx, dw
+
+
+def norm_train(x, w, b=None, eps=1e-5, kind="rms", delta=None):
+    h = x if delta is None else (x.float() + delta.float()).to(x.dtype)
+    hf = h.reshape(-1, h.shape[-1]).float()
+    mu = hf.mean(-1, keepdim=True) if kind == "layer" else torch.zeros_like(hf[:, :1])
+    r = torch.rsqrt((hf - mu).pow(2).mean(-1, keepdim=True) + eps)
+    y = (hf - mu) * r * w.float()
+    if b is not None:
+        y = y + b.float()
+    return y.to(x.dtype).view(x.shape), h, torch.cat([mu, r], 1)
+
+
+def norm_train_bwd(dy, h, w, stats, kind="rms", bias=False, dh=None):
+    D = h.shape[-1]
+    g = dy.reshape(-1, D).float()
+    r = stats[:, 1:]
+    n = (h.reshape(-1, D).float() - stats[:, :1]) * r
+    a = g * w.float()
+    dx = a - n * (a * n).mean(-1, keepdim=True)
+    if kind == "layer":
+        dx = dx - a.mean(-1, keepdim=True)
+    dx = dx * r
+    if dh is not None:
+        dx = dx + dh.reshape(-1, D).float()
+    return dx.to(h.dtype).view(h.shape), (g * n).sum(0).to(w.dtype), g.sum(0).to(w.dtype) if bias else None

@@ -589,7 +589,7 @@ static CUtensorMap map_bthd(const torch::Tensor& x) {
   CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, x.data_ptr(), dims, strides, box, es,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "attention_bwd: cuTensorMapEncodeTiled failed: ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "attention_bwd: cuTensorMapEncodeTiled failed: ", num((int)r));
   return m;
 }
 
@@ -626,31 +626,40 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
 
 }  // namespace om
 
+namespace {
+
+// [B, T, H, D] bf16 with D contiguous and every other stride a multiple of 8 (16 bytes)
+void check_rows(const torch::Tensor& t, const char* name, int64_t b, int64_t n, int64_t h, int64_t d, bool dense) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(0) == b && t.size(1) == n &&
+                  t.size(2) == h && t.size(3) == d,
+              "attention_bwd: ", name, " must be a bf16 CUDA tensor [", om::num(b), ", ", om::num(n), ", ",
+              om::num(h), ", ", om::num(d), "]");
+  if (t.numel() == 0) return;
+  bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
+  TORCH_CHECK(ok && (!dense || t.is_contiguous()), "attention_bwd: layout of ", name);
+}
+
+}  // namespace
+
 // q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D] bf16 (D contiguous, other strides multiples of 8),
 // lse fp32 [B, T, H] natural log, lens int32 [B] (T == S). dq, dk, dv contiguous.
 void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
                       torch::Tensor dout, c10::optional<torch::Tensor> lens, double scale, bool causal,
                       torch::Tensor dq, torch::Tensor dk, torch::Tensor dv, torch::Tensor status) {
-  auto rows = [&](const torch::Tensor& t, const char* name, at::IntArrayRef shape, bool dense) {
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.sizes() == shape,
-                "attention_bwd: ", name, " must be a bf16 CUDA tensor of shape ", shape);
-    bool ok = (t.stride(3) == 1 || t.size(3) == 1) && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
-    if (t.numel()) TORCH_CHECK(ok && (!dense || t.is_contiguous()), "attention_bwd: layout of ", name);
-  };
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "attention_bwd: q [B, T, H, D], k / v [B, S, Hkv, D]");
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), S = k.size(1), Hkv = k.size(2);
-  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention_bwd: head_dim must be a multiple of 8 up to 128 (got ", D,
-              ")");
+  TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention_bwd: head_dim must be a multiple of 8 up to 128 (got ",
+              om::num(D), ")");
   TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "attention_bwd: query heads must be a multiple of KV heads");
-  rows(q, "q", {B, T, H, D}, false);
-  rows(k, "k", {B, S, Hkv, D}, false);
-  rows(v, "v", {B, S, Hkv, D}, false);
-  rows(out, "out", {B, T, H, D}, false);
-  rows(dout, "dout", {B, T, H, D}, false);
-  rows(dq, "dq", {B, T, H, D}, true);
-  rows(dk, "dk", {B, S, Hkv, D}, true);
-  rows(dv, "dv", {B, S, Hkv, D}, true);
+  check_rows(q, "q", B, T, H, D, false);
+  check_rows(k, "k", B, S, Hkv, D, false);
+  check_rows(v, "v", B, S, Hkv, D, false);
+  check_rows(out, "out", B, T, H, D, false);
+  check_rows(dout, "dout", B, T, H, D, false);
+  check_rows(dq, "dq", B, T, H, D, true);
+  check_rows(dk, "dk", B, S, Hkv, D, true);
+  check_rows(dv, "dv", B, S, Hkv, D, true);
   TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 3 &&
                   lse.size(0) == B && lse.size(1) == T && lse.size(2) == H,
               "attention_bwd: lse must be contiguous fp32 [B, T, H]");

@@ -166,7 +166,7 @@ static void launch_d(const AttnArgs& a, int rows, int G, cudaStream_t st) {
     case 5: paged_attn_kernel<D, 5><<<grid, 128, 0, st>>>(a); break;
     case 8: paged_attn_kernel<D, 8><<<grid, 128, 0, st>>>(a); break;
     case 16: paged_attn_kernel<D, 16><<<grid, 128, 0, st>>>(a); break;
-    default: TORCH_CHECK(false, "paged_attention: unsupported GQA group ", G);
+    default: TORCH_CHECK(false, "paged_attention: unsupported GQA group ", om::num(G));
   }
   OM_LAUNCH_CHECK();
   attn_merge_kernel<D><<<dim3(rows, a.Hq), 128, 0, st>>>(a);

@@ -9,13 +9,20 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <atomic>
 #include <mutex>
+#include <string>
 
 #define OM_CUDA_CHECK(x)                                                                   \
   do {                                                                                     \
     cudaError_t _e = (x);                                                                  \
     TORCH_CHECK(_e == cudaSuccess, "CUDA error ", cudaGetErrorString(_e), " at ", __FILE__, \
-                ":", __LINE__);                                                            \
+                ":", om::num(__LINE__));                                                   \
   } while (0)
+
+namespace om {
+// Numbers enter error messages as text: an extension that carries its own libstdc++ beside
+// torch's may fail inside the stream's number formatting.
+inline std::string num(long long v) { return std::to_string(v); }
+}  // namespace om
 
 // Check the last launch and count it.
 #define OM_LAUNCH_CHECK()                  \
@@ -64,7 +71,7 @@ inline CUtensorMap make_tmap_2d(const void* ptr, CUtensorMapDataType dt, int ele
   CUresult r = encode_fn()(&m, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed: ", num((int)r));
   return m;
 }
 
@@ -82,7 +89,7 @@ inline CUtensorMap make_tmap_3d(const void* ptr, CUtensorMapDataType dt, int ele
   CUresult r = encode_fn()(&m, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (3d) failed: ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (3d) failed: ", num((int)r));
   return m;
 }
 

@@ -441,7 +441,7 @@ void om_dsa_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_ca
     case 4: OM_DSA_LAUNCH(4)
     case 5: OM_DSA_LAUNCH(5)
     case 8: OM_DSA_LAUNCH(8)
-    default: TORCH_CHECK(false, "dsa_attention: unsupported GQA group ", G);
+    default: TORCH_CHECK(false, "dsa_attention: unsupported GQA group ", om::num(G));
   }
 #undef OM_DSA_LAUNCH
   OM_LAUNCH_CHECK();

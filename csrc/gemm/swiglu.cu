@@ -5,8 +5,8 @@
 // Forward: one GEMM whose column tile holds BN / 2 gate columns beside the BN / 2 up columns of
 // the same features (gemm_ex.cuh loads B in two halves F rows apart), so the activation and the
 // product happen on the fp32 accumulators as they leave tensor memory; h is rounded once. For
-// training, g and u are also stored (16 bits each: 4 M F bytes kept, which saves the gradient a
-// third of its products; the rounding enters dg and du at 2^-9 relative, once).
+// training, g and u are also stored, in 32 bits: dg and du are then rounded once, as operands of
+// their products, and keeping them saves the gradient a third of its products.
 //
 // Gradient: s = 1 / (1 + exp(-g))
 //   dg = dh u s (1 + g (1 - s)),  du = dh g s      one pass over g, u, dh
@@ -19,10 +19,26 @@
 
 namespace om {
 
+// exp(-g) = inf gives 0, as it should
+__device__ __forceinline__ float sigmoid_f(float g) { return fast_rcp(1.f + fast_exp2(-1.4426950408889634f * g)); }
+
+// n of 32 fp32 columns
+__device__ __forceinline__ void store_row32(float* dst, const float (&f)[32], int n, bool vec) {
+  if (n >= 32 && vec) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+      *reinterpret_cast<float4*>(dst + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j < n) dst[j] = f[j];
+  }
+}
+
 struct EpiSwiglu {
   struct Args {
     __nv_bfloat16* h;
-    __nv_bfloat16* gu;  // optional [M, ldgu]: g at column f, u at column F + f
+    float* gu;  // optional [M, ldgu]: g at column f, u at column F + f
     int ldh, ldgu, vec_h, vec_gu;
   };
   template <int BN>
@@ -45,13 +61,12 @@ struct EpiSwiglu {
       for (int j = 0; j < 32; ++j) {
         gf[j] = __uint_as_float(gv[j]);
         uf[j] = __uint_as_float(uv[j]);
-        // g / (1 + exp(-g)): exp(-g) = inf gives 0, as it should
-        hf[j] = __fdividef(gf[j], 1.f + fast_exp2(fminf(-1.4426950408889634f * gf[j], 126.f))) * uf[j];
+        hf[j] = gf[j] * sigmoid_f(gf[j]) * uf[j];
       }
       store_row32(e.h + (size_t)r * e.ldh + c0, hf, n, e.vec_h);
       if (e.gu != nullptr) {
         store_row32(e.gu + (size_t)r * e.ldgu + c0, gf, n, e.vec_gu);
-        store_row32(e.gu + (size_t)r * e.ldgu + F + c0, uf, n, e.vec_gu && (F & 7) == 0);
+        store_row32(e.gu + (size_t)r * e.ldgu + F + c0, uf, n, e.vec_gu && (F & 3) == 0);
       }
     }
   }
@@ -59,7 +74,7 @@ struct EpiSwiglu {
 
 // dg, du of one row block; V = 8 where every row start and F allow 16-byte accesses, else 1.
 template <int V>
-__global__ void __launch_bounds__(256) swiglu_grad_kernel(const __nv_bfloat16* __restrict__ gu, long long ldgu,
+__global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restrict__ gu, long long ldgu,
                                                           const __nv_bfloat16* __restrict__ dh, long long lddh,
                                                           __nv_bfloat16* __restrict__ dgu, long long lddgu,
                                                           long long M, int F) {
@@ -70,17 +85,20 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const __nv_bfloat16* _
     const int c = (int)(i - r * nv) * V;
     float g[V], u[V], d[V];
     if constexpr (V == 8) {
-      unpack8(*reinterpret_cast<const uint4*>(gu + r * ldgu + c), g);
-      unpack8(*reinterpret_cast<const uint4*>(gu + r * ldgu + F + c), u);
+      const float4* pg = reinterpret_cast<const float4*>(gu + r * ldgu + c);
+      const float4* pu = reinterpret_cast<const float4*>(gu + r * ldgu + F + c);
+      const float4 g0 = pg[0], g1 = pg[1], u0 = pu[0], u1 = pu[1];
+      g[0] = g0.x; g[1] = g0.y; g[2] = g0.z; g[3] = g0.w; g[4] = g1.x; g[5] = g1.y; g[6] = g1.z; g[7] = g1.w;
+      u[0] = u0.x; u[1] = u0.y; u[2] = u0.z; u[3] = u0.w; u[4] = u1.x; u[5] = u1.y; u[6] = u1.z; u[7] = u1.w;
       unpack8(*reinterpret_cast<const uint4*>(dh + r * lddh + c), d);
     } else {
-      g[0] = __bfloat162float(gu[r * ldgu + c]);
-      u[0] = __bfloat162float(gu[r * ldgu + F + c]);
+      g[0] = gu[r * ldgu + c];
+      u[0] = gu[r * ldgu + F + c];
       d[0] = __bfloat162float(dh[r * lddh + c]);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const float s = __fdividef(1.f, 1.f + fast_exp2(fminf(-1.4426950408889634f * g[j], 126.f)));
+      const float s = sigmoid_f(g[j]);
       const float dg = d[j] * u[j] * s * (1.f + g[j] * (1.f - s));
       u[j] = d[j] * g[j] * s;
       g[j] = dg;
@@ -116,7 +134,13 @@ static void check_bf16_rows(const torch::Tensor& t, const char* op, const char* 
               " is too large");
 }
 
-// h [M, F] = silu(x Wg^T) * (x Wu^T); gu [M, >= 2F] optional.
+static void check_gu(const torch::Tensor& t, const char* op, int64_t M, int64_t F) {
+  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == M && t.size(1) == 2 * F &&
+                  t.is_contiguous() && 2 * F < (1ll << 31),
+              op, ": gu must be fp32 [M, 2F]");
+}
+
+// h [M, F] = silu(x Wg^T) * (x Wu^T); gu fp32 [M, 2F] optional.
 void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<torch::Tensor> gu,
                torch::Tensor status) {
   check_bf16_rows(x, "swiglu", "x");
@@ -134,11 +158,10 @@ void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<
   e.ldh = (int)h.stride(0);
   e.vec_h = h.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(e.h) & 15) == 0;
   if (gu.has_value()) {
-    check_bf16_rows(*gu, "swiglu", "gu");
-    TORCH_CHECK(gu->size(0) == M && gu->size(1) == 2 * F, "swiglu: gu must be [M, 2F]");
-    e.gu = reinterpret_cast<__nv_bfloat16*>(gu->data_ptr());
-    e.ldgu = (int)gu->stride(0);
-    e.vec_gu = gu->stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(e.gu) & 15) == 0;
+    check_gu(*gu, "swiglu", M, F);
+    e.gu = gu->data_ptr<float>();
+    e.ldgu = (int)(2 * F);
+    e.vec_gu = F % 2 == 0 && (reinterpret_cast<uintptr_t>(e.gu) & 15) == 0;
   }
   GemmX g{};
   g.rows = (int)M;
@@ -161,12 +184,11 @@ void om_swiglu_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor gu, torch::Te
                    c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status) {
   check_bf16_rows(x, "swiglu_bwd", "x");
   check_bf16_rows(w, "swiglu_bwd", "w");
-  check_bf16_rows(gu, "swiglu_bwd", "gu");
   check_bf16_rows(dh, "swiglu_bwd", "dh");
   const int64_t M = x.size(0), K = x.size(1), F = w.size(0) / 2;
   TORCH_CHECK(w.size(0) == 2 * F && w.size(1) == K, "swiglu_bwd: w must be [2F, K]");
-  TORCH_CHECK(gu.size(0) == M && gu.size(1) == 2 * F && dh.size(0) == M && dh.size(1) == F,
-              "swiglu_bwd: gu must be [M, 2F] and dh [M, F]");
+  check_gu(gu, "swiglu_bwd", M, F);
+  TORCH_CHECK(dh.size(0) == M && dh.size(1) == F, "swiglu_bwd: dh must be [M, F]");
   TORCH_CHECK(K > 0 && K % 8 == 0, "swiglu_bwd: K must be a positive multiple of 8");
   const c10::cuda::CUDAGuard guard(x.device());
   auto st = at::cuda::getCurrentCUDAStream().stream();
@@ -181,14 +203,14 @@ void om_swiglu_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor gu, torch::Te
   auto al = [](const torch::Tensor& t) {
     return t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   };
-  const bool v8 = F % 8 == 0 && al(gu) && al(dh);
+  const bool v8 = F % 8 == 0 && (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0 && al(dh);
   const long long work = M * (v8 ? F / 8 : F);
   const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)om::num_sms() * 16);
   if (v8)
-    om::swiglu_grad_kernel<8><<<blocks, 256, 0, st>>>(ptr(gu), gu.stride(0), ptr(dh), dh.stride(0), ptr(dgu), ld, M,
+    om::swiglu_grad_kernel<8><<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(dh), dh.stride(0), ptr(dgu), ld, M,
                                                       (int)F);
   else
-    om::swiglu_grad_kernel<1><<<blocks, 256, 0, st>>>(ptr(gu), gu.stride(0), ptr(dh), dh.stride(0), ptr(dgu), ld, M,
+    om::swiglu_grad_kernel<1><<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(dh), dh.stride(0), ptr(dgu), ld, M,
                                                       (int)F);
   OM_LAUNCH_CHECK();
   auto product = [&](om::GxOperand a, om::GxOperand b, int64_t rows, int64_t cols, int64_t k, torch::Tensor& out,

@@ -337,7 +337,7 @@ static void norm_shape(const char* op, int D, bool vec, F&& f) {
     if (D <= 16384) OM_NORM_CASE(1024, 1, 16);
   }
 #undef OM_NORM_CASE
-  TORCH_CHECK(false, op, ": rows of more than 16384 elements are not supported (got ", D, ")");
+  TORCH_CHECK(false, op, ": rows of more than 16384 elements are not supported (got ", num(D), ")");
 }
 
 template <typename F>

@@ -330,7 +330,7 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
 
 def swiglu(x, w, save=False):
     """silu(x Wg^T) * (x Wu^T) of x [..., K] and w [2F, K] (gate rows first) -> [..., F]. With
-    ``save`` also the projections [rows, 2F] that :func:`swiglu_bwd` reads."""
+    ``save`` also the projections, fp32 [rows, 2F], that :func:`swiglu_bwd` reads."""
     _same_device("swiglu", x, w)
     if not x.is_cuda:
         return ref.swiglu(x, w, save)
@@ -338,7 +338,7 @@ def swiglu(x, w, save=False):
         raise ValueError("swiglu: w must be [2F, K]")
     x2, F = _rows(x), w.shape[0] // 2
     h = torch.empty(x2.shape[0], F, dtype=x.dtype, device=x.device)
-    gu = torch.empty(x2.shape[0], 2 * F, dtype=x.dtype, device=x.device) if save else None
+    gu = torch.empty(x2.shape[0], 2 * F, dtype=torch.float32, device=x.device) if save else None
     _native.C().swiglu(x2, _rows(w), h, gu, ctx(x.device).status)
     h = h.view(*x.shape[:-1], F)
     return (h, gu) if save else h

@@ -330,7 +330,7 @@ def swiglu(x, w, save=False):
     z = x.float() @ w.float().t()
     g, u = z[..., :F], z[..., F:]
     h = (g / (1 + torch.exp(-g)) * u).to(x.dtype)
-    return (h, z.reshape(-1, 2 * F).to(x.dtype)) if save else h
+    return (h, z.reshape(-1, 2 * F)) if save else h
 
 
 def swiglu_bwd(x, w, gu, dh, need_dx=True, need_dw=True):

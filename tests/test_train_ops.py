@@ -554,3 +554,13 @@ def test_same_result_on_every_run_and_stream():
     ops.check_status()
     for p, q, r, s in zip(first, again, a, b):
         assert torch.equal(p, q) and torch.equal(p, r) and torch.equal(p, s)
+
+
+def test_native_refusals_name_their_numbers():
+    """An error raised by the native entry (sizes in its text) reaches Python as an exception."""
+    from openmini_v1_b200 import _native
+    if not _native.have_C():
+        pytest.skip("native extension not built")
+    t = torch.zeros(1, 2, 2, 60, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="got 60"):
+        _native.C().attention_bwd(t, t, t, t, t, t, None, 1.0, True, t, t, t, t)

@@ -6,28 +6,30 @@
 //   dS = P * (dO V^T - rowsum(dO * O))
 //   dQ = c dS K,   dK = c dS^T Q
 //
-// Two kernels, so that no gradient is summed by atomics (the same result on every run):
-//   dK, dV  one CTA per 128 keys of a KV head walks the 64-query tiles of its query heads
-//   dQ      one CTA per 128 queries of a head walks the 64-key tiles
+// No gradient is summed by atomics (the same result on every run): one launch holds two kinds of
+// CTAs, the heavy ones first, and the others fill the SMs behind them.
+//   kv  one CTA per 128 keys of a KV head walks the 64-query tiles of its query heads: dK, dV
+//   q   one CTA per 128 queries of a head walks the 64-key tiles: dQ
 // Both keep their rows (keys, or queries) in the MMA's 128 lanes and compute S and dP of a
-// 64-column tile from shared memory; the softmax threads turn a lane's 64 values into P and dS
-// and write them, as 16-bit pairs, over S and dP in tensor memory, from where they are the A
-// operand of the accumulating products. P and dS therefore never touch shared memory, and the
-// transposed form (S^T) needs no transposition. Rounding P and dS to 16 bits enters each
-// gradient at 2^-9 relative per term, independently; sums are fp32 in tensor memory.
+// 64-column tile from shared memory; the softmax threads turn the tile into P and dS and write
+// them, as 16-bit pairs, over S and dP in tensor memory, from where they are the A operand of the
+// accumulating products. P and dS therefore never touch shared memory, and the transposed form
+// (S^T) needs no transposition. Rounding P and dS to 16 bits enters each gradient at 2^-8
+// relative per term at the most, independently; sums are fp32 in tensor memory.
 //
-// Tensor memory of the dK/dV kernel: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512
-// columns, all there are; this is what sets the 64-query tile. Two softmax warpgroups take the
-// two stages in turn, so that the tensor pipe works on one tile while the other is exponentiated.
+// Tensor memory of a kv CTA: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512 columns, all
+// there are; this is what sets the 64-query tile. All eight softmax warps work on one tile, 32
+// columns a thread, because the tile's latency (the exponentials alone take 512 cycles of the
+// SM's 16 a cycle) has to fit into the 1280 cycles of products that run beside it.
 //
-// Seven products instead of the five of a single kernel is the price of the fixed summation
-// order (and of no fp32 dQ in memory).
+// Seven products instead of the five of a single loop is the price of the fixed summation order
+// (and of no fp32 dQ in memory).
 //
 // Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared
 // memory before a product contracts over them, so that whatever padding holds (NaN too) adds 0.
 //
-// Work split: where the key tiles x KV heads leave SMs idle, the query heads of a KV head are
-// divided among `nsplit` CTAs, which leave fp32 partials that a third kernel adds in order.
+// Work split: where all CTAs together would leave SMs idle, the query heads of a KV head are
+// divided among `nsplit` CTAs, which leave fp32 partials that a last kernel adds in order.
 #include <c10/cuda/CUDAGuard.h>
 #include "../common/om_host.h"
 #include "../common/om_ptx.cuh"
@@ -59,7 +61,8 @@ struct AttnBwdArgs {
   int B, T, S, H, Hkv, G, hd;
   int Tp;               // T rounded up to 64
   int causal, off;      // key j visible to query i when j <= i + off
-  int nsplit, gper;     // query heads of one CTA
+  int nsplit, gper;     // kv CTAs of a KV head and key tile, and the query heads of one
+  int kv_blocks;        // the grid's first blocks
   float scale, scale_log2;
   int* status;
 };
@@ -72,24 +75,23 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// (-lse log2 e, rowsum(dO * O)) of every query row, laid out [B, H, Tp] for the kernels below.
+// (-lse log2 e, rowsum(dO * O)) of every query row, laid out [B, H, Tp] for the kernel below.
 // Rows without a visible key (lse = -inf), beyond the length or beyond T get (-inf, 0): P = 0.
-// 16 lanes a row, 8 elements each.
+// 16 lanes a row, 8 elements each; blockIdx.y is the sequence. Bound by reading out and dout.
 __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16* __restrict__ o,
                                                             const __nv_bfloat16* __restrict__ go,
                                                             const float* __restrict__ lse, const int* lens,
-                                                            float2* __restrict__ stat, int B, int T, int Tp, int H,
-                                                            int hd, long long ob, long long ot, long long oh,
-                                                            long long gb, long long gt, long long gh) {
-  const int sub = threadIdx.x & 15;
-  const long long n = (long long)B * Tp * H;
-  for (long long i = (blockIdx.x * 256ll + threadIdx.x) >> 4; i < ((n + 1) & ~1ll); i += gridDim.x * 16ll) {
-    const int h = (int)(i % H);
-    const int t = (int)(i / H % Tp);
-    const int b = (int)(i / H / Tp);
+                                                            float2* __restrict__ stat, int T, int Tp, int H, int hd,
+                                                            long long ob, long long ot, long long oh, long long gb,
+                                                            long long gt, long long gh) {
+  const int sub = threadIdx.x & 15, b = blockIdx.y;
+  const unsigned n = (unsigned)Tp * H;  // below 2^31
+  const int len = lens ? min(lens[b], T) : T;
+  // Tp is a multiple of 64, so both halves of a warp take the same number of turns
+  for (unsigned i = blockIdx.x * 16 + (threadIdx.x >> 4); i < n; i += gridDim.x * 16) {
+    const int t = (int)(i / (unsigned)H), h = (int)(i - (unsigned)t * H);
     float d = 0.f, l = -INFINITY;
-    const bool live = i < n && t < (lens ? min(lens[b], T) : T);
-    if (live) {
+    if (t < len) {
       l = lse[((long long)b * T + t) * H + h];
       if (sub * 8 < hd) {
         float x[8], y[8];
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16*
     }
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (sub == 0 && i < n)
+    if (sub == 0)
       stat[((long long)b * H + h) * Tp + t] =
           l == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-l * fa_bw::LOG2E, d);
   }
@@ -116,45 +118,44 @@ __device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
   }
 }
 
-// One lane's 64 columns of S and dP (tensor memory) -> P and dS, 16 bits, written over them.
-// COLQ: columns are queries (S^T): stat per column from shared memory; else one stat per lane.
-// Column j is visible when lo <= j < hi.
+// A thread's 32 columns of S and dP (tensor memory) -> P and dS, 16 bits, written over the
+// tile's S and dP. COLQ: columns are queries (S^T), their stats come from shared memory; else the
+// thread's row has one stat. The results take the first 16 of the columns that the thread itself
+// has read (P and dS of tile columns 32 .. 63 therefore start at column 32, not 16). Column j (of
+// the tile) is visible when lo <= j < hi.
 template <bool COLQ>
 __device__ __forceinline__ void softmax_grad(uint32_t s_tmem, uint32_t dp_tmem, uint32_t stat_smem, float2 own,
-                                             float c2, int lo, int hi, bool masked, bool want_p) {
+                                             float c2, int col0, int lo, int hi, bool masked) {
+  uint32_t sv[32], dv[32];
+  tmem_ld_32x32b_x32(s_tmem + col0, sv);
+  tmem_ld_32x32b_x32(dp_tmem + col0, dv);
+  tc_wait_ld();
+  uint32_t pk[16], dk[16];
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t sv[32], dv[32];
-    tmem_ld_32x32b_x32(s_tmem + half * 32, sv);
-    tmem_ld_32x32b_x32(dp_tmem + half * 32, dv);
-    tc_wait_ld();
-    uint32_t pk[16], dk[16];
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      float2 a = own, b = own;
-      if constexpr (COLQ) {
-        const uint4 u = lds128(stat_smem + (half * 32 + j) * 8);
-        a = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-        b = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
-      }
-      float p0 = fast_exp2(fmaf(__uint_as_float(sv[j]), c2, a.x));
-      float p1 = fast_exp2(fmaf(__uint_as_float(sv[j + 1]), c2, b.x));
-      float d0 = p0 * (__uint_as_float(dv[j]) - a.y);
-      float d1 = p1 * (__uint_as_float(dv[j + 1]) - b.y);
-      if (masked) {  // selected, not multiplied: what lies under a mask may be anything
-        const int c = half * 32 + j;
-        const bool v0 = c >= lo && c < hi, v1 = c + 1 >= lo && c + 1 < hi;
-        p0 = v0 ? p0 : 0.f;
-        d0 = v0 ? d0 : 0.f;
-        p1 = v1 ? p1 : 0.f;
-        d1 = v1 ? d1 : 0.f;
-      }
-      pk[j / 2] = pack_bf16x2(p0, p1);
-      dk[j / 2] = pack_bf16x2(d0, d1);
+  for (int j = 0; j < 32; j += 2) {
+    float2 a = own, b = own;
+    if constexpr (COLQ) {
+      const uint4 u = lds128(stat_smem + (col0 + j) * 8);
+      a = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+      b = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
     }
-    if (want_p) tmem_st_32x32b_x16(s_tmem + half * 16, pk);
-    tmem_st_32x32b_x16(dp_tmem + half * 16, dk);
+    float p0 = fast_exp2(fmaf(__uint_as_float(sv[j]), c2, a.x));
+    float p1 = fast_exp2(fmaf(__uint_as_float(sv[j + 1]), c2, b.x));
+    float d0 = p0 * (__uint_as_float(dv[j]) - a.y);
+    float d1 = p1 * (__uint_as_float(dv[j + 1]) - b.y);
+    if (masked) {  // selected, not multiplied: what lies under a mask may be anything
+      const int c = col0 + j;
+      const bool v0 = c >= lo && c < hi, v1 = c + 1 >= lo && c + 1 < hi;
+      p0 = v0 ? p0 : 0.f;
+      d0 = v0 ? d0 : 0.f;
+      p1 = v1 ? p1 : 0.f;
+      d1 = v1 ? d1 : 0.f;
+    }
+    pk[j / 2] = pack_bf16x2(p0, p1);
+    dk[j / 2] = pack_bf16x2(d0, d1);
   }
+  if constexpr (COLQ) tmem_st_32x32b_x16(s_tmem + col0, pk);
+  tmem_st_32x32b_x16(dp_tmem + col0, dk);
   tc_wait_st();
 }
 
@@ -184,18 +185,17 @@ __device__ __forceinline__ void write_acc(uint32_t tmem, OUT* dst, bool live, bo
   }
 }
 
-// ------------------------------------------------------------------ dK, dV
-template <int D>
-__global__ void __launch_bounds__(384, 1)
-    attn_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const AttnBwdArgs a) {
+// ------------------------------------------------------------------ the CTA of either kind
+// KV: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
+// else: resident Q, dO; streamed K, V; accumulates dQ.
+template <int D, bool KV>
+__device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUtensorMap& tmG, const CUtensorMap& tmK,
+                                             const CUtensorMap& tmV, const AttnBwdArgs& a, int block, uint8_t* smem) {
   using C = fa_bw::Cfg<D>;
   constexpr int NS = fa_bw::NSTAGE;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* full = kv_full + 1;     // [NS]
+  constexpr int STAGE0 = KV ? 256 : 128;  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D), then the stages
+  uint64_t* fix_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* full = fix_full + 1;    // [NS]
   uint64_t* empty = full + NS;      // [NS]
   uint64_t* land = empty + NS;      // a padded tile before its rows are cleared
   uint64_t* s_full = land + 1;      // [2]
@@ -204,24 +204,42 @@ __global__ void __launch_bounds__(384, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  // heaviest tiles (the first keys, under a causal mask) first
-  const int per = a.B * a.Hkv * a.nsplit;
-  const int kt = blockIdx.x / per;
-  int rest = blockIdx.x % per;
-  const int split = rest % a.nsplit;
-  rest /= a.nsplit;
-  const int kvh = rest % a.Hkv, b = rest / a.Hkv;
-  const int k0 = kt * 128;
-  const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
-  const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
-  const int g0 = split * a.gper, g1 = min(a.G, g0 + a.gper);
-  const int qt0 = a.causal ? max(0, k0 - a.off) / 64 : 0;
-  const int qt1 = (nq + 63) / 64;
-  const int nqt = k0 < nk ? max(0, qt1 - qt0) : 0;
-  const int total = nqt * max(0, g1 - g0);
+  // which rows, heads and tiles; the heaviest tiles come first: under a causal mask the first
+  // keys (kv) and the last queries (q)
+  int b, kvh, head = 0, split = 0, row0, first, ntile, total;
+  {
+    const int heads = KV ? a.Hkv * a.nsplit : a.H;
+    const int per = a.B * heads;
+    int tile = block / per, rest = block % per;
+    b = rest / heads;
+    rest %= heads;
+    const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
+    const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
+    if constexpr (KV) {
+      split = rest % a.nsplit;
+      kvh = rest / a.nsplit;
+      row0 = tile * 128;
+      head = kvh * a.G + split * a.gper;
+      first = a.causal ? max(0, row0 - a.off) / 64 : 0;
+      ntile = row0 < nk ? max(0, (nq + 63) / 64 - first) : 0;
+      total = ntile * max(0, min(a.G - split * a.gper, a.gper));
+    } else {
+      head = rest;
+      kvh = head / a.G;
+      row0 = ((a.T + 127) / 128 - 1 - tile) * 128;
+      const int last = min(nq, row0 + 128) - 1;
+      const int kend = last < row0 ? 0 : (a.causal ? min(nk, last + a.off + 1) : nk);
+      first = 0;
+      total = ntile = kend > 0 ? (kend + 63) / 64 : 0;
+    }
+  }
+  const int len_b = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;    // T == S with lens
+  const int nstream = KV ? (a.lens ? len_b : a.T) : len_b;         // valid rows of the streamed operands
+  const int nrow = KV ? len_b : (a.lens ? len_b : a.T);            // valid rows of the resident ones
+  const bool may_pad = a.lens != nullptr && nstream < a.S;         // beyond T the copies fill zeros themselves
 
   if (threadIdx.x == 0) {
-    mbar_init(kv_full, 1);
+    mbar_init(fix_full, 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -229,7 +247,7 @@ __global__ void __launch_bounds__(384, 1)
     mbar_init(land, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[s], 256);
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
@@ -238,36 +256,38 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // dV [0, D), dK [128, 128 + D), stage s: S^T at 256 + 128 s, dP^T 64 on
+  const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (the whole warp)
     bool ok = true;
     int it = 0, landed = 0;
     if (total > 0 && lane == 0) {
-      mbar_arrive_expect_tx(kv_full, C::FIX_BYTES);
+      mbar_arrive_expect_tx(fix_full, C::FIX_BYTES);
       for (int h = 0; h < C::H; ++h)
         for (int r = 0; r < 2; ++r) {
-          tma_load_4d(smem + h * C::BIG + r * C::SMALL, &tmK, kv_full, h * 64, kvh, k0 + r * 64, b);
-          tma_load_4d(smem + (C::H + h) * C::BIG + r * C::SMALL, &tmV, kv_full, h * 64, kvh, k0 + r * 64, b);
+          const int off = h * C::BIG + r * C::SMALL;
+          tma_load_4d(smem + off, KV ? &tmK : &tmQ, fix_full, h * 64, KV ? kvh : head, row0 + r * 64, b);
+          tma_load_4d(smem + C::H * C::BIG + off, KV ? &tmV : &tmG, fix_full, h * 64, KV ? kvh : head, row0 + r * 64, b);
         }
     }
+    int tile = 0, hd = head;
     for (; it < total; ++it) {
-      const int s = it % NS;
-      const int head = kvh * a.G + g0 + it / nqt, q0 = (qt0 + it % nqt) * 64;
+      const int s = it % NS, x0 = (first + tile) * 64;
       ok = mbar_wait(&empty[s], ((it / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
-      const bool pad = nq - q0 < 64 && nq < a.T;  // rows beyond T are zero already (the copy fills them)
+      const bool pad = may_pad && nstream - x0 < 64;
       uint64_t* bar = pad ? land : &full[s];
       if (lane == 0) {
-        mbar_arrive_expect_tx(bar, C::ST_BYTES + C::STAT);
+        mbar_arrive_expect_tx(bar, C::ST_BYTES + (KV ? C::STAT : 0));
         for (int h = 0; h < C::H; ++h) {
-          tma_load_4d(st + h * C::SMALL, &tmQ, bar, h * 64, head, q0, b);
-          tma_load_4d(st + (C::H + h) * C::SMALL, &tmG, bar, h * 64, head, q0, b);
+          tma_load_4d(st + h * C::SMALL, KV ? &tmQ : &tmK, bar, h * 64, KV ? hd : kvh, x0, b);
+          tma_load_4d(st + (C::H + h) * C::SMALL, KV ? &tmG : &tmV, bar, h * 64, KV ? hd : kvh, x0, b);
         }
-        bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + ((size_t)b * a.H + head) * a.Tp + q0, C::STAT, bar);
+        if constexpr (KV)
+          bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + ((size_t)b * a.H + hd) * a.Tp + x0, C::STAT, bar);
       }
       __syncwarp();
       if (pad) {
@@ -275,57 +295,62 @@ __global__ void __launch_bounds__(384, 1)
         ++landed;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        clear_rows<2 * C::H>(st, nq - q0, lane);
+        clear_rows<2 * C::H>(st, nstream - x0, lane);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[s]);
       }
+      if (++tile == ntile) {
+        tile = 0;
+        ++hd;
+      }
     }
     if (!ok) {  // wait (bounded) for the loads that may still be in flight
       for (int j = max(0, it - NS); j < it; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
-      mbar_wait(kv_full, 0, nullptr, 0);
+      mbar_wait(fix_full, 0, nullptr, 0);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (total > 0 && elect_one()) {
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
       constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
-      const uint32_t k_addr = smem_u32(smem), v_addr = k_addr + C::H * C::BIG;
-      bool ok = mbar_wait(kv_full, 0, a.status, OM_ERR_WAIT_FULL);
+      const uint32_t r0 = smem_u32(smem), r1 = r0 + C::H * C::BIG;  // K, V or Q, dO
+      bool ok = mbar_wait(fix_full, 0, a.status, OM_ERR_WAIT_FULL);
       for (int it = 0; it <= total && ok; ++it) {
         if (it < total) {
           const int s = it % NS;
           if (!mbar_wait(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t q_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
-          const uint32_t g_addr = q_addr + C::H * C::SMALL;
-          const uint32_t d = tmem + 256 + (it & 1) * 128;
-          // stage it & 1 was last read by the products of tile it - 2, issued before: they run in order
+          const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
+          const uint32_t d = tmem + STAGE0 + (it & 1) * 128;
+          // stage it & 1 was last read by the products of tile it - 2, issued before by this
+          // thread: the tensor pipe runs them in order
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d, smem_desc_sw128(k_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(q_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+            tc_mma_f16(d, smem_desc_sw128(r0 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(x0 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d + 64, smem_desc_sw128(v_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(g_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+            tc_mma_f16(d + 64, smem_desc_sw128(r1 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                       smem_desc_sw128(x1 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
           tc_commit(&s_full[it & 1]);
         }
         if (it > 0) {
           const int j = it - 1, s = j % NS;
           if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t q_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
-          const uint32_t g_addr = q_addr + C::H * C::SMALL;
-          const uint32_t p = tmem + 256 + (j & 1) * 128;
+          const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
+          const uint32_t p = tmem + STAGE0 + (j & 1) * 128;
+          if constexpr (KV) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 queries a step
-            tc_mma_f16_ts(tmem, p + k * 8, smem_desc_sw128_mn(g_addr + k * 2048, C::SMALL, 1024), IDESC_A,
-                          j > 0 || k > 0);
+            for (int k = 0; k < 4; ++k)  // 16 queries a step
+              tc_mma_f16_ts(tmem, p + (k >> 1) * 32 + (k & 1) * 8, smem_desc_sw128_mn(x1 + k * 2048, C::SMALL, 1024), IDESC_A,
+                            j > 0 || k > 0);
+          }
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc_mma_f16_ts(tmem + 128, p + 64 + k * 8, smem_desc_sw128_mn(q_addr + k * 2048, C::SMALL, 1024), IDESC_A,
-                          j > 0 || k > 0);
+          for (int k = 0; k < 4; ++k)  // dK += dS^T Q, or dQ += dS K
+            tc_mma_f16_ts(tmem + (KV ? 128 : 0), p + 64 + (k >> 1) * 32 + (k & 1) * 8,
+                          smem_desc_sw128_mn(x0 + k * 2048, C::SMALL, 1024), IDESC_A, j > 0 || k > 0);
           tc_commit(&empty[s]);
         }
       }
@@ -333,41 +358,60 @@ __global__ void __launch_bounds__(384, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax and output
-    const int wg = (warp - 4) >> 2;
-    const int t = threadIdx.x & 127;  // key row == TMEM lane
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int key = k0 + t;
+    const int half = (warp - 4) >> 2;            // columns 32 half .. of a tile
+    const int t = (warp & 3) * 32 + lane;        // row == TMEM lane
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int row = row0 + t;
+    float2 own = make_float2(0.f, 0.f);
+    bool zero = total == 0;
+    if constexpr (!KV) {
+      own.x = -INFINITY;
+      if (row < nrow) own = a.stat[((size_t)b * a.H + head) * a.Tp + row];
+      zero = zero || own.x == -INFINITY;         // padding, or no visible key: gradient 0
+    }
     bool ok = true;
-    for (int it = wg; it < total; it += 2) {
-      const int q0 = (qt0 + it % nqt) * 64;
-      ok = mbar_wait(&s_full[wg], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-      // every thread that waits for a tile's statistics waits for its load as well
-      ok = ok && mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+    int tile = 0;
+    for (int it = 0; it < total; ++it) {
+      const int x0 = (first + tile) * 64;
+      if (++tile == ntile) tile = 0;
+      ok = mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+      // whoever reads a tile's statistics waits for their copy as well
+      if constexpr (KV) ok = ok && mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const bool masked = k0 + 128 > nk || (a.causal && k0 + 127 > q0 + a.off);
-      const int lo = key >= nk ? 64 : (a.causal ? key - a.off - q0 : 0);
-      const uint32_t st = tmem + lanes + 256 + wg * 128;
-      softmax_grad<true>(st, st + 64, smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT), make_float2(0.f, 0.f),
-                         a.scale_log2, lo, 64, masked, true);
+      const uint32_t st = lanes + STAGE0 + (it & 1) * 128;
+      if constexpr (KV) {
+        const bool masked = row0 + 128 > nrow || (a.causal && row0 + 127 > x0 + a.off);
+        const int lo = row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0);
+        softmax_grad<true>(st, st + 64, smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT), own, a.scale_log2,
+                           half * 32, lo, 64, masked);
+      } else {
+        const bool masked = x0 + 64 > nstream || (a.causal && x0 + 63 > row0 + a.off);
+        const int hi = min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64);
+        softmax_grad<false>(st, st + 64, 0, own, a.scale_log2, half * 32, 0, hi, masked);
+      }
       tc_fence_before();
-      mbar_arrive(&p_full[wg]);
+      mbar_arrive(&p_full[it & 1]);
     }
     if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      // warpgroup 0 writes dV, warpgroup 1 writes dK
-      const bool live = key < a.S;
-      const size_t at = (((size_t)b * a.S + key) * a.Hkv + kvh) * a.hd;
-      const float f = wg ? a.scale : 1.f;
-      const uint32_t acc = tmem + lanes + wg * 128;
-      if (a.nsplit > 1) {
-        const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
-        write_acc<D>(acc, a.part + (split * 2 + wg) * plane + at, live, total == 0, f, a.hd);
-      } else {
-        write_acc<D>(acc, (wg ? a.dk : a.dv) + at, live, total == 0, f, a.hd);
+      if constexpr (KV) {
+        // the first four warps write dV, the others dK
+        const bool live = row < a.S;
+        const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd;
+        const float f = half ? a.scale : 1.f;
+        if (a.nsplit > 1) {
+          const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
+          write_acc<D>(lanes + half * 128, a.part + (split * 2 + half) * plane + at, live, zero, f, a.hd);
+        } else {
+          write_acc<D>(lanes + half * 128, (half ? a.dk : a.dv) + at, live, zero, f, a.hd);
+        }
+      } else {  // each half writes half of the columns
+        write_acc<D / 2>(lanes + half * (D / 2), a.dq + (((size_t)b * a.T + row) * a.H + head) * a.hd + half * (D / 2),
+                            row < a.T, zero, a.scale, a.hd - half * (D / 2));
       }
     }
   }
@@ -378,6 +422,19 @@ __global__ void __launch_bounds__(384, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const AttnBwdArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  if ((int)blockIdx.x < a.kv_blocks)
+    attn_bwd_cta<D, true>(tmQ, tmG, tmK, tmV, a, blockIdx.x, smem);
+  else
+    attn_bwd_cta<D, false>(tmQ, tmG, tmK, tmV, a, blockIdx.x - a.kv_blocks, smem);
 }
 
 // Adds the query-head splits' fp32 partials in split order.
@@ -396,183 +453,6 @@ __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const float* __restr
     o.x = pack_bf16x2(s.x, s.y);
     o.y = pack_bf16x2(s.z, s.w);
     *reinterpret_cast<uint2*>((k ? dk : dv) + at) = o;
-  }
-}
-
-// ------------------------------------------------------------------ dQ
-template <int D>
-__global__ void __launch_bounds__(384, 1)
-    attn_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                      const AttnBwdArgs a) {
-  using C = fa_bw::Cfg<D>;
-  constexpr int NS = fa_bw::NSTAGE;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* full = q_full + 1;
-  uint64_t* empty = full + NS;
-  uint64_t* land = empty + NS;
-  uint64_t* s_full = land + 1;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* acc_full = p_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // heaviest tiles (the last queries, under a causal mask) first; the heads of a KV head side by side
-  const int per = a.B * a.H;
-  const int tiles = (a.T + 127) / 128;
-  const int qt = tiles - 1 - blockIdx.x / per;
-  const int head = blockIdx.x % per % a.H, b = blockIdx.x % per / a.H;
-  const int kvh = head / a.G;
-  const int q0 = qt * 128;
-  const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
-  const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
-  const int last = min(nq, q0 + 128) - 1;  // last valid query of the tile
-  const int kend = last < q0 ? 0 : (a.causal ? min(nk, last + a.off + 1) : nk);
-  const int total = kend > 0 ? (kend + 63) / 64 : 0;
-
-  if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(land, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
-    }
-    mbar_init(acc_full, 1);
-    fence_barrier_init();
-  }
-  if (warp == 2) tmem_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;  // dQ [0, D), stage s: S at 128 + 128 s, dP 64 on
-
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer (the whole warp)
-    bool ok = true;
-    int it = 0, landed = 0;
-    if (total > 0 && lane == 0) {
-      mbar_arrive_expect_tx(q_full, C::FIX_BYTES);
-      for (int h = 0; h < C::H; ++h)
-        for (int r = 0; r < 2; ++r) {
-          tma_load_4d(smem + h * C::BIG + r * C::SMALL, &tmQ, q_full, h * 64, head, q0 + r * 64, b);
-          tma_load_4d(smem + (C::H + h) * C::BIG + r * C::SMALL, &tmG, q_full, h * 64, head, q0 + r * 64, b);
-        }
-    }
-    for (; it < total; ++it) {
-      const int s = it % NS, k0 = it * 64;
-      ok = mbar_wait(&empty[s], ((it / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
-      const bool pad = nk - k0 < 64 && nk < a.S;
-      uint64_t* bar = pad ? land : &full[s];
-      if (lane == 0) {
-        mbar_arrive_expect_tx(bar, C::ST_BYTES);
-        for (int h = 0; h < C::H; ++h) {
-          tma_load_4d(st + h * C::SMALL, &tmK, bar, h * 64, kvh, k0, b);
-          tma_load_4d(st + (C::H + h) * C::SMALL, &tmV, bar, h * 64, kvh, k0, b);
-        }
-      }
-      __syncwarp();
-      if (pad) {
-        ok = mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL);
-        ++landed;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        clear_rows<2 * C::H>(st, nk - k0, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
-      }
-    }
-    if (!ok) {
-      for (int j = max(0, it - NS); j < it; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
-      mbar_wait(q_full, 0, nullptr, 0);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (total > 0 && elect_one()) {
-      constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
-      constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
-      const uint32_t q_addr = smem_u32(smem), g_addr = q_addr + C::H * C::BIG;
-      bool ok = mbar_wait(q_full, 0, a.status, OM_ERR_WAIT_FULL);
-      for (int it = 0; it <= total && ok; ++it) {
-        if (it < total) {
-          const int s = it % NS;
-          if (!mbar_wait(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t k_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
-          const uint32_t v_addr = k_addr + C::H * C::SMALL;
-          const uint32_t d = tmem + 128 + (it & 1) * 128;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d, smem_desc_sw128(q_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(k_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d + 64, smem_desc_sw128(g_addr + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(v_addr + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-          tc_commit(&s_full[it & 1]);
-        }
-        if (it > 0) {
-          const int j = it - 1, s = j % NS;
-          if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t k_addr = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES);
-          const uint32_t p = tmem + 128 + (j & 1) * 128 + 64;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // 16 keys a step
-            tc_mma_f16_ts(tmem, p + k * 8, smem_desc_sw128_mn(k_addr + k * 2048, C::SMALL, 1024), IDESC_A,
-                          j > 0 || k > 0);
-          tc_commit(&empty[s]);
-        }
-      }
-      if (ok) tc_commit(acc_full);
-    }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------ softmax and output
-    const int wg = (warp - 4) >> 2;
-    const int t = threadIdx.x & 127;  // query row == TMEM lane
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const int q = q0 + t;
-    const bool row = q < nq;
-    float2 own = make_float2(-INFINITY, 0.f);
-    if (row) own = a.stat[((size_t)b * a.H + head) * a.Tp + q];
-    const bool empty_row = own.x == -INFINITY;  // padding, or no visible key: gradient 0
-    bool ok = true;
-    for (int it = wg; it < total; it += 2) {
-      const int k0 = it * 64;
-      ok = mbar_wait(&s_full[wg], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      const bool masked = k0 + 64 > nk || (a.causal && k0 + 63 > q0 + a.off);
-      const int hi = min(nk - k0, a.causal ? q + a.off + 1 - k0 : 64);
-      const uint32_t st = tmem + lanes + 128 + wg * 128;
-      softmax_grad<false>(st, st + 64, 0, own, a.scale_log2, 0, hi, masked, false);
-      tc_fence_before();
-      mbar_arrive(&p_full[wg]);
-    }
-    if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok && wg == 0) {
-      tc_fence_after();
-      write_acc<D>(tmem + lanes, a.dq + (((size_t)b * a.T + q) * a.H + head) * a.hd, q < a.T,
-                   total == 0 || empty_row, a.scale, a.hd);
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 2) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -601,25 +481,17 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
   int dev;
   OM_CUDA_CHECK(cudaGetDevice(&dev));
   if (!attr_set[dev].load()) {
-    OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_kv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_q_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_set[dev].store(true);
   }
-  const long long kv = (long long)((a.S + 127) / 128) * a.B * a.Hkv * a.nsplit;
-  const long long qb = (long long)((a.T + 127) / 128) * a.B * a.H;
-  TORCH_CHECK(kv < (1ll << 31) && qb < (1ll << 31), "attention_bwd: too many tiles");
-  if (kv) {
-    attn_bwd_kv_kernel<D><<<(unsigned)kv, 384, C::SMEM, st>>>(q, g, k, v, a);
-    OM_LAUNCH_CHECK();
-  }
-  if (a.nsplit > 1 && kv) {
+  const long long blocks = a.kv_blocks + (long long)((a.T + 127) / 128) * a.B * a.H;
+  TORCH_CHECK(blocks < (1ll << 31), "attention_bwd: too many tiles");
+  attn_bwd_kernel<D><<<(unsigned)blocks, 384, C::SMEM, st>>>(q, g, k, v, a);
+  OM_LAUNCH_CHECK();
+  if (a.nsplit > 1) {
     const long long n = (long long)a.B * a.S * a.Hkv * a.hd;
-    const int blocks = (int)std::min<long long>((2 * n + 1023) / 1024, (long long)num_sms() * 8);
-    attn_bwd_join_kernel<<<blocks, 256, 0, st>>>(a.part, a.nsplit, n, a.dv, a.dk);
-    OM_LAUNCH_CHECK();
-  }
-  if (qb) {
-    attn_bwd_q_kernel<D><<<(unsigned)qb, 384, C::SMEM, st>>>(q, g, k, v, a);
+    const int jb = (int)std::min<long long>((2 * n + 1023) / 1024, (long long)num_sms() * 8);
+    attn_bwd_join_kernel<<<jb, 256, 0, st>>>(a.part, a.nsplit, n, a.dv, a.dk);
     OM_LAUNCH_CHECK();
   }
 }
@@ -628,58 +500,61 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
 
 namespace {
 
-// [B, T, H, D] bf16 with D contiguous and every other stride a multiple of 8 (16 bytes)
-void check_rows(const torch::Tensor& t, const char* name, int64_t b, int64_t n, int64_t h, int64_t d, bool dense) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 4 && t.size(0) == b && t.size(1) == n &&
-                  t.size(2) == h && t.size(3) == d,
-              "attention_bwd: ", name, " must be a bf16 CUDA tensor [", om::num(b), ", ", om::num(n), ", ",
-              om::num(h), ", ", om::num(d), "]");
-  if (t.numel() == 0) return;
+// [B, T, H, D] bf16 as the kernels read it: D contiguous, every other stride a positive multiple
+// of 8 (16 bytes). Anything else is copied.
+torch::Tensor read_rows(const torch::Tensor& t, const char* name, int64_t b, int64_t n, int64_t h, int64_t d) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 4 && t.size(0) == b && t.size(1) == n && t.size(2) == h && t.size(3) == d,
+              "attention_bwd: ", name, " must be a CUDA tensor [", om::num(b), ", ", om::num(n), ", ", om::num(h),
+              ", ", om::num(d), "]");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, "attention_bwd: ", name, " must be bf16");
+  if (t.numel() == 0) return t;
   bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) > 0));
-  TORCH_CHECK(ok && (!dense || t.is_contiguous()), "attention_bwd: layout of ", name);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 }  // namespace
 
-// q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D] bf16 (D contiguous, other strides multiples of 8),
-// lse fp32 [B, T, H] natural log, lens int32 [B] (T == S). dq, dk, dv contiguous.
-void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
-                      torch::Tensor dout, c10::optional<torch::Tensor> lens, double scale, bool causal,
-                      torch::Tensor dq, torch::Tensor dk, torch::Tensor dv, torch::Tensor status) {
+// (dq, dk, dv) of q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D], lse fp32 [B, T, H] natural log,
+// lens int32 [B] (T == S).
+std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out,
+                                            torch::Tensor lse, torch::Tensor dout, c10::optional<torch::Tensor> lens,
+                                            double scale, bool causal, torch::Tensor status) {
   TORCH_CHECK(q.dim() == 4 && k.dim() == 4, "attention_bwd: q [B, T, H, D], k / v [B, S, Hkv, D]");
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2), D = q.size(3), S = k.size(1), Hkv = k.size(2);
   TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0, "attention_bwd: head_dim must be a multiple of 8 up to 128 (got ",
               om::num(D), ")");
   TORCH_CHECK(Hkv > 0 && H % Hkv == 0, "attention_bwd: query heads must be a multiple of KV heads");
-  check_rows(q, "q", B, T, H, D, false);
-  check_rows(k, "k", B, S, Hkv, D, false);
-  check_rows(v, "v", B, S, Hkv, D, false);
-  check_rows(out, "out", B, T, H, D, false);
-  check_rows(dout, "dout", B, T, H, D, false);
-  check_rows(dq, "dq", B, T, H, D, true);
-  check_rows(dk, "dk", B, S, Hkv, D, true);
-  check_rows(dv, "dv", B, S, Hkv, D, true);
-  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() && lse.dim() == 3 &&
-                  lse.size(0) == B && lse.size(1) == T && lse.size(2) == H,
-              "attention_bwd: lse must be contiguous fp32 [B, T, H]");
+  TORCH_CHECK(T < (1 << 30) && S < (1 << 30) && ((T + 63) / 64 * 64) * H < (1ll << 31) && B < 65536,
+              "attention_bwd: batch, sequence or head count too large");
+  TORCH_CHECK(q.is_cuda(), "attention_bwd: CUDA tensors required");
+  const c10::cuda::CUDAGuard guard(q.device());
+  q = read_rows(q, "q", B, T, H, D);
+  k = read_rows(k, "k", B, S, Hkv, D);
+  v = read_rows(v, "v", B, S, Hkv, D);
+  out = read_rows(out, "out", B, T, H, D);
+  dout = read_rows(dout, "dout", B, T, H, D);
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == B &&
+                  lse.size(1) == T && lse.size(2) == H,
+              "attention_bwd: lse must be fp32 [B, T, H]");
+  lse = lse.contiguous();
   om::AttnBwdArgs a{};
   if (lens.has_value()) {
     TORCH_CHECK(T == S, "attention_bwd: lens needs as many queries as keys");
-    TORCH_CHECK(lens->is_cuda() && lens->scalar_type() == at::kInt && lens->is_contiguous() && lens->dim() == 1 &&
-                    lens->size(0) == B,
-                "attention_bwd: lens must be int32 [B]");
+    TORCH_CHECK(lens->is_cuda() && lens->dim() == 1 && lens->size(0) == B, "attention_bwd: lens must be int32 [B]");
+    lens = lens->to(at::kInt).contiguous();
     a.lens = lens->data_ptr<int>();
   }
-  TORCH_CHECK(T < (1 << 30) && S < (1 << 30), "attention_bwd: sequence too long");
-  const c10::cuda::CUDAGuard guard(q.device());
-  auto st = at::cuda::getCurrentCUDAStream().stream();
+  auto dq = torch::empty({B, T, H, D}, q.options());
+  auto dk = torch::empty({B, S, Hkv, D}, q.options());
+  auto dv = torch::empty({B, S, Hkv, D}, q.options());
   if (B == 0 || T == 0 || S == 0) {
     dq.zero_();
     dk.zero_();
     dv.zero_();
-    return;
+    return {dq, dk, dv};
   }
+  auto st = at::cuda::getCurrentCUDAStream().stream();
   auto ptr = [](const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); };
   a.B = (int)B; a.T = (int)T; a.S = (int)S; a.H = (int)H; a.Hkv = (int)Hkv; a.G = (int)(H / Hkv); a.hd = (int)D;
   a.Tp = (int)((T + 63) / 64 * 64);
@@ -691,28 +566,32 @@ void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::
   a.dk = ptr(dk);
   a.dv = ptr(dv);
   a.status = status.data_ptr<int>();
-  auto stat = torch::empty({B * H * a.Tp, 2}, lse.options());
-  a.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
-  // query heads of a KV head are divided until the CTAs are twice the SMs (a causal mask makes
-  // them uneven) or each has one head
-  const int64_t base = (S + 127) / 128 * B * Hkv, want = 2 * om::num_sms();
-  a.nsplit = (int)std::min<int64_t>(a.G, std::max<int64_t>(1, want / base));
-  a.gper = (a.G + a.nsplit - 1) / a.nsplit;
+  // A kv CTA with all query heads of its KV head walks up to G T / 64 tiles. The launch ends about
+  // when the longest CTA or the average SM does, so a CTA gets as many heads as fit into the
+  // average (a q tile counts 0.75 of a kv tile), and all of them where that is a few tiles anyway
+  // (a join costs more).
+  const int64_t qt = (T + 63) / 64, kt = (S + 127) / 128;
+  const double average = (double)B * H * qt * kt * (causal ? 0.5 : 1.0) * 1.75 / om::num_sms();
+  a.gper = a.G * qt <= 16 ? a.G : (int)std::min<double>(a.G, std::max(1.0, average / qt));
   a.nsplit = (a.G + a.gper - 1) / a.gper;
-  torch::Tensor part;
-  if (a.nsplit > 1) {
-    part = torch::empty({(int64_t)a.nsplit * 2 * B * S * Hkv * D}, lse.options());
-    a.part = part.data_ptr<float>();
-  }
-  const long long n = (long long)B * a.Tp * H;
-  const int blocks = (int)std::min<long long>((n + 15) / 16, (long long)om::num_sms() * 16);
-  om::attn_bwd_stat_kernel<<<blocks, 256, 0, st>>>(
-      ptr(out), ptr(dout), lse.data_ptr<float>(), a.lens, reinterpret_cast<float2*>(stat.data_ptr<float>()), a.B, a.T,
-      a.Tp, a.H, a.hd, out.stride(0), out.stride(1), out.stride(2), dout.stride(0), dout.stride(1), dout.stride(2));
+  TORCH_CHECK(kt * B * Hkv * a.nsplit < (1ll << 30), "attention_bwd: too many tiles");
+  a.kv_blocks = (int)(kt * B * Hkv * a.nsplit);
+  // scratch: the rows' statistics, then the split heads' partials
+  const int64_t stat_floats = B * H * a.Tp * 2, plane = B * S * Hkv * D;
+  auto ws = torch::empty({stat_floats + (a.nsplit > 1 ? 2 * a.nsplit * plane : 0)}, lse.options());
+  float2* stat = reinterpret_cast<float2*>(ws.data_ptr<float>());
+  a.stat = stat;
+  a.part = a.nsplit > 1 ? ws.data_ptr<float>() + stat_floats : nullptr;
+  const int64_t rows = (int64_t)a.Tp * H;
+  const int blocks = (int)std::min<int64_t>((rows + 15) / 16, std::max<int64_t>(1, om::num_sms() * 16 / B));
+  om::attn_bwd_stat_kernel<<<dim3(blocks, (unsigned)B), 256, 0, st>>>(
+      ptr(out), ptr(dout), lse.data_ptr<float>(), a.lens, stat, a.T, a.Tp, a.H, a.hd, out.stride(0), out.stride(1),
+      out.stride(2), dout.stride(0), dout.stride(1), dout.stride(2));
   OM_LAUNCH_CHECK();
   const CUtensorMap mq = om::map_bthd(q), mg = om::map_bthd(dout), mk = om::map_bthd(k), mv = om::map_bthd(v);
   if (D <= 64)
     om::attn_bwd_launch<64>(a, mq, mg, mk, mv, st);
   else
     om::attn_bwd_launch<128>(a, mq, mg, mk, mv, st);
+  return {dq, dk, dv};
 }

@@ -79,25 +79,28 @@ void om_moe_permute(torch::Tensor x, torch::Tensor ids, torch::Tensor counts, to
 void om_moe_combine(torch::Tensor yp, torch::Tensor row_of, torch::Tensor wts, torch::Tensor out, bool add);
 void om_grouped_gemm(torch::Tensor x, torch::Tensor w, torch::Tensor offsets, torch::Tensor y, torch::Tensor status);
 
-void om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out, torch::Tensor lse,
-                      torch::Tensor dout, c10::optional<torch::Tensor> lens, double scale, bool causal,
-                      torch::Tensor dq, torch::Tensor dk, torch::Tensor dv, torch::Tensor status);
-void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<torch::Tensor> gu,
-               torch::Tensor status);
-void om_swiglu_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor gu, torch::Tensor dh,
-                   c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status);
-void om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
-                    double scale, double smoothing, int64_t ignore, torch::Tensor loss, torch::Tensor lse,
-                    torch::Tensor status);
-void om_linear_xent_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
-                        double scale, double smoothing, int64_t ignore, torch::Tensor lse, torch::Tensor dloss,
-                        c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status);
-void om_norm_train(torch::Tensor x, c10::optional<torch::Tensor> delta, torch::Tensor w,
-                   c10::optional<torch::Tensor> b, bool layer, double eps, torch::Tensor y,
-                   c10::optional<torch::Tensor> h, torch::Tensor stats);
-void om_norm_train_bwd(torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats,
-                       c10::optional<torch::Tensor> dh, bool layer, torch::Tensor dx, torch::Tensor dw,
-                       c10::optional<torch::Tensor> db);
+std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor out,
+                                            torch::Tensor lse, torch::Tensor dout, c10::optional<torch::Tensor> lens,
+                                            double scale, bool causal, torch::Tensor status);
+std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x, torch::Tensor w, bool save,
+                                                                 torch::Tensor status);
+std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_swiglu_bwd(torch::Tensor x, torch::Tensor w,
+                                                                                    torch::Tensor gu, torch::Tensor dh,
+                                                                                    bool need_dx, bool need_dw,
+                                                                                    torch::Tensor status);
+std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                                                       c10::optional<torch::Tensor> keep, double scale,
+                                                       double smoothing, int64_t ignore, torch::Tensor status);
+std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_xent_bwd(
+    torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep, double scale,
+    double smoothing, int64_t ignore, torch::Tensor lse, torch::Tensor dloss, bool need_dx, bool need_dw,
+    torch::Tensor status);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Tensor x, torch::Tensor w,
+                                                                      c10::optional<torch::Tensor> b, double eps,
+                                                                      bool layer, c10::optional<torch::Tensor> delta);
+std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_train_bwd(
+    torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats, bool layer, bool bias,
+    c10::optional<torch::Tensor> dh);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("launch_count", [] { return (int64_t)om::g_launches.load(); }, "kernel launches issued so far");

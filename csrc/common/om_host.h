@@ -93,4 +93,20 @@ inline CUtensorMap make_tmap_3d(const void* ptr, CUtensorMapDataType dt, int ele
   return m;
 }
 
+// `x` [..., K] as [rows, K] with contiguous rows: a view where its strides allow one.
+inline torch::Tensor rows_view(const torch::Tensor& x) {
+  if (x.dim() == 2 && x.stride(1) == 1) return x;
+  const int64_t K = x.dim() ? x.size(-1) : 0;
+  torch::Tensor r = x.dim() == 2 ? x : x.reshape({K ? x.numel() / K : 0, K});
+  return r.dim() == 2 && (r.stride(1) == 1 || K == 1) ? r : r.contiguous();
+}
+// The same, and readable by TMA copies: rows a multiple of 16 bytes apart from a 16-byte boundary.
+inline torch::Tensor tma_rows(const torch::Tensor& x) {
+  torch::Tensor r = rows_view(x);
+  const int64_t e = r.element_size();
+  const bool ok = (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0 && r.stride(0) * e % 16 == 0 &&
+                  r.stride(0) >= r.size(1);
+  return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
 }  // namespace om

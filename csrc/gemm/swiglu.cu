@@ -127,41 +127,42 @@ static void swiglu_fwd_bn(const CUtensorMap& ta, const void* w, int64_t ldw, Gem
 
 using om::GemmX;
 
-static void check_bf16_rows(const torch::Tensor& t, const char* op, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, op, ": ", name,
-              " must be a 2-D bf16 CUDA tensor with contiguous rows");
-  TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31) && t.stride(0) < (1ll << 31), op, ": ", name,
-              " is too large");
+namespace {
+
+void check_swiglu(const char* op, const torch::Tensor& x, const torch::Tensor& w) {
+  for (const auto& t : {x, w})
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() >= 1, op,
+                ": x and w must be bf16 CUDA tensors");
+  const int64_t K = x.size(-1);
+  TORCH_CHECK(w.dim() == 2 && w.size(0) % 2 == 0 && w.size(1) == K, op, ": w must be [2F, K]");
+  TORCH_CHECK(K > 0 && K % 8 == 0, op, ": K must be a positive multiple of 8");
+  TORCH_CHECK(x.numel() / K < (1ll << 31) && w.size(0) < (1ll << 31) && K < (1ll << 30), op, ": too large");
 }
 
-static void check_gu(const torch::Tensor& t, const char* op, int64_t M, int64_t F) {
-  TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.dim() == 2 && t.size(0) == M && t.size(1) == 2 * F &&
-                  t.is_contiguous() && 2 * F < (1ll << 31),
-              op, ": gu must be fp32 [M, 2F]");
-}
+}  // namespace
 
-// h [M, F] = silu(x Wg^T) * (x Wu^T); gu fp32 [M, 2F] optional.
-void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<torch::Tensor> gu,
-               torch::Tensor status) {
-  check_bf16_rows(x, "swiglu", "x");
-  check_bf16_rows(w, "swiglu", "w");
-  check_bf16_rows(h, "swiglu", "h");
-  const int64_t M = x.size(0), K = x.size(1), F = w.size(0) / 2;
-  TORCH_CHECK(w.size(0) == 2 * F && w.size(1) == K, "swiglu: w must be [2F, K]");
-  TORCH_CHECK(h.size(0) == M && h.size(1) == F, "swiglu: h must be [M, F]");
-  TORCH_CHECK(K > 0 && K % 8 == 0, "swiglu: K must be a positive multiple of 8");
-  if (M == 0 || F == 0) return;
+// (h [..., F] = silu(x Wg^T) * (x Wu^T), gu fp32 [rows, 2F] if saved)
+std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x, torch::Tensor w, bool save,
+                                                                 torch::Tensor status) {
+  check_swiglu("swiglu", x, w);
   const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t K = x.size(x.dim() - 1), F = w.size(0) / 2, M = x.numel() / K;
+  auto shape = x.sizes().vec();
+  shape.back() = F;
+  auto h = torch::empty(shape, x.options());
+  c10::optional<torch::Tensor> gu;
+  if (save) gu = torch::empty({M, 2 * F}, x.options().dtype(at::kFloat));
+  if (M == 0 || F == 0) return {h, gu};
+  const torch::Tensor x2 = om::tma_rows(x), w2 = om::tma_rows(w);
   auto st = at::cuda::getCurrentCUDAStream().stream();
   om::EpiSwiglu::Args e{};
   e.h = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
-  e.ldh = (int)h.stride(0);
-  e.vec_h = h.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(e.h) & 15) == 0;
-  if (gu.has_value()) {
-    check_gu(*gu, "swiglu", M, F);
+  e.ldh = (int)F;
+  e.vec_h = F % 8 == 0;
+  if (save) {
     e.gu = gu->data_ptr<float>();
     e.ldgu = (int)(2 * F);
-    e.vec_gu = F % 2 == 0 && (reinterpret_cast<uintptr_t>(e.gu) & 15) == 0;
+    e.vec_gu = F % 2 == 0;
   }
   GemmX g{};
   g.rows = (int)M;
@@ -171,61 +172,56 @@ void om_swiglu(torch::Tensor x, torch::Tensor w, torch::Tensor h, c10::optional<
   g.kb_per_split = g.num_kb;
   g.tiles_r = om::ceil_div(M, 128);
   g.status = status.data_ptr<int>();
-  const CUtensorMap ta = om::gx_map(x.data_ptr(), false, M, K, x.stride(0), 128);
+  const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), 128);
   // 128 features a tile once those tiles fill the SMs; fewer tiles than SMs: 32 features a tile
   if ((int64_t)g.tiles_r * om::ceil_div(F, 128) >= om::num_sms())
-    om::swiglu_fwd_bn<256>(ta, w.data_ptr(), w.stride(0), g, e, F, K, st);
+    om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), g, e, F, K, st);
   else
-    om::swiglu_fwd_bn<64>(ta, w.data_ptr(), w.stride(0), g, e, F, K, st);
+    om::swiglu_fwd_bn<64>(ta, w2.data_ptr(), w2.stride(0), g, e, F, K, st);
+  return {h, gu};
 }
 
-// dx [M, K], dw [2F, K] from x, w, gu (as the forward stored it) and dh [M, F].
-void om_swiglu_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor gu, torch::Tensor dh,
-                   c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status) {
-  check_bf16_rows(x, "swiglu_bwd", "x");
-  check_bf16_rows(w, "swiglu_bwd", "w");
-  check_bf16_rows(dh, "swiglu_bwd", "dh");
-  const int64_t M = x.size(0), K = x.size(1), F = w.size(0) / 2;
-  TORCH_CHECK(w.size(0) == 2 * F && w.size(1) == K, "swiglu_bwd: w must be [2F, K]");
-  check_gu(gu, "swiglu_bwd", M, F);
-  TORCH_CHECK(dh.size(0) == M && dh.size(1) == F, "swiglu_bwd: dh must be [M, F]");
-  TORCH_CHECK(K > 0 && K % 8 == 0, "swiglu_bwd: K must be a positive multiple of 8");
+// (dx [..., K], dw [2F, K]) from x, w, gu (as the forward stored it) and dh [..., F].
+std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_swiglu_bwd(torch::Tensor x, torch::Tensor w,
+                                                                                    torch::Tensor gu, torch::Tensor dh,
+                                                                                    bool need_dx, bool need_dw,
+                                                                                    torch::Tensor status) {
+  check_swiglu("swiglu_bwd", x, w);
   const c10::cuda::CUDAGuard guard(x.device());
-  auto st = at::cuda::getCurrentCUDAStream().stream();
+  const int64_t K = x.size(x.dim() - 1), F = w.size(0) / 2, M = x.numel() / K;
+  TORCH_CHECK(gu.is_cuda() && gu.scalar_type() == at::kFloat && gu.dim() == 2 && gu.size(0) == M &&
+                  gu.size(1) == 2 * F && gu.is_contiguous(),
+              "swiglu_bwd: gu must be fp32 [rows, 2F] as swiglu saved it");
+  TORCH_CHECK(dh.is_cuda() && dh.numel() == M * F && (F == 0 || dh.size(-1) == F), "swiglu_bwd: dh must be [..., F]");
+  c10::optional<torch::Tensor> dx, dw;
+  if (need_dx) dx = torch::empty(x.sizes(), x.options());
+  if (need_dw) dw = torch::empty(w.sizes(), w.options());
   if (M == 0 || F == 0) {
-    if (dx.has_value()) dx->zero_();
-    if (dw.has_value()) dw->zero_();
-    return;
+    if (need_dx) dx->zero_();
+    if (need_dw) dw->zero_();
+    return {dx, dw};
   }
+  const torch::Tensor x2 = om::tma_rows(x), w2 = om::tma_rows(w), d2 = om::rows_view(dh.to(at::kBFloat16));
+  auto st = at::cuda::getCurrentCUDAStream().stream();
   const int64_t ld = (2 * F + 7) / 8 * 8;
   auto dgu = torch::empty({M, ld}, x.options());
   auto ptr = [](const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); };
-  auto al = [](const torch::Tensor& t) {
-    return t.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
-  };
-  const bool v8 = F % 8 == 0 && (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0 && al(dh);
+  const bool v8 = F % 8 == 0 && (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0 && d2.stride(0) % 8 == 0 &&
+                  (reinterpret_cast<uintptr_t>(d2.data_ptr()) & 15) == 0;
   const long long work = M * (v8 ? F / 8 : F);
   const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)om::num_sms() * 16);
-  if (v8)
-    om::swiglu_grad_kernel<8><<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(dh), dh.stride(0), ptr(dgu), ld, M,
-                                                      (int)F);
-  else
-    om::swiglu_grad_kernel<1><<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(dh), dh.stride(0), ptr(dgu), ld, M,
-                                                      (int)F);
+  auto grad = v8 ? om::swiglu_grad_kernel<8> : om::swiglu_grad_kernel<1>;
+  grad<<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(d2), d2.stride(0), ptr(dgu), ld, M, (int)F);
   OM_LAUNCH_CHECK();
-  auto product = [&](om::GxOperand a, om::GxOperand b, int64_t rows, int64_t cols, int64_t k, torch::Tensor& out,
-                     const char* name) {
-    check_bf16_rows(out, "swiglu_bwd", name);
-    TORCH_CHECK(out.size(0) == rows && out.size(1) == cols, "swiglu_bwd: ", name, " has the wrong shape");
+  auto product = [&](om::GxOperand a, om::GxOperand b, int64_t rows, int64_t cols, int64_t k, torch::Tensor& out) {
     const om::GxPlan p = om::gx_plan(rows, cols, k);
     const int64_t n = om::gx_acc_floats(p, rows, cols, false);
     torch::Tensor acc;
-    if (n) acc = torch::empty({n}, x.options().dtype(at::kFloat));
-    om::gx_product(p, a, b, rows, cols, k, ptr(out), out.stride(0), n ? acc.data_ptr<float>() : nullptr, true, true,
+    if (n) acc = torch::empty({n}, gu.options());
+    om::gx_product(p, a, b, rows, cols, k, ptr(out), cols, n ? acc.data_ptr<float>() : nullptr, true, true,
                    status.data_ptr<int>(), st);
   };
-  if (dx.has_value())
-    product({dgu.data_ptr(), false, ld}, {w.data_ptr(), true, w.stride(0)}, M, K, 2 * F, *dx, "dx");
-  if (dw.has_value())
-    product({dgu.data_ptr(), true, ld}, {x.data_ptr(), true, x.stride(0)}, 2 * F, K, M, *dw, "dw");
+  if (need_dx) product({dgu.data_ptr(), false, ld}, {w2.data_ptr(), true, w2.stride(0)}, M, K, 2 * F, *dx);
+  if (need_dw) product({dgu.data_ptr(), true, ld}, {x2.data_ptr(), true, x2.stride(0)}, 2 * F, K, M, *dw);
+  return {dx, dw};
 }

@@ -223,71 +223,82 @@ static int64_t piece_columns(int64_t M, int64_t V) {
 
 namespace {
 
-void check_xent(const char* op, const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets,
-                const c10::optional<torch::Tensor>& keep, double smoothing, om::XentRows& rows, double scale,
-                int64_t ignore) {
-  auto mat = [&](const torch::Tensor& t, const char* name) {
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() == 2 && t.stride(1) == 1, op, ": ", name,
-                " must be a 2-D bf16 CUDA tensor with contiguous rows");
-    TORCH_CHECK(t.size(0) < (1ll << 31) && t.stride(0) < (1ll << 31), op, ": ", name, " is too large");
-  };
-  mat(x, "x");
-  mat(w, "w");
-  const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
-  TORCH_CHECK(w.size(1) == K && V > 0, op, ": w must be [V, K] with V > 0");
-  TORCH_CHECK(K > 0 && K % 8 == 0, op, ": K must be a positive multiple of 8");
-  TORCH_CHECK(targets.is_cuda() && targets.scalar_type() == at::kLong && targets.is_contiguous() &&
-                  targets.dim() == 1 && targets.size(0) == M,
-              op, ": targets must be int64 [M]");
-  rows = om::XentRows{};
-  rows.targets = reinterpret_cast<const long long*>(targets.data_ptr<int64_t>());
-  rows.ignore = ignore;
-  rows.scale = (float)scale;
-  rows.V = (int)V;
+struct XentIn {
+  torch::Tensor x, w, targets, keep;  // as the kernels read them
+  int64_t M, K, V;
+  om::XentRows rows{};
+};
+
+XentIn check_xent(const char* op, const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& targets,
+                  const c10::optional<torch::Tensor>& keep, double smoothing, double scale, int64_t ignore) {
+  for (const auto& t : {x, w})
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kBFloat16 && t.dim() >= 1, op,
+                ": x and w must be bf16 CUDA tensors");
+  XentIn in;
+  in.K = x.size(x.dim() - 1);
+  TORCH_CHECK(w.dim() == 2 && w.size(1) == in.K && w.size(0) > 0, op, ": w must be [V, K] with V > 0");
+  TORCH_CHECK(in.K > 0 && in.K % 8 == 0, op, ": K must be a positive multiple of 8");
+  in.M = x.numel() / in.K;
+  in.V = w.size(0);
+  TORCH_CHECK(in.M < (1ll << 31) - 256 && in.V < (1ll << 31) - 256 && in.K < (1ll << 30), op, ": too large");
+  TORCH_CHECK(targets.is_cuda() && targets.numel() == in.M, op, ": targets must have one entry a row");
+  in.x = om::tma_rows(x);
+  in.w = om::tma_rows(w);
+  in.targets = targets.to(at::kLong).contiguous();
+  in.rows.targets = reinterpret_cast<const long long*>(in.targets.data_ptr<int64_t>());
+  in.rows.ignore = ignore;
+  in.rows.scale = (float)scale;
+  in.rows.V = (int)in.V;
   if (keep.has_value()) {
     TORCH_CHECK(smoothing == 0.0, op, ": label smoothing over a keep mask is not defined");
-    TORCH_CHECK(keep->is_cuda() && keep->scalar_type() == at::kInt && keep->dim() == 2 && keep->size(0) == M &&
-                    keep->size(1) >= (V + 31) / 32 && keep->stride(1) == 1,
-                op, ": keep must be int32 [M, ceil(V / 32)] words");
-    rows.keep = keep->data_ptr<int>();
-    rows.ldk = keep->stride(0);
+    TORCH_CHECK(keep->is_cuda() && keep->scalar_type() == at::kInt && keep->dim() == 2 && keep->size(0) == in.M &&
+                    keep->size(1) >= (in.V + 31) / 32 && keep->stride(1) == 1,
+                op, ": keep must be int32 [rows, ceil(V / 32)] words");
+    in.keep = *keep;
+    in.rows.keep = keep->data_ptr<int>();
+    in.rows.ldk = keep->stride(0);
   }
+  return in;
+}
+
+om::GemmX xent_gemm(const XentIn& in, int64_t cols, int* status) {
+  om::GemmX g{};
+  g.rows = (int)in.M;
+  g.cols = (int)cols;
+  g.num_kb = om::ceil_div(in.K, 64);
+  g.splits = 1;
+  g.kb_per_split = g.num_kb;
+  g.tiles_r = om::ceil_div(in.M, 128);
+  g.tiles_c = om::ceil_div(cols, 256);
+  g.b_step = 256;
+  g.b_second = 128;
+  g.status = status;
+  return g;
 }
 
 }  // namespace
 
-void om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
-                    double scale, double smoothing, int64_t ignore, torch::Tensor loss, torch::Tensor lse,
-                    torch::Tensor status) {
-  om::XentRows rows;
-  check_xent("linear_xent", x, w, targets, keep, smoothing, rows, scale, ignore);
-  const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
-  for (const auto& t : {loss, lse})
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == M,
-                "linear_xent: loss and lse must be fp32 [M]");
-  if (M == 0) return;
-  const c10::cuda::CUDAGuard guard(x.device());
+// (loss, lse) fp32 in targets' shape
+std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets,
+                                                       c10::optional<torch::Tensor> keep, double scale,
+                                                       double smoothing, int64_t ignore, torch::Tensor status) {
+  const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::make_optional(x.device()) : c10::nullopt);
+  const XentIn in = check_xent("linear_xent", x, w, targets, keep, smoothing, scale, ignore);
+  const auto f32 = x.options().dtype(at::kFloat);
+  auto loss = torch::empty(targets.sizes(), f32), lse = torch::empty(targets.sizes(), f32);
+  const int64_t M = in.M;
+  if (M == 0) return {loss, lse};
   auto st = at::cuda::getCurrentCUDAStream().stream();
-  om::GemmX g{};
-  g.rows = (int)M;
-  g.cols = (int)V;
-  g.num_kb = om::ceil_div(K, 64);
-  g.splits = 1;
-  g.kb_per_split = g.num_kb;
-  g.tiles_r = om::ceil_div(M, 128);
-  g.tiles_c = om::ceil_div(V, 256);
-  g.b_step = 256;
-  g.b_second = 128;
-  g.status = status.data_ptr<int>();
+  const om::GemmX g = xent_gemm(in, in.V, status.data_ptr<int>());
   const int64_t n = (int64_t)g.tiles_c * M;
   const bool smooth = smoothing != 0.0;
-  auto ws = torch::empty({n * (smooth ? 3 : 2) + M}, loss.options());
+  auto ws = torch::empty({n * (smooth ? 3 : 2) + M}, f32);
   float* p = ws.data_ptr<float>();
-  const CUtensorMap ta = om::gx_map(x.data_ptr(), false, M, K, x.stride(0), 128);
-  const CUtensorMap tb = om::gx_map(w.data_ptr(), false, V, K, w.stride(0), 128);
+  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, M, in.K, in.x.stride(0), 128);
+  const CUtensorMap tb = om::gx_map(in.w.data_ptr(), false, in.V, in.K, in.w.stride(0), 128);
   auto run = [&](auto epi) {
     using E = decltype(epi);
-    typename E::Args e{rows, reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n};
+    typename E::Args e{in.rows, reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n};
     om::gx_launch<256, false, false, E>(ta, tb, g, e, st);
   };
   if (smooth)
@@ -295,71 +306,60 @@ void om_linear_xent(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10
   else
     run(om::EpiXentFwd<false>{});
   om::xent_join_kernel<<<om::ceil_div(M, 32), 256, 0, st>>>(
-      reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n, rows, (int)M, g.tiles_c,
+      reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n, in.rows, (int)M, g.tiles_c,
       (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
   OM_LAUNCH_CHECK();
+  return {loss, lse};
 }
 
-void om_linear_xent_bwd(torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep,
-                        double scale, double smoothing, int64_t ignore, torch::Tensor lse, torch::Tensor dloss,
-                        c10::optional<torch::Tensor> dx, c10::optional<torch::Tensor> dw, torch::Tensor status) {
-  om::XentRows rows;
-  check_xent("linear_xent_bwd", x, w, targets, keep, smoothing, rows, scale, ignore);
-  const int64_t M = x.size(0), K = x.size(1), V = w.size(0);
-  for (const auto& t : {lse, dloss})
-    TORCH_CHECK(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == M,
-                "linear_xent_bwd: lse and dloss must be fp32 [M]");
-  auto grad = [&](const c10::optional<torch::Tensor>& t, int64_t r, const char* name) -> __nv_bfloat16* {
-    if (!t.has_value()) return nullptr;
-    TORCH_CHECK(t->is_cuda() && t->scalar_type() == at::kBFloat16 && t->dim() == 2 && t->size(0) == r &&
-                    t->size(1) == K && t->is_contiguous(),
-                "linear_xent_bwd: ", name, " has the wrong shape or type");
-    return reinterpret_cast<__nv_bfloat16*>(t->data_ptr());
-  };
-  __nv_bfloat16* dxp = grad(dx, M, "dx");
-  __nv_bfloat16* dwp = grad(dw, V, "dw");
-  const c10::cuda::CUDAGuard guard(x.device());
-  auto st = at::cuda::getCurrentCUDAStream().stream();
+// (dx [..., K], dw [V, K])
+std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_xent_bwd(
+    torch::Tensor x, torch::Tensor w, torch::Tensor targets, c10::optional<torch::Tensor> keep, double scale,
+    double smoothing, int64_t ignore, torch::Tensor lse, torch::Tensor dloss, bool need_dx, bool need_dw,
+    torch::Tensor status) {
+  const c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::make_optional(x.device()) : c10::nullopt);
+  const XentIn in = check_xent("linear_xent_bwd", x, w, targets, keep, smoothing, scale, ignore);
+  const int64_t M = in.M, K = in.K, V = in.V;
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.numel() == M,
+              "linear_xent_bwd: lse must be fp32 with one entry a row");
+  TORCH_CHECK(dloss.is_cuda() && dloss.numel() == M, "linear_xent_bwd: dloss must have one entry a row");
+  lse = lse.contiguous();
+  dloss = dloss.to(at::kFloat).contiguous();
+  c10::optional<torch::Tensor> dx, dw;
+  if (need_dx) dx = torch::empty(x.sizes(), x.options());
+  if (need_dw) dw = torch::empty(w.sizes(), w.options());
   if (M == 0) {
-    if (dwp) dw->zero_();
-    return;
+    if (need_dw) dw->zero_();
+    return {dx, dw};
   }
-  if (!dxp && !dwp) return;
+  if (!need_dx && !need_dw) return {dx, dw};
+  auto ptr = [](const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); };
+  auto st = at::cuda::getCurrentCUDAStream().stream();
   const int64_t C = om::piece_columns(M, V);
   const int64_t ld = std::min(C, (V + 31) / 32 * 32);
   auto dz = torch::empty({M, ld}, x.options());
-  const bool pieces = C < V;
   const om::GxPlan px = om::gx_plan(M, K, std::min(C, V));
   const om::GxPlan pw = om::gx_plan(std::min(C, V), K, M);
-  const int64_t nx = dxp ? om::gx_acc_floats(px, M, K, pieces) : 0;
-  const int64_t nw = dwp ? om::gx_acc_floats(pw, std::min(C, V), K, false) : 0;
-  torch::Tensor ax, aw;
-  if (nx) ax = torch::empty({nx}, lse.options());
-  if (nw) aw = torch::empty({nw}, lse.options());
-  om::GemmX g{};
-  g.rows = (int)M;
-  g.num_kb = om::ceil_div(K, 64);
-  g.splits = 1;
-  g.kb_per_split = g.num_kb;
-  g.tiles_r = om::ceil_div(M, 128);
-  g.b_step = 256;
-  g.b_second = 128;
-  g.status = status.data_ptr<int>();
-  const CUtensorMap ta = om::gx_map(x.data_ptr(), false, M, K, x.stride(0), 128);
-  const __nv_bfloat16* wp = reinterpret_cast<const __nv_bfloat16*>(w.data_ptr());
+  const int64_t nx = need_dx ? om::gx_acc_floats(px, M, K, C < V) : 0;
+  const int64_t nw = need_dw ? om::gx_acc_floats(pw, std::min(C, V), K, false) : 0;
+  torch::Tensor acc;
+  if (nx + nw) acc = torch::empty({nx + nw}, lse.options());
+  float* ax = nx ? acc.data_ptr<float>() : nullptr;
+  float* aw = nw ? acc.data_ptr<float>() + nx : nullptr;  // nx is a multiple of 32
+  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, M, K, in.x.stride(0), 128);
   for (int64_t v0 = 0; v0 < V; v0 += C) {
     const int64_t n = std::min(C, V - v0);
-    const __nv_bfloat16* wv = wp + v0 * w.stride(0);
-    g.cols = (int)n;
-    g.tiles_c = om::ceil_div(n, 256);
-    om::EpiXentBwd::Args e{rows,      lse.data_ptr<float>(), dloss.data_ptr<float>(),
-                           (float)smoothing, (int)v0, reinterpret_cast<__nv_bfloat16*>(dz.data_ptr()), (int)ld};
-    om::gx_launch<256, false, false, om::EpiXentBwd>(ta, om::gx_map(wv, false, n, K, w.stride(0), 128), g, e, st);
-    if (dxp)
-      om::gx_product(px, {dz.data_ptr(), false, ld}, {wv, true, w.stride(0)}, M, K, n, dxp, K,
-                     nx ? ax.data_ptr<float>() : nullptr, v0 == 0, v0 + n == V, g.status, st);
-    if (dwp)
-      om::gx_product(pw, {dz.data_ptr(), true, ld}, {x.data_ptr(), true, x.stride(0)}, n, K, M, dwp + v0 * K, K,
-                     nw ? aw.data_ptr<float>() : nullptr, true, true, g.status, st);
+    const __nv_bfloat16* wv = ptr(in.w) + v0 * in.w.stride(0);
+    const om::GemmX g = xent_gemm(in, n, status.data_ptr<int>());
+    om::EpiXentBwd::Args e{in.rows, lse.data_ptr<float>(), dloss.data_ptr<float>(), (float)smoothing, (int)v0,
+                           ptr(dz), (int)ld};
+    om::gx_launch<256, false, false, om::EpiXentBwd>(ta, om::gx_map(wv, false, n, K, in.w.stride(0), 128), g, e, st);
+    if (need_dx)
+      om::gx_product(px, {dz.data_ptr(), false, ld}, {wv, true, in.w.stride(0)}, M, K, n, ptr(*dx), K, ax, v0 == 0,
+                     v0 + n == V, g.status, st);
+    if (need_dw)
+      om::gx_product(pw, {dz.data_ptr(), true, ld}, {in.x.data_ptr(), true, in.x.stride(0)}, n, K, M,
+                     ptr(*dw) + v0 * K, K, aw, true, true, g.status, st);
   }
+  return {dx, dw};
 }

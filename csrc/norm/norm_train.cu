@@ -356,66 +356,64 @@ static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 namespace {
 
-// 2-D [M, D] with contiguous rows; returns the row distance
-long long norm_rows(const char* op, const char* name, const torch::Tensor& t, int64_t M, int64_t D,
-                    at::ScalarType ty) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.size(0) == M && t.size(1) == D && t.scalar_type() == ty &&
-                  (t.stride(1) == 1 || D == 1),
-              op, ": ", name, " must be a CUDA [M, D] tensor of the rows' type with contiguous rows");
-  return t.stride(0);
+// [..., D] as [M, D] rows of the expected type
+torch::Tensor norm_rows(const char* op, const char* name, const torch::Tensor& t, int64_t M, int64_t D,
+                        at::ScalarType ty) {
+  TORCH_CHECK(t.is_cuda() && t.dim() >= 1 && t.size(t.dim() - 1) == D && t.numel() == M * D && t.scalar_type() == ty,
+              op, ": ", name, " must be a CUDA tensor of the rows' shape and type");
+  return om::rows_view(t);
 }
-void norm_cols(const char* op, const char* name, const torch::Tensor& t, int64_t D, at::ScalarType ty) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 1 && t.size(0) == D && t.scalar_type() == ty && t.is_contiguous(), op, ": ",
-              name, " must be a contiguous CUDA [D] tensor of the weight's type");
+torch::Tensor norm_cols(const char* op, const char* name, const torch::Tensor& t, int64_t D, at::ScalarType ty) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 1 && t.size(0) == D && t.scalar_type() == ty, op, ": ", name,
+              " must be a CUDA [D] tensor of the weight's type");
+  return t.contiguous();
+}
+bool norm_vec(const torch::Tensor& t) {
+  return (t.dim() == 1 || t.stride(0) % 8 == 0) && om::aligned16(t.data_ptr());
 }
 
 }  // namespace
 
-// y [M, D]; h [M, D] (with delta); stats fp32 [M, 2]
-void om_norm_train(torch::Tensor x, c10::optional<torch::Tensor> delta, torch::Tensor w,
-                   c10::optional<torch::Tensor> b, bool layer, double eps, torch::Tensor y,
-                   c10::optional<torch::Tensor> h, torch::Tensor stats) {
+// (y [..., D], h (x itself without delta), stats fp32 [M, 2])
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Tensor x, torch::Tensor w,
+                                                                      c10::optional<torch::Tensor> b, double eps,
+                                                                      bool layer, c10::optional<torch::Tensor> delta) {
   const char* op = "norm_train";
-  TORCH_CHECK(x.dim() == 2 && x.is_cuda(), "norm_train: x must be a CUDA [M, D] tensor");
-  const int64_t M = x.size(0), D = x.size(1);
+  TORCH_CHECK(x.dim() >= 1 && x.is_cuda(), "norm_train: x must be a CUDA tensor [..., D]");
+  const int64_t D = x.size(x.dim() - 1);
   TORCH_CHECK(D > 0, "norm_train: empty rows");
+  const int64_t M = x.numel() / D;
+  const c10::cuda::CUDAGuard guard(x.device());
   om::NormFwd a{};
   const auto ty = x.scalar_type(), wt = w.scalar_type();
-  a.ldx = norm_rows(op, "x", x, M, D, ty);
-  norm_cols(op, "w", w, D, wt);
-  bool vec = D % 8 == 0 && a.ldx % 8 == 0 && om::aligned16(x.data_ptr()) && om::aligned16(w.data_ptr()) &&
-             om::aligned16(y.data_ptr()) && (!h.has_value() || om::aligned16(h->data_ptr()));
+  const torch::Tensor x2 = norm_rows(op, "x", x, M, D, ty), w2 = norm_cols(op, "w", w, D, wt);
+  torch::Tensor d2, b2, h;
+  bool vec = D % 8 == 0 && norm_vec(x2) && norm_vec(w2);
   if (delta.has_value()) {
-    TORCH_CHECK(h.has_value(), "norm_train: delta needs h");
-    a.ldd = norm_rows(op, "delta", *delta, M, D, ty);
-    a.delta = delta->data_ptr();
-    vec = vec && a.ldd % 8 == 0 && om::aligned16(a.delta);
+    d2 = norm_rows(op, "delta", *delta, M, D, ty);
+    a.ldd = d2.stride(0);
+    a.delta = d2.data_ptr();
+    vec = vec && norm_vec(d2);
   }
   if (b.has_value()) {
     TORCH_CHECK(layer, "norm_train: RMSNorm takes no bias");
-    norm_cols(op, "b", *b, D, wt);
-    a.b = b->data_ptr();
-    vec = vec && om::aligned16(a.b);
+    b2 = norm_cols(op, "b", *b, D, wt);
+    a.b = b2.data_ptr();
+    vec = vec && norm_vec(b2);
   }
-  norm_rows(op, "y", y, M, D, ty);
-  TORCH_CHECK(y.is_contiguous(), "norm_train: y must be contiguous");
-  if (h.has_value()) {
-    norm_rows(op, "h", *h, M, D, ty);
-    TORCH_CHECK(h->is_contiguous(), "norm_train: h must be contiguous");
-    a.h = h->data_ptr();
-  }
-  TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * M,
-              "norm_train: stats must be fp32 [M, 2]");
-  if (M == 0) return;
-  const c10::cuda::CUDAGuard guard(x.device());
-  auto st = at::cuda::getCurrentCUDAStream().stream();
-  a.x = x.data_ptr();
-  a.w = w.data_ptr();
+  auto y = torch::empty(x.sizes(), x.options());
+  h = delta.has_value() ? torch::empty(x.sizes(), x.options()) : x;
+  auto stats = torch::empty({M, 2}, x.options().dtype(at::kFloat));
+  a.x = x2.data_ptr();
+  a.ldx = x2.stride(0);
+  a.w = w2.data_ptr();
   a.y = y.data_ptr();
+  a.h = delta.has_value() ? h.data_ptr() : nullptr;
   a.stats = stats.data_ptr<float>();
   a.M = M;
   a.D = (int)std::min<int64_t>(D, INT32_MAX);
   a.eps = (float)eps;
+  auto st = at::cuda::getCurrentCUDAStream().stream();
   om::norm_types(op, ty, wt, [&](auto t0, auto w0) {
     om::norm_shape(op, a.D, vec, [&](auto G, auto V, auto P) {
       using T = decltype(t0);
@@ -424,6 +422,7 @@ void om_norm_train(torch::Tensor x, c10::optional<torch::Tensor> delta, torch::T
       constexpr int NT = om::norm_threads<g>();
       const long long blocks = (M + NT / g - 1) / (NT / g);
       TORCH_CHECK(blocks < (1ll << 31), "norm_train: too many rows");
+      if (M == 0) return;
       if (layer)
         om::norm_fwd_kernel<T, W, true, g, v, p><<<(unsigned)blocks, NT, 0, st>>>(a);
       else
@@ -431,77 +430,85 @@ void om_norm_train(torch::Tensor x, c10::optional<torch::Tensor> delta, torch::T
       OM_LAUNCH_CHECK();
     });
   });
+  return {y, h, stats};
 }
 
-// dx [M, D], dw [D], db [D] (LayerNorm with bias)
-void om_norm_train_bwd(torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats,
-                       c10::optional<torch::Tensor> dh, bool layer, torch::Tensor dx, torch::Tensor dw,
-                       c10::optional<torch::Tensor> db) {
+// (dx [..., D], dw [D], db [D] (LayerNorm with bias))
+std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_train_bwd(
+    torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats, bool layer, bool bias,
+    c10::optional<torch::Tensor> dh) {
   const char* op = "norm_train_bwd";
-  TORCH_CHECK(h.dim() == 2 && h.is_cuda(), "norm_train_bwd: h must be a CUDA [M, D] tensor");
-  const int64_t M = h.size(0), D = h.size(1);
+  TORCH_CHECK(h.dim() >= 1 && h.is_cuda(), "norm_train_bwd: h must be a CUDA tensor [..., D]");
+  const int64_t D = h.size(h.dim() - 1);
   TORCH_CHECK(D > 0, "norm_train_bwd: empty rows");
+  TORCH_CHECK(layer || !bias, "norm_train_bwd: RMSNorm has no bias");
+  const int64_t M = h.numel() / D;
+  const c10::cuda::CUDAGuard guard(h.device());
   const auto ty = h.scalar_type(), wt = w.scalar_type();
   om::NormBwd a{};
-  a.ldh = norm_rows(op, "h", h, M, D, ty);
-  a.ldy = norm_rows(op, "dy", dy, M, D, ty);
-  norm_cols(op, "w", w, D, wt);
-  norm_rows(op, "dx", dx, M, D, ty);
-  TORCH_CHECK(dx.is_contiguous(), "norm_train_bwd: dx must be contiguous");
-  norm_cols(op, "dw", dw, D, wt);
-  bool vec = D % 8 == 0 && a.ldh % 8 == 0 && a.ldy % 8 == 0 && om::aligned16(h.data_ptr()) &&
-             om::aligned16(dy.data_ptr()) && om::aligned16(w.data_ptr()) && om::aligned16(dx.data_ptr());
+  const torch::Tensor h2 = norm_rows(op, "h", h, M, D, ty), y2 = norm_rows(op, "dy", dy.to(ty), M, D, ty);
+  const torch::Tensor w2 = norm_cols(op, "w", w, D, wt);
+  torch::Tensor d2;
+  bool vec = D % 8 == 0 && norm_vec(h2) && norm_vec(y2) && norm_vec(w2);
   if (dh.has_value()) {
-    a.lddh = norm_rows(op, "dh", *dh, M, D, ty);
-    a.dh = dh->data_ptr();
-    vec = vec && a.lddh % 8 == 0 && om::aligned16(a.dh);
-  }
-  if (db.has_value()) {
-    TORCH_CHECK(layer, "norm_train_bwd: RMSNorm has no bias");
-    norm_cols(op, "db", *db, D, wt);
+    d2 = norm_rows(op, "dh", dh->to(ty), M, D, ty);
+    a.lddh = d2.stride(0);
+    a.dh = d2.data_ptr();
+    vec = vec && norm_vec(d2);
   }
   TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * M,
               "norm_train_bwd: stats must be fp32 [M, 2]");
-  const c10::cuda::CUDAGuard guard(h.device());
-  auto st = at::cuda::getCurrentCUDAStream().stream();
+  auto dx = torch::empty(h.sizes(), h.options());
+  auto dw = torch::empty({D}, w.options());
+  c10::optional<torch::Tensor> db;
+  if (bias) db = torch::empty({D}, w.options());
   if (M == 0) {
     dw.zero_();
-    if (db.has_value()) db->zero_();
-    return;
+    if (bias) db->zero_();
+    return {dx, dw, db};
   }
-  a.dy = dy.data_ptr();
-  a.h = h.data_ptr();
-  a.w = w.data_ptr();
+  a.dy = y2.data_ptr();
+  a.ldy = y2.stride(0);
+  a.h = h2.data_ptr();
+  a.ldh = h2.stride(0);
+  a.w = w2.data_ptr();
   a.dx = dx.data_ptr();
   a.stats = stats.data_ptr<float>();
   a.M = M;
   a.D = (int)std::min<int64_t>(D, INT32_MAX);
   const int n = layer ? 2 : 1;
+  auto st = at::cuda::getCurrentCUDAStream().stream();
   om::norm_types(op, ty, wt, [&](auto t0, auto w0) {
     om::norm_shape(op, a.D, vec, [&](auto G, auto V, auto P) {
       using T = decltype(t0);
       using W = decltype(w0);
       constexpr int g = decltype(G)::value, v = decltype(V)::value, p = decltype(P)::value;
       constexpr int NT = om::norm_threads<g>(), RPB = NT / g;
-      auto go = [&](auto kernel) {
-        int per_sm = 0;
+      auto go = [&](auto kernel, std::atomic<int>& resident) {
         const size_t smem = RPB > 1 ? (size_t)a.D * sizeof(float) : 0;
-        OM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, smem));
+        int per_sm = resident.load();  // the same for every call of this instance (smem is at most 8 KB)
+        if (per_sm == 0) {
+          OM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, smem));
+          per_sm = std::max(1, per_sm);
+          resident.store(per_sm);
+        }
         const long long most = (M + RPB - 1) / RPB;
-        const int blocks = (int)std::min<long long>(most, (long long)om::num_sms() * std::max(1, per_sm));
+        const int blocks = (int)std::min<long long>(most, (long long)om::num_sms() * per_sm);
         auto part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());
         a.part = part.data_ptr<float>();
         kernel<<<blocks, NT, smem, st>>>(a);
         OM_LAUNCH_CHECK();
-        om::norm_join_kernel<W><<<dim3((a.D + 31) / 32, db.has_value() ? 2 : 1), 256, 0, st>>>(
+        om::norm_join_kernel<W><<<dim3((a.D + 31) / 32, bias ? 2 : 1), 256, 0, st>>>(
             a.part, blocks, n, a.D, reinterpret_cast<W*>(dw.data_ptr()),
-            db.has_value() ? reinterpret_cast<W*>(db->data_ptr()) : nullptr);
+            bias ? reinterpret_cast<W*>(db->data_ptr()) : nullptr);
         OM_LAUNCH_CHECK();
       };
+      static std::atomic<int> resident[2];
       if (layer)
-        go(om::norm_bwd_kernel<T, W, true, g, v, p>);
+        go(om::norm_bwd_kernel<T, W, true, g, v, p>, resident[1]);
       else
-        go(om::norm_bwd_kernel<T, W, false, g, v, p>);
+        go(om::norm_bwd_kernel<T, W, false, g, v, p>, resident[0]);
     });
   });
+  return {dx, dw, db};
 }

@@ -282,29 +282,14 @@ def repetition_penalty(logits, prev, penalty):
 
 
 # ------------------------------------------------------------------ training operators
-# Scratch of these is allocated per call on the current stream (the caching allocator keeps
-# it), so calls on different streams never share any.
-
-def _rows(x):
-    """``x`` as [rows, K] whose rows a TMA copy can read: contiguous, 16-byte aligned."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(-1) != 1 or x2.stride(0) % 8 or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2
-
-
-def _heads(x):
-    """``x`` [B, T, H, D] with D contiguous and every other stride a positive multiple of 8."""
-    if x.stride(3) != 1 or x.data_ptr() % 16 or any(n > 1 and (s % 8 or s <= 0)
-                                                    for n, s in zip(x.shape[:3], x.stride()[:3])):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
-
+# The native entries take tensors as they are (a layout that a TMA copy cannot read is copied) and
+# allocate results and scratch on the current stream, so calls on different streams never share any.
 
 def _same_device(op, *tensors):
     d = tensors[0].device
-    if any(t is not None and t.device != d for t in tensors):
-        raise ValueError(f"{op}: all tensors must be on {d}")
+    for t in tensors:
+        if t is not None and t.device != d:
+            raise ValueError(f"{op}: all tensors must be on {d}")
 
 
 def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
@@ -318,29 +303,20 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
     _same_device("attention_bwd", q, k, v, out, lse, dout, lens)
     if not q.is_cuda:
         return ref.attention_bwd(q, k, v, out, lse, dout, scale, causal, lens)
-    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or out.shape != q.shape or dout.shape != q.shape:
+    if v.shape != k.shape or out.shape != q.shape or dout.shape != q.shape:
         raise ValueError("attention_bwd: q, out, dout [B, T, H, D] and k, v [B, S, Hkv, D]")
-    q, k, v, out, dout = (_heads(t) for t in (q, k, v, out.to(q.dtype), dout.to(q.dtype)))
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-    _native.C().attention_bwd(q, k, v, out, lse.contiguous(), dout,
-                              None if lens is None else lens.to(torch.int32).contiguous(), float(scale), bool(causal),
-                              dq, dk, dv, ctx(q.device).status)
-    return dq, dk, dv
+    return _native.C().attention_bwd(q, k, v, out, lse, dout, lens, scale, causal, ctx(q.device).status)
 
 
 def swiglu(x, w, save=False):
     """silu(x Wg^T) * (x Wu^T) of x [..., K] and w [2F, K] (gate rows first) -> [..., F]. With
     ``save`` also the projections, fp32 [rows, 2F], that :func:`swiglu_bwd` reads."""
     _same_device("swiglu", x, w)
-    if not x.is_cuda:
-        return ref.swiglu(x, w, save)
     if w.dim() != 2 or w.shape[0] % 2 or w.shape[1] != x.shape[-1]:
         raise ValueError("swiglu: w must be [2F, K]")
-    x2, F = _rows(x), w.shape[0] // 2
-    h = torch.empty(x2.shape[0], F, dtype=x.dtype, device=x.device)
-    gu = torch.empty(x2.shape[0], 2 * F, dtype=torch.float32, device=x.device) if save else None
-    _native.C().swiglu(x2, _rows(w), h, gu, ctx(x.device).status)
-    h = h.view(*x.shape[:-1], F)
+    if not x.is_cuda:
+        return ref.swiglu(x, w, save)
+    h, gu = _native.C().swiglu(x, w, save, ctx(x.device).status)
     return (h, gu) if save else h
 
 
@@ -349,13 +325,7 @@ def swiglu_bwd(x, w, gu, dh, need_dx=True, need_dw=True):
     _same_device("swiglu_bwd", x, w, gu, dh)
     if not x.is_cuda:
         return ref.swiglu_bwd(x, w, gu, dh, need_dx, need_dw)
-    x2 = _rows(x)
-    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
-    d2 = dh.to(x.dtype).reshape(-1, dh.shape[-1])
-    _native.C().swiglu_bwd(x2, _rows(w), gu, d2 if d2.stride(-1) == 1 else d2.contiguous(), dx, dw,
-                           ctx(x.device).status)
-    return dx.view(x.shape) if need_dx else None, dw
+    return _native.C().swiglu_bwd(x, w, gu, dh, need_dx, need_dw, ctx(x.device).status)
 
 
 def _xent_args(op, x, w, targets, smoothing, keep):
@@ -381,32 +351,24 @@ def linear_xent(x, w, targets, scale=1.0, smoothing=0.0, ignore_index=-100, keep
     _xent_args("linear_xent", x, w, targets, smoothing, keep)
     if not x.is_cuda:
         return ref.linear_xent(x, w, targets, scale, smoothing, ignore_index, keep)
-    loss = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
-    lse = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
-    _native.C().linear_xent(_rows(x), _rows(w), targets.long().reshape(-1), keep, float(scale), float(smoothing),
-                            int(ignore_index), loss, lse, ctx(x.device).status)
-    return loss, lse
+    return _native.C().linear_xent(x, w, targets, keep, scale, smoothing, ignore_index, ctx(x.device).status)
 
 
 def linear_xent_bwd(x, w, targets, lse, dloss, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None, need_dx=True,
                     need_dw=True):
-    """Gradient (dx, dw) of :func:`linear_xent`; ``dloss`` fp32 [...] is the loss's gradient row by row."""
+    """Gradient (dx, dw) of :func:`linear_xent`; ``dloss`` [...] is the loss's gradient row by row."""
     _xent_args("linear_xent_bwd", x, w, targets, smoothing, keep)
+    _same_device("linear_xent_bwd", x, lse, dloss)
     if not x.is_cuda:
         return ref.linear_xent_bwd(x, w, targets, lse, dloss, scale, smoothing, ignore_index, keep, need_dx, need_dw)
-    x2 = _rows(x)
-    dx = torch.empty(x2.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
-    _native.C().linear_xent_bwd(x2, _rows(w), targets.long().reshape(-1), keep, float(scale), float(smoothing),
-                                int(ignore_index), lse.reshape(-1).contiguous(),
-                                dloss.float().reshape(-1).contiguous(), dx, dw, ctx(x.device).status)
-    return dx.view(x.shape) if need_dx else None, dw
+    return _native.C().linear_xent_bwd(x, w, targets, keep, scale, smoothing, ignore_index, lse, dloss, need_dx,
+                                       need_dw, ctx(x.device).status)
 
 
-def _norm_kind(kind, b):
+def _norm_kind(kind, bias):
     if kind not in ("rms", "layer"):
         raise ValueError(f"norm kind {kind!r}: 'rms' or 'layer'")
-    if kind == "rms" and b is not None:
+    if kind == "rms" and bias:
         raise ValueError("RMSNorm takes no bias")
     return kind == "layer"
 
@@ -414,42 +376,20 @@ def _norm_kind(kind, b):
 def norm_train(x, w, b=None, eps=1e-5, kind="rms", delta=None):
     """(y, h, stats): y = norm(h) * w (+ b) with h = x (+ delta, rounded to x's type), and the rows'
     fp32 (mean, 1 / std) that :func:`norm_train_bwd` reads. x bf16 (w, b bf16 or fp32) or fp32."""
-    layer = _norm_kind(kind, b)
+    layer = _norm_kind(kind, b is not None)
     _same_device("norm_train", x, w, b, delta)
+    if delta is not None and (delta.shape != x.shape or delta.dtype != x.dtype):
+        raise ValueError("norm_train: delta must be like x")
     if not x.is_cuda:
         return ref.norm_train(x, w, b, eps, kind, delta)
-    x2 = x.reshape(-1, x.shape[-1])
-    x2 = x2 if x2.stride(-1) == 1 else x2.contiguous()
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(x2.shape[0], 2, dtype=torch.float32, device=x.device)
-    h = d2 = None
-    if delta is not None:
-        if delta.shape != x.shape or delta.dtype != x.dtype:
-            raise ValueError("norm_train: delta must be like x")
-        d2 = delta.reshape(x2.shape)
-        d2 = d2 if d2.stride(-1) == 1 else d2.contiguous()
-        h = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-    _native.C().norm_train(x2, d2, w.contiguous(), None if b is None else b.contiguous(), layer, float(eps), y, h,
-                           stats)
-    return y.view(x.shape), x if h is None else h.view(x.shape), stats
+    return _native.C().norm_train(x, w, b, eps, layer, delta)
 
 
 def norm_train_bwd(dy, h, w, stats, kind="rms", bias=False, dh=None):
     """(dx, dw, db) of :func:`norm_train`: ``dh`` is the gradient that h itself receives (the residual
     stream's), added to dx; dw, db have w's type; db is None without ``bias``."""
-    layer = _norm_kind(kind, w if bias else None)
+    layer = _norm_kind(kind, bias)
     _same_device("norm_train_bwd", dy, h, w, stats, dh)
     if not h.is_cuda:
         return ref.norm_train_bwd(dy, h, w, stats, kind, bias, dh)
-
-    def rows(t):
-        t = t.to(h.dtype).reshape(-1, h.shape[-1])
-        return t if t.stride(-1) == 1 else t.contiguous()
-
-    h2 = rows(h)
-    dx = torch.empty(h2.shape, dtype=h.dtype, device=h.device)
-    dw = torch.empty(w.shape, dtype=w.dtype, device=h.device)
-    db = torch.empty(w.shape, dtype=w.dtype, device=h.device) if bias else None
-    _native.C().norm_train_bwd(rows(dy), h2, w.contiguous(), stats, None if dh is None else rows(dh), layer, dx, dw,
-                               db)
-    return dx.view(h.shape), dw, db
+    return _native.C().norm_train_bwd(dy, h, w, stats, layer, bias, dh)

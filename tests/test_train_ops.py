@@ -563,4 +563,4 @@ def test_native_refusals_name_their_numbers():
         pytest.skip("native extension not built")
     t = torch.zeros(1, 2, 2, 60, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="got 60"):
-        _native.C().attention_bwd(t, t, t, t, t, t, None, 1.0, True, t, t, t, t)
+        _native.C().attention_bwd(t, t, t, t, t, t, None, 1.0, True, t)

@@ -46,7 +46,7 @@ struct Cfg {
   static constexpr int SMALL = 64 * 64 * 2;      // one half of 64 rows
   static constexpr int FIX_BYTES = 2 * H * BIG;  // the two resident operands (K, V or Q, dO)
   static constexpr int ST_BYTES = 2 * H * SMALL; // the two streamed ones
-  static constexpr int STAT = 64 * 8;            // (-lse log2 e, delta) of 64 queries
+  static constexpr int STAT = 64 * 8;            // -lse log2 e and -delta of 64 queries
   static constexpr int STAT_OFF = FIX_BYTES + NSTAGE * ST_BYTES;
   static constexpr int BAR_OFF = STAT_OFF + NSTAGE * STAT;
   static constexpr int SMEM = BAR_OFF + 256 + 1024;
@@ -54,7 +54,7 @@ struct Cfg {
 }  // namespace fa_bw
 
 struct AttnBwdArgs {
-  const float2* stat;   // [B, H, Tp] (-lse log2 e or -inf, delta)
+  const float* stat;    // [B, H, Tp / 64][2][64]: -lse log2 e (or -inf), -delta
   const int* lens;      // optional [B] valid tokens
   __nv_bfloat16 *dq, *dk, *dv;  // contiguous [B, T, H, D], [B, S, Hkv, D]
   float* part;          // nsplit > 1: [nsplit][2][B, S, Hkv, D]
@@ -75,13 +75,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// (-lse log2 e, rowsum(dO * O)) of every query row, laid out [B, H, Tp] for the kernel below.
-// Rows without a visible key (lse = -inf), beyond the length or beyond T get (-inf, 0): P = 0.
+// -lse log2 e and -rowsum(dO * O) of every query row, 64 of each side by side for a tile of the
+// kernel below. Rows without a visible key (lse = -inf), beyond the length or beyond T get
+// (-inf, 0): P = 0.
 // 16 lanes a row, 8 elements each; blockIdx.y is the sequence. Bound by reading out and dout.
 __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16* __restrict__ o,
                                                             const __nv_bfloat16* __restrict__ go,
                                                             const float* __restrict__ lse, const int* lens,
-                                                            float2* __restrict__ stat, int T, int Tp, int H, int hd,
+                                                            float* __restrict__ stat, int T, int Tp, int H, int hd,
                                                             long long ob, long long ot, long long oh, long long gb,
                                                             long long gt, long long gh) {
   const int sub = threadIdx.x & 15, b = blockIdx.y;
@@ -103,9 +104,11 @@ __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16*
     }
 #pragma unroll
     for (int s = 8; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
-    if (sub == 0)
-      stat[((long long)b * H + h) * Tp + t] =
-          l == -INFINITY ? make_float2(-INFINITY, 0.f) : make_float2(-l * fa_bw::LOG2E, d);
+    if (sub == 0) {
+      float* p = stat + (((long long)b * H + h) * Tp + (t & ~63)) * 2 + (t & 63);
+      p[0] = l == -INFINITY ? -INFINITY : -l * fa_bw::LOG2E;
+      p[64] = l == -INFINITY ? 0.f : -d;
+    }
   }
 }
 
@@ -118,43 +121,72 @@ __device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
   }
 }
 
-// A thread's 32 columns of S and dP (tensor memory) -> P and dS, 16 bits, written over the
-// tile's S and dP. COLQ: columns are queries (S^T), their stats come from shared memory; else the
-// thread's row has one stat. The results take the first 16 of the columns that the thread itself
-// has read (P and dS of tile columns 32 .. 63 therefore start at column 32, not 16). Column j (of
-// the tile) is visible when lo <= j < hi.
-template <bool COLQ>
-__device__ __forceinline__ void softmax_grad(uint32_t s_tmem, uint32_t dp_tmem, uint32_t stat_smem, float2 own,
-                                             float c2, int col0, int lo, int hi, bool masked) {
-  uint32_t sv[32], dv[32];
+// A thread's 32 columns (from col0) of a tile's S -> P, kept in fp32 pairs; with PUT also written
+// in 16 bits. COLQ: columns are queries (S^T), their -lse come from shared memory; else the
+// thread's row has one. Results take the first 16 of the columns that the thread itself has read
+// (P and dS of tile columns 32 .. 63 therefore start at column 32, not 16). MASK: column j of
+// the tile is visible when lo <= j < hi; selected, not multiplied: what lies under a mask may be
+// anything.
+template <bool COLQ, bool MASK>
+__device__ __forceinline__ void tile_p(uint32_t s_tmem, uint32_t stat, float own, float c2, int col0, int lo, int hi,
+                                       uint64_t (&p)[16]) {
+  uint32_t sv[32];
   tmem_ld_32x32b_x32(s_tmem + col0, sv);
+  tc_wait_ld();
+  const uint64_t c = pair_f32(c2, c2);
+  uint32_t pk[16];
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    uint4 u;
+    if constexpr (COLQ) u = lds128(stat + (col0 + j) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e ? u.z : u.x), __uint_as_float(e ? u.w : u.y))
+                              : pair_f32(own, own);
+      const float2 x = unpair_f32(
+          fma_f32x2(pair_f32(__uint_as_float(sv[j + e]), __uint_as_float(sv[j + e + 1])), c, l));
+      float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+      if constexpr (MASK) {
+        const int i = col0 + j + e;
+        p0 = i >= lo && i < hi ? p0 : 0.f;
+        p1 = i + 1 >= lo && i + 1 < hi ? p1 : 0.f;
+      }
+      p[(j + e) / 2] = pair_f32(p0, p1);
+      if constexpr (COLQ) pk[(j + e) / 2] = pack_bf16x2(p0, p1);
+    }
+  }
+  if constexpr (COLQ) {
+    tmem_st_32x32b_x16(s_tmem + col0, pk);
+    tc_wait_st();
+  }
+}
+
+// dS = P (dP - delta) of the same columns, written over dP in 16 bits. stat / own: -delta.
+template <bool COLQ, bool MASK>
+__device__ __forceinline__ void tile_ds(uint32_t dp_tmem, uint32_t stat, float own, int col0, int lo, int hi,
+                                        const uint64_t (&p)[16]) {
+  uint32_t dv[32];
   tmem_ld_32x32b_x32(dp_tmem + col0, dv);
   tc_wait_ld();
-  uint32_t pk[16], dk[16];
+  uint32_t dk[16];
 #pragma unroll
-  for (int j = 0; j < 32; j += 2) {
-    float2 a = own, b = own;
-    if constexpr (COLQ) {
-      const uint4 u = lds128(stat_smem + (col0 + j) * 8);
-      a = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-      b = make_float2(__uint_as_float(u.z), __uint_as_float(u.w));
+  for (int j = 0; j < 32; j += 4) {
+    uint4 u;
+    if constexpr (COLQ) u = lds128(stat + (col0 + j) * 4);
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e ? u.z : u.x), __uint_as_float(e ? u.w : u.y))
+                              : pair_f32(own, own);
+      float2 d = unpair_f32(mul_f32x2(
+          p[(j + e) / 2], add_f32x2(pair_f32(__uint_as_float(dv[j + e]), __uint_as_float(dv[j + e + 1])), l)));
+      if constexpr (MASK) {
+        const int i = col0 + j + e;
+        d.x = i >= lo && i < hi ? d.x : 0.f;
+        d.y = i + 1 >= lo && i + 1 < hi ? d.y : 0.f;
+      }
+      dk[(j + e) / 2] = pack_bf16x2(d.x, d.y);
     }
-    float p0 = fast_exp2(fmaf(__uint_as_float(sv[j]), c2, a.x));
-    float p1 = fast_exp2(fmaf(__uint_as_float(sv[j + 1]), c2, b.x));
-    float d0 = p0 * (__uint_as_float(dv[j]) - a.y);
-    float d1 = p1 * (__uint_as_float(dv[j + 1]) - b.y);
-    if (masked) {  // selected, not multiplied: what lies under a mask may be anything
-      const int c = col0 + j;
-      const bool v0 = c >= lo && c < hi, v1 = c + 1 >= lo && c + 1 < hi;
-      p0 = v0 ? p0 : 0.f;
-      d0 = v0 ? d0 : 0.f;
-      p1 = v1 ? p1 : 0.f;
-      d1 = v1 ? d1 : 0.f;
-    }
-    pk[j / 2] = pack_bf16x2(p0, p1);
-    dk[j / 2] = pack_bf16x2(d0, d1);
   }
-  if constexpr (COLQ) tmem_st_32x32b_x16(s_tmem + col0, pk);
   tmem_st_32x32b_x16(dp_tmem + col0, dk);
   tc_wait_st();
 }
@@ -198,9 +230,11 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   uint64_t* full = fix_full + 1;    // [NS]
   uint64_t* empty = full + NS;      // [NS]
   uint64_t* land = empty + NS;      // a padded tile before its rows are cleared
-  uint64_t* s_full = land + 1;      // [2]
-  uint64_t* p_full = s_full + 2;    // [2]
-  uint64_t* acc_full = p_full + 2;
+  uint64_t* s_full = land + 1;      // [2] S of a stage is there
+  uint64_t* dp_full = s_full + 2;   // [2] dP is
+  uint64_t* p_full = dp_full + 2;   // [2] P is (kv)
+  uint64_t* ds_full = p_full + 2;   // [2] dS is
+  uint64_t* acc_full = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -247,7 +281,9 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     mbar_init(land, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
+      mbar_init(&dp_full[s], 1);
       mbar_init(&p_full[s], 256);
+      mbar_init(&ds_full[s], 256);
     }
     mbar_init(acc_full, 1);
     fence_barrier_init();
@@ -287,7 +323,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
           tma_load_4d(st + (C::H + h) * C::SMALL, KV ? &tmG : &tmV, bar, h * 64, KV ? hd : kvh, x0, b);
         }
         if constexpr (KV)
-          bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + ((size_t)b * a.H + hd) * a.Tp + x0, C::STAT, bar);
+          bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + (((size_t)b * a.H + hd) * a.Tp + x0) * 2, C::STAT, bar);
       }
       __syncwarp();
       if (pad) {
@@ -319,7 +355,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       for (int it = 0; it <= total && ok; ++it) {
         if (it < total) {
           const int s = it % NS;
-          if (!mbar_wait(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+          if (!mbar_poll(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
           const uint32_t d = tmem + STAGE0 + (it & 1) * 128;
@@ -329,24 +365,27 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
           for (int k = 0; k < D / 16; ++k)
             tc_mma_f16(d, smem_desc_sw128(r0 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
                        smem_desc_sw128(x0 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+          tc_commit(&s_full[it & 1]);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k)
             tc_mma_f16(d + 64, smem_desc_sw128(r1 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
                        smem_desc_sw128(x1 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-          tc_commit(&s_full[it & 1]);
+          tc_commit(&dp_full[it & 1]);
         }
         if (it > 0) {
           const int j = it - 1, s = j % NS;
-          if (!mbar_wait(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
-          tc_fence_after();
           const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
           const uint32_t p = tmem + STAGE0 + (j & 1) * 128;
           if constexpr (KV) {
+            if (!mbar_poll(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
+            tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; ++k)  // 16 queries a step
               tc_mma_f16_ts(tmem, p + (k >> 1) * 32 + (k & 1) * 8, smem_desc_sw128_mn(x1 + k * 2048, C::SMALL, 1024), IDESC_A,
                             j > 0 || k > 0);
           }
+          if (!mbar_poll(&ds_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
+          tc_fence_after();
 #pragma unroll
           for (int k = 0; k < 4; ++k)  // dK += dS^T Q, or dQ += dS K
             tc_mma_f16_ts(tmem + (KV ? 128 : 0), p + 64 + (k >> 1) * 32 + (k & 1) * 8,
@@ -366,7 +405,10 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     bool zero = total == 0;
     if constexpr (!KV) {
       own.x = -INFINITY;
-      if (row < nrow) own = a.stat[((size_t)b * a.H + head) * a.Tp + row];
+      if (row < nrow) {
+        const float* p = a.stat + (((size_t)b * a.H + head) * a.Tp + (row & ~63)) * 2 + (row & 63);
+        own = make_float2(p[0], p[64]);
+      }
       zero = zero || own.x == -INFINITY;         // padding, or no visible key: gradient 0
     }
     bool ok = true;
@@ -381,18 +423,30 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       if (!ok) break;
       tc_fence_after();
       const uint32_t st = lanes + STAGE0 + (it & 1) * 128;
+      const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT);
+      const bool masked = KV ? row0 + 128 > nrow || (a.causal && row0 + 127 > x0 + a.off)
+                             : x0 + 64 > nstream || (a.causal && x0 + 63 > row0 + a.off);
+      const int lo = !KV ? 0 : row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0);
+      const int hi = KV ? 64 : min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64);
+      uint64_t p[16];
+      if (masked)
+        tile_p<KV, true>(st, stat, own.x, a.scale_log2, half * 32, lo, hi, p);
+      else
+        tile_p<KV, false>(st, stat, own.x, a.scale_log2, half * 32, lo, hi, p);
       if constexpr (KV) {
-        const bool masked = row0 + 128 > nrow || (a.causal && row0 + 127 > x0 + a.off);
-        const int lo = row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0);
-        softmax_grad<true>(st, st + 64, smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT), own, a.scale_log2,
-                           half * 32, lo, 64, masked);
-      } else {
-        const bool masked = x0 + 64 > nstream || (a.causal && x0 + 63 > row0 + a.off);
-        const int hi = min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64);
-        softmax_grad<false>(st, st + 64, 0, own, a.scale_log2, half * 32, 0, hi, masked);
+        tc_fence_before();
+        mbar_arrive(&p_full[it & 1]);
       }
+      ok = mbar_wait(&dp_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      if (masked)
+        tile_ds<KV, true>(st + 64, stat + 256, own.y, half * 32, lo, hi, p);
+      else
+        tile_ds<KV, false>(st + 64, stat + 256, own.y, half * 32, lo, hi, p);
       tc_fence_before();
-      mbar_arrive(&p_full[it & 1]);
+      mbar_arrive(&ds_full[it & 1]);
     }
     if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
     ok = __all_sync(0xffffffffu, ok);
@@ -579,7 +633,7 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   // scratch: the rows' statistics, then the split heads' partials
   const int64_t stat_floats = B * H * a.Tp * 2, plane = B * S * Hkv * D;
   auto ws = torch::empty({stat_floats + (a.nsplit > 1 ? 2 * a.nsplit * plane : 0)}, lse.options());
-  float2* stat = reinterpret_cast<float2*>(ws.data_ptr<float>());
+  float* stat = ws.data_ptr<float>();
   a.stat = stat;
   a.part = a.nsplit > 1 ? ws.data_ptr<float>() + stat_floats : nullptr;
   const int64_t rows = (int64_t)a.Tp * H;

@@ -18,9 +18,10 @@
 // relative per term at the most, independently; sums are fp32 in tensor memory.
 //
 // Tensor memory of a kv CTA: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512 columns, all
-// there are; this is what sets the 64-query tile. All eight softmax warps work on one tile, 32
-// columns a thread, because the tile's latency (the exponentials alone take 512 cycles of the
-// SM's 16 a cycle) has to fit into the 1280 cycles of products that run beside it.
+// there are; this is what sets the 64-query tile. Eight softmax warps work on one tile, 32 columns
+// a thread, and two such groups take the tiles in turn: a tile's exponentials (512 cycles at the
+// SM's 16 a cycle) and its loads and stores of tensor memory have to fit beside the 1280 cycles of
+// products of the tile before and after.
 //
 // Seven products instead of the five of a single loop is the price of the fixed summation order
 // (and of no fp32 dQ in memory).
@@ -39,6 +40,7 @@ namespace om {
 namespace fa_bw {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NSTAGE = 4;
+constexpr int THREADS = 640;  // copy, MMA, TMEM and one idle warp; two groups of eight softmax warps
 template <int D>
 struct Cfg {
   static constexpr int H = D / 64;               // 64-wide halves of the head dimension
@@ -397,7 +399,8 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax and output
-    const int half = (warp - 4) >> 2;            // columns 32 half .. of a tile
+    const int group = (warp - 4) >> 3;           // tiles group, group + 2, ...
+    const int half = ((warp - 4) >> 2) & 1;      // columns 32 half .. of a tile
     const int t = (warp & 3) * 32 + lane;        // row == TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int row = row0 + t;
@@ -412,10 +415,11 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       zero = zero || own.x == -INFINITY;         // padding, or no visible key: gradient 0
     }
     bool ok = true;
-    int tile = 0;
-    for (int it = 0; it < total; ++it) {
+    int tile = ntile ? group % ntile : 0;
+    for (int it = group; it < total; it += 2) {
       const int x0 = (first + tile) * 64;
-      if (++tile == ntile) tile = 0;
+      tile += 2;
+      while (tile >= ntile) tile -= ntile;
       ok = mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
       // whoever reads a tile's statistics waits for their copy as well
       if constexpr (KV) ok = ok && mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
@@ -452,20 +456,21 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      if constexpr (KV) {
-        // the first four warps write dV, the others dK
+      const int col0 = half * (D / 2);  // each half writes half of the columns
+      if constexpr (KV) {               // group 0 writes dV, group 1 dK
         const bool live = row < a.S;
-        const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd;
-        const float f = half ? a.scale : 1.f;
+        const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd + col0;
+        const float f = group ? a.scale : 1.f;
+        const uint32_t acc = lanes + group * 128 + col0;
         if (a.nsplit > 1) {
           const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
-          write_acc<D>(lanes + half * 128, a.part + (split * 2 + half) * plane + at, live, zero, f, a.hd);
+          write_acc<D / 2>(acc, a.part + (split * 2 + group) * plane + at, live, zero, f, a.hd - col0);
         } else {
-          write_acc<D>(lanes + half * 128, (half ? a.dk : a.dv) + at, live, zero, f, a.hd);
+          write_acc<D / 2>(acc, (group ? a.dk : a.dv) + at, live, zero, f, a.hd - col0);
         }
-      } else {  // each half writes half of the columns
-        write_acc<D / 2>(lanes + half * (D / 2), a.dq + (((size_t)b * a.T + row) * a.H + head) * a.hd + half * (D / 2),
-                            row < a.T, zero, a.scale, a.hd - half * (D / 2));
+      } else if (group == 0) {
+        write_acc<D / 2>(lanes + col0, a.dq + (((size_t)b * a.T + row) * a.H + head) * a.hd + col0, row < a.T, zero,
+                         a.scale, a.hd - col0);
       }
     }
   }
@@ -479,7 +484,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
 }
 
 template <int D>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(fa_bw::THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const AttnBwdArgs a) {
@@ -540,7 +545,7 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
   }
   const long long blocks = a.kv_blocks + (long long)((a.T + 127) / 128) * a.B * a.H;
   TORCH_CHECK(blocks < (1ll << 31), "attention_bwd: too many tiles");
-  attn_bwd_kernel<D><<<(unsigned)blocks, 384, C::SMEM, st>>>(q, g, k, v, a);
+  attn_bwd_kernel<D><<<(unsigned)blocks, fa_bw::THREADS, C::SMEM, st>>>(q, g, k, v, a);
   OM_LAUNCH_CHECK();
   if (a.nsplit > 1) {
     const long long n = (long long)a.B * a.S * a.Hkv * a.hd;

@@ -123,73 +123,72 @@ __device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
   }
 }
 
-// A thread's 32 columns (from col0) of a tile's S -> P, kept in fp32 pairs; with PUT also written
-// in 16 bits. COLQ: columns are queries (S^T), their -lse come from shared memory; else the
-// thread's row has one. Results take the first 16 of the columns that the thread itself has read
-// (P and dS of tile columns 32 .. 63 therefore start at column 32, not 16). MASK: column j of
-// the tile is visible when lo <= j < hi; selected, not multiplied: what lies under a mask may be
-// anything.
+// Where tile i keeps its S (which = 0) and dP (1): four regions of 64 columns, two for each parity
+// of i. P and dS are written over S, so the region of dP is free once dS is there; the next tile
+// of the parity puts its S into it, before P and dS are used up, and its dP over P and dS after.
+__device__ __forceinline__ uint32_t tile_region(int i, int which) {
+  return (uint32_t)((i & 1) * 128 + (((i >> 1) ^ which) & 1) * 64);
+}
+
+// A thread's 32 columns of S -> P, kept in fp32 pairs; COLQ: also written in 16 bits over the
+// first 16 of these columns (the caller waits for the store). COLQ: columns are queries (S^T),
+// their -lse come from shared memory; else the thread's row has one. MASK: column j is visible
+// when lo <= j < hi; selected, not multiplied: what lies under a mask may be anything.
 template <bool COLQ, bool MASK>
-__device__ __forceinline__ void tile_p(uint32_t s_tmem, uint32_t stat, float own, float c2, int col0, int lo, int hi,
+__device__ __forceinline__ void tile_p(uint32_t s_at, uint32_t stat, float own, float c2, int lo, int hi,
                                        uint64_t (&p)[16]) {
   uint32_t sv[32];
-  tmem_ld_32x32b_x32(s_tmem + col0, sv);
+  tmem_ld_32x32b_x32(s_at, sv);
   tc_wait_ld();
   const uint64_t c = pair_f32(c2, c2);
   uint32_t pk[16];
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     uint4 u;
-    if constexpr (COLQ) u = lds128(stat + (col0 + j) * 4);
+    if constexpr (COLQ) u = lds128(stat + j * 4);
 #pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e ? u.z : u.x), __uint_as_float(e ? u.w : u.y))
+    for (int e = j; e < j + 4; e += 2) {
+      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e > j ? u.z : u.x), __uint_as_float(e > j ? u.w : u.y))
                               : pair_f32(own, own);
-      const float2 x = unpair_f32(
-          fma_f32x2(pair_f32(__uint_as_float(sv[j + e]), __uint_as_float(sv[j + e + 1])), c, l));
+      const float2 x = unpair_f32(fma_f32x2(pair_f32(__uint_as_float(sv[e]), __uint_as_float(sv[e + 1])), c, l));
       float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
       if constexpr (MASK) {
-        const int i = col0 + j + e;
-        p0 = i >= lo && i < hi ? p0 : 0.f;
-        p1 = i + 1 >= lo && i + 1 < hi ? p1 : 0.f;
+        p0 = e >= lo && e < hi ? p0 : 0.f;
+        p1 = e + 1 >= lo && e + 1 < hi ? p1 : 0.f;
       }
-      p[(j + e) / 2] = pair_f32(p0, p1);
-      if constexpr (COLQ) pk[(j + e) / 2] = pack_bf16x2(p0, p1);
+      p[e / 2] = pair_f32(p0, p1);
+      if constexpr (COLQ) pk[e / 2] = pack_bf16x2(p0, p1);
     }
   }
-  if constexpr (COLQ) {
-    tmem_st_32x32b_x16(s_tmem + col0, pk);
-    tc_wait_st();
-  }
+  if constexpr (COLQ) tmem_st_32x32b_x16(s_at, pk);
 }
 
-// dS = P (dP - delta) of the same columns, written over dP in 16 bits. stat / own: -delta.
+// dS = P (dP - delta) of the same columns, in 16 bits to ds_at. stat / own: -delta.
 template <bool COLQ, bool MASK>
-__device__ __forceinline__ void tile_ds(uint32_t dp_tmem, uint32_t stat, float own, int col0, int lo, int hi,
+__device__ __forceinline__ void tile_ds(uint32_t dp_at, uint32_t ds_at, uint32_t stat, float own, int lo, int hi,
                                         const uint64_t (&p)[16]) {
   uint32_t dv[32];
-  tmem_ld_32x32b_x32(dp_tmem + col0, dv);
+  tmem_ld_32x32b_x32(dp_at, dv);
   tc_wait_ld();
   uint32_t dk[16];
 #pragma unroll
   for (int j = 0; j < 32; j += 4) {
     uint4 u;
-    if constexpr (COLQ) u = lds128(stat + (col0 + j) * 4);
+    if constexpr (COLQ) u = lds128(stat + j * 4);
 #pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e ? u.z : u.x), __uint_as_float(e ? u.w : u.y))
+    for (int e = j; e < j + 4; e += 2) {
+      const uint64_t l = COLQ ? pair_f32(__uint_as_float(e > j ? u.z : u.x), __uint_as_float(e > j ? u.w : u.y))
                               : pair_f32(own, own);
-      float2 d = unpair_f32(mul_f32x2(
-          p[(j + e) / 2], add_f32x2(pair_f32(__uint_as_float(dv[j + e]), __uint_as_float(dv[j + e + 1])), l)));
+      float2 d = unpair_f32(
+          mul_f32x2(p[e / 2], add_f32x2(pair_f32(__uint_as_float(dv[e]), __uint_as_float(dv[e + 1])), l)));
       if constexpr (MASK) {
-        const int i = col0 + j + e;
-        d.x = i >= lo && i < hi ? d.x : 0.f;
-        d.y = i + 1 >= lo && i + 1 < hi ? d.y : 0.f;
+        d.x = e >= lo && e < hi ? d.x : 0.f;
+        d.y = e + 1 >= lo && e + 1 < hi ? d.y : 0.f;
       }
-      dk[(j + e) / 2] = pack_bf16x2(d.x, d.y);
+      dk[e / 2] = pack_bf16x2(d.x, d.y);
     }
   }
-  tmem_st_32x32b_x16(dp_tmem + col0, dk);
+  tmem_st_32x32b_x16(ds_at, dk);
   tc_wait_st();
 }
 
@@ -234,8 +233,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   uint64_t* land = empty + NS;      // a padded tile before its rows are cleared
   uint64_t* s_full = land + 1;      // [2] S of a stage is there
   uint64_t* dp_full = s_full + 2;   // [2] dP is
-  uint64_t* p_full = dp_full + 2;   // [2] P is (kv)
-  uint64_t* ds_full = p_full + 2;   // [2] dS is
+  uint64_t* ds_full = dp_full + 2;  // [2] P and dS are
   uint64_t* acc_full = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -284,7 +282,6 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&dp_full[s], 1);
-      mbar_init(&p_full[s], 256);
       mbar_init(&ds_full[s], 256);
     }
     mbar_init(acc_full, 1);
@@ -353,47 +350,55 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
       constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
       const uint32_t r0 = smem_u32(smem), r1 = r0 + C::H * C::BIG;  // K, V or Q, dO
+      // S (which = 0) or dP (1) of tile i, from the resident rows and the tile's 64
+      auto scores = [&](int i, int which) {
+        const uint32_t x = smem_u32(smem + C::FIX_BYTES + (i % NS) * C::ST_BYTES) + which * C::H * C::SMALL;
+        const uint32_t r = which ? r1 : r0;
+        const uint32_t d = tmem + STAGE0 + tile_region(i, which);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_f16(d, smem_desc_sw128(r + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
+                     smem_desc_sw128(x + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
+        tc_commit(which ? &dp_full[i & 1] : &s_full[i & 1]);
+      };
+      auto loaded = [&](int i) {
+        const bool there = mbar_poll(&full[i % NS], (i / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+        tc_fence_after();
+        return there;
+      };
       bool ok = mbar_wait(fix_full, 0, a.status, OM_ERR_WAIT_FULL);
-      for (int it = 0; it <= total && ok; ++it) {
-        if (it < total) {
-          const int s = it % NS;
-          if (!mbar_poll(&full[s], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
-          const uint32_t d = tmem + STAGE0 + (it & 1) * 128;
-          // stage it & 1 was last read by the products of tile it - 2, issued before by this
-          // thread: the tensor pipe runs them in order
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d, smem_desc_sw128(r0 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(x0 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-          tc_commit(&s_full[it & 1]);
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            tc_mma_f16(d + 64, smem_desc_sw128(r1 + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                       smem_desc_sw128(x1 + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-          tc_commit(&dp_full[it & 1]);
+      for (int i = 0; i < 2 && i < total && ok; ++i) {
+        ok = loaded(i);
+        if (!ok) break;
+        scores(i, 0);
+        scores(i, 1);
+      }
+      for (int i = 0; i < total && ok; ++i) {
+        ok = mbar_poll(&ds_full[i & 1], (i >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+        if (!ok) break;
+        tc_fence_after();
+        // dP of tile i has been read: its columns take the next S of this parity at once
+        if (i + 2 < total) {
+          ok = loaded(i + 2);
+          if (!ok) break;
+          scores(i + 2, 0);
         }
-        if (it > 0) {
-          const int j = it - 1, s = j % NS;
-          const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + s * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
-          const uint32_t p = tmem + STAGE0 + (j & 1) * 128;
-          if constexpr (KV) {
-            if (!mbar_poll(&p_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
-            tc_fence_after();
+        const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + (i % NS) * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
+        const uint32_t p = tmem + STAGE0 + tile_region(i, 0);
+        if constexpr (KV) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)  // 16 queries a step
-              tc_mma_f16_ts(tmem, p + (k >> 1) * 32 + (k & 1) * 8, smem_desc_sw128_mn(x1 + k * 2048, C::SMALL, 1024), IDESC_A,
-                            j > 0 || k > 0);
-          }
-          if (!mbar_poll(&ds_full[j & 1], (j >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < 4; ++k)  // dK += dS^T Q, or dQ += dS K
-            tc_mma_f16_ts(tmem + (KV ? 128 : 0), p + 64 + (k >> 1) * 32 + (k & 1) * 8,
-                          smem_desc_sw128_mn(x0 + k * 2048, C::SMALL, 1024), IDESC_A, j > 0 || k > 0);
-          tc_commit(&empty[s]);
+          for (int k = 0; k < 4; ++k)  // dV += P^T dO, 16 queries a step
+            tc_mma_f16_ts(tmem, p + (k >> 1) * 32 + (k & 1) * 8, smem_desc_sw128_mn(x1 + k * 2048, C::SMALL, 1024),
+                          IDESC_A, i > 0 || k > 0);
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // dK += dS^T Q, or dQ += dS K
+          tc_mma_f16_ts(tmem + (KV ? 128 : 0), p + 16 + (k >> 1) * 32 + (k & 1) * 8,
+                        smem_desc_sw128_mn(x0 + k * 2048, C::SMALL, 1024), IDESC_A, i > 0 || k > 0);
+        tc_commit(&empty[i % NS]);
+        // P and dS of tile i are read by the products just issued; the tensor pipe runs this
+        // thread's products in order, so the next dP may take their columns
+        if (i + 2 < total) scores(i + 2, 1);
       }
       if (ok) tc_commit(acc_full);
     }
@@ -420,35 +425,32 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       const int x0 = (first + tile) * 64;
       tile += 2;
       while (tile >= ntile) tile -= ntile;
-      ok = mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
       // whoever reads a tile's statistics waits for their copy as well
-      if constexpr (KV) ok = ok && mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+      if constexpr (KV) ok = mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+      ok = ok && mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t st = lanes + STAGE0 + (it & 1) * 128;
-      const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT);
+      const uint32_t s_at = lanes + STAGE0 + tile_region(it, 0) + half * 32;
+      const uint32_t dp_at = lanes + STAGE0 + tile_region(it, 1) + half * 32;
+      const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT) + half * 128;
       const bool masked = KV ? row0 + 128 > nrow || (a.causal && row0 + 127 > x0 + a.off)
                              : x0 + 64 > nstream || (a.causal && x0 + 63 > row0 + a.off);
-      const int lo = !KV ? 0 : row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0);
-      const int hi = KV ? 64 : min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64);
+      const int lo = (!KV ? 0 : row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0)) - half * 32;
+      const int hi = (KV ? 64 : min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64)) - half * 32;
       uint64_t p[16];
       if (masked)
-        tile_p<KV, true>(st, stat, own.x, a.scale_log2, half * 32, lo, hi, p);
+        tile_p<KV, true>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
       else
-        tile_p<KV, false>(st, stat, own.x, a.scale_log2, half * 32, lo, hi, p);
-      if constexpr (KV) {
-        tc_fence_before();
-        mbar_arrive(&p_full[it & 1]);
-      }
+        tile_p<KV, false>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
       ok = mbar_wait(&dp_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       if (masked)
-        tile_ds<KV, true>(st + 64, stat + 256, own.y, half * 32, lo, hi, p);
+        tile_ds<KV, true>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
       else
-        tile_ds<KV, false>(st + 64, stat + 256, own.y, half * 32, lo, hi, p);
+        tile_ds<KV, false>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
       tc_fence_before();
       mbar_arrive(&ds_full[it & 1]);
     }

@@ -97,10 +97,11 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_
     torch::Tensor status);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Tensor x, torch::Tensor w,
                                                                       c10::optional<torch::Tensor> b, double eps,
-                                                                      bool layer, c10::optional<torch::Tensor> delta);
+                                                                      bool layer, c10::optional<torch::Tensor> delta,
+                                                                      torch::Tensor status);
 std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_train_bwd(
     torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats, bool layer, bool bias,
-    c10::optional<torch::Tensor> dh);
+    c10::optional<torch::Tensor> dh, torch::Tensor status);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("launch_count", [] { return (int64_t)om::g_launches.load(); }, "kernel launches issued so far");

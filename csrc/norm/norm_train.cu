@@ -5,13 +5,15 @@
 //   r = 1 / sqrt(mean((h - mu)^2) + eps),  mu = mean(h) (RMSNorm: 0)
 //   a = dy w;  dx = r (a - n mean(a n) - [mean(a)]) (+ dh);  dw = sum_rows dy n;  db = sum_rows dy
 //
-// What bounds it: the rows' bytes, each read once and written once (4 or 7 values a column).
-// A row is held in the registers of G threads (16 elements each with 16-byte accesses), so the
-// two passes of the variance and of the gradient cost no second read. In the gradient every
-// group of threads walks rows grid-strided and keeps its columns' dw and db in registers; the
-// partial sums of the blocks are joined in block order by a second kernel: fp32, no atomics,
-// the same result on every run. The next row's loads are issued before the current row's
-// reductions, so the reductions' latency is hidden behind the loads.
+// What bounds it: the rows' bytes, each read once and written once (4 or 7 values a column). A row
+// is held in the registers of G threads, so the two passes of the variance and of the gradient
+// cost no second read, and every group of threads walks rows grid-strided with the weights (and
+// its columns' dw and db) in registers. Rows come into a ring in shared memory by bulk copies,
+// several rows ahead: registers alone could hold one row ahead, which left the memory idle during
+// the reductions. Rows that do not start on 16 bytes, or of which two do not fit into shared
+// memory, are read straight into registers.
+// The partial dw, db of the blocks are joined in block order by a second kernel: fp32, no atomics,
+// the same result on every run.
 #include <c10/cuda/CUDAGuard.h>
 #include "../common/om_host.h"
 #include "../common/om_ptx.cuh"
@@ -94,6 +96,33 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* sh, int& flip) {
 template <int G>
 constexpr int norm_threads() { return G < 256 ? 256 : G; }
 
+// A ring of rows in shared memory, one per group of G threads: NA arrays a stage, filled by bulk
+// copies that the group's first thread starts. Only arrival is signalled: a stage is filled again
+// after a barrier of the group that follows its last read.
+template <typename T, int G, int NA>
+struct RowRing {
+  uint8_t* base;      // this group's stages
+  uint64_t* full;     // this group's barriers
+  const T* src[NA];
+  long long ld[NA];
+  int stages;
+  uint32_t bytes;     // of a row
+  __device__ __forceinline__ void fill(int k, long long row) const {  // one thread
+    const int s = k % stages;
+    mbar_arrive_expect_tx(&full[s], NA * bytes);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) bulk_load(base + (size_t)(s * NA + i) * bytes, src[i] + row * ld[i], bytes, &full[s]);
+  }
+  __device__ __forceinline__ bool wait(int k, int* status) const {
+    return mbar_wait(&full[k % stages], (k / stages) & 1, status, OM_ERR_WAIT_FULL);
+  }
+  __device__ __forceinline__ const T* row(int k, int i) const {
+    return reinterpret_cast<const T*>(base + (size_t)((k % stages) * NA + i) * bytes);
+  }
+};
+
+constexpr int RING_MAX = 8;  // stages
+
 struct NormFwd {
   const void *x, *delta, *w, *b;
   void *y, *h;
@@ -101,6 +130,8 @@ struct NormFwd {
   long long M, ldx, ldd;
   int D;
   float eps;
+  int stages;  // of the ring
+  int* status;
 };
 
 template <typename T, typename W, bool LAYER, int G, int V, int P>
@@ -163,6 +194,97 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_kernel(const NormF
   }
 }
 
+// The same with the rows in a ring and the weights in registers.
+template <typename T, typename W, bool LAYER, bool DELTA, int G, int P>
+__global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const NormFwd a) {
+  constexpr int NT = norm_threads<G>(), RPB = NT / G, V = 8, NA = DELTA ? 2 : 1;
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float sh[2 * (NT / 32)];
+  __shared__ uint64_t bars[RPB * RING_MAX];
+  const int grp = threadIdx.x / G, lane = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
+  RowRing<T, G, NA> ring;
+  ring.stages = a.stages;
+  ring.bytes = a.D * sizeof(T);
+  ring.base = ring_mem + (size_t)grp * a.stages * NA * ring.bytes;
+  ring.full = bars + grp * RING_MAX;
+  ring.src[0] = static_cast<const T*>(a.x);
+  ring.ld[0] = a.ldx;
+  if constexpr (DELTA) {
+    ring.src[1] = static_cast<const T*>(a.delta);
+    ring.ld[1] = a.ldd;
+  }
+  if (lane == 0) {
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+    fence_barrier_init();
+    for (int k = 0; k < a.stages; ++k)
+      if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
+  }
+  Vec<W, V> w[P], b[LAYER ? P : 1];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int c = (lane + i * G) * V;
+    w[i].zero();
+    if (c < a.D) w[i].load(static_cast<const W*>(a.w) + c);
+    if constexpr (LAYER) {
+      b[i].zero();
+      if (a.b && c < a.D) b[i].load(static_cast<const W*>(a.b) + c);
+    }
+  }
+  __syncthreads();
+  int flip = 0, k = 0;
+  for (long long base = row0; base < a.M; base += step, ++k) {
+    const long long row = base + grp;
+    const bool live = row < a.M && ring.wait(k, a.status);
+    float f[P][V], sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + i * G) * V;
+      Vec<T, V> v, d;
+      v.zero();
+      d.zero();
+      if (live && c < a.D) {
+        v.load(ring.row(k, 0) + c);
+        if constexpr (DELTA) d.load(ring.row(k, 1) + c);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        f[i][j] = DELTA ? round_to<T>(v.get(j) + d.get(j)) : v.get(j);
+        sum[0] += LAYER ? f[i][j] : f[i][j] * f[i][j];
+      }
+      if (DELTA && live && c < a.D) store_vec<T, V>(static_cast<T*>(a.h) + row * a.D + c, f[i]);
+    }
+    group_sum<G, 1>(sum, sh, flip);
+    if constexpr (G == 32) __syncwarp();
+    if (lane == 0 && row + a.stages * step < a.M) ring.fill(k + a.stages, row + a.stages * step);
+    float mu = 0.f;
+    if constexpr (LAYER) {
+      mu = sum[0] / a.D;
+      sum[0] = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float t = (lane + i * G) * V < a.D ? f[i][j] - mu : 0.f;
+          sum[0] += t * t;
+        }
+      group_sum<G, 1>(sum, sh, flip);
+    }
+    if (!live) continue;
+    const float r = rsqrtf(sum[0] / a.D + a.eps);
+    if (lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mu, r);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + i * G) * V;
+      if (c >= a.D) continue;
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = (f[i][j] - mu) * r * w[i].get(j) + (LAYER ? b[LAYER ? i : 0].get(j) : 0.f);
+      store_vec<T, V>(static_cast<T*>(a.y) + row * a.D + c, o);
+    }
+  }
+}
+
 struct NormBwd {
   const void *dy, *h, *w, *dh;
   void* dx;
@@ -170,7 +292,51 @@ struct NormBwd {
   float* part;  // [blocks][1 or 2][D]: dw, db
   long long M, ldy, ldh, lddh;
   int D;
+  int stages;
+  int* status;
 };
+
+// The block's row groups are added up in group order through shared memory (acc: [D]).
+template <int G, int V, int P, int N, int RPB>
+__device__ __forceinline__ void write_partials(const NormBwd& a, const float (&dw)[P][V],
+                                               const float (&db)[N == 2 ? P : 1][V], float* acc) {
+  const int lane = threadIdx.x % G;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    float* out = a.part + ((size_t)blockIdx.x * N + k) * a.D;
+    if constexpr (RPB == 1) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int c = (lane + i * G) * V;
+        if (c >= a.D) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[c + j] = k == 0 ? dw[i][j] : db[N == 2 ? i : 0][j];
+      }
+    } else {
+      for (int grp = 0; grp < RPB; ++grp) {
+        __syncthreads();
+        if ((int)threadIdx.x / G == grp) {
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const int c = (lane + i * G) * V;
+            if (c >= a.D) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              const float t = k == 0 ? dw[i][j] : db[N == 2 ? i : 0][j];
+              if (grp == 0)
+                acc[c + j] = t;
+              else if (grp < RPB - 1)
+                acc[c + j] += t;
+              else
+                out[c + j] = acc[c + j] + t;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
 
 template <typename T, typename W, bool LAYER, int G, int V, int P>
 __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_kernel(const NormBwd a) {
@@ -251,43 +417,107 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_kernel(const NormB
       store_vec<T, V>(static_cast<T*>(a.dx) + row * a.D + c, o);
     }
   }
-  // the block's row groups are added up in group order through shared memory
   extern __shared__ float acc[];  // [D] when RPB > 1
+  write_partials<G, V, P, N, RPB>(a, dw, db, acc);
+}
+
+// The same with the rows in a ring.
+template <typename T, typename W, bool LAYER, bool DH, int G, int P>
+__global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const NormBwd a) {
+  constexpr int NT = norm_threads<G>(), RPB = NT / G, N = LAYER ? 2 : 1, V = 8, NA = DH ? 3 : 2;
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float sh[2 * N * (NT / 32)];
+  __shared__ uint64_t bars[RPB * RING_MAX];
+  const int grp = threadIdx.x / G, lane = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
+  RowRing<T, G, NA> ring;
+  ring.stages = a.stages;
+  ring.bytes = a.D * sizeof(T);
+  ring.base = ring_mem + (size_t)grp * a.stages * NA * ring.bytes;
+  ring.full = bars + grp * RING_MAX;
+  ring.src[0] = static_cast<const T*>(a.h);
+  ring.ld[0] = a.ldh;
+  ring.src[1] = static_cast<const T*>(a.dy);
+  ring.ld[1] = a.ldy;
+  if constexpr (DH) {
+    ring.src[2] = static_cast<const T*>(a.dh);
+    ring.ld[2] = a.lddh;
+  }
+  if (lane == 0) {
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+    fence_barrier_init();
+    for (int k = 0; k < a.stages; ++k)
+      if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
+  }
+  float dw[P][V], db[LAYER ? P : 1][V];
+  Vec<W, V> w[P];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    float* out = a.part + ((size_t)blockIdx.x * N + k) * a.D;
-    if constexpr (RPB == 1) {
+  for (int i = 0; i < P; ++i) {
+    const int c = (lane + i * G) * V;
+    w[i].zero();
+    if (c < a.D) w[i].load(static_cast<const W*>(a.w) + c);
 #pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const int c = (lane + i * G) * V;
-        if (c >= a.D) continue;
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[c + j] = k == 0 ? dw[i][j] : db[LAYER ? i : 0][j];
-      }
-    } else {
-      for (int grp = 0; grp < RPB; ++grp) {
-        __syncthreads();
-        if ((int)threadIdx.x / G == grp) {
-#pragma unroll
-          for (int i = 0; i < P; ++i) {
-            const int c = (lane + i * G) * V;
-            if (c >= a.D) continue;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const float t = k == 0 ? dw[i][j] : db[LAYER ? i : 0][j];
-              if (grp == 0)
-                acc[c + j] = t;
-              else if (grp < RPB - 1)
-                acc[c + j] += t;
-              else
-                out[c + j] = acc[c + j] + t;
-            }
-          }
-        }
-      }
-      __syncthreads();
+    for (int j = 0; j < V; ++j) {
+      dw[i][j] = 0.f;
+      if constexpr (LAYER) db[i][j] = 0.f;
     }
   }
+  float2 next = make_float2(0.f, 0.f);
+  if (row0 + grp < a.M) next = *reinterpret_cast<const float2*>(a.stats + 2 * (row0 + grp));
+  __syncthreads();
+  int flip = 0, k = 0;
+  for (long long base = row0; base < a.M; base += step, ++k) {
+    const long long row = base + grp;
+    const bool live = row < a.M && ring.wait(k, a.status);
+    const float mu = next.x, r = live ? next.y : 0.f;
+    if (row + step < a.M) next = *reinterpret_cast<const float2*>(a.stats + 2 * (row + step));
+    float n[P][V], ga[P][V];
+    Vec<T, V> d[DH ? P : 1];
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + i * G) * V;
+      Vec<T, V> hv, yv;
+      hv.zero();
+      yv.zero();
+      if constexpr (DH) d[i].zero();
+      if (live && c < a.D) {
+        hv.load(ring.row(k, 0) + c);
+        yv.load(ring.row(k, 1) + c);
+        if constexpr (DH) d[i].load(ring.row(k, 2) + c);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float y = yv.get(j);
+        n[i][j] = (hv.get(j) - mu) * r;
+        ga[i][j] = y * w[i].get(j);  // 0 beyond the row's end: w and dy are 0 there
+        s[0] += ga[i][j] * n[i][j];
+        dw[i][j] += y * n[i][j];
+        if constexpr (LAYER) {
+          s[N - 1] += ga[i][j];
+          db[i][j] += y;
+        }
+      }
+    }
+    group_sum<G, N>(s, sh, flip);
+    if constexpr (G == 32) __syncwarp();
+    if (lane == 0 && row + a.stages * step < a.M) ring.fill(k + a.stages, row + a.stages * step);
+    if (!live) continue;  // no barrier below
+    const float c1 = s[0] / a.D, c2 = LAYER ? s[N - 1] / a.D : 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = (lane + i * G) * V;
+      if (c >= a.D) continue;
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = r * (ga[i][j] - n[i][j] * c1 - c2) + (DH ? d[DH ? i : 0].get(j) : 0.f);
+      store_vec<T, V>(static_cast<T*>(a.dx) + row * a.D + c, o);
+    }
+  }
+  __syncthreads();  // every copy has been waited for and read: the ring's memory is free
+  write_partials<G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }
 
 // dw (db) = sum over blocks, in block order: 32 columns a block, 8 warps each take every eighth
@@ -350,6 +580,38 @@ static void norm_types(const char* op, at::ScalarType t, at::ScalarType w, F&& f
   return f(0.f, 0.f);
 }
 
+// Stages of a ring: what makes about 64 KB a block, at least two; fewer than two: no ring.
+static int ring_stages(size_t stage_bytes) {
+  const size_t two = 2 * stage_bytes;
+  if (two > 200 * 1024) return 0;
+  return (int)std::min<size_t>(RING_MAX, std::max<size_t>(2, (64 * 1024) / stage_bytes));
+}
+
+// Blocks of a kernel that an SM holds, for the shared memory last asked for (a program runs few
+// row lengths). The kernel is allowed that much first.
+struct Residents {
+  std::mutex lock;
+  size_t smem = (size_t)-1, allowed = 40 * 1024;
+  int dev = -1, blocks = 0;
+  template <typename K>
+  int get(K kernel, int threads, size_t bytes) {
+    std::lock_guard<std::mutex> hold(lock);
+    int d;
+    OM_CUDA_CHECK(cudaGetDevice(&d));
+    if (d != dev) allowed = 40 * 1024;
+    if (d == dev && bytes == smem) return blocks;
+    if (bytes > allowed) {
+      OM_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+      allowed = bytes;
+    }
+    OM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, bytes));
+    blocks = std::max(1, blocks);
+    dev = d;
+    smem = bytes;
+    return blocks;
+  }
+};
+
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace om
@@ -377,7 +639,8 @@ bool norm_vec(const torch::Tensor& t) {
 // (y [..., D], h (x itself without delta), stats fp32 [M, 2])
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Tensor x, torch::Tensor w,
                                                                       c10::optional<torch::Tensor> b, double eps,
-                                                                      bool layer, c10::optional<torch::Tensor> delta) {
+                                                                      bool layer, c10::optional<torch::Tensor> delta,
+                                                                      torch::Tensor status) {
   const char* op = "norm_train";
   TORCH_CHECK(x.dim() >= 1 && x.is_cuda(), "norm_train: x must be a CUDA tensor [..., D]");
   const int64_t D = x.size(x.dim() - 1);
@@ -413,6 +676,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
   a.M = M;
   a.D = (int)std::min<int64_t>(D, INT32_MAX);
   a.eps = (float)eps;
+  a.status = status.data_ptr<int>();
   auto st = at::cuda::getCurrentCUDAStream().stream();
   om::norm_types(op, ty, wt, [&](auto t0, auto w0) {
     om::norm_shape(op, a.D, vec, [&](auto G, auto V, auto P) {
@@ -423,6 +687,29 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
       const long long blocks = (M + NT / g - 1) / (NT / g);
       TORCH_CHECK(blocks < (1ll << 31), "norm_train: too many rows");
       if (M == 0) return;
+      if constexpr (v == 8) {
+        constexpr int RPB = NT / g;
+        const size_t stage = (size_t)RPB * (delta.has_value() ? 2 : 1) * D * sizeof(T);
+        a.stages = om::ring_stages(stage);
+        if (a.stages >= 2) {
+          auto go = [&](auto kernel, om::Residents& res) {
+            const size_t smem = a.stages * stage;
+            const int grid = (int)std::min<long long>(blocks, om::num_sms() * res.get(kernel, NT, smem));
+            kernel<<<grid, NT, smem, st>>>(a);
+            OM_LAUNCH_CHECK();
+          };
+          static om::Residents res[4];
+          if (layer && a.delta)
+            go(om::norm_fwd_ring_kernel<T, W, true, true, g, p>, res[0]);
+          else if (layer)
+            go(om::norm_fwd_ring_kernel<T, W, true, false, g, p>, res[1]);
+          else if (a.delta)
+            go(om::norm_fwd_ring_kernel<T, W, false, true, g, p>, res[2]);
+          else
+            go(om::norm_fwd_ring_kernel<T, W, false, false, g, p>, res[3]);
+          return;
+        }
+      }
       if (layer)
         om::norm_fwd_kernel<T, W, true, g, v, p><<<(unsigned)blocks, NT, 0, st>>>(a);
       else
@@ -436,7 +723,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
 // (dx [..., D], dw [D], db [D] (LayerNorm with bias))
 std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_train_bwd(
     torch::Tensor dy, torch::Tensor h, torch::Tensor w, torch::Tensor stats, bool layer, bool bias,
-    c10::optional<torch::Tensor> dh) {
+    c10::optional<torch::Tensor> dh, torch::Tensor status) {
   const char* op = "norm_train_bwd";
   TORCH_CHECK(h.dim() >= 1 && h.is_cuda(), "norm_train_bwd: h must be a CUDA tensor [..., D]");
   const int64_t D = h.size(h.dim() - 1);
@@ -474,6 +761,7 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
   a.w = w2.data_ptr();
   a.dx = dx.data_ptr();
   a.stats = stats.data_ptr<float>();
+  a.status = status.data_ptr<int>();
   a.M = M;
   a.D = (int)std::min<int64_t>(D, INT32_MAX);
   const int n = layer ? 2 : 1;
@@ -484,16 +772,9 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
       using W = decltype(w0);
       constexpr int g = decltype(G)::value, v = decltype(V)::value, p = decltype(P)::value;
       constexpr int NT = om::norm_threads<g>(), RPB = NT / g;
-      auto go = [&](auto kernel, std::atomic<int>& resident) {
-        const size_t smem = RPB > 1 ? (size_t)a.D * sizeof(float) : 0;
-        int per_sm = resident.load();  // the same for every call of this instance (smem is at most 8 KB)
-        if (per_sm == 0) {
-          OM_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, NT, smem));
-          per_sm = std::max(1, per_sm);
-          resident.store(per_sm);
-        }
+      auto go = [&](auto kernel, om::Residents& res, size_t smem) {
         const long long most = (M + RPB - 1) / RPB;
-        const int blocks = (int)std::min<long long>(most, (long long)om::num_sms() * per_sm);
+        const int blocks = (int)std::min<long long>(most, om::num_sms() * res.get(kernel, NT, smem));
         auto part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());
         a.part = part.data_ptr<float>();
         kernel<<<blocks, NT, smem, st>>>(a);
@@ -503,11 +784,29 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
             bias ? reinterpret_cast<W*>(db->data_ptr()) : nullptr);
         OM_LAUNCH_CHECK();
       };
-      static std::atomic<int> resident[2];
+      const size_t joined = RPB > 1 ? (size_t)a.D * sizeof(float) : 0;
+      if constexpr (v == 8) {
+        const size_t stage = (size_t)RPB * (a.dh ? 3 : 2) * D * sizeof(T);
+        a.stages = om::ring_stages(stage);
+        if (a.stages >= 2) {
+          const size_t smem = std::max(a.stages * stage, joined);
+          static om::Residents res[4];
+          if (layer && a.dh)
+            go(om::norm_bwd_ring_kernel<T, W, true, true, g, p>, res[0], smem);
+          else if (layer)
+            go(om::norm_bwd_ring_kernel<T, W, true, false, g, p>, res[1], smem);
+          else if (a.dh)
+            go(om::norm_bwd_ring_kernel<T, W, false, true, g, p>, res[2], smem);
+          else
+            go(om::norm_bwd_ring_kernel<T, W, false, false, g, p>, res[3], smem);
+          return;
+        }
+      }
+      static om::Residents res[2];
       if (layer)
-        go(om::norm_bwd_kernel<T, W, true, g, v, p>, resident[1]);
+        go(om::norm_bwd_kernel<T, W, true, g, v, p>, res[1], joined);
       else
-        go(om::norm_bwd_kernel<T, W, false, g, v, p>, resident[0]);
+        go(om::norm_bwd_kernel<T, W, false, g, v, p>, res[0], joined);
     });
   });
   return {dx, dw, db};

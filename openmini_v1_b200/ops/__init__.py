@@ -382,7 +382,7 @@ def norm_train(x, w, b=None, eps=1e-5, kind="rms", delta=None):
         raise ValueError("norm_train: delta must be like x")
     if not x.is_cuda:
         return ref.norm_train(x, w, b, eps, kind, delta)
-    return _native.C().norm_train(x, w, b, eps, layer, delta)
+    return _native.C().norm_train(x, w, b, eps, layer, delta, ctx(x.device).status)
 
 
 def norm_train_bwd(dy, h, w, stats, kind="rms", bias=False, dh=None):
@@ -392,4 +392,4 @@ def norm_train_bwd(dy, h, w, stats, kind="rms", bias=False, dh=None):
     _same_device("norm_train_bwd", dy, h, w, stats, dh)
     if not h.is_cuda:
         return ref.norm_train_bwd(dy, h, w, stats, kind, bias, dh)
-    return _native.C().norm_train_bwd(dy, h, w, stats, layer, bias, dh)
+    return _native.C().norm_train_bwd(dy, h, w, stats, layer, bias, dh, ctx(h.device).status)

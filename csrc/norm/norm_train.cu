@@ -41,6 +41,10 @@ struct Vec {
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(u) / 4); ++i) u[i] = 0u;
   }
+  __device__ __forceinline__ uint64_t pair(int j) const {  // elements 2 j, 2 j + 1
+    if constexpr (sizeof(T) == 4) return pair_f32(__uint_as_float(u[2 * j]), __uint_as_float(u[2 * j + 1]));
+    return pair_f32(bf16lo(u[j]), bf16hi(u[j]));
+  }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(u[j]);
     return (j & 1) ? bf16hi(u[j >> 1]) : bf16lo(u[j >> 1]);
@@ -60,13 +64,38 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
   }
 }
 template <typename T>
+__device__ __forceinline__ void store_pairs(T* p, const uint64_t (&f)[4]) {
+  const float2 a = unpair_f32(f[0]), b = unpair_f32(f[1]), c = unpair_f32(f[2]), d = unpair_f32(f[3]);
+  if constexpr (sizeof(T) == 2) {
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y), pack_bf16x2(c.x, c.y), pack_bf16x2(d.x, d.y));
+  } else {
+    reinterpret_cast<float4*>(p)[0] = make_float4(a.x, a.y, b.x, b.y);
+    reinterpret_cast<float4*>(p)[1] = make_float4(c.x, c.y, d.x, d.y);
+  }
+}
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+  const float2 a = unpair_f32(v);
+  return a.x + a.y;
+}
+template <typename T>
+__device__ __forceinline__ uint64_t round_pair(uint64_t v) {
+  if constexpr (sizeof(T) == 2) {
+    const float2 a = unpair_f32(v);
+    const uint32_t u = pack_bf16x2(a.x, a.y);
+    return pair_f32(bf16lo(u), bf16hi(u));
+  }
+  return v;
+}
+template <typename T>
 __device__ __forceinline__ float round_to(float v) {
   if constexpr (sizeof(T) == 2) return __bfloat162float(__float2bfloat16_rn(v));
   return v;
 }
 
-// Sums of N values over the G threads of a row; `sh` has 2 * N * (threads / 32) floats and is
-// used by halves in turn (`flip`), so that one barrier a reduction is enough.
+// Sums of N values over the G threads of a row, which meet at a barrier of their own; `sh` has
+// 2 * N * (threads / 32) floats and is used by halves in turn (`flip`), so that one barrier a
+// reduction is enough.
 template <int G, int N>
 __device__ __forceinline__ void group_sum(float (&v)[N], float* sh, int& flip) {
 #pragma unroll
@@ -81,7 +110,10 @@ __device__ __forceinline__ void group_sum(float (&v)[N], float* sh, int& flip) {
 #pragma unroll
       for (int i = 0; i < N; ++i) s[i * warps + warp] = v[i];
     }
-    __syncthreads();
+    if (G == (int)blockDim.x)
+      __syncthreads();
+    else
+      named_bar_sync(1 + threadIdx.x / G, G);
     const int w0 = threadIdx.x / G * (G / 32);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -107,17 +139,23 @@ struct RowRing {
   long long ld[NA];
   int stages;
   uint32_t bytes;     // of a row
-  __device__ __forceinline__ void fill(int k, long long row) const {  // one thread
-    const int s = k % stages;
-    mbar_arrive_expect_tx(&full[s], NA * bytes);
+  int s;              // the stage in turn and the phase of its barrier
+  uint32_t phase;
+  __device__ __forceinline__ void fill(int stage, long long row) const {  // one thread
+    mbar_arrive_expect_tx(&full[stage], NA * bytes);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) bulk_load(base + (size_t)(s * NA + i) * bytes, src[i] + row * ld[i], bytes, &full[s]);
+    for (int i = 0; i < NA; ++i)
+      bulk_load(base + (size_t)(stage * NA + i) * bytes, src[i] + row * ld[i], bytes, &full[stage]);
   }
-  __device__ __forceinline__ bool wait(int k, int* status) const {
-    return mbar_wait(&full[k % stages], (k / stages) & 1, status, OM_ERR_WAIT_FULL);
+  __device__ __forceinline__ bool wait(int* status) const { return mbar_wait(&full[s], phase, status, OM_ERR_WAIT_FULL); }
+  __device__ __forceinline__ const T* row(int i) const {
+    return reinterpret_cast<const T*>(base + (size_t)(s * NA + i) * bytes);
   }
-  __device__ __forceinline__ const T* row(int k, int i) const {
-    return reinterpret_cast<const T*>(base + (size_t)((k % stages) * NA + i) * bytes);
+  __device__ __forceinline__ void next() {
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
   }
 };
 
@@ -205,6 +243,8 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const 
   const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
   RowRing<T, G, NA> ring;
   ring.stages = a.stages;
+  ring.s = 0;
+  ring.phase = 0;
   ring.bytes = a.D * sizeof(T);
   ring.base = ring_mem + (size_t)grp * a.stages * NA * ring.bytes;
   ring.full = bars + grp * RING_MAX;
@@ -220,23 +260,28 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const 
     for (int k = 0; k < a.stages; ++k)
       if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
   }
-  Vec<W, V> w[P], b[LAYER ? P : 1];
+  uint64_t w[P][4], b[LAYER ? P : 1][4];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int c = (lane + i * G) * V;
-    w[i].zero();
-    if (c < a.D) w[i].load(static_cast<const W*>(a.w) + c);
-    if constexpr (LAYER) {
-      b[i].zero();
-      if (a.b && c < a.D) b[i].load(static_cast<const W*>(a.b) + c);
+    Vec<W, V> wv, bv;
+    wv.zero();
+    bv.zero();
+    if (c < a.D) wv.load(static_cast<const W*>(a.w) + c);
+    if (LAYER && a.b && c < a.D) bv.load(static_cast<const W*>(a.b) + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[i][j] = wv.pair(j);
+      if constexpr (LAYER) b[i][j] = bv.pair(j);
     }
   }
   __syncthreads();
-  int flip = 0, k = 0;
-  for (long long base = row0; base < a.M; base += step, ++k) {
+  int flip = 0;
+  // every group takes the same number of turns
+  for (long long base = row0; base < a.M; base += step) {
     const long long row = base + grp;
-    const bool live = row < a.M && ring.wait(k, a.status);
-    float f[P][V], sum[1] = {0.f};
+    const bool live = row < a.M && ring.wait(a.status);
+    uint64_t f[P][4], acc = 0;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int c = (lane + i * G) * V;
@@ -244,30 +289,35 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const 
       v.zero();
       d.zero();
       if (live && c < a.D) {
-        v.load(ring.row(k, 0) + c);
-        if constexpr (DELTA) d.load(ring.row(k, 1) + c);
+        v.load(ring.row(0) + c);
+        if constexpr (DELTA) d.load(ring.row(1) + c);
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        f[i][j] = DELTA ? round_to<T>(v.get(j) + d.get(j)) : v.get(j);
-        sum[0] += LAYER ? f[i][j] : f[i][j] * f[i][j];
+      for (int j = 0; j < 4; ++j) {
+        f[i][j] = DELTA ? round_pair<T>(add_f32x2(v.pair(j), d.pair(j))) : v.pair(j);
+        acc = LAYER ? add_f32x2(acc, f[i][j]) : fma_f32x2(f[i][j], f[i][j], acc);
       }
-      if (DELTA && live && c < a.D) store_vec<T, V>(static_cast<T*>(a.h) + row * a.D + c, f[i]);
+      if (DELTA && live && c < a.D) store_pairs(static_cast<T*>(a.h) + row * a.D + c, f[i]);
     }
+    float sum[1] = {pair_sum(acc)};
     group_sum<G, 1>(sum, sh, flip);
     if constexpr (G == 32) __syncwarp();
-    if (lane == 0 && row + a.stages * step < a.M) ring.fill(k + a.stages, row + a.stages * step);
+    if (lane == 0 && row + a.stages * step < a.M) ring.fill(ring.s, row + a.stages * step);
+    ring.next();
     float mu = 0.f;
     if constexpr (LAYER) {
       mu = sum[0] / a.D;
-      sum[0] = 0.f;
+      acc = 0;
 #pragma unroll
-      for (int i = 0; i < P; ++i)
+      for (int i = 0; i < P; ++i) {
+        const bool in = (lane + i * G) * V < a.D;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float t = (lane + i * G) * V < a.D ? f[i][j] - mu : 0.f;
-          sum[0] += t * t;
+        for (int j = 0; j < 4; ++j) {
+          f[i][j] = add_f32x2(f[i][j], pair_f32(-mu, -mu));
+          if (in) acc = fma_f32x2(f[i][j], f[i][j], acc);
         }
+      }
+      sum[0] = pair_sum(acc);
       group_sum<G, 1>(sum, sh, flip);
     }
     if (!live) continue;
@@ -277,10 +327,13 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const 
     for (int i = 0; i < P; ++i) {
       const int c = (lane + i * G) * V;
       if (c >= a.D) continue;
-      float o[V];
+      uint64_t o[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = (f[i][j] - mu) * r * w[i].get(j) + (LAYER ? b[LAYER ? i : 0].get(j) : 0.f);
-      store_vec<T, V>(static_cast<T*>(a.y) + row * a.D + c, o);
+      for (int j = 0; j < 4; ++j) {
+        o[j] = mul_f32x2(f[i][j], pair_f32(r, r));
+        o[j] = LAYER ? fma_f32x2(o[j], w[i][j], b[LAYER ? i : 0][j]) : mul_f32x2(o[j], w[i][j]);
+      }
+      store_pairs(static_cast<T*>(a.y) + row * a.D + c, o);
     }
   }
 }
@@ -432,6 +485,8 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
   const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
   RowRing<T, G, NA> ring;
   ring.stages = a.stages;
+  ring.s = 0;
+  ring.phase = 0;
   ring.bytes = a.D * sizeof(T);
   ring.base = ring_mem + (size_t)grp * a.stages * NA * ring.bytes;
   ring.full = bars + grp * RING_MAX;
@@ -449,33 +504,31 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
     for (int k = 0; k < a.stages; ++k)
       if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
   }
-  float dw[P][V], db[LAYER ? P : 1][V];
-  Vec<W, V> w[P];
+  uint64_t dw2[P][4], db2[LAYER ? P : 1][4], w[P][4];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int c = (lane + i * G) * V;
-    w[i].zero();
-    if (c < a.D) w[i].load(static_cast<const W*>(a.w) + c);
+    Vec<W, V> wv;
+    wv.zero();
+    if (c < a.D) wv.load(static_cast<const W*>(a.w) + c);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      dw[i][j] = 0.f;
-      if constexpr (LAYER) db[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) {
+      w[i][j] = wv.pair(j);
+      dw2[i][j] = 0;
+      if constexpr (LAYER) db2[i][j] = 0;
     }
   }
   float2 next = make_float2(0.f, 0.f);
   if (row0 + grp < a.M) next = *reinterpret_cast<const float2*>(a.stats + 2 * (row0 + grp));
   __syncthreads();
-  int flip = 0, k = 0;
-  for (long long base = row0; base < a.M; base += step, ++k) {
+  int flip = 0;
+  for (long long base = row0; base < a.M; base += step) {
     const long long row = base + grp;
-    const bool live = row < a.M && ring.wait(k, a.status);
+    const bool live = row < a.M && ring.wait(a.status);
     const float mu = next.x, r = live ? next.y : 0.f;
     if (row + step < a.M) next = *reinterpret_cast<const float2*>(a.stats + 2 * (row + step));
-    float n[P][V], ga[P][V];
+    uint64_t n[P][4], ga[P][4], s0 = 0, s1 = 0;
     Vec<T, V> d[DH ? P : 1];
-    float s[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int c = (lane + i * G) * V;
@@ -484,38 +537,61 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
       yv.zero();
       if constexpr (DH) d[i].zero();
       if (live && c < a.D) {
-        hv.load(ring.row(k, 0) + c);
-        yv.load(ring.row(k, 1) + c);
-        if constexpr (DH) d[i].load(ring.row(k, 2) + c);
+        hv.load(ring.row(0) + c);
+        yv.load(ring.row(1) + c);
+        if constexpr (DH) d[i].load(ring.row(2) + c);
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float y = yv.get(j);
-        n[i][j] = (hv.get(j) - mu) * r;
-        ga[i][j] = y * w[i].get(j);  // 0 beyond the row's end: w and dy are 0 there
-        s[0] += ga[i][j] * n[i][j];
-        dw[i][j] += y * n[i][j];
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t y = yv.pair(j);
+        n[i][j] = LAYER ? add_f32x2(hv.pair(j), pair_f32(-mu, -mu)) : hv.pair(j);
+        n[i][j] = mul_f32x2(n[i][j], pair_f32(r, r));
+        ga[i][j] = mul_f32x2(y, w[i][j]);  // 0 beyond the row's end: w and dy are 0 there
+        s0 = fma_f32x2(ga[i][j], n[i][j], s0);
+        dw2[i][j] = fma_f32x2(y, n[i][j], dw2[i][j]);
         if constexpr (LAYER) {
-          s[N - 1] += ga[i][j];
-          db[i][j] += y;
+          s1 = add_f32x2(s1, ga[i][j]);
+          db2[i][j] = add_f32x2(db2[i][j], y);
         }
       }
     }
+    float s[N];
+    s[0] = pair_sum(s0);
+    if constexpr (LAYER) s[N - 1] = pair_sum(s1);
     group_sum<G, N>(s, sh, flip);
     if constexpr (G == 32) __syncwarp();
-    if (lane == 0 && row + a.stages * step < a.M) ring.fill(k + a.stages, row + a.stages * step);
+    if (lane == 0 && row + a.stages * step < a.M) ring.fill(ring.s, row + a.stages * step);
+    ring.next();
     if (!live) continue;  // no barrier below
-    const float c1 = s[0] / a.D, c2 = LAYER ? s[N - 1] / a.D : 0.f;
+    const float c1 = -s[0] / a.D, c2 = LAYER ? -s[N - 1] / a.D : 0.f;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int c = (lane + i * G) * V;
       if (c >= a.D) continue;
-      float o[V];
+      uint64_t o[4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = r * (ga[i][j] - n[i][j] * c1 - c2) + (DH ? d[DH ? i : 0].get(j) : 0.f);
-      store_vec<T, V>(static_cast<T*>(a.dx) + row * a.D + c, o);
+      for (int j = 0; j < 4; ++j) {
+        o[j] = fma_f32x2(n[i][j], pair_f32(c1, c1), ga[i][j]);
+        if constexpr (LAYER) o[j] = add_f32x2(o[j], pair_f32(c2, c2));
+        o[j] = DH ? fma_f32x2(o[j], pair_f32(r, r), d[DH ? i : 0].pair(j)) : mul_f32x2(o[j], pair_f32(r, r));
+      }
+      store_pairs(static_cast<T*>(a.dx) + row * a.D + c, o);
     }
   }
+  float dw[P][V], db[LAYER ? P : 1][V];
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = unpair_f32(dw2[i][j]);
+      dw[i][2 * j] = t.x;
+      dw[i][2 * j + 1] = t.y;
+      if constexpr (LAYER) {
+        const float2 q = unpair_f32(db2[LAYER ? i : 0][j]);
+        db[i][2 * j] = q.x;
+        db[i][2 * j + 1] = q.y;
+      }
+    }
   __syncthreads();  // every copy has been waited for and read: the ring's memory is free
   write_partials<G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }

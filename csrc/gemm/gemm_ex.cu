@@ -14,6 +14,7 @@ __global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __rest
     const int c = (int)(i - r * nv) * 4;
     if (c >= cols) continue;
     float4 a = *reinterpret_cast<const float4*>(P + r * ldacc + c);
+#pragma unroll 8
     for (int s = 1; s < splits; ++s) {
       const float4 b = *reinterpret_cast<const float4*>(P + s * plane + r * ldacc + c);
       a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
@@ -34,11 +35,21 @@ __global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __rest
 GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
   const int sms = num_sms();
   const int64_t tr = ceil_div(rows, 128);
-  GxPlan p;
-  // 128 x 256 tiles feed the tensor cores best; half as wide ones where those would not fill the SMs
-  p.bn = cols <= 128 || tr * ceil_div(cols, 256) < sms ? 128 : 256;
-  const int64_t tiles = tr * ceil_div(cols, p.bn);
   const int kb = ceil_div(K, 64);
+  // The launch lasts as long as its fullest SM: waves of tiles x the time of one. A 128-wide tile
+  // takes 64 of the MMA's cycles a step, a 192-wide one 96 and a 256-wide one 128; shared memory
+  // (A is read again for each) leaves the narrow ones 4 and 2 % behind.
+  GxPlan p{256, 1};
+  double best = 1e300;
+  for (int bn : {256, 192, 128}) {
+    const int64_t tiles = tr * ceil_div(cols, bn);
+    const double t = (double)ceil_div(tiles, sms) * bn * (bn == 128 ? 1.04 : bn == 192 ? 1.02 : 1.0);
+    if (t < best) {
+      best = t;
+      p.bn = bn;
+    }
+  }
+  const int64_t tiles = tr * ceil_div(cols, p.bn);
   // a split has to be worth its fp32 plane (written and read once): 8 steps of 64 at least
   int s = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
   const int per = ceil_div(kb, s);
@@ -50,9 +61,32 @@ int64_t gx_acc_floats(const GxPlan& p, int64_t rows, int64_t cols, bool pieces) 
   return p.splits > 1 || pieces ? (int64_t)p.splits * rows * ceil_div(cols, 32) * 32 : 0;
 }
 
-template <int BN>
-static void product_bn(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
-                       const EpiStore::Args& e, int* status, cudaStream_t st) {
+template <int BN, class Epi>
+static void product_bn(GxOperand a, GxOperand b, const OutMaps& o, GemmX g, const typename Epi::Args& e, int64_t K,
+                       cudaStream_t st) {
+  g.tiles_c = ceil_div(g.cols, BN);
+  const CUtensorMap ta = gx_map(a.p, a.mn, g.rows, K, a.ld, 128);
+  const CUtensorMap tb = gx_map(b.p, true, g.cols, K, b.ld, 64);
+  if (a.mn)
+    gx_launch<BN, true, true, Epi>(ta, tb, o, g, e, st);
+  else
+    gx_launch<BN, false, true, Epi>(ta, tb, o, g, e, st);
+}
+
+template <class Epi>
+static void product(int bn, GxOperand a, GxOperand b, const OutMaps& o, const GemmX& g, const typename Epi::Args& e,
+                    int64_t K, cudaStream_t st) {
+  if (bn == 128)
+    product_bn<128, Epi>(a, b, o, g, e, K, st);
+  else if (bn == 192)
+    product_bn<192, Epi>(a, b, o, g, e, K, st);
+  else
+    product_bn<256, Epi>(a, b, o, g, e, K, st);
+}
+
+void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
+                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st) {
+  TORCH_CHECK(b.mn, "gx_product: B is MN-major");
   GemmX g{};
   g.rows = (int)rows;
   g.cols = (int)cols;
@@ -61,40 +95,23 @@ static void product_bn(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, 
   // a piece shorter than the planned one may have fewer splits: the planes it leaves out keep
   // the sums of the pieces before it (the first piece is never shorter than the plan's K)
   g.splits = ceil_div(g.num_kb, g.kb_per_split);
-  TORCH_CHECK(e.add || g.splits == p.splits, "gx_product: the first piece is shorter than planned");
+  TORCH_CHECK(!first || g.splits == p.splits, "gx_product: the first piece is shorter than planned");
   g.tiles_r = ceil_div(rows, 128);
-  g.tiles_c = ceil_div(cols, BN);
-  g.b_step = BN;
-  g.b_second = BN / 2;
   g.status = status;
-  const CUtensorMap ta = gx_map(a.p, a.mn, rows, K, a.ld, 128);
-  const CUtensorMap tb = gx_map(b.p, b.mn, cols, K, b.ld, BN / 2);
-  TORCH_CHECK(b.mn, "gx_product: B is MN-major");
-  if (a.mn)
-    gx_launch<BN, true, true, EpiStore>(ta, tb, g, e, st);
-  else
-    gx_launch<BN, false, true, EpiStore>(ta, tb, g, e, st);
-}
-
-void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
-                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st) {
-  EpiStore::Args e{};
-  e.out = out;
-  e.ldo = (int)ldo;
-  e.vec = ldo % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  const bool direct = p.splits == 1 && first && last;
-  e.acc = direct ? nullptr : acc;
-  e.ldacc = ceil_div(cols, 32) * 32;
-  e.add = !first;
-  e.last = last && p.splits == 1;
-  if (p.bn == 128)
-    product_bn<128>(p, a, b, rows, cols, K, e, status, st);
-  else
-    product_bn<256>(p, a, b, rows, cols, K, e, status, st);
-  if (last && p.splits > 1) {
-    const long long work = (long long)rows * (e.ldacc / 4);
+  OutMaps o{};
+  if (p.splits == 1 && first && last) {
+    o.m[0] = gx_out(out, rows, cols, ldo);
+    product<EpiStore>(p.bn, a, b, o, g, {}, K, st);
+    return;
+  }
+  const int ldacc = ceil_div(cols, 32) * 32;
+  o.m[0] = make_tmap_3d(acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, rows, p.splits, ldacc,
+                        (uint64_t)rows * ldacc, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B);
+  product<EpiSum>(p.bn, a, b, o, g, {first ? 0 : 1}, K, st);
+  if (last) {
+    const long long work = (long long)rows * (ldacc / 4);
     const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)num_sms() * 8);
-    planes_to_bf16_kernel<<<blocks, 256, 0, st>>>(acc, p.splits, rows, (int)cols, e.ldacc, out, ldo,
+    planes_to_bf16_kernel<<<blocks, 256, 0, st>>>(acc, p.splits, rows, (int)cols, ldacc, out, ldo,
                                                   ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0);
     OM_LAUNCH_CHECK();
   }

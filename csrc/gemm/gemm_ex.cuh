@@ -17,8 +17,15 @@
 // 128 cycles), so the tensor pipe, not shared memory, is the limit for BN = 256; BN = 64 and
 // 128 are for grids that would otherwise leave SMs idle.
 //
+// Results leave through shared memory: an epilogue warp lays 32 rows x 128 bytes into one of its
+// two 4 KB buffers (128-byte swizzle, no bank conflicts) and a TMA store writes whole lines, while
+// the warp goes on with the next columns. Direct 16-byte stores, one row a lane, touch 32 lines an
+// instruction; they remain for outputs whose rows do not start on 16 bytes.
+//
 // Epi is a functor type with Args and
-//   static void tile(const GemmX&, const Args&, uint32_t tbase, int r, int tc, int sp)
+//   static Row row(const GemmX&, const Args&, int r)
+//   template <int BN> static void tile(const GemmX&, const Args&, const Row&, const OutMaps&, RowStage&,
+//                                      uint32_t tbase, int r, int tc, int sp)
 // called by every epilogue thread (accumulator row r, TMEM lane address tbase).
 #pragma once
 #include <cuda.h>
@@ -34,6 +41,51 @@ struct GemmX {
   int b_step;        // rows of B per column tile (K-major B): BN, or BN / 2 for a gated pair
   int b_second;      // distance of the second half's rows (K-major B): BN / 2, or F
   int* status;
+};
+
+struct OutMaps {
+  CUtensorMap m[3];  // what an Epi stores through; unused ones are zero
+};
+
+// The two buffers of one epilogue warp, used in turn.
+struct RowStage {
+  uint8_t* base;  // 2 x 4096 bytes, 1024-byte aligned
+  int lane, turn;
+  __device__ __forceinline__ uint8_t* begin() {  // a buffer whose last store has been read
+    if (lane == 0) bulk_wait_read<1>();
+    __syncwarp();
+    uint8_t* b = base + turn * 4096;
+    turn ^= 1;
+    return b;
+  }
+  // 32 bf16 columns into half `h` of the lane's 64-column row / 32 fp32 columns
+  __device__ __forceinline__ void put(uint8_t* b, int h, const float (&f)[32]) const {
+    const uint32_t row = smem_u32(b) + lane * 128;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sts128(row + (((h * 4 + j) ^ (lane & 7)) << 4), pack8(f + 8 * j));
+  }
+  // 32 bf16 columns as rows of 64 bytes (64-byte swizzle)
+  __device__ __forceinline__ void put32(uint8_t* b, const float (&f)[32]) const {
+    const uint32_t row = smem_u32(b) + lane * 64;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sts128(row + ((j ^ ((lane >> 1) & 3)) << 4), pack8(f + 8 * j));
+  }
+  __device__ __forceinline__ void put_f32(uint8_t* b, const float (&f)[32]) const {
+    const uint32_t row = smem_u32(b) + lane * 128;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      sts128(row + ((j ^ (lane & 7)) << 4), make_uint4(__float_as_uint(f[4 * j]), __float_as_uint(f[4 * j + 1]),
+                                                       __float_as_uint(f[4 * j + 2]), __float_as_uint(f[4 * j + 3])));
+  }
+  template <class F>
+  __device__ __forceinline__ void end(F&& store) const {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      store();
+      bulk_commit();
+    }
+  }
 };
 
 constexpr int GX_GROUP = 16;  // row tiles walked before the next column tile: 16 x 9 tiles in flight share L2 lines
@@ -60,19 +112,21 @@ struct GemmXCfg {
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = BN * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (200 * 1024) / STAGE_BYTES > 8 ? 8 : (200 * 1024) / STAGE_BYTES;
-  static constexpr int TMEM_COLS = 2 * BN;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align slack*/ + 256;
+  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES > 8 ? 8 : (192 * 1024) / STAGE_BYTES;
+  static constexpr int TMEM_COLS = BN <= 128 ? 2 * BN : 512;  // a power of two
+  static constexpr int OUT_BYTES = 4 * 2 * 4096;  // four epilogue warps
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 /*align slack*/ + 256;
 };
 
 template <int BN, bool AMN, bool BMN, class Epi>
 __global__ void __launch_bounds__(256, 1)
-    gemm_ex_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const GemmX g,
-                   const typename Epi::Args e) {
+    gemm_ex_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ OutMaps outs, const GemmX g, const typename Epi::Args e) {
   using C = GemmXCfg<BN>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE_BYTES);
+  uint8_t* out_bytes = smem + C::STAGES * C::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_bytes + C::OUT_BYTES);
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 2;
@@ -170,17 +224,22 @@ __global__ void __launch_bounds__(256, 1)
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
     const int q = warp & 3;
+    RowStage stage{out_bytes + q * 8192, lane, 0};
     int local = 0;
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++local) {
       int tr, tc, sp;
       gx_coords(g, u, tr, tc, sp);
       const int acc = local & 1;
-      if (!mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM)) break;
+      const int r = tr * 128 + q * 32 + lane;
+      const auto row = Epi::row(g, e, r);  // the row's own inputs, read while the products run
+      bool ok = mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      Epi::template tile<BN>(g, e, tmem + ((uint32_t)(q * 32) << 16) + acc * BN, tr * 128 + q * 32 + lane, tc, sp);
+      Epi::template tile<BN>(g, e, row, outs, stage, tmem + ((uint32_t)(q * 32) << 16) + acc * BN, r, tc, sp);
       tc_fence_before();
       mbar_arrive(&tempty[acc]);
     }
+    if (lane == 0) bulk_wait<0>();  // the stores are complete before the CTA's memory goes
   }
 
   tc_fence_before();
@@ -203,45 +262,64 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const float (&f)
   }
 }
 
-// Plain result: bf16 rows, or fp32 sums that several launches (pieces of a long contraction)
-// and splits add up. A piece adds to what the launch before it left: no atomics, one order.
+struct NoRow {};
+
+// bf16 rows through map 0, 64 columns a store.
 struct EpiStore {
-  struct Args {
-    __nv_bfloat16* out;
-    int ldo, vec;
-    float* acc;        // [splits][rows][ldacc] fp32, ldacc a multiple of 32; null: straight to out
-    int ldacc;
-    int add, last;     // add: acc holds earlier pieces; last: write out instead of acc (splits == 1)
-  };
+  struct Args {};
+  static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, uint32_t tbase, int r, int tc, int sp) {
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args&, const NoRow&, const OutMaps& o,
+                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
+#pragma unroll 1
+    for (int cc = 0; cc < BN / 64; ++cc) {
+      const int c0 = tc * BN + cc * 64;
+      if (c0 >= g.cols || r - st.lane >= g.rows) break;  // the same for the whole warp
+      uint8_t* b = st.begin();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tbase + cc * 64 + h * 32, v);
+        tc_wait_ld();
+        float f[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+        st.put(b, h, f);
+      }
+      st.end([&] { tma_store_2d(&o.m[0], b, c0, r - st.lane); });
+    }
+  }
+};
+
+// fp32 sums [splits][rows][cols] through map 0: pieces of a long contraction (`add`: launches after
+// the first) and splits are added up here. Every element has one writer a launch, so the order of
+// the sum is the launches' order.
+struct EpiSum {
+  struct Args {
+    int add;
+  };
+  static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
+  template <int BN>
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const NoRow&, const OutMaps& o,
+                                              RowStage& st, uint32_t tbase, int r, int tc, int sp) {
 #pragma unroll 1
     for (int cc = 0; cc < BN / 32; ++cc) {
       const int c0 = tc * BN + cc * 32;
-      if (c0 >= g.cols) break;  // the same for the whole warp
+      if (c0 >= g.cols || r - st.lane >= g.rows) break;
+      uint8_t* b = st.begin();
       uint32_t v[32];
       tmem_ld_32x32b_x32(tbase + cc * 32, v);
       tc_wait_ld();
-      if (r >= g.rows) continue;
       float f[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-      if (e.acc != nullptr) {
-        float4* a = reinterpret_cast<float4*>(e.acc + ((size_t)sp * g.rows + r) * e.ldacc + c0);
-        if (e.add) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 o = a[j];
-            f[4 * j] += o.x; f[4 * j + 1] += o.y; f[4 * j + 2] += o.z; f[4 * j + 3] += o.w;
-          }
-        }
-        if (!e.last) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) a[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-          continue;
-        }
-      }
-      store_row32(e.out + (size_t)r * e.ldo + c0, f, g.cols - c0, e.vec);
+      st.put_f32(b, f);
+      st.end([&] {
+        if (e.add)
+          tma_add_3d(&o.m[0], b, c0, r - st.lane, sp);
+        else
+          tma_store_3d(&o.m[0], b, c0, r - st.lane, sp);
+      });
     }
   }
 };

@@ -15,9 +15,24 @@ inline CUtensorMap gx_map(const void* p, bool mn, uint64_t rows, uint64_t K, uin
             : make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, K, rows, ld, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Output maps of RowStage: boxes of 32 rows x 128 bytes. Rows start on 16 bytes.
+inline bool gx_storable(const void* p, int64_t ld, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * bytes % 16 == 0;
+}
+inline CUtensorMap gx_out(__nv_bfloat16* p, uint64_t rows, uint64_t cols, uint64_t ld) {
+  return make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, cols, rows, ld, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// 32 columns a store (RowStage::put32)
+inline CUtensorMap gx_out32(__nv_bfloat16* p, uint64_t rows, uint64_t cols, uint64_t ld) {
+  return make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+inline CUtensorMap gx_out(float* p, uint64_t rows, uint64_t cols, uint64_t ld) {
+  return make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 template <int BN, bool AMN, bool BMN, class Epi>
-void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmX& g, const typename Epi::Args& e,
-               cudaStream_t st) {
+void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs, const GemmX& g,
+               const typename Epi::Args& e, cudaStream_t st) {
   using C = GemmXCfg<BN>;
   static std::atomic<bool> attr_set[64];
   int dev;
@@ -30,7 +45,7 @@ void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const GemmX& g, con
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 31), "gemm: too many tiles");
   const int grid = (int)std::min<long long>(units, num_sms());
-  gemm_ex_kernel<BN, AMN, BMN, Epi><<<grid, 256, C::SMEM_BYTES, st>>>(ta, tb, g, e);
+  gemm_ex_kernel<BN, AMN, BMN, Epi><<<grid, 256, C::SMEM_BYTES, st>>>(ta, tb, outs, g, e);
   OM_LAUNCH_CHECK();
 }
 

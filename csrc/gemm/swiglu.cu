@@ -35,27 +35,27 @@ __device__ __forceinline__ void store_row32(float* dst, const float (&f)[32], in
   }
 }
 
+// Maps: 0 h, 1 g, 2 u (`maps`: all that is written has one; else plain stores).
 struct EpiSwiglu {
   struct Args {
     __nv_bfloat16* h;
     float* gu;  // optional [M, ldgu]: g at column f, u at column F + f
-    int ldh, ldgu, vec_h, vec_gu;
+    int ldh, ldgu, vec_h, vec_gu, maps;
   };
+  static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, uint32_t tbase, int r, int tc, int) {
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const NoRow&, const OutMaps& o,
+                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
     constexpr int HALF = BN / 2;
-    constexpr int CH = HALF < 32 ? HALF : 32;
-    const int F = g.cols;
+    const int F = g.cols, r0 = r - st.lane;
 #pragma unroll 1
-    for (int cc = 0; cc < HALF / CH; ++cc) {
-      const int c0 = tc * HALF + cc * CH;
-      if (c0 >= F) break;
+    for (int cc = 0; cc < HALF / 32; ++cc) {
+      const int c0 = tc * HALF + cc * 32;
+      if (c0 >= F || r0 >= g.rows) break;
       uint32_t gv[32], uv[32];
-      tmem_ld_32x32b_x32(tbase + cc * CH, gv);
-      tmem_ld_32x32b_x32(tbase + HALF + cc * CH, uv);
+      tmem_ld_32x32b_x32(tbase + cc * 32, gv);
+      tmem_ld_32x32b_x32(tbase + HALF + cc * 32, uv);
       tc_wait_ld();
-      if (r >= g.rows) continue;
-      const int n = min(CH, F - c0);
       float gf[32], uf[32], hf[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
@@ -63,6 +63,22 @@ struct EpiSwiglu {
         uf[j] = __uint_as_float(uv[j]);
         hf[j] = gf[j] * sigmoid_f(gf[j]) * uf[j];
       }
+      if (HALF >= 64 && e.maps) {
+        if (e.gu != nullptr) {
+          uint8_t* b = st.begin();
+          st.put_f32(b, gf);
+          st.end([&] { tma_store_2d(&o.m[1], b, c0, r0); });
+          b = st.begin();
+          st.put_f32(b, uf);
+          st.end([&] { tma_store_2d(&o.m[2], b, c0, r0); });
+        }
+        uint8_t* b = st.begin();
+        st.put32(b, hf);
+        st.end([&] { tma_store_2d(&o.m[0], b, c0, r0); });
+        continue;
+      }
+      if (r >= g.rows) continue;
+      const int n = min(32, F - c0);
       store_row32(e.h + (size_t)r * e.ldh + c0, hf, n, e.vec_h);
       if (e.gu != nullptr) {
         store_row32(e.gu + (size_t)r * e.ldgu + c0, gf, n, e.vec_gu);
@@ -115,12 +131,12 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restric
 }
 
 template <int BN>
-static void swiglu_fwd_bn(const CUtensorMap& ta, const void* w, int64_t ldw, GemmX g, const EpiSwiglu::Args& e,
-                          int64_t F, int64_t K, cudaStream_t st) {
+static void swiglu_fwd_bn(const CUtensorMap& ta, const void* w, int64_t ldw, const OutMaps& o, GemmX g,
+                          const EpiSwiglu::Args& e, int64_t F, int64_t K, cudaStream_t st) {
   g.tiles_c = ceil_div(F, BN / 2);
   g.b_step = BN / 2;
   g.b_second = (int)F;
-  gx_launch<BN, false, false, EpiSwiglu>(ta, gx_map(w, false, 2 * F, K, ldw, BN / 2), g, e, st);
+  gx_launch<BN, false, false, EpiSwiglu>(ta, gx_map(w, false, 2 * F, K, ldw, BN / 2), o, g, e, st);
 }
 
 }  // namespace om
@@ -174,10 +190,20 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
   g.status = status.data_ptr<int>();
   const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), 128);
   // 128 features a tile once those tiles fill the SMs; fewer tiles than SMs: 32 features a tile
-  if ((int64_t)g.tiles_r * om::ceil_div(F, 128) >= om::num_sms())
-    om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), g, e, F, K, st);
-  else
-    om::swiglu_fwd_bn<64>(ta, w2.data_ptr(), w2.stride(0), g, e, F, K, st);
+  om::OutMaps o{};
+  if ((int64_t)g.tiles_r * om::ceil_div(F, 128) >= om::num_sms()) {
+    e.maps = om::gx_storable(e.h, F, 2);  // F a multiple of 8: every row of h, g and u starts on 16 bytes
+    if (e.maps) {
+      o.m[0] = om::gx_out32(e.h, M, F, F);
+      if (save) {
+        o.m[1] = om::gx_out(e.gu, M, F, 2 * F);
+        o.m[2] = om::gx_out(e.gu + F, M, F, 2 * F);
+      }
+    }
+    om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+  } else {
+    om::swiglu_fwd_bn<64>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+  }
   return {h, gu};
 }
 

@@ -43,16 +43,17 @@ struct EpiXentFwd {
     float* sumz;    // [tiles_c][M] sums of z (SMOOTH)
     float* zt;      // [M] z of the target, -inf if masked
   };
+  static __device__ __forceinline__ long long row(const GemmX& g, const Args& e, int r) {
+    return r < g.rows ? e.x.targets[r] : -1;
+  }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, uint32_t tbase, int r, int tc, int) {
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const long long& target, const OutMaps&,
+                                              RowStage&, uint32_t tbase, int r, int tc, int) {
     const bool row = r < g.rows;
     const int t0 = tc * BN;
     // the target's column within this tile, or a value no column has
-    int tcol = -1;
-    if (row) {
-      const long long t = e.x.targets[r] - t0;
-      tcol = t >= 0 && t < BN ? (int)t : -1;
-    }
+    const long long in = target - t0;
+    const int tcol = target >= 0 && in >= 0 && in < BN ? (int)in : -1;
     const float c2 = e.x.scale * XE_LOG2E;
     float m = -INFINITY, s = 0.f, zs = 0.f;
 #pragma unroll 1
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
   loss[r] = out;
 }
 
-// dz of one vocabulary piece, 16 bits.
+// dz of one vocabulary piece, 16 bits, through map 0 ([M, piece], rows a multiple of 64 bytes).
 struct EpiXentBwd {
   struct Args {
     XentRows x;
@@ -162,52 +163,58 @@ struct EpiXentBwd {
     const float* dloss;  // [M]
     float smoothing;
     int v0;              // the piece's first column
-    __nv_bfloat16* dz;   // [M, ld], ld a multiple of 32
-    int ld;
   };
+  struct Row {
+    float gz, l2;  // c gloss (0: ignored), lse log2 e
+    int tcol;      // the target's column in the piece, or -1
+  };
+  static __device__ __forceinline__ Row row(const GemmX& g, const Args& e, int r) {
+    Row o{0.f, 0.f, -1};
+    if (r >= g.rows) return o;
+    const long long t = e.x.targets[r];
+    if (t < 0 || t >= e.x.V || t == e.x.ignore) return o;
+    o.gz = e.dloss[r] * e.x.scale;
+    o.l2 = e.lse[r] * XE_LOG2E;
+    if (t >= e.v0 && t < e.v0 + (long long)g.cols) o.tcol = (int)(t - e.v0);
+    return o;
+  }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, uint32_t tbase, int r, int tc, int) {
-    const int t0 = tc * BN;
-    float gz = 0.f, l2 = 0.f;
-    int tcol = -1;
-    if (r < g.rows) {
-      const long long t = e.x.targets[r];
-      if (t >= 0 && t < e.x.V && t != e.x.ignore) {
-        gz = e.dloss[r] * e.x.scale;
-        l2 = e.lse[r] * XE_LOG2E;
-        const long long tt = t - e.v0 - t0;
-        tcol = tt >= 0 && tt < BN ? (int)tt : -1;
-      }
-    }
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const Row& w, const OutMaps& o,
+                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
     const float c2 = e.x.scale * XE_LOG2E;
     const float base = e.smoothing / (float)e.x.V;
 #pragma unroll 1
-    for (int cc = 0; cc < BN / 32; ++cc) {
-      const int c0 = t0 + cc * 32;
-      if (c0 >= g.cols) break;
-      uint32_t v[32];
-      tmem_ld_32x32b_x32(tbase + cc * 32, v);
-      uint32_t bits = 0xffffffffu;
-      if (e.x.keep != nullptr && r < g.rows) bits = (uint32_t)e.x.keep[r * e.x.ldk + ((e.v0 + c0) >> 5)];
-      tc_wait_ld();
-      if (r >= g.rows) continue;
-      float f[32];
-      if (gz == 0.f) {  // an ignored row: nothing, whatever its logits are
+    for (int cc = 0; cc < BN / 64; ++cc) {
+      const int c64 = tc * BN + cc * 64;
+      if (c64 >= g.cols || r - st.lane >= g.rows) break;
+      uint8_t* b = st.begin();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = 0.f;
-      } else {
+      for (int h = 0; h < 2; ++h) {
+        const int c0 = c64 + h * 32;
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(tbase + cc * 64 + h * 32, v);
+        uint32_t bits = 0xffffffffu;
+        if (e.x.keep != nullptr && r < g.rows && c0 < g.cols)
+          bits = (uint32_t)e.x.keep[r * e.x.ldk + ((e.v0 + c0) >> 5)];
+        tc_wait_ld();
+        float f[32];
+        if (w.gz == 0.f) {  // an ignored row: nothing, whatever its logits are
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = fast_exp2(__uint_as_float(v[j]) * c2 - l2) - base;
-        if ((tcol >> 5) == cc) {
+          for (int j = 0; j < 32; ++j) f[j] = 0.f;
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j == (tcol & 31)) f[j] -= 1.f - e.smoothing;
+          for (int j = 0; j < 32; ++j) f[j] = fast_exp2(__uint_as_float(v[j]) * c2 - w.l2) - base;
+          if ((w.tcol >> 5) == (c0 >> 5)) {  // tcol = -1 matches no column
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == (w.tcol & 31)) f[j] -= 1.f - e.smoothing;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? f[j] * w.gz : 0.f;
         }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? f[j] * gz : 0.f;
+        st.put(b, h, f);
       }
-      // ld is a multiple of 32 and the workspace has whole rows: a short last chunk may fill its row's end
-      store_row32(e.dz + (size_t)r * e.ld + c0, f, 32, true);
+      st.end([&] { tma_store_2d(&o.m[0], b, c64, r - st.lane); });
     }
   }
 };
@@ -299,7 +306,7 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
   auto run = [&](auto epi) {
     using E = decltype(epi);
     typename E::Args e{in.rows, reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n};
-    om::gx_launch<256, false, false, E>(ta, tb, g, e, st);
+    om::gx_launch<256, false, false, E>(ta, tb, om::OutMaps{}, g, e, st);
   };
   if (smooth)
     run(om::EpiXentFwd<true>{});
@@ -351,9 +358,11 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_
     const int64_t n = std::min(C, V - v0);
     const __nv_bfloat16* wv = ptr(in.w) + v0 * in.w.stride(0);
     const om::GemmX g = xent_gemm(in, n, status.data_ptr<int>());
-    om::EpiXentBwd::Args e{in.rows, lse.data_ptr<float>(), dloss.data_ptr<float>(), (float)smoothing, (int)v0,
-                           ptr(dz), (int)ld};
-    om::gx_launch<256, false, false, om::EpiXentBwd>(ta, om::gx_map(wv, false, n, K, in.w.stride(0), 128), g, e, st);
+    const om::EpiXentBwd::Args e{in.rows, lse.data_ptr<float>(), dloss.data_ptr<float>(), (float)smoothing, (int)v0};
+    om::OutMaps o{};
+    o.m[0] = om::gx_out(ptr(dz), M, n, ld);
+    om::gx_launch<256, false, false, om::EpiXentBwd>(ta, om::gx_map(wv, false, n, K, in.w.stride(0), 128), o, g, e,
+                                                     st);
     if (need_dx)
       om::gx_product(px, {dz.data_ptr(), false, ld}, {wv, true, in.w.stride(0)}, M, K, n, ptr(*dx), K, ax, v0 == 0,
                      v0 + n == V, g.status, st);

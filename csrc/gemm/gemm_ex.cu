@@ -39,7 +39,11 @@ GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
   // The launch lasts as long as its fullest SM: waves of tiles x the time of one. A 128-wide tile
   // takes 64 of the MMA's cycles a step, a 192-wide one 96 and a 256-wide one 128; shared memory
   // (A is read again for each) leaves the narrow ones 4 and 2 % behind.
-  GxPlan p{256, 1};
+  GxPlan p{256, 1, 0};
+  if (gx_pairs(rows, cols)) {
+    p.pair = 1;
+    return p;
+  }
   double best = 1e300;
   for (int bn : {256, 192, 128}) {
     const int64_t tiles = tr * ceil_div(cols, bn);
@@ -74,11 +78,26 @@ static void product_bn(GxOperand a, GxOperand b, const OutMaps& o, GemmX g, cons
 }
 
 template <class Epi>
-static void product(int bn, GxOperand a, GxOperand b, const OutMaps& o, const GemmX& g, const typename Epi::Args& e,
-                    int64_t K, cudaStream_t st) {
-  if (bn == 128)
+static void product_pair(GxOperand a, GxOperand b, const OutMaps& o, GemmX g, const typename Epi::Args& e, int64_t K,
+                         cudaStream_t st) {
+  g.tiles_r = ceil_div(g.rows, 256);
+  g.tiles_c = ceil_div(g.cols, 256);
+  const CUtensorMap ta = gx_map(a.p, a.mn, g.rows, K, a.ld, 128);
+  const CUtensorMap tb = gx_map(b.p, true, g.cols, K, b.ld, 64);
+  if (a.mn)
+    gx_launch_pair<true, true, Epi>(ta, tb, o, g, e, st);
+  else
+    gx_launch_pair<false, true, Epi>(ta, tb, o, g, e, st);
+}
+
+template <class Epi>
+static void product(const GxPlan& p, GxOperand a, GxOperand b, const OutMaps& o, const GemmX& g,
+                    const typename Epi::Args& e, int64_t K, cudaStream_t st) {
+  if (p.pair)
+    product_pair<Epi>(a, b, o, g, e, K, st);
+  else if (p.bn == 128)
     product_bn<128, Epi>(a, b, o, g, e, K, st);
-  else if (bn == 192)
+  else if (p.bn == 192)
     product_bn<192, Epi>(a, b, o, g, e, K, st);
   else
     product_bn<256, Epi>(a, b, o, g, e, K, st);
@@ -101,13 +120,13 @@ void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t
   OutMaps o{};
   if (p.splits == 1 && first && last) {
     o.m[0] = gx_out(out, rows, cols, ldo);
-    product<EpiStore>(p.bn, a, b, o, g, {}, K, st);
+    product<EpiStore>(p, a, b, o, g, {}, K, st);
     return;
   }
   const int ldacc = ceil_div(cols, 32) * 32;
   o.m[0] = make_tmap_3d(acc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, rows, p.splits, ldacc,
                         (uint64_t)rows * ldacc, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B);
-  product<EpiSum>(p.bn, a, b, o, g, {first ? 0 : 1}, K, st);
+  product<EpiSum>(p, a, b, o, g, {first ? 0 : 1}, K, st);
   if (last) {
     const long long work = (long long)rows * (ldacc / 4);
     const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)num_sms() * 8);

@@ -49,6 +49,30 @@ void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs
   OM_LAUNCH_CHECK();
 }
 
+// On CTA pairs; g.tiles_r counts 256-row tiles, K-major operands have boxes of 128 rows.
+template <bool AMN, bool BMN, class Epi>
+void gx_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs, const GemmX& g,
+                    const typename Epi::Args& e, cudaStream_t st) {
+  static std::atomic<bool> attr_set[64];
+  int dev;
+  OM_CUDA_CHECK(cudaGetDevice(&dev));
+  if (!attr_set[dev].load()) {
+    OM_CUDA_CHECK(cudaFuncSetAttribute(gemm_pair_kernel<AMN, BMN, Epi>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       GemmPairCfg::SMEM_BYTES));
+    attr_set[dev].store(true);
+  }
+  const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
+  TORCH_CHECK(units < (1ll << 30), "gemm: too many tiles");
+  const int pairs = (int)std::min<long long>(units, num_sms() / 2);
+  gemm_pair_kernel<AMN, BMN, Epi><<<2 * pairs, 256, GemmPairCfg::SMEM_BYTES, st>>>(ta, tb, outs, g, e);
+  OM_LAUNCH_CHECK();
+}
+
+// Whether a grid has the tiles for pairs: at least one 256 x 256 tile for every pair of SMs.
+inline bool gx_pairs(int64_t rows, int64_t cols) {
+  return (int64_t)ceil_div(rows, 256) * ceil_div(cols, 256) >= num_sms() / 2;
+}
+
 struct GxOperand {
   const void* p;
   bool mn;
@@ -58,7 +82,7 @@ struct GxOperand {
 // out[rows, cols] (+)= A . B over K, split over K where the tiles alone leave SMs idle.
 // `acc` (from gx_acc_floats) carries fp32 sums from piece to piece; first / last tell the piece's place.
 struct GxPlan {
-  int bn, splits;
+  int bn, splits, pair;
 };
 GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K);
 int64_t gx_acc_floats(const GxPlan& p, int64_t rows, int64_t cols, bool pieces);

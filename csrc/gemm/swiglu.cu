@@ -200,7 +200,16 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
         o.m[2] = om::gx_out(e.gu + F, M, F, 2 * F);
       }
     }
-    om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+    if (om::gx_pairs(M, 2 * F)) {
+      g.tiles_r = om::ceil_div(M, 256);
+      g.tiles_c = om::ceil_div(F, 128);
+      g.b_step = 128;
+      g.b_second = (int)F;
+      om::gx_launch_pair<false, false, om::EpiSwiglu>(ta, om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), 128),
+                                                      o, g, e, st);
+    } else {
+      om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+    }
   } else {
     om::swiglu_fwd_bn<64>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
   }

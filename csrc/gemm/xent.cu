@@ -93,12 +93,11 @@ struct EpiXentFwd {
       s = s * fast_exp2(m - ref) + (a0 + a1);
       m = mn;
       if ((tcol >> 5) == cc) {  // tcol = -1 matches no chunk
-        const int j = tcol & 31;
-        float z = -INFINITY;
+        const uint32_t hit = bits & (1u << (tcol & 31));  // a mask, not an index: registers stay registers
+        float z = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i == j && ((bits >> i) & 1u)) z = __uint_as_float(v[i]) * e.x.scale;
-        e.zt[r] = z;
+        for (int i = 0; i < 32; ++i) z += (hit >> i) & 1u ? __uint_as_float(v[i]) : 0.f;
+        e.zt[r] = hit ? z * e.x.scale : -INFINITY;
       }
     }
     if (row) {
@@ -204,13 +203,19 @@ struct EpiXentBwd {
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) f[j] = fast_exp2(__uint_as_float(v[j]) * c2 - w.l2) - base;
-          if ((w.tcol >> 5) == (c0 >> 5)) {  // tcol = -1 matches no column
+          // tcol = -1 matches no column; a mask, not an index: registers stay registers
+          const uint32_t hit = (w.tcol >> 5) == (c0 >> 5) ? 1u << (w.tcol & 31) : 0u;
+          if (hit) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j == (w.tcol & 31)) f[j] -= 1.f - e.smoothing;
+            for (int j = 0; j < 32; ++j) f[j] -= (hit >> j) & 1u ? 1.f - e.smoothing : 0.f;
           }
+          if (bits == 0xffffffffu) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? f[j] * w.gz : 0.f;
+            for (int j = 0; j < 32; ++j) f[j] *= w.gz;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? f[j] * w.gz : 0.f;
+          }
         }
         st.put(b, h, f);
       }
@@ -268,6 +273,21 @@ XentIn check_xent(const char* op, const torch::Tensor& x, const torch::Tensor& w
   return in;
 }
 
+// The product x W^T of `cols` vocabulary rows from wv with either logits epilogue, on CTA pairs where
+// there are enough tiles.
+template <class Epi>
+void xent_logits(const XentIn& in, const void* wv, const om::OutMaps& o, om::GemmX g, const typename Epi::Args& e,
+                 cudaStream_t st) {
+  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, in.M, in.K, in.x.stride(0), 128);
+  const CUtensorMap tb = om::gx_map(wv, false, g.cols, in.K, in.w.stride(0), 128);
+  if (om::gx_pairs(in.M, g.cols)) {
+    g.tiles_r = om::ceil_div(in.M, 256);
+    om::gx_launch_pair<false, false, Epi>(ta, tb, o, g, e, st);
+  } else {
+    om::gx_launch<256, false, false, Epi>(ta, tb, o, g, e, st);
+  }
+}
+
 om::GemmX xent_gemm(const XentIn& in, int64_t cols, int* status) {
   om::GemmX g{};
   g.rows = (int)in.M;
@@ -301,12 +321,10 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
   const bool smooth = smoothing != 0.0;
   auto ws = torch::empty({n * (smooth ? 3 : 2) + M}, f32);
   float* p = ws.data_ptr<float>();
-  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, M, in.K, in.x.stride(0), 128);
-  const CUtensorMap tb = om::gx_map(in.w.data_ptr(), false, in.V, in.K, in.w.stride(0), 128);
   auto run = [&](auto epi) {
     using E = decltype(epi);
     typename E::Args e{in.rows, reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n};
-    om::gx_launch<256, false, false, E>(ta, tb, om::OutMaps{}, g, e, st);
+    xent_logits<E>(in, in.w.data_ptr(), om::OutMaps{}, g, e, st);
   };
   if (smooth)
     run(om::EpiXentFwd<true>{});
@@ -353,7 +371,6 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_
   if (nx + nw) acc = torch::empty({nx + nw}, lse.options());
   float* ax = nx ? acc.data_ptr<float>() : nullptr;
   float* aw = nw ? acc.data_ptr<float>() + nx : nullptr;  // nx is a multiple of 32
-  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, M, K, in.x.stride(0), 128);
   for (int64_t v0 = 0; v0 < V; v0 += C) {
     const int64_t n = std::min(C, V - v0);
     const __nv_bfloat16* wv = ptr(in.w) + v0 * in.w.stride(0);
@@ -361,8 +378,7 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_
     const om::EpiXentBwd::Args e{in.rows, lse.data_ptr<float>(), dloss.data_ptr<float>(), (float)smoothing, (int)v0};
     om::OutMaps o{};
     o.m[0] = om::gx_out(ptr(dz), M, n, ld);
-    om::gx_launch<256, false, false, om::EpiXentBwd>(ta, om::gx_map(wv, false, n, K, in.w.stride(0), 128), o, g, e,
-                                                     st);
+    xent_logits<om::EpiXentBwd>(in, wv, o, g, e, st);
     if (need_dx)
       om::gx_product(px, {dz.data_ptr(), false, ld}, {wv, true, in.w.stride(0)}, M, K, n, ptr(*dx), K, ax, v0 == 0,
                      v0 + n == V, g.status, st);

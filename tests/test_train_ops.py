@@ -218,6 +218,27 @@ def test_swiglu(dev, M, K, F):
     assert torch.equal(ops.swiglu_bwd(x, w, gu, dh, need_dw=False)[0], dx)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,F", [(2600, 72, 1100), (2700, 200, 1104), (4100, 64, 4001)])
+def test_swiglu_many_tiles(M, K, F):
+    """Enough tiles for the CTA-pair GEMM, whole and ragged ones, rows on and off 16-byte boundaries."""
+    x, w, dh, want, tol = swiglu_case("cuda", M, K, F)
+    h, gu = ops.swiglu(x, w, save=True)
+    dx, dw = ops.swiglu_bwd(x, w, gu, dh)
+    for name, g, a, t in zip(("h", "dx", "dw"), (h, dx, dw), want, tol):
+        close(g, a, t, name)
+    assert torch.equal(ops.swiglu(x, w), h)
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [dict(M=2049, K=136, V=4100, smoothing=0.1), dict(M=1500, K=4096, V=6500, scale=1.2),
+                               dict(M=700, K=72, V=9000, keep=0.1)], ids=str)
+def test_linear_xent_many_tiles(c):
+    check_xent(xent_case("cuda", **c))
+    ops.check_status()
+
+
 @on_devices
 def test_swiglu_extreme_gates(dev):
     """Gates of +-1000: the activation saturates to the product or to 0 without NaN."""

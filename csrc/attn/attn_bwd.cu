@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16*
                                                             float* __restrict__ stat, int T, int Tp, int H, int hd,
                                                             long long ob, long long ot, long long oh, long long gb,
                                                             long long gt, long long gh) {
+  grid_wait();
+  grid_release();
   const int sub = threadIdx.x & 15, b = blockIdx.y;
   const unsigned n = (unsigned)Tp * H;  // below 2^31
   const int len = lens ? min(lens[b], T) : T;
@@ -238,6 +240,29 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 0) {
+    mbar_init(fix_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(land, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&dp_full[s], 1);
+      mbar_init(&ds_full[s], 256);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_wait();
+  grid_release();
+
   // which rows, heads and tiles; the heaviest tiles come first: under a causal mask the first
   // keys (kv) and the last queries (q)
   int b, kvh, head = 0, split = 0, row0, first, ntile, total;
@@ -271,27 +296,6 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   const int nstream = KV ? (a.lens ? len_b : a.T) : len_b;         // valid rows of the streamed operands
   const int nrow = KV ? len_b : (a.lens ? len_b : a.T);            // valid rows of the resident ones
   const bool may_pad = a.lens != nullptr && nstream < a.S;         // beyond T the copies fill zeros themselves
-
-  if (threadIdx.x == 0) {
-    mbar_init(fix_full, 1);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(land, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&dp_full[s], 1);
-      mbar_init(&ds_full[s], 256);
-    }
-    mbar_init(acc_full, 1);
-    fence_barrier_init();
-  }
-  if (warp == 2) tmem_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (the whole warp)
@@ -502,6 +506,8 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
 __global__ void __launch_bounds__(256) attn_bwd_join_kernel(const float* __restrict__ part, int nsplit, long long n,
                                                             __nv_bfloat16* __restrict__ dv,
                                                             __nv_bfloat16* __restrict__ dk) {
+  grid_wait();
+  grid_release();
   for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < 2 * n; i += gridDim.x * 1024ll) {
     const int k = i >= n;
     const long long at = i - k * n;  // n is a multiple of 8
@@ -547,13 +553,11 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
   }
   const long long blocks = a.kv_blocks + (long long)((a.T + 127) / 128) * a.B * a.H;
   TORCH_CHECK(blocks < (1ll << 31), "attention_bwd: too many tiles");
-  attn_bwd_kernel<D><<<(unsigned)blocks, fa_bw::THREADS, C::SMEM, st>>>(q, g, k, v, a);
-  OM_LAUNCH_CHECK();
+  launch_dependent(attn_bwd_kernel<D>, (unsigned)blocks, fa_bw::THREADS, C::SMEM, st, q, g, k, v, a);
   if (a.nsplit > 1) {
     const long long n = (long long)a.B * a.S * a.Hkv * a.hd;
     const int jb = (int)std::min<long long>((2 * n + 1023) / 1024, (long long)num_sms() * 8);
-    attn_bwd_join_kernel<<<jb, 256, 0, st>>>(a.part, a.nsplit, n, a.dv, a.dk);
-    OM_LAUNCH_CHECK();
+    launch_dependent(attn_bwd_join_kernel, jb, 256, 0, st, (const float*)a.part, a.nsplit, n, a.dv, a.dk);
   }
 }
 
@@ -645,10 +649,10 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   a.part = a.nsplit > 1 ? ws.data_ptr<float>() + stat_floats : nullptr;
   const int64_t rows = (int64_t)a.Tp * H;
   const int blocks = (int)std::min<int64_t>((rows + 15) / 16, std::max<int64_t>(1, om::num_sms() * 16 / B));
-  om::attn_bwd_stat_kernel<<<dim3(blocks, (unsigned)B), 256, 0, st>>>(
-      ptr(out), ptr(dout), lse.data_ptr<float>(), a.lens, stat, a.T, a.Tp, a.H, a.hd, out.stride(0), out.stride(1),
-      out.stride(2), dout.stride(0), dout.stride(1), dout.stride(2));
-  OM_LAUNCH_CHECK();
+  om::launch_dependent(om::attn_bwd_stat_kernel, dim3(blocks, (unsigned)B), 256, 0, st, ptr(out), ptr(dout),
+                       lse.data_ptr<float>(), a.lens, stat, a.T, a.Tp, a.H, a.hd, (long long)out.stride(0),
+                       (long long)out.stride(1), (long long)out.stride(2), (long long)dout.stride(0),
+                       (long long)dout.stride(1), (long long)dout.stride(2));
   const CUtensorMap mq = om::map_bthd(q), mg = om::map_bthd(dout), mk = om::map_bthd(k), mv = om::map_bthd(v);
   if (D <= 64)
     om::attn_bwd_launch<64>(a, mq, mg, mk, mv, st);

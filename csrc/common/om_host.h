@@ -10,6 +10,7 @@
 #include <atomic>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #define OM_CUDA_CHECK(x)                                                                   \
   do {                                                                                     \
@@ -36,6 +37,24 @@ namespace om {
 // Host-side count of kernel launches issued by this library (also counts
 // launches recorded into a CUDA graph during capture).
 inline std::atomic<long long> g_launches{0};
+
+// Launch that may overlap its prologue with the end of the kernel before it in the stream; the
+// kernel calls grid_wait() in every thread before it touches memory.
+template <typename... P, typename... A>
+void launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  OM_CUDA_CHECK(cudaLaunchKernelEx(&c, kernel, std::forward<A>(args)...));
+  g_launches.fetch_add(1);
+}
 
 inline int num_sms(int dev = -1) {
   static int cache[64] = {0};

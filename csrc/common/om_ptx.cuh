@@ -254,6 +254,13 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// ---------------------------------------------------------------- dependent launches
+// A kernel launched with launch_dependent (om_host.h) may start before its predecessor in the
+// stream has ended: every thread calls grid_wait() before it touches memory (the predecessor and
+// all before it are complete then), and grid_release() lets the successor start its own prologue.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- tcgen05
 // Allocate `ncols` TMEM columns (power of two >= 32). Whole warp must call.
 // The TMEM base address is written to *smem_slot.

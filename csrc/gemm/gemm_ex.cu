@@ -3,22 +3,43 @@
 
 namespace om {
 
-// Sums the fp32 planes of a split contraction in plane order and rounds once.
+// Sums the fp32 planes of a split contraction and rounds once. SUB lanes share four columns: lane
+// group s adds planes s, s + SUB, ..., and the groups are added in order (one order, whatever the
+// grid). SUB = 8 from 16 planes on, where the walk over the planes is what takes the time.
+template <int SUB>
 __global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __restrict__ P, int splits, long long rows,
                                                              int cols, int ldacc, __nv_bfloat16* __restrict__ out,
                                                              long long ldo, int vec) {
-  const int nv = ldacc >> 2;
-  const long long plane = rows * ldacc;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < rows * nv; i += gridDim.x * 256ll) {
+  __shared__ float4 sh[SUB > 1 ? 256 : 1];
+  grid_wait();
+  grid_release();
+  const int nv = ldacc >> 2, lanes = 256 / SUB, sub = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+  const long long plane = rows * ldacc, n = rows * nv;
+  for (long long i0 = blockIdx.x * (long long)lanes; i0 < n; i0 += gridDim.x * (long long)lanes) {
+    const long long i = i0 + lane;
     const long long r = i / nv;
     const int c = (int)(i - r * nv) * 4;
-    if (c >= cols) continue;
-    float4 a = *reinterpret_cast<const float4*>(P + r * ldacc + c);
+    const bool live = i < n && c < cols;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
 #pragma unroll 8
-    for (int s = 1; s < splits; ++s) {
-      const float4 b = *reinterpret_cast<const float4*>(P + s * plane + r * ldacc + c);
-      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      for (int s = sub; s < splits; s += SUB) {
+        const float4 b = *reinterpret_cast<const float4*>(P + s * plane + r * ldacc + c);
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      }
     }
+    if constexpr (SUB > 1) {
+      __syncthreads();
+      sh[threadIdx.x] = a;
+      __syncthreads();
+      if (sub != 0) continue;
+#pragma unroll
+      for (int s = 1; s < SUB; ++s) {
+        const float4 b = sh[s * lanes + lane];
+        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+      }
+    }
+    if (!live) continue;
     __nv_bfloat16* o = out + r * ldo + c;
     if (vec && c + 4 <= cols) {
       uint2 w;
@@ -40,8 +61,10 @@ GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
   // takes 64 of the MMA's cycles a step, a 192-wide one 96 and a 256-wide one 128; shared memory
   // (A is read again for each) leaves the narrow ones 4 and 2 % behind.
   GxPlan p{256, 1, 0};
-  if (gx_pairs(rows, cols)) {
+  if (gx_pairs(rows, cols, K)) {
     p.pair = 1;
+    // Not split where the last wave leaves pairs idle: under the power limit the others run faster
+    // meanwhile, and the fp32 planes cost more (4096 x 4096 x 22016: 519 us whole, 560 in two).
     return p;
   }
   double best = 1e300;
@@ -128,11 +151,12 @@ void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t
                         (uint64_t)rows * ldacc, 32, 32, 1, CU_TENSOR_MAP_SWIZZLE_128B);
   product<EpiSum>(p, a, b, o, g, {first ? 0 : 1}, K, st);
   if (last) {
-    const long long work = (long long)rows * (ldacc / 4);
-    const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)num_sms() * 8);
-    planes_to_bf16_kernel<<<blocks, 256, 0, st>>>(acc, p.splits, rows, (int)cols, ldacc, out, ldo,
-                                                  ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0);
-    OM_LAUNCH_CHECK();
+    const bool many = p.splits >= 16;
+    const long long work = (long long)rows * (ldacc / 4), lanes = many ? 32 : 256;
+    const int blocks = (int)std::min<long long>((work + lanes - 1) / lanes, (long long)num_sms() * 8);
+    launch_dependent(many ? planes_to_bf16_kernel<8> : planes_to_bf16_kernel<1>, blocks, 256, 0, st, acc, p.splits,
+                     (long long)rows, (int)cols, ldacc, out, (long long)ldo,
+                     (int)(ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0));
   }
 }
 

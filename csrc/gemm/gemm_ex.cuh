@@ -154,6 +154,8 @@ __global__ void __launch_bounds__(256, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_wait();
+  grid_release();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
@@ -304,6 +306,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   __syncthreads();
   pair_sync();
   tc_fence_after();
+  grid_wait();
+  grid_release();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {

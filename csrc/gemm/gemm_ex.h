@@ -45,8 +45,7 @@ void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 31), "gemm: too many tiles");
   const int grid = (int)std::min<long long>(units, num_sms());
-  gemm_ex_kernel<BN, AMN, BMN, Epi><<<grid, 256, C::SMEM_BYTES, st>>>(ta, tb, outs, g, e);
-  OM_LAUNCH_CHECK();
+  launch_dependent(gemm_ex_kernel<BN, AMN, BMN, Epi>, grid, 256, C::SMEM_BYTES, st, ta, tb, outs, g, e);
 }
 
 // On CTA pairs; g.tiles_r counts 256-row tiles, K-major operands have boxes of 128 rows.
@@ -64,13 +63,14 @@ void gx_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps&
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 30), "gemm: too many tiles");
   const int pairs = (int)std::min<long long>(units, num_sms() / 2);
-  gemm_pair_kernel<AMN, BMN, Epi><<<2 * pairs, 256, GemmPairCfg::SMEM_BYTES, st>>>(ta, tb, outs, g, e);
-  OM_LAUNCH_CHECK();
+  launch_dependent(gemm_pair_kernel<AMN, BMN, Epi>, 2 * pairs, 256, GemmPairCfg::SMEM_BYTES, st, ta, tb, outs, g, e);
 }
 
-// Whether a grid has the tiles for pairs: at least one 256 x 256 tile for every pair of SMs.
-inline bool gx_pairs(int64_t rows, int64_t cols) {
-  return (int64_t)ceil_div(rows, 256) * ceil_div(cols, 256) >= num_sms() / 2;
+// Whether a product goes to pairs: a 256 x 256 tile for every pair of SMs, rows that fill more than
+// one half of a tile, and a contraction of 512 or more, below which setting up the pair costs more
+// than it saves.
+inline bool gx_pairs(int64_t rows, int64_t cols, int64_t K) {
+  return rows > 128 && K >= 512 && (int64_t)ceil_div(rows, 256) * ceil_div(cols, 256) >= num_sms() / 2;
 }
 
 struct GxOperand {

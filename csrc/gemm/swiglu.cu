@@ -94,6 +94,8 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restric
                                                           const __nv_bfloat16* __restrict__ dh, long long lddh,
                                                           __nv_bfloat16* __restrict__ dgu, long long lddgu,
                                                           long long M, int F) {
+  grid_wait();
+  grid_release();
   const int nv = F / V;
   const long long n = M * nv;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
@@ -200,7 +202,7 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
         o.m[2] = om::gx_out(e.gu + F, M, F, 2 * F);
       }
     }
-    if (om::gx_pairs(M, 2 * F)) {
+    if (om::gx_pairs(M, 2 * F, K)) {
       g.tiles_r = om::ceil_div(M, 256);
       g.tiles_c = om::ceil_div(F, 128);
       g.b_step = 128;
@@ -246,8 +248,8 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_swiglu_
   const long long work = M * (v8 ? F / 8 : F);
   const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)om::num_sms() * 16);
   auto grad = v8 ? om::swiglu_grad_kernel<8> : om::swiglu_grad_kernel<1>;
-  grad<<<blocks, 256, 0, st>>>(gu.data_ptr<float>(), 2 * F, ptr(d2), d2.stride(0), ptr(dgu), ld, M, (int)F);
-  OM_LAUNCH_CHECK();
+  om::launch_dependent(grad, blocks, 256, 0, st, gu.data_ptr<float>(), (long long)(2 * F), ptr(d2),
+                       (long long)d2.stride(0), ptr(dgu), (long long)ld, (long long)M, (int)F);
   auto product = [&](om::GxOperand a, om::GxOperand b, int64_t rows, int64_t cols, int64_t k, torch::Tensor& out) {
     const om::GxPlan p = om::gx_plan(rows, cols, k);
     const int64_t n = om::gx_acc_floats(p, rows, cols, false);

@@ -108,19 +108,23 @@ struct EpiXentFwd {
   }
 };
 
-// Joins the column tiles of 32 rows: warp w takes tiles w, w + 8, ...; the eight partial results
+// Joins the column tiles of 32 rows: warp w takes tiles w, w + 16, ...; the sixteen partial results
 // are joined in warp order (fixed order: the same result on every run).
-__global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict__ part, const float* __restrict__ sumz,
-                                                        const float* __restrict__ zt, XentRows x, int M, int tiles,
-                                                        float smoothing, float* __restrict__ loss,
-                                                        float* __restrict__ lse, int* status) {
-  __shared__ float sm[8][32], ss[8][32], sz[8][32];
+constexpr int XE_JOIN = 16;
+__global__ void __launch_bounds__(32 * XE_JOIN) xent_join_kernel(const float2* __restrict__ part,
+                                                                 const float* __restrict__ sumz,
+                                                                 const float* __restrict__ zt, XentRows x, int M,
+                                                                 int tiles, float smoothing, float* __restrict__ loss,
+                                                                 float* __restrict__ lse, int* status) {
+  __shared__ float sm[XE_JOIN][32], ss[XE_JOIN][32], sz[XE_JOIN][32];
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int r = blockIdx.x * 32 + lane;
   float m = -INFINITY, s = 0.f, z = 0.f;
   if (r < M) {
-#pragma unroll 4
-    for (int t = warp; t < tiles; t += 8) {
+#pragma unroll 8
+    for (int t = warp; t < tiles; t += XE_JOIN) {
       const float2 p = part[(size_t)t * M + r];
       const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.f : mn;
       s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
@@ -133,8 +137,9 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
   sz[warp][lane] = z;
   __syncthreads();
   if (warp != 0 || r >= M) return;
+  const long long t = x.targets[r];
 #pragma unroll
-  for (int w = 1; w < 8; ++w) {
+  for (int w = 1; w < XE_JOIN; ++w) {
     const float mn = fmaxf(m, sm[w][lane]), ref = mn == -INFINITY ? 0.f : mn;
     s = s * exp2f(m - ref) + ss[w][lane] * exp2f(sm[w][lane] - ref);
     m = mn;
@@ -142,7 +147,6 @@ __global__ void __launch_bounds__(256) xent_join_kernel(const float2* __restrict
   }
   const float l = m == -INFINITY ? -INFINITY : (m + log2f(s)) * XE_LN2;
   lse[r] = l;
-  const long long t = x.targets[r];
   float out = 0.f;
   if (t >= 0 && t < x.V && t != x.ignore) {
     const float a = zt[r];
@@ -280,7 +284,7 @@ void xent_logits(const XentIn& in, const void* wv, const om::OutMaps& o, om::Gem
                  cudaStream_t st) {
   const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, in.M, in.K, in.x.stride(0), 128);
   const CUtensorMap tb = om::gx_map(wv, false, g.cols, in.K, in.w.stride(0), 128);
-  if (om::gx_pairs(in.M, g.cols)) {
+  if (om::gx_pairs(in.M, g.cols, in.K)) {
     g.tiles_r = om::ceil_div(in.M, 256);
     om::gx_launch_pair<false, false, Epi>(ta, tb, o, g, e, st);
   } else {
@@ -330,10 +334,9 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
     run(om::EpiXentFwd<true>{});
   else
     run(om::EpiXentFwd<false>{});
-  om::xent_join_kernel<<<om::ceil_div(M, 32), 256, 0, st>>>(
-      reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n, in.rows, (int)M, g.tiles_c,
-      (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
-  OM_LAUNCH_CHECK();
+  om::launch_dependent(om::xent_join_kernel, om::ceil_div(M, 32), 32 * om::XE_JOIN, 0, st, (const float2*)p,
+                       (const float*)(smooth ? p + 2 * n + M : nullptr), (const float*)(p + 2 * n), in.rows, (int)M,
+                       g.tiles_c, (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
   return {loss, lse};
 }
 

@@ -176,6 +176,8 @@ template <typename T, typename W, bool LAYER, int G, int V, int P>
 __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_kernel(const NormFwd a) {
   __shared__ float sh[2 * (norm_threads<G>() / 32)];
   constexpr int RPB = norm_threads<G>() / G;
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x % G;
   const long long row = (long long)blockIdx.x * RPB + threadIdx.x / G;
   const bool live = row < a.M;
@@ -257,6 +259,10 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_ring_kernel(const 
   if (lane == 0) {
     for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
     fence_barrier_init();
+  }
+  grid_wait();
+  grid_release();
+  if (lane == 0) {
     for (int k = 0; k < a.stages; ++k)
       if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
   }
@@ -398,6 +404,8 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_kernel(const NormB
   const int lane = threadIdx.x % G;
   const long long step = (long long)gridDim.x * RPB;
   int flip = 0;
+  grid_wait();
+  grid_release();
   float dw[P][V], db[LAYER ? P : 1][V];
   Vec<W, V> w[P];
   Vec<T, V> hv[P], yv[P];
@@ -501,6 +509,10 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
   if (lane == 0) {
     for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
     fence_barrier_init();
+  }
+  grid_wait();
+  grid_release();
+  if (lane == 0) {
     for (int k = 0; k < a.stages; ++k)
       if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
   }
@@ -596,24 +608,27 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
   write_partials<G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }
 
-// dw (db) = sum over blocks, in block order: 32 columns a block, 8 warps each take every eighth
-// partial row, joined in warp order.
+// dw (db) = sum over blocks, in a fixed order: 32 columns a block, each of 16 warps takes every
+// sixteenth partial row, joined in warp order.
+constexpr int NORM_JOIN = 16;
 template <typename W>
-__global__ void __launch_bounds__(256) norm_join_kernel(const float* __restrict__ part, int blocks, int n, int D,
+__global__ void __launch_bounds__(32 * NORM_JOIN) norm_join_kernel(const float* __restrict__ part, int blocks, int n, int D,
                                                         W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ float sh[8][32];
+  __shared__ float sh[NORM_JOIN][32];
+  grid_wait();
+  grid_release();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane, k = blockIdx.y;
   float t = 0.f;
   if (c < D) {
-#pragma unroll 4
-    for (int b = warp; b < blocks; b += 8) t += part[((size_t)b * n + k) * D + c];
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += NORM_JOIN) t += part[((size_t)b * n + k) * D + c];
   }
   sh[warp][lane] = t;
   __syncthreads();
   if (warp != 0 || c >= D) return;
 #pragma unroll
-  for (int w = 1; w < 8; ++w) t += sh[w][lane];
+  for (int w = 1; w < NORM_JOIN; ++w) t += sh[w][lane];
   W* out = k == 0 ? dw : db;
   if constexpr (sizeof(W) == 2)
     out[c] = __float2bfloat16_rn(t);
@@ -771,8 +786,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
           auto go = [&](auto kernel, om::Residents& res) {
             const size_t smem = a.stages * stage;
             const int grid = (int)std::min<long long>(blocks, om::num_sms() * res.get(kernel, NT, smem));
-            kernel<<<grid, NT, smem, st>>>(a);
-            OM_LAUNCH_CHECK();
+            om::launch_dependent(kernel, grid, NT, smem, st, a);
           };
           static om::Residents res[4];
           if (layer && a.delta)
@@ -786,11 +800,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
           return;
         }
       }
-      if (layer)
-        om::norm_fwd_kernel<T, W, true, g, v, p><<<(unsigned)blocks, NT, 0, st>>>(a);
-      else
-        om::norm_fwd_kernel<T, W, false, g, v, p><<<(unsigned)blocks, NT, 0, st>>>(a);
-      OM_LAUNCH_CHECK();
+      om::launch_dependent(layer ? om::norm_fwd_kernel<T, W, true, g, v, p> : om::norm_fwd_kernel<T, W, false, g, v, p>,
+                           (unsigned)blocks, NT, 0, st, a);
     });
   });
   return {y, h, stats};
@@ -853,12 +864,10 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
         const int blocks = (int)std::min<long long>(most, om::num_sms() * res.get(kernel, NT, smem));
         auto part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());
         a.part = part.data_ptr<float>();
-        kernel<<<blocks, NT, smem, st>>>(a);
-        OM_LAUNCH_CHECK();
-        om::norm_join_kernel<W><<<dim3((a.D + 31) / 32, bias ? 2 : 1), 256, 0, st>>>(
-            a.part, blocks, n, a.D, reinterpret_cast<W*>(dw.data_ptr()),
-            bias ? reinterpret_cast<W*>(db->data_ptr()) : nullptr);
-        OM_LAUNCH_CHECK();
+        om::launch_dependent(kernel, blocks, NT, smem, st, a);
+        om::launch_dependent(om::norm_join_kernel<W>, dim3((a.D + 31) / 32, bias ? 2 : 1), 32 * om::NORM_JOIN, 0, st,
+                             (const float*)a.part, blocks, n, a.D, reinterpret_cast<W*>(dw.data_ptr()),
+                             bias ? reinterpret_cast<W*>(db->data_ptr()) : (W*)nullptr);
       };
       const size_t joined = RPB > 1 ? (size_t)a.D * sizeof(float) : 0;
       if constexpr (v == 8) {

@@ -220,6 +220,33 @@ __device__ __forceinline__ void write_acc(uint32_t tmem, OUT* dst, bool live, bo
   }
 }
 
+// Zeros for the 128 rows of a CTA that has no tile to walk.
+template <int D, bool KV>
+__device__ __forceinline__ void write_zero(const AttnBwdArgs& a, int b, int kvh, int head, int split, int row0) {
+  const int vecs = a.hd / 8, rows = min(128, (KV ? a.S : a.T) - row0);
+  const uint4 z = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < rows * vecs; i += blockDim.x) {
+    const int row = row0 + i / vecs, c = i % vecs * 8;
+    if constexpr (KV) {
+      const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd + c;
+      if (a.nsplit > 1) {
+        const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint4* p = reinterpret_cast<uint4*>(a.part + (split * 2 + k) * plane + at);
+          p[0] = z;
+          p[1] = z;
+        }
+      } else {
+        *reinterpret_cast<uint4*>(a.dk + at) = z;
+        *reinterpret_cast<uint4*>(a.dv + at) = z;
+      }
+    } else {
+      *reinterpret_cast<uint4*>(a.dq + (((size_t)b * a.T + row) * a.H + head) * a.hd + c) = z;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ the CTA of either kind
 // KV: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
 // else: resident Q, dO; streamed K, V; accumulates dQ.
@@ -239,29 +266,6 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   uint64_t* acc_full = ds_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  if (threadIdx.x == 0) {
-    mbar_init(fix_full, 1);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(land, 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&dp_full[s], 1);
-      mbar_init(&ds_full[s], 256);
-    }
-    mbar_init(acc_full, 1);
-    fence_barrier_init();
-  }
-  if (warp == 2) tmem_alloc(tmem_slot, 512);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  grid_wait();
-  grid_release();
 
   // which rows, heads and tiles; the heaviest tiles come first: under a causal mask the first
   // keys (kv) and the last queries (q)
@@ -297,11 +301,37 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
   const int nrow = KV ? len_b : (a.lens ? len_b : a.T);            // valid rows of the resident ones
   const bool may_pad = a.lens != nullptr && nstream < a.S;         // beyond T the copies fill zeros themselves
 
+  if (total == 0) {  // nothing but padding: zeros, without tensor memory
+    write_zero<D, KV>(a, b, kvh, head, split, row0);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(fix_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(land, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&dp_full[s], 1);
+      mbar_init(&ds_full[s], 256);
+    }
+    mbar_init(acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
   if (warp == 0) {
     // ------------------------------------------------------------ producer (the whole warp)
     bool ok = true;
     int it = 0, landed = 0;
-    if (total > 0 && lane == 0) {
+    if (lane == 0) {
       mbar_arrive_expect_tx(fix_full, C::FIX_BYTES);
       for (int h = 0; h < C::H; ++h)
         for (int r = 0; r < 2; ++r) {
@@ -350,7 +380,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (total > 0 && elect_one()) {
+    if (elect_one()) {
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
       constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
       const uint32_t r0 = smem_u32(smem), r1 = r0 + C::H * C::BIG;  // K, V or Q, dO
@@ -414,17 +444,17 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int row = row0 + t;
     float2 own = make_float2(0.f, 0.f);
-    bool zero = total == 0;
+    bool zero = false;
     if constexpr (!KV) {
       own.x = -INFINITY;
       if (row < nrow) {
         const float* p = a.stat + (((size_t)b * a.H + head) * a.Tp + (row & ~63)) * 2 + (row & 63);
         own = make_float2(p[0], p[64]);
       }
-      zero = zero || own.x == -INFINITY;         // padding, or no visible key: gradient 0
+      zero = own.x == -INFINITY;                 // padding, or no visible key: gradient 0
     }
     bool ok = true;
-    int tile = ntile ? group % ntile : 0;
+    int tile = group % ntile;
     for (int it = group; it < total; it += 2) {
       const int x0 = (first + tile) * 64;
       tile += 2;
@@ -458,7 +488,7 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       tc_fence_before();
       mbar_arrive(&ds_full[it & 1]);
     }
-    if (ok && total > 0) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
+    if (ok) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
@@ -496,6 +526,8 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
                     const AttnBwdArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  grid_wait();
+  grid_release();
   if ((int)blockIdx.x < a.kv_blocks)
     attn_bwd_cta<D, true>(tmQ, tmG, tmK, tmV, a, blockIdx.x, smem);
   else

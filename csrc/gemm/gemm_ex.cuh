@@ -38,7 +38,8 @@ struct GemmX {
   int num_kb;        // 64-deep steps of the whole contraction
   int splits, kb_per_split;
   int tiles_r, tiles_c;
-  int b_step;        // rows of B per column tile (K-major B): BN, or BN / 2 for a gated pair
+  int b_step;        // rows of B per column tile (K-major B): BN, or for a gated pair the features of a tile
+  int b_box;         // rows of B that one of the two loads of a step brings (K-major B): BN / 2 or fewer
   int b_second;      // distance of the second half's rows (K-major B): BN / 2, or F
   int* status;
 };
@@ -106,23 +107,26 @@ __host__ __device__ constexpr uint32_t idesc_bf16_x(int M, int N, bool amn, bool
   return idesc_bf16_f32(M, N) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
 }
 
-template <int BN>
+// AR: rows of A that are loaded. The MMA reads 128; for a few tokens the rest is whatever follows in
+// shared memory, which ends in accumulator rows that are never read, and the room goes to stages.
+template <int BN, int AR = 128>
 struct GemmXCfg {
-  static constexpr int BM = 128, BK = 64;
-  static constexpr int A_BYTES = BM * BK * 2;
+  static constexpr int BK = 64;
+  static constexpr int A_BYTES = AR * BK * 2;
   static constexpr int B_BYTES = BN * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES > 8 ? 8 : (192 * 1024) / STAGE_BYTES;
+  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES > 16 ? 16 : (192 * 1024) / STAGE_BYTES;
   static constexpr int TMEM_COLS = BN <= 128 ? 2 * BN : 512;  // a power of two
-  static constexpr int OUT_BYTES = 4 * 2 * 4096;  // four epilogue warps
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 /*align slack*/ + 256;
+  static constexpr int OUT_BYTES = 4 * 2 * 4096;  // four epilogue warps; also what lies behind a short A
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 /*align slack*/ + 512;
+  static_assert((128 - AR) * BK * 2 <= B_BYTES + OUT_BYTES, "the MMA reads 128 rows of A");
 };
 
-template <int BN, bool AMN, bool BMN, class Epi>
+template <int BN, int AR, bool AMN, bool BMN, class Epi>
 __global__ void __launch_bounds__(256, 1)
     gemm_ex_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ OutMaps outs, const GemmX g, const typename Epi::Args e) {
-  using C = GemmXCfg<BN>;
+  using C = GemmXCfg<BN, AR>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* out_bytes = smem + C::STAGES * C::STAGE_BYTES;
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(256, 1)
           if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, g.status, OM_ERR_WAIT_EMPTY)) { ok = false; break; }
           uint8_t* a_dst = smem + s * C::STAGE_BYTES;
           uint8_t* b_dst = a_dst + C::A_BYTES;
-          mbar_arrive_expect_tx(&full[s], C::STAGE_BYTES);
+          mbar_arrive_expect_tx(&full[s], C::A_BYTES + (BMN ? C::B_BYTES : 2 * g.b_box * 128));
           if constexpr (AMN) {
             tma_load_2d(a_dst, &tmA, &full[s], tr * 128, kb * 64);
             tma_load_2d(a_dst + 8192, &tmA, &full[s], tr * 128 + 64, kb * 64);

@@ -30,22 +30,22 @@ inline CUtensorMap gx_out(float* p, uint64_t rows, uint64_t cols, uint64_t ld) {
   return make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, cols, rows, ld, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int BN, bool AMN, bool BMN, class Epi>
+template <int BN, bool AMN, bool BMN, class Epi, int AR = 128>
 void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs, const GemmX& g,
                const typename Epi::Args& e, cudaStream_t st) {
-  using C = GemmXCfg<BN>;
+  using C = GemmXCfg<BN, AR>;
   static std::atomic<bool> attr_set[64];
   int dev;
   OM_CUDA_CHECK(cudaGetDevice(&dev));
   if (!attr_set[dev].load()) {
-    OM_CUDA_CHECK(cudaFuncSetAttribute(gemm_ex_kernel<BN, AMN, BMN, Epi>,
+    OM_CUDA_CHECK(cudaFuncSetAttribute(gemm_ex_kernel<BN, AR, AMN, BMN, Epi>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES));
     attr_set[dev].store(true);
   }
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 31), "gemm: too many tiles");
   const int grid = (int)std::min<long long>(units, num_sms());
-  launch_dependent(gemm_ex_kernel<BN, AMN, BMN, Epi>, grid, 256, C::SMEM_BYTES, st, ta, tb, outs, g, e);
+  launch_dependent(gemm_ex_kernel<BN, AR, AMN, BMN, Epi>, grid, 256, C::SMEM_BYTES, st, ta, tb, outs, g, e);
 }
 
 // On CTA pairs; g.tiles_r counts 256-row tiles, K-major operands have boxes of 128 rows.

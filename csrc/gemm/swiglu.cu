@@ -50,7 +50,7 @@ struct EpiSwiglu {
     const int F = g.cols, r0 = r - st.lane;
 #pragma unroll 1
     for (int cc = 0; cc < HALF / 32; ++cc) {
-      const int c0 = tc * HALF + cc * 32;
+      const int c0 = tc * g.b_step + cc * 32;
       if (c0 >= F || r0 >= g.rows) break;
       uint32_t gv[32], uv[32];
       tmem_ld_32x32b_x32(tbase + cc * 32, gv);
@@ -78,7 +78,7 @@ struct EpiSwiglu {
         continue;
       }
       if (r >= g.rows) continue;
-      const int n = min(32, F - c0);
+      const int n = min(min(32, g.b_step - cc * 32), F - c0);
       store_row32(e.h + (size_t)r * e.ldh + c0, hf, n, e.vec_h);
       if (e.gu != nullptr) {
         store_row32(e.gu + (size_t)r * e.ldgu + c0, gf, n, e.vec_gu);
@@ -132,15 +132,6 @@ __global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restric
   }
 }
 
-template <int BN>
-static void swiglu_fwd_bn(const CUtensorMap& ta, const void* w, int64_t ldw, const OutMaps& o, GemmX g,
-                          const EpiSwiglu::Args& e, int64_t F, int64_t K, cudaStream_t st) {
-  g.tiles_c = ceil_div(F, BN / 2);
-  g.b_step = BN / 2;
-  g.b_second = (int)F;
-  gx_launch<BN, false, false, EpiSwiglu>(ta, gx_map(w, false, 2 * F, K, ldw, BN / 2), o, g, e, st);
-}
-
 }  // namespace om
 
 using om::GemmX;
@@ -190,10 +181,16 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
   g.kb_per_split = g.num_kb;
   g.tiles_r = om::ceil_div(M, 128);
   g.status = status.data_ptr<int>();
-  const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), 128);
-  // 128 features a tile once those tiles fill the SMs; fewer tiles than SMs: 32 features a tile
+  const int sms = om::num_sms();
+  g.b_second = (int)F;
   om::OutMaps o{};
-  if ((int64_t)g.tiles_r * om::ceil_div(F, 128) >= om::num_sms()) {
+  // 128 features a tile once those tiles fill the SMs and there is more than one row tile's worth of
+  // work for each weight byte
+  if (M > 128 && (int64_t)g.tiles_r * om::ceil_div(F, 128) >= sms) {
+    const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), 128);
+    const CUtensorMap tb = om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), 128);
+    g.b_step = g.b_box = 128;
+    g.tiles_c = om::ceil_div(F, 128);
     e.maps = om::gx_storable(e.h, F, 2);  // F a multiple of 8: every row of h, g and u starts on 16 bytes
     if (e.maps) {
       o.m[0] = om::gx_out32(e.h, M, F, F);
@@ -204,17 +201,26 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
     }
     if (om::gx_pairs(M, 2 * F, K)) {
       g.tiles_r = om::ceil_div(M, 256);
-      g.tiles_c = om::ceil_div(F, 128);
-      g.b_step = 128;
-      g.b_second = (int)F;
-      om::gx_launch_pair<false, false, om::EpiSwiglu>(ta, om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), 128),
-                                                      o, g, e, st);
+      om::gx_launch_pair<false, false, om::EpiSwiglu>(ta, tb, o, g, e, st);
     } else {
-      om::swiglu_fwd_bn<256>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+      om::gx_launch<256, false, false, om::EpiSwiglu>(ta, tb, o, g, e, st);
     }
-  } else {
-    om::swiglu_fwd_bn<64>(ta, w2.data_ptr(), w2.stride(0), o, g, e, F, K, st);
+    return {h, gu};
   }
+  // Few tokens, or a small layer: bound by the weight's bytes or by latency. At most 32 features a
+  // tile, and as many (not a multiple of anything) as give every SM the same number of tiles:
+  // 28672 features are 7 tiles of 28 on each of 148 SMs, where 32 each would leave a seventh idle.
+  // With 32 tokens or fewer, A is loaded 32 rows high and the room is 16 stages of weights.
+  const int waves = om::ceil_div((int64_t)g.tiles_r * om::ceil_div(F, 32), sms);
+  const int64_t tiles = std::max<int64_t>(1, (int64_t)waves * sms / g.tiles_r);
+  g.b_step = g.b_box = (int)std::min<int64_t>(32, std::max<int64_t>(8, om::ceil_div(F, tiles)));
+  g.tiles_c = om::ceil_div(F, g.b_step);
+  const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), M <= 32 ? 32 : 128);
+  const CUtensorMap tb = om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), g.b_box);
+  if (M <= 32)
+    om::gx_launch<64, false, false, om::EpiSwiglu, 32>(ta, tb, o, g, e, st);
+  else
+    om::gx_launch<64, false, false, om::EpiSwiglu>(ta, tb, o, g, e, st);
   return {h, gu};
 }
 

@@ -302,7 +302,7 @@ om::GemmX xent_gemm(const XentIn& in, int64_t cols, int* status) {
   g.tiles_r = om::ceil_div(in.M, 128);
   g.tiles_c = om::ceil_div(cols, 256);
   g.b_step = 256;
-  g.b_second = 128;
+  g.b_second = g.b_box = 128;
   g.status = status;
   return g;
 }

@@ -2,10 +2,10 @@
 
 Holds fp32 master parameters (``nn.Parameter``) of a decoder with the same
 architecture and weight layout as :class:`DecoderLM`, computes in bf16 on the
-GPU through the differentiable tcgen05 GEMM (``ops.autograd.linear``) and the
-differentiable FlashAttention (``ops.autograd.attention``: tcgen05 kernel forward,
-gradient recomputed from its log-sum-exp), and can
-push its weights into an inference ``DecoderLM`` (rollout weight sync).
+GPU through the differentiable kernels of ``ops.autograd`` (tcgen05 GEMM,
+FlashAttention with its recomputing gradient, the gated projection, residual add and
+RMSNorm, and a cross entropy that never stores logits: ``loss`` and ``logprobs``), and
+can push its weights into an inference ``DecoderLM`` (rollout weight sync).
 
 The forward takes whole sequences (no paged cache) and supports Keep-Routing
 replay: ``forced_routing[layer] = expert ids [B*T, k]`` makes each MoE layer
@@ -68,32 +68,53 @@ class Policy(nn.Module):
     def _w(self, p):
         return p.to(self.cdt)
 
-    def forward(self, ids: torch.Tensor, forced_routing: dict | None = None, record_routing: dict | None = None):
-        """ids [B, T] -> logits [B, T, V] (fp32)."""
+    def hidden(self, ids: torch.Tensor, forced_routing: dict | None = None, record_routing: dict | None = None,
+               lens: torch.Tensor | None = None):
+        """ids [B, T] -> final normed hidden states [B, T, D] (what lm_head multiplies). ``lens`` int32
+        [B]: valid tokens of right-padded rows; attention's gradient then skips the padding."""
         cfg = self.cfg
         B, T = ids.shape
         H, Hkv, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
         pos = torch.arange(T, device=ids.device)
-        x = F.embedding(ids, self._w(self.embed))
+        x, d = F.embedding(ids, self._w(self.embed)), None
+
+        def norm(x, d, w):  # (norm(x + d), x + d)
+            if d is None:
+                return ag.rmsnorm(x, self._w(w), cfg.rms_eps), x
+            return ag.add_rmsnorm(x, d, self._w(w), cfg.rms_eps)
+
         for i, L in enumerate(self.layers):
-            a = ag.rmsnorm(x, self._w(L.attn_norm), cfg.rms_eps)
+            a, x = norm(x, d, L.attn_norm)
             qkv = ag.linear(a, self._w(L.qkv))
             q = qkv[..., :H * hd].view(B, T, H, hd)
             k = qkv[..., H * hd:(H + Hkv) * hd].view(B, T, Hkv, hd)
             v = qkv[..., (H + Hkv) * hd:].view(B, T, Hkv, hd)
             q = _rope(q, pos, self.inv_freq, cfg.rope_mode)
             k = _rope(k, pos, self.inv_freq, cfg.rope_mode)
-            o = ag.attention(q, k, v, 1.0 / math.sqrt(hd)).reshape(B, T, H * hd)
-            x = x + ag.linear(o, self._w(L.o))
-            h = ag.rmsnorm(x, self._w(L.ffn_norm), cfg.rms_eps)
+            o = ag.attention(q, k, v, 1.0 / math.sqrt(hd), lens).reshape(B, T, H * hd)
+            h, x = norm(x, ag.linear(o, self._w(L.o)), L.ffn_norm)
             if L.is_moe:
-                x = x + self._moe(i, L, h.reshape(B * T, -1), forced_routing, record_routing).view(B, T, -1)
+                d = self._moe(i, L, h.reshape(B * T, -1), forced_routing, record_routing).view(B, T, -1)
             else:
-                gu = ag.linear(h, self._w(L.gate_up))
-                Fd = gu.shape[-1] // 2
-                x = x + ag.linear(F.silu(gu[..., :Fd]) * gu[..., Fd:], self._w(L.down))
-        x = ag.rmsnorm(x, self._w(self.norm), cfg.rms_eps)
-        return ag.linear(x, self._w(self.lm_head)).float()
+                d = ag.linear(ag.swiglu(h, self._w(L.gate_up)), self._w(L.down))
+        return norm(x, d, self.norm)[0]
+
+    def forward(self, ids: torch.Tensor, forced_routing: dict | None = None, record_routing: dict | None = None):
+        """ids [B, T] -> logits [B, T, V] (fp32)."""
+        return ag.linear(self.hidden(ids, forced_routing, record_routing), self._w(self.lm_head)).float()
+
+    def loss(self, ids: torch.Tensor, labels: torch.Tensor, label_smoothing: float = 0.0) -> torch.Tensor:
+        """Mean next-token cross entropy (``train.loss.causal_lm_loss`` of the logits) without the
+        logits: position t predicts labels[t + 1], labels of -100 do not count."""
+        tgt = torch.full_like(labels, -100)
+        tgt[:, :-1] = labels[:, 1:]
+        rows = ag.linear_xent(self.hidden(ids), self._w(self.lm_head), tgt, smoothing=label_smoothing)
+        return rows.sum() / (tgt != -100).sum().clamp(min=1)
+
+    def logprobs(self, hidden: torch.Tensor, targets: torch.Tensor, temperature: float = 1.0, keep=None):
+        """log p(target) under softmax(logits / temperature) of hidden rows [N, D], restricted to the
+        packed keep mask (int32 [N, ceil(V / 32)]), without the logits."""
+        return -ag.linear_xent(hidden, self._w(self.lm_head), targets, scale=1.0 / max(temperature, 1e-6), keep=keep)
 
     def _moe(self, i, L, h, forced, record):
         k = self.cfg.moe.top_k
@@ -111,9 +132,8 @@ class Policy(nn.Module):
             if sel.numel() == 0:
                 continue
             t_idx = tok[sel]
-            gu = ag.linear(h.index_select(0, t_idx), self._w(L.experts_gate_up[e]))
-            Fe = gu.shape[-1] // 2
-            y = ag.linear(F.silu(gu[:, :Fe]) * gu[:, Fe:], self._w(L.experts_down[e]))
+            y = ag.linear(ag.swiglu(h.index_select(0, t_idx), self._w(L.experts_gate_up[e])),
+                          self._w(L.experts_down[e]))
             out = out.index_add(0, t_idx, y.float() * wt[sel, None])
         return out.to(h.dtype)
 

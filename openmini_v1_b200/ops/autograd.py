@@ -43,62 +43,168 @@ def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return y.reshape(*shp[:-1], w.shape[0])
 
 
+class _Norm(torch.autograd.Function):
+    """y = norm(x (+ delta)) w (+ b) on the native kernels (``ops.norm_train``); with delta the sum
+    h comes back too, and its gradient joins dx in the same pass."""
+
+    @staticmethod
+    def forward(ctx, x, delta, w, b, eps, kind):
+        y, h, stats = ops.norm_train(x, w, b, eps, kind=kind, delta=delta)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(h, w, stats)
+        ctx.kind, ctx.bias, ctx.summed = kind, b is not None, delta is not None
+        return (y, h) if delta is not None else y
+
+    @staticmethod
+    def backward(ctx, gy, gh=None):
+        h, w, stats = ctx.saved_tensors
+        if gy is None:
+            gy = torch.zeros_like(h)
+        dx, dw, db = ops.norm_train_bwd(gy, h, w, stats, kind=ctx.kind, bias=ctx.bias, dh=gh)
+        return dx, dx if ctx.summed else None, dw, db, None, None
+
+
+def _norm_native(x, w):
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and w.dtype in (x.dtype, torch.float32)
+            and x.shape[-1] <= 16384)
+
+
 def rmsnorm(x, w, eps):
+    if _norm_native(x, w):
+        return _Norm.apply(x, None, w, None, eps, "rms")
     xf = x.float()
     return (xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps) * w.float()).to(x.dtype)
+
+
+def add_rmsnorm(x, delta, w, eps):
+    """(rmsnorm(h), h) with h = x + delta: the residual add and the norm that follows it."""
+    if _norm_native(x, w):
+        return _Norm.apply(x, delta, w, None, eps, "rms")
+    h = x + delta
+    return rmsnorm(h, w, eps), h
+
+
+def layernorm(x, w, b, eps):
+    """LayerNorm with gain and (optional) bias over the last dimension."""
+    if _norm_native(x, w):
+        return _Norm.apply(x, None, w, b, eps, "layer")
+    xf = x.float()
+    mu = xf.mean(-1, keepdim=True)
+    y = (xf - mu) * torch.rsqrt((xf - mu).pow(2).mean(-1, keepdim=True) + eps) * w.float()
+    return (y if b is None else y + b.float()).to(x.dtype)
+
+
+class _SwiGLU(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w):
+        h, gu = ops.swiglu(x, w, save=True)
+        ctx.save_for_backward(x, w, gu)
+        return h
+
+    @staticmethod
+    def backward(ctx, gh):
+        x, w, gu = ctx.saved_tensors
+        return ops.swiglu_bwd(x, w, gu, gh, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+
+
+def swiglu(x, w):
+    """silu(x Wg^T) * (x Wu^T) of x [..., K], w [2F, K] (gate rows first): one GEMM forward, the
+    gradient from its fp32 projections."""
+    if not x.is_cuda:
+        z = x @ w.t()
+        F = w.shape[0] // 2
+        return torch.nn.functional.silu(z[..., :F]) * z[..., F:]
+    if not (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)):
+        return ops.swiglu(x, w)
+    return _SwiGLU.apply(x, w)
+
+
+class _LinearXent(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, targets, scale, smoothing, ignore_index, keep):
+        loss, lse = ops.linear_xent(x, w, targets, scale, smoothing, ignore_index, keep)
+        ctx.save_for_backward(x, w, targets, lse, keep)
+        ctx.args = (scale, smoothing, ignore_index)
+        return loss
+
+    @staticmethod
+    def backward(ctx, gl):
+        x, w, targets, lse, keep = ctx.saved_tensors
+        dx, dw = ops.linear_xent_bwd(x, w, targets, lse, gl, *ctx.args, keep=keep, need_dx=ctx.needs_input_grad[0],
+                                     need_dw=ctx.needs_input_grad[1])
+        return dx, dw, None, None, None, None, None
+
+
+def linear_xent(x, w, targets, scale=1.0, smoothing=0.0, ignore_index=-100, keep=None):
+    """Cross entropy [...] (fp32, row by row) of the logits scale * x w^T against ``targets`` [...],
+    without the logits; ``keep`` restricts the vocabulary (see ``ops.linear_xent``)."""
+    if x.is_cuda:
+        return _LinearXent.apply(x, w, targets, scale, smoothing, ignore_index, keep)
+    z = (x @ w.t()).float().reshape(-1, w.shape[0]) * scale
+    if keep is not None:
+        if smoothing:
+            raise ValueError("linear_xent: label smoothing over a keep mask is not defined")
+        bits = (keep[:, :, None] >> torch.arange(32, dtype=torch.int32, device=keep.device)) & 1
+        z = z.masked_fill(bits.reshape(keep.shape[0], -1)[:, :w.shape[0]] == 0, float("-inf"))
+    loss = torch.nn.functional.cross_entropy(z, targets.reshape(-1).long(), ignore_index=ignore_index,
+                                             label_smoothing=smoothing, reduction="none")
+    return loss.view(targets.shape)
+
+
+def _attend_batch(q, k, v, scale):
+    """Causal attention of a whole batch in one launch of the tcgen05 prefill kernel: K and V laid
+    out as a paged cache (16-token blocks), heads narrower than 128 filled up with zeros.
+    (out [B, T, H, D], lse fp32 [B, T, H])."""
+    B, T, H, D = q.shape
+    Hkv, dev = k.shape[2], q.device
+    nb = (T + 15) // 16
+    fill = lambda x, t: torch.nn.functional.pad(x, (0, 128 - D, 0, 0, 0, t)) if t or D < 128 else x  # noqa: E731
+
+    def paged(x):
+        return fill(x, nb * 16 - T).reshape(B * nb, 16, Hkv, 128).transpose(1, 2).contiguous()
+
+    tiles = [(b * T + t, min(128, T - t), b, min(T, t + 128)) for t in range((T - 1) // 128 * 128, -1, -128)
+             for b in range(B)]   # longest first
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    out = torch.empty(B * T, H * 128, dtype=q.dtype, device=dev)
+    lse = torch.empty(B * T, H, dtype=torch.float32, device=dev)
+    ops.flash_prefill(fill(q, 0).reshape(B * T, H * 128), paged(k), paged(v),
+                      torch.arange(B * nb, dtype=torch.int32, device=dev).view(B, nb),
+                      torch.arange(B, dtype=torch.int32, device=dev).repeat_interleave(T),
+                      torch.arange(1, T + 1, dtype=torch.int32, device=dev).repeat(B), ints(tiles), H, scale, out=out,
+                      lse=lse)
+    return out.view(B, T, H, 128)[..., :D], lse.view(B, T, H)
 
 
 class _Attention(torch.autograd.Function):
     """Causal attention of q [B, T, H, D] over k, v [B, T, Hkv, D].
 
-    Forward: the repo's attention per sequence (``parallel.ring_attention.attend``: the
-    tcgen05 FlashAttention kernel on CUDA for head_dim 128, the fp32 statement on CPU),
-    which also returns the natural-log sum of exponentials L of every row.
-    Backward (flash-attention gradient from L, no stored probabilities):
-        P = exp(scale q k^T - L),  dV = P^T dO,  dP = dO V^T,
-        delta = rowsum(dO * O),    dS = P * (dP - delta),
-        dQ = scale dS K,           dK = scale dS^T Q   (GQA: summed over each KV head's queries)."""
+    Forward: the repo's attention (on CUDA one launch of the tcgen05 FlashAttention kernel, on the
+    CPU the fp32 statement per sequence), which also returns the natural-log sum of exponentials L
+    of every row. Backward: ``ops.attention_bwd``, which recomputes the probabilities from L."""
 
     @staticmethod
-    def forward(ctx, q, k, v, scale):
-        from ..parallel.ring_attention import attend
-        B = q.shape[0]
-        outs, lses = [], []
-        for b in range(B):
-            o, lse = attend(q[b].contiguous(), k[b].contiguous(), v[b].contiguous(), scale, causal=True)
-            outs.append(o)
-            lses.append(lse)
-        out = torch.stack(outs)                    # fp32 [B, T, H, D]
-        lse = torch.stack(lses)                    # [B, T, H]
-        ctx.save_for_backward(q, k, v, out, lse)
+    def forward(ctx, q, k, v, scale, lens):
+        if q.is_cuda and q.numel():
+            out, lse = _attend_batch(q, k, v, scale)
+        else:
+            from ..parallel.ring_attention import attend
+            got = [attend(q[b], k[b], v[b], scale, causal=True) for b in range(q.shape[0])]
+            out, lse = (torch.stack(t) for t in zip(*got)) if got else (q.float(), q[..., 0].float())
+        ctx.save_for_backward(q, k, v, out, lse, lens)
         ctx.scale = scale
         return out.to(q.dtype)
 
     @staticmethod
     def backward(ctx, go):
-        q, k, v, out, lse = ctx.saved_tensors
-        scale = ctx.scale
-        B, T, H, D = q.shape
-        Hkv = k.shape[2]
-        G = H // Hkv
-        qf, gof = q.float(), go.float()
-        kf = k.float().repeat_interleave(G, dim=2)
-        vf = v.float().repeat_interleave(G, dim=2)
-        s = torch.einsum("bqhd,bkhd->bhqk", qf, kf) * scale
-        causal = torch.ones(T, T, dtype=torch.bool, device=q.device).triu(1)
-        p = torch.exp(s - lse.permute(0, 2, 1)[..., None]).masked_fill(causal, 0.0)
-        dv = torch.einsum("bhqk,bqhd->bkhd", p, gof)
-        dp = torch.einsum("bqhd,bkhd->bhqk", gof, vf)
-        delta = (gof * out).sum(-1).permute(0, 2, 1)[..., None]   # [B, H, T, 1]
-        ds = p * (dp - delta)
-        dq = torch.einsum("bhqk,bkhd->bqhd", ds, kf) * scale
-        dk = torch.einsum("bhqk,bqhd->bkhd", ds, qf) * scale
-        if G > 1:
-            dk = dk.view(B, T, Hkv, G, D).sum(3)
-            dv = dv.view(B, T, Hkv, G, D).sum(3)
-        return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype), None
+        q, k, v, out, lse, lens = ctx.saved_tensors
+        dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, go, ctx.scale, causal=True, lens=lens)
+        return dq, dk, dv, None, None
 
 
-def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float) -> torch.Tensor:
-    """Differentiable causal attention, q [B, T, H, D], k / v [B, T, Hkv, D] -> [B, T, H, D]."""
-    return _Attention.apply(q, k, v, scale)
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, lens=None) -> torch.Tensor:
+    """Differentiable causal attention, q [B, T, H, D], k / v [B, T, Hkv, D] -> [B, T, H, D].
+
+    ``lens`` int32 [B]: valid tokens of right-padded sequences. Their rows do not depend on it (a
+    causal row sees no padding); the gradient leaves the padding out, in work and in value."""
+    return _Attention.apply(q, k, v, scale, lens)

@@ -105,6 +105,9 @@ class GRPOTrainer:
                         for i, r in enumerate(per):
                             rows[i, :r[layer].shape[0]] = r[layer]
                         routing[layer] = rows.view(len(grp) * T, k)
+            if dev.type == "cuda" and hasattr(model, "logprobs"):
+                out += self._logp_rows(model, grp, seqs, ids.to(dev), routing)
+                continue
             logits = model(ids.to(dev), forced_routing=routing)
             for i, s in enumerate(grp):
                 P, C = len(s["prompt"]), len(s["completion"])
@@ -114,6 +117,24 @@ class GRPOTrainer:
                 keep = unpack_words(item[0][:C].to(dev), V) if item is not None else None
                 out.append(token_logprobs(lg, tgt, self.temperature, keep))
         return out
+
+    def _logp_rows(self, model, grp, seqs, ids, routing):
+        """Completion log-probs of one padded batch from its hidden rows: neither the prompt's nor the
+        padding's logits are computed, and the completion's are never stored."""
+        dev, V = ids.device, self.policy.cfg.vocab_size
+        lens = torch.tensor([len(x) - 1 for x in seqs], dtype=torch.int32, device=dev)
+        hidden = model.hidden(ids, forced_routing=routing, lens=lens)
+        items = [self.keep_mask.get(s["key"]) for s in grp]
+        rows, words, n = [], [], [len(s["completion"]) for s in grp]
+        for i, (s, item) in enumerate(zip(grp, items)):
+            p = len(s["prompt"])
+            rows.append(hidden[i, p - 1:p - 1 + n[i]])
+            if any(x is not None for x in items):
+                words.append(item[0][:n[i]].to(dev) if item is not None else
+                             torch.full((n[i], (V + 31) // 32), -1, dtype=torch.int32, device=dev))
+        tgt = torch.tensor([t for s in grp for t in s["completion"]], device=dev)
+        logp = model.logprobs(torch.cat(rows), tgt, self.temperature, torch.cat(words) if words else None)
+        return list(logp.split(n))
 
     def train_step(self, prompts) -> dict:
         t0 = time.time()

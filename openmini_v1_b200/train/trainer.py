@@ -116,6 +116,8 @@ class Trainer:
     def _loss(self, batch):
         ids = batch["input_ids"].to(self.device)
         labels = batch["labels"].to(self.device)
+        if ids.is_cuda and hasattr(self.model, "loss"):  # no logits in memory
+            return self.model.loss(ids, labels, self.cfg.label_smoothing_factor)
         logits = self.model(ids)
         return causal_lm_loss(logits, labels, self.cfg.label_smoothing_factor)
 

@@ -585,3 +585,105 @@ def test_native_refusals_name_their_numbers():
     t = torch.zeros(1, 2, 2, 60, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="got 60"):
         _native.C().attention_bwd(t, t, t, t, t, t, None, 1.0, True, t)
+
+
+# ----------------------------------------------------------------------------- through autograd and the policy
+def test_autograd_forms_on_cpu():
+    """The CPU forms of ops.autograd differentiate to the reference statements of the kernels."""
+    from openmini_v1_b200.ops import autograd as ag
+    g = gen("cpu", 3)
+    x, w = randn(g, 2, 5, 16, dtype=F32).requires_grad_(True), randn(g, 24, 16, dtype=F32).requires_grad_(True)
+    t = torch.randint(0, 24, (2, 5), generator=g)
+    t[0, 1] = -100
+    words = words_of(torch.rand(10, 24, generator=g) < 0.7)
+    for kw in (dict(smoothing=0.1), dict(scale=0.5), dict(keep=words)):
+        loss = ag.linear_xent(x, w, t, **kw)
+        want, lse = ops.linear_xent(x.detach(), w.detach(), t, **kw)
+        torch.testing.assert_close(loss.detach(), want)
+        gl = torch.where(torch.isfinite(want), torch.ones_like(want), torch.zeros_like(want))
+        dx, dw = torch.autograd.grad(loss.masked_fill(~torch.isfinite(want), 0.0), (x, w), gl)
+        rx, rw = ops.linear_xent_bwd(x.detach(), w.detach(), t, lse, gl, **kw)
+        torch.testing.assert_close(dx, rx, atol=1e-5, rtol=1e-5)
+        torch.testing.assert_close(dw, rw, atol=1e-5, rtol=1e-5)
+    h = ag.swiglu(x, w)
+    dx, dw = torch.autograd.grad(h, (x, w), torch.ones_like(h))
+    rh, gu = ops.swiglu(x.detach(), w.detach(), save=True)
+    rx, rw = ops.swiglu_bwd(x.detach(), w.detach(), gu, torch.ones_like(h))
+    for a, b in ((h.detach(), rh), (dx, rx), (dw, rw)):
+        torch.testing.assert_close(a, b, atol=1e-5, rtol=1e-5)
+
+
+def small_policy(dev, moe=False, head_dim=64):
+    from openmini_v1_b200.models.config import ModelConfig, MoEConfig
+    from openmini_v1_b200.models.policy import Policy
+    cfg = ModelConfig(name="p", vocab_size=520, hidden_size=192, num_layers=2, num_heads=4, num_kv_heads=2,
+                      head_dim=head_dim, intermediate_size=344, max_position=512, dtype="float32",
+                      moe=MoEConfig(num_experts=4, top_k=2, expert_ffn=72, layer_rule="all") if moe else MoEConfig())
+    return Policy(cfg, device=dev, seed=5)
+
+
+def test_policy_loss_is_the_logits_loss():
+    from openmini_v1_b200.train.loss import causal_lm_loss
+    p = small_policy("cpu")
+    ids = torch.randint(0, 520, (3, 20), generator=gen("cpu", 1))
+    labels = ids.clone()
+    labels[:, :6] = -100
+    for s in (0.0, 0.1):
+        torch.testing.assert_close(p.loss(ids, labels, s), causal_lm_loss(p(ids), labels, s))
+    assert float(p.loss(ids, torch.full_like(ids, -100))) == 0.0
+    from openmini_v1_b200.models.policy import token_logprobs
+    h, lg = p.hidden(ids)[0], p(ids)[0]
+    mask = torch.rand(20, 520, generator=gen("cpu", 2)) < 0.5
+    mask[torch.arange(20), ids[1]] = True
+    torch.testing.assert_close(p.logprobs(h, ids[1], 0.7, words_of(mask)), token_logprobs(lg, ids[1], 0.7, mask),
+                               atol=1e-5, rtol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("moe,head_dim", [(False, 64), (False, 128), (True, 48)])
+def test_policy_loss_and_gradients_on_gpu(moe, head_dim):
+    """A training step on the kernels against the same weights in fp32 on the CPU (bf16 activations
+    through two layers: compared in norm)."""
+    import copy
+    cpu = small_policy("cpu", moe, head_dim)
+    gpu = copy.deepcopy(cpu).to("cuda")
+    gpu.device, gpu.cdt, gpu.inv_freq = torch.device("cuda"), torch.bfloat16, gpu.inv_freq.to("cuda")
+    ids = torch.randint(0, 520, (3, 150), generator=gen("cpu", 1))
+    labels = ids.clone()
+    labels[:, :20] = -100
+    labels[2, 90:] = -100
+    a, b = cpu.loss(ids, labels, 0.05), gpu.loss(ids.cuda(), labels.cuda(), 0.05)
+    assert abs(float(a) - float(b)) < 2e-3 * float(a)
+    a.backward()
+    b.backward()
+    ops.check_status()
+    for (n, pc), (_, pg) in zip(cpu.named_parameters(), gpu.named_parameters()):
+        if pc.grad is None:
+            continue
+        rel = float((pg.grad.cpu() - pc.grad).norm() / (pc.grad.norm() + 1e-12))
+        assert rel < 0.1, (n, rel)
+
+
+@pytest.mark.gpu
+def test_trainer_step_on_gpu_uses_no_logits():
+    from openmini_v1_b200.train.trainer import Trainer, TrainingConfig
+    p = small_policy("cuda")
+
+    def no_logits(*a, **k):
+        raise AssertionError("the logits were computed")
+
+    p.forward = no_logits
+    ids = torch.randint(0, 520, (4, 64), generator=gen("cpu", 4))
+
+    class Loader(list):
+        def set_epoch(self, e):
+            pass
+
+    import tempfile
+    with tempfile.TemporaryDirectory() as d:
+        cfg = TrainingConfig(num_train_epochs=1, learning_rate=1e-3, output_dir=d, save_steps=0, logging_steps=1)
+        tr = Trainer(p, cfg, Loader([{"input_ids": ids, "labels": ids}] * 8))
+        st = tr.train()
+    losses = [r["loss"] for r in st.history if "loss" in r]
+    assert losses[-1] < losses[0] and all(math.isfinite(v) for v in losses)
+    ops.check_status()

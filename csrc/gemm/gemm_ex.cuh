@@ -11,22 +11,31 @@
 // an argument: BN / 2 for one matrix, F for the two stacked projections of a gated block, so
 // gate and up columns of the same features meet in one accumulator tile.
 //
-// Roles as in gemm_tc.cuh (256 threads: TMA warp, MMA warp, TMEM warp, four epilogue warps),
-// two TMEM accumulators, so that the epilogue of tile i runs beside the products of tile i+1.
+// Roles: TMA warp, MMA warp, TMEM warp, and eight epilogue warps (two for each quarter of the
+// accumulator's lanes, taking its columns in turn, because the epilogues here are more than a
+// store); two TMEM accumulators, so that the epilogue of tile i runs beside the products of tile
+// i+1.
 // What bounds it: 128 x 256 tiles read 12 KB of shared memory per 16-deep MMA step (96 of its
 // 128 cycles), so the tensor pipe, not shared memory, is the limit for BN = 256; BN = 64 and
 // 128 are for grids that would otherwise leave SMs idle.
 //
-// Results leave through shared memory: an epilogue warp lays 32 rows x 128 bytes into one of its
-// two 4 KB buffers (128-byte swizzle, no bank conflicts) and a TMA store writes whole lines, while
-// the warp goes on with the next columns. Direct 16-byte stores, one row a lane, touch 32 lines an
-// instruction; they remain for outputs whose rows do not start on 16 bytes.
+// Results leave through shared memory: an epilogue warp lays 32 rows x 128 bytes into its 4 KB
+// buffer (128-byte swizzle, no bank conflicts) and a TMA store writes whole lines, while the warp
+// goes on with the next columns. (Direct 16-byte stores, one row a lane, touch 32 lines an
+// instruction.)
 //
-// Epi is a functor type with Args and
+// The tensor cores add in fp32 but cut off instead of rounding, which over thousands of additions
+// is a bias of 1e-6 relative and more. An Epi whose results are kept in fp32 asks for segments
+// (SEG steps of 64): each is accumulated apart, and the epilogue adds them in registers, rounded.
+//
+// Epi is a functor type with Args, SEG and
 //   static Row row(const GemmX&, const Args&, int r)
-//   template <int BN> static void tile(const GemmX&, const Args&, const Row&, const OutMaps&, RowStage&,
-//                                      uint32_t tbase, int r, int tc, int sp)
-// called by every epilogue thread (accumulator row r, TMEM lane address tbase).
+//   SEG == 0: template <int BN> static void tile(const GemmX&, const Args&, const Row&, const OutMaps&,
+//                                 RowStage&, uint32_t tbase, int r, int tc, int sp, int half)
+//   SEG > 0:  template <int BN> static void finish(const GemmX&, const Args&, const Row&,
+//                                 float (&z)[BN / 2], int r, int tc, int half)
+// called by every epilogue thread (accumulator row r, TMEM lane address tbase); `half` takes the
+// 32- or 64-column pieces half, half + 2, ... of the tile.
 #pragma once
 #include <cuda.h>
 #include "../common/om_ptx.cuh"
@@ -48,16 +57,14 @@ struct OutMaps {
   CUtensorMap m[3];  // what an Epi stores through; unused ones are zero
 };
 
-// The two buffers of one epilogue warp, used in turn.
+// The buffer of one epilogue warp.
 struct RowStage {
-  uint8_t* base;  // 2 x 4096 bytes, 1024-byte aligned
-  int lane, turn;
-  __device__ __forceinline__ uint8_t* begin() {  // a buffer whose last store has been read
-    if (lane == 0) bulk_wait_read<1>();
+  uint8_t* base;  // 4096 bytes, 1024-byte aligned
+  int lane;
+  __device__ __forceinline__ uint8_t* begin() const {  // its last store has been read
+    if (lane == 0) bulk_wait_read<0>();
     __syncwarp();
-    uint8_t* b = base + turn * 4096;
-    turn ^= 1;
-    return b;
+    return base;
   }
   // 32 bf16 columns into half `h` of the lane's 64-column row / 32 fp32 columns
   __device__ __forceinline__ void put(uint8_t* b, int h, const float (&f)[32]) const {
@@ -89,6 +96,7 @@ struct RowStage {
   }
 };
 
+constexpr int GX_THREADS = 384;
 constexpr int GX_GROUP = 16;  // row tiles walked before the next column tile: 16 x 9 tiles in flight share L2 lines
 
 __device__ __forceinline__ void gx_coords(const GemmX& g, int u, int& tr, int& tc, int& sp) {
@@ -117,13 +125,19 @@ struct GemmXCfg {
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = (192 * 1024) / STAGE_BYTES > 16 ? 16 : (192 * 1024) / STAGE_BYTES;
   static constexpr int TMEM_COLS = BN <= 128 ? 2 * BN : 512;  // a power of two
-  static constexpr int OUT_BYTES = 4 * 2 * 4096;  // four epilogue warps; also what lies behind a short A
+  static constexpr int OUT_BYTES = 8 * 4096;  // eight epilogue warps; also what lies behind a short A
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 /*align slack*/ + 512;
   static_assert((128 - AR) * BK * 2 <= B_BYTES + OUT_BYTES, "the MMA reads 128 rows of A");
 };
 
+// Steps of one segment: the whole contraction (`kb1` is past its end) unless the Epi wants shorter ones.
+template <class Epi>
+__device__ __forceinline__ int gx_seg(int kb1) {
+  return Epi::SEG ? Epi::SEG : kb1;
+}
+
 template <int BN, int AR, bool AMN, bool BMN, class Epi>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(GX_THREADS, 1)
     gemm_ex_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ OutMaps outs, const GemmX g, const typename Epi::Args e) {
   using C = GemmXCfg<BN, AR>;
@@ -146,7 +160,7 @@ __global__ void __launch_bounds__(256, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 128);
+      mbar_init(&tempty[a], 256);
     }
     fence_barrier_init();
   }
@@ -202,48 +216,75 @@ __global__ void __launch_bounds__(256, 1)
       constexpr uint32_t IDESC = idesc_bf16_x(128, BN, AMN, BMN);
       int it = 0, local = 0;
       bool ok = true;
-      for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++local) {
+      for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
         int tr, tc, sp;
         gx_coords(g, u, tr, tc, sp);
         const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
-        const int acc = local & 1;
-        if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, g.status, OM_ERR_WAIT_ACCUM)) break;
-        tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          if (!mbar_wait(&full[s], (it / C::STAGES) & 1, g.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+        for (int s0 = kb0; s0 < kb1 && ok; s0 += gx_seg<Epi>(kb1), ++local) {
+          const int acc = local & 1, s1 = min(kb1, s0 + gx_seg<Epi>(kb1));
+          if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, g.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::A_BYTES;
+          for (int kb = s0; kb < s1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (!mbar_wait(&full[s], (it / C::STAGES) & 1, g.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::A_BYTES;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // 16 deep: 32 bytes of a K-major row, two 8-row atoms MN-major
-            const uint64_t ad = AMN ? smem_desc_sw128_mn(a_addr + k * 2048, 8192, 1024)
-                                    : smem_desc_sw128(a_addr + k * 32, 1024);
-            const uint64_t bd = BMN ? smem_desc_sw128_mn(b_addr + k * 2048, 8192, 1024)
-                                    : smem_desc_sw128(b_addr + k * 32, 1024);
-            tc_mma_f16(tmem + acc * BN, ad, bd, IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) {  // 16 deep: 32 bytes of a K-major row, two 8-row atoms MN-major
+              const uint64_t ad = AMN ? smem_desc_sw128_mn(a_addr + k * 2048, 8192, 1024)
+                                      : smem_desc_sw128(a_addr + k * 32, 1024);
+              const uint64_t bd = BMN ? smem_desc_sw128_mn(b_addr + k * 2048, 8192, 1024)
+                                      : smem_desc_sw128(b_addr + k * 32, 1024);
+              tc_mma_f16(tmem + acc * BN, ad, bd, IDESC, (kb > s0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit(&empty[s]);
           }
-          tc_commit(&empty[s]);
+          if (ok) tc_commit(&tfull[acc]);
         }
-        if (ok) tc_commit(&tfull[acc]);
       }
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;
-    RowStage stage{out_bytes + q * 8192, lane, 0};
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const RowStage stage{out_bytes + (warp - 4) * 4096, lane};
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     int local = 0;
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++local) {
+    bool ok = true;
+    for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       int tr, tc, sp;
       gx_coords(g, u, tr, tc, sp);
-      const int acc = local & 1;
       const int r = tr * 128 + q * 32 + lane;
       const auto row = Epi::row(g, e, r);  // the row's own inputs, read while the products run
-      bool ok = mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      Epi::template tile<BN>(g, e, row, outs, stage, tmem + ((uint32_t)(q * 32) << 16) + acc * BN, r, tc, sp);
-      tc_fence_before();
-      mbar_arrive(&tempty[acc]);
+      if constexpr (Epi::SEG == 0) {
+        const int acc = local & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM));
+        if (!ok) break;
+        ++local;
+        tc_fence_after();
+        Epi::template tile<BN>(g, e, row, outs, stage, lanes + acc * BN, r, tc, sp, half);
+        tc_fence_before();
+        mbar_arrive(&tempty[acc]);
+      } else {
+        float z[BN / 2];
+        const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+        for (int s0 = kb0; s0 < kb1; s0 += gx_seg<Epi>(kb1), ++local) {
+          const int acc = local & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < BN / 32; ++i) {  // 16 columns at a time: z takes most of the registers
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(lanes + acc * BN + (2 * (i >> 1) + half) * 32 + (i & 1) * 16, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[i * 16 + j] = (s0 == kb0 ? 0.f : z[i * 16 + j]) + __uint_as_float(v[j]);
+          }
+          tc_fence_before();
+          mbar_arrive(&tempty[acc]);
+        }
+        if (ok) Epi::template finish<BN>(g, e, row, z, r, tc, half);
+      }
     }
     if (lane == 0) bulk_wait<0>();  // the stores are complete before the CTA's memory goes
   }
@@ -266,12 +307,12 @@ struct GemmPairCfg {
   static constexpr int A_BYTES = 128 * 64 * 2;
   static constexpr int STAGE_BYTES = 2 * A_BYTES;
   static constexpr int STAGES = 6;
-  static constexpr int OUT_BYTES = 4 * 2 * 4096;
+  static constexpr int OUT_BYTES = 8 * 4096;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
 };
 
 template <bool AMN, bool BMN, class Epi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GX_THREADS, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ OutMaps outs, const GemmX g, const typename Epi::Args e) {
   using C = GemmPairCfg;
@@ -297,7 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);
+      mbar_init(&tempty[a], 16);
     }
     fence_barrier_init();
   }
@@ -363,49 +404,77 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
       constexpr uint32_t IDESC = idesc_bf16_x(256, 256, AMN, BMN);
       int it = 0, local = 0;
       bool ok = true;
-      for (int u = pair; u < units && ok; u += pairs, ++local) {
+      for (int u = pair; u < units && ok; u += pairs) {
         int tr, tc, sp;
         gx_coords(g, u, tr, tc, sp);
         const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
-        const int acc = local & 1;
-        if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, g.status, OM_ERR_WAIT_ACCUM)) break;
-        tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % C::STAGES;
-          if (!mbar_wait(&full[s], (it / C::STAGES) & 1, g.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+        for (int s0 = kb0; s0 < kb1 && ok; s0 += gx_seg<Epi>(kb1), ++local) {
+          const int acc = local & 1, s1 = min(kb1, s0 + gx_seg<Epi>(kb1));
+          if (!mbar_wait(&tempty[acc], ((local >> 1) & 1) ^ 1, g.status, OM_ERR_WAIT_ACCUM)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::A_BYTES;
+          for (int kb = s0; kb < s1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (!mbar_wait(&full[s], (it / C::STAGES) & 1, g.status, OM_ERR_WAIT_FULL)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t a_addr = smem_u32(smem + s * C::STAGE_BYTES), b_addr = a_addr + C::A_BYTES;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = AMN ? smem_desc_sw128_mn(a_addr + k * 2048, 8192, 1024)
-                                    : smem_desc_sw128(a_addr + k * 32, 1024);
-            const uint64_t bd = BMN ? smem_desc_sw128_mn(b_addr + k * 2048, 8192, 1024)
-                                    : smem_desc_sw128(b_addr + k * 32, 1024);
-            tc_mma_f16_pair(tmem + acc * 256, ad, bd, IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < 4; ++k) {  // 16 deep: 32 bytes of a K-major row, two 8-row atoms MN-major
+              const uint64_t ad = AMN ? smem_desc_sw128_mn(a_addr + k * 2048, 8192, 1024)
+                                      : smem_desc_sw128(a_addr + k * 32, 1024);
+              const uint64_t bd = BMN ? smem_desc_sw128_mn(b_addr + k * 2048, 8192, 1024)
+                                      : smem_desc_sw128(b_addr + k * 32, 1024);
+              tc_mma_f16_pair(tmem + acc * 256, ad, bd, IDESC, (kb > s0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit_pair(&empty[s]);
           }
-          tc_commit_pair(&empty[s]);
+          if (ok) tc_commit_pair(&tfull[acc]);
         }
-        if (ok) tc_commit_pair(&tfull[acc]);
       }
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue (each CTA its 128 rows)
-    const int q = warp & 3;
-    RowStage stage{out_bytes + q * 8192, lane, 0};
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const RowStage stage{out_bytes + (warp - 4) * 4096, lane};
+    const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
     int local = 0;
-    for (int u = pair; u < units; u += pairs, ++local) {
+    bool ok = true;
+    for (int u = pair; u < units && ok; u += pairs) {
       int tr, tc, sp;
       gx_coords(g, u, tr, tc, sp);
-      const int acc = local & 1;
       const int r = tr * 256 + (int)rank * 128 + q * 32 + lane;
-      const auto row = Epi::row(g, e, r);
-      bool ok = mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tc_fence_after();
-      Epi::template tile<256>(g, e, row, outs, stage, tmem + ((uint32_t)(q * 32) << 16) + acc * 256, r, tc, sp);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(pair_addr(&tempty[acc], 0));
+      const auto row = Epi::row(g, e, r);  // the row's own inputs, read while the products run
+      if constexpr (Epi::SEG == 0) {
+        const int acc = local & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM));
+        if (!ok) break;
+        ++local;
+        tc_fence_after();
+        Epi::template tile<256>(g, e, row, outs, stage, lanes + acc * 256, r, tc, sp, half);
+        tc_fence_before();
+        __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(pair_addr(&tempty[acc], 0));
+      } else {
+        float z[256 / 2];
+        const int kb0 = sp * g.kb_per_split, kb1 = min(g.num_kb, kb0 + g.kb_per_split);
+        for (int s0 = kb0; s0 < kb1; s0 += gx_seg<Epi>(kb1), ++local) {
+          const int acc = local & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&tfull[acc], (local >> 1) & 1, g.status, OM_ERR_WAIT_ACCUM));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 256 / 32; ++i) {  // 16 columns at a time: z takes most of the registers
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(lanes + acc * 256 + (2 * (i >> 1) + half) * 32 + (i & 1) * 16, v);
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[i * 16 + j] = (s0 == kb0 ? 0.f : z[i * 16 + j]) + __uint_as_float(v[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(pair_addr(&tempty[acc], 0));
+        }
+        if (ok) Epi::template finish<256>(g, e, row, z, r, tc, half);
+      }
     }
     if (lane == 0) bulk_wait<0>();
   }
@@ -419,15 +488,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(256, 1)
   }
 }
 
-// 32 fp32 of one accumulator row, columns c0 .. c0 + 31, to bf16. `n` of them exist.
+// n of 32 columns of one accumulator row, in 16-byte stores where they are whole.
 __device__ __forceinline__ void store_row32(__nv_bfloat16* dst, const float (&f)[32], int n, bool vec) {
-  if (n >= 32 && vec) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) *reinterpret_cast<uint4*>(dst + j) = pack8(f + j);
-  } else {
+  for (int j = 0; j < 32; j += 8) {
+    if (j + 8 <= n && vec) {
+      *reinterpret_cast<uint4*>(dst + j) = pack8(f + j);
+    } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) dst[j] = __float2bfloat16_rn(f[j]);
+      for (int i = 0; i < 8; ++i)
+        if (j + i < n) dst[j + i] = __float2bfloat16_rn(f[j + i]);
+    }
+  }
+}
+__device__ __forceinline__ void store_row32(float* dst, const float (&f)[32], int n, bool vec) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    if (j + 4 <= n && vec) {
+      *reinterpret_cast<float4*>(dst + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i < n) dst[j + i] = f[j + i];
+    }
   }
 }
 
@@ -436,12 +519,13 @@ struct NoRow {};
 // bf16 rows through map 0, 64 columns a store.
 struct EpiStore {
   struct Args {};
+  static constexpr int SEG = 0;
   static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
   template <int BN>
   static __device__ __forceinline__ void tile(const GemmX& g, const Args&, const NoRow&, const OutMaps& o,
-                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
+                                              const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
 #pragma unroll 1
-    for (int cc = 0; cc < BN / 64; ++cc) {
+    for (int cc = half; cc < BN / 64; cc += 2) {
       const int c0 = tc * BN + cc * 64;
       if (c0 >= g.cols || r - st.lane >= g.rows) break;  // the same for the whole warp
       uint8_t* b = st.begin();
@@ -467,12 +551,13 @@ struct EpiSum {
   struct Args {
     int add;
   };
+  static constexpr int SEG = 0;
   static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
   template <int BN>
   static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const NoRow&, const OutMaps& o,
-                                              RowStage& st, uint32_t tbase, int r, int tc, int sp) {
+                                              const RowStage& st, uint32_t tbase, int r, int tc, int sp, int half) {
 #pragma unroll 1
-    for (int cc = 0; cc < BN / 32; ++cc) {
+    for (int cc = half; cc < BN / 32; cc += 2) {
       const int c0 = tc * BN + cc * 32;
       if (c0 >= g.cols || r - st.lane >= g.rows) break;
       uint8_t* b = st.begin();

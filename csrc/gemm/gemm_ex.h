@@ -45,7 +45,7 @@ void gx_launch(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps& outs
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 31), "gemm: too many tiles");
   const int grid = (int)std::min<long long>(units, num_sms());
-  launch_dependent(gemm_ex_kernel<BN, AR, AMN, BMN, Epi>, grid, 256, C::SMEM_BYTES, st, ta, tb, outs, g, e);
+  launch_dependent(gemm_ex_kernel<BN, AR, AMN, BMN, Epi>, grid, GX_THREADS, C::SMEM_BYTES, st, ta, tb, outs, g, e);
 }
 
 // On CTA pairs; g.tiles_r counts 256-row tiles, K-major operands have boxes of 128 rows.
@@ -63,7 +63,7 @@ void gx_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps&
   const long long units = (long long)g.tiles_r * g.tiles_c * g.splits;
   TORCH_CHECK(units < (1ll << 30), "gemm: too many tiles");
   const int pairs = (int)std::min<long long>(units, num_sms() / 2);
-  launch_dependent(gemm_pair_kernel<AMN, BMN, Epi>, 2 * pairs, 256, GemmPairCfg::SMEM_BYTES, st, ta, tb, outs, g, e);
+  launch_dependent(gemm_pair_kernel<AMN, BMN, Epi>, 2 * pairs, GX_THREADS, GemmPairCfg::SMEM_BYTES, st, ta, tb, outs, g, e);
 }
 
 // Whether a product goes to pairs: a 256 x 256 tile for every pair of SMs, rows that fill more than

@@ -22,34 +22,23 @@ namespace om {
 // exp(-g) = inf gives 0, as it should
 __device__ __forceinline__ float sigmoid_f(float g) { return fast_rcp(1.f + fast_exp2(-1.4426950408889634f * g)); }
 
-// n of 32 fp32 columns
-__device__ __forceinline__ void store_row32(float* dst, const float (&f)[32], int n, bool vec) {
-  if (n >= 32 && vec) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 4)
-      *reinterpret_cast<float4*>(dst + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (j < n) dst[j] = f[j];
-  }
-}
-
-// Maps: 0 h, 1 g, 2 u (`maps`: all that is written has one; else plain stores).
+// Rows of h, g and u are laid out a multiple of 8 elements apart (ldh, ldu: F rounded up), whatever F is.
+// Maps: 0 h, 1 g, 2 u; without `maps` (narrow tiles) plain stores.
 struct EpiSwiglu {
   struct Args {
     __nv_bfloat16* h;
-    float* gu;  // optional [M, ldgu]: g at column f, u at column F + f
-    int ldh, ldgu, vec_h, vec_gu, maps;
+    float* gu;  // optional [M, 2 ld]: g at column f, u at column ld + f
+    int ld, maps;
   };
+  static constexpr int SEG = 0;
   static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
   template <int BN>
   static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const NoRow&, const OutMaps& o,
-                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
+                                              const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
     constexpr int HALF = BN / 2;
     const int F = g.cols, r0 = r - st.lane;
 #pragma unroll 1
-    for (int cc = 0; cc < HALF / 32; ++cc) {
+    for (int cc = half; cc < HALF / 32; cc += 2) {
       const int c0 = tc * g.b_step + cc * 32;
       if (c0 >= F || r0 >= g.rows) break;
       uint32_t gv[32], uv[32];
@@ -79,39 +68,39 @@ struct EpiSwiglu {
       }
       if (r >= g.rows) continue;
       const int n = min(min(32, g.b_step - cc * 32), F - c0);
-      store_row32(e.h + (size_t)r * e.ldh + c0, hf, n, e.vec_h);
+      const bool vec = (c0 & 7) == 0;
+      store_row32(e.h + (size_t)r * e.ld + c0, hf, n, vec);
       if (e.gu != nullptr) {
-        store_row32(e.gu + (size_t)r * e.ldgu + c0, gf, n, e.vec_gu);
-        store_row32(e.gu + (size_t)r * e.ldgu + F + c0, uf, n, e.vec_gu && (F & 3) == 0);
+        store_row32(e.gu + (size_t)r * 2 * e.ld + c0, gf, n, vec);
+        store_row32(e.gu + ((size_t)r * 2 + 1) * e.ld + c0, uf, n, vec);
       }
     }
   }
 };
 
-// dg, du of one row block; V = 8 where every row start and F allow 16-byte accesses, else 1.
+// dg, du, V columns a thread: 8 where dh's and the result's rows start on 16 bytes, else 1. The block
+// is blockDim.x columns' worth by blockDim.y rows.
 template <int V>
-__global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restrict__ gu, long long ldgu,
+__global__ void __launch_bounds__(256) swiglu_grad_kernel(const float* __restrict__ gu, int ld,
                                                           const __nv_bfloat16* __restrict__ dh, long long lddh,
                                                           __nv_bfloat16* __restrict__ dgu, long long lddgu,
                                                           long long M, int F) {
   grid_wait();
   grid_release();
-  const int nv = F / V;
-  const long long n = M * nv;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long r = i / nv;
-    const int c = (int)(i - r * nv) * V;
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * V;
+  if (c >= F) return;
+  for (long long r = blockIdx.y * (long long)blockDim.y + threadIdx.y; r < M; r += gridDim.y * (long long)blockDim.y) {
     float g[V], u[V], d[V];
+    const float* pg = gu + r * 2 * ld + c;
     if constexpr (V == 8) {
-      const float4* pg = reinterpret_cast<const float4*>(gu + r * ldgu + c);
-      const float4* pu = reinterpret_cast<const float4*>(gu + r * ldgu + F + c);
-      const float4 g0 = pg[0], g1 = pg[1], u0 = pu[0], u1 = pu[1];
+      const float4 g0 = reinterpret_cast<const float4*>(pg)[0], g1 = reinterpret_cast<const float4*>(pg)[1];
+      const float4 u0 = reinterpret_cast<const float4*>(pg + ld)[0], u1 = reinterpret_cast<const float4*>(pg + ld)[1];
+      unpack8(*reinterpret_cast<const uint4*>(dh + r * lddh + c), d);
       g[0] = g0.x; g[1] = g0.y; g[2] = g0.z; g[3] = g0.w; g[4] = g1.x; g[5] = g1.y; g[6] = g1.z; g[7] = g1.w;
       u[0] = u0.x; u[1] = u0.y; u[2] = u0.z; u[3] = u0.w; u[4] = u1.x; u[5] = u1.y; u[6] = u1.z; u[7] = u1.w;
-      unpack8(*reinterpret_cast<const uint4*>(dh + r * lddh + c), d);
     } else {
-      g[0] = gu[r * ldgu + c];
-      u[0] = gu[r * ldgu + F + c];
+      g[0] = pg[0];
+      u[0] = pg[ld];
       d[0] = __bfloat162float(dh[r * lddh + c]);
     }
 #pragma unroll
@@ -150,29 +139,27 @@ void check_swiglu(const char* op, const torch::Tensor& x, const torch::Tensor& w
 
 }  // namespace
 
-// (h [..., F] = silu(x Wg^T) * (x Wu^T), gu fp32 [rows, 2F] if saved)
+// (h [..., F] = silu(x Wg^T) * (x Wu^T), gu fp32 [rows, 2 Fp] if saved). Fp is F rounded up to 8: rows
+// of h are Fp apart, so that F need not be a multiple of anything for whole-line stores.
 std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x, torch::Tensor w, bool save,
                                                                  torch::Tensor status) {
   check_swiglu("swiglu", x, w);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t K = x.size(x.dim() - 1), F = w.size(0) / 2, M = x.numel() / K;
+  const int64_t Fp = (F + 7) / 8 * 8;
   auto shape = x.sizes().vec();
-  shape.back() = F;
+  shape.back() = Fp;
   auto h = torch::empty(shape, x.options());
+  if (Fp != F) h = h.narrow(-1, 0, F);
   c10::optional<torch::Tensor> gu;
-  if (save) gu = torch::empty({M, 2 * F}, x.options().dtype(at::kFloat));
+  if (save) gu = torch::empty({M, 2 * Fp}, x.options().dtype(at::kFloat));
   if (M == 0 || F == 0) return {h, gu};
   const torch::Tensor x2 = om::tma_rows(x), w2 = om::tma_rows(w);
   auto st = at::cuda::getCurrentCUDAStream().stream();
   om::EpiSwiglu::Args e{};
   e.h = reinterpret_cast<__nv_bfloat16*>(h.data_ptr());
-  e.ldh = (int)F;
-  e.vec_h = F % 8 == 0;
-  if (save) {
-    e.gu = gu->data_ptr<float>();
-    e.ldgu = (int)(2 * F);
-    e.vec_gu = F % 2 == 0;
-  }
+  e.ld = (int)Fp;
+  if (save) e.gu = gu->data_ptr<float>();
   GemmX g{};
   g.rows = (int)M;
   g.cols = (int)F;
@@ -191,13 +178,11 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
     const CUtensorMap tb = om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), 128);
     g.b_step = g.b_box = 128;
     g.tiles_c = om::ceil_div(F, 128);
-    e.maps = om::gx_storable(e.h, F, 2);  // F a multiple of 8: every row of h, g and u starts on 16 bytes
-    if (e.maps) {
-      o.m[0] = om::gx_out32(e.h, M, F, F);
-      if (save) {
-        o.m[1] = om::gx_out(e.gu, M, F, 2 * F);
-        o.m[2] = om::gx_out(e.gu + F, M, F, 2 * F);
-      }
+    e.maps = 1;
+    o.m[0] = om::gx_out32(e.h, M, F, Fp);
+    if (save) {
+      o.m[1] = om::gx_out(e.gu, M, F, 2 * Fp);
+      o.m[2] = om::gx_out(e.gu + Fp, M, F, 2 * Fp);
     }
     if (om::gx_pairs(M, 2 * F, K)) {
       g.tiles_r = om::ceil_div(M, 256);
@@ -213,7 +198,9 @@ std::pair<torch::Tensor, c10::optional<torch::Tensor>> om_swiglu(torch::Tensor x
   // With 32 tokens or fewer, A is loaded 32 rows high and the room is 16 stages of weights.
   const int waves = om::ceil_div((int64_t)g.tiles_r * om::ceil_div(F, 32), sms);
   const int64_t tiles = std::max<int64_t>(1, (int64_t)waves * sms / g.tiles_r);
-  g.b_step = g.b_box = (int)std::min<int64_t>(32, std::max<int64_t>(8, om::ceil_div(F, tiles)));
+  int64_t step = std::min<int64_t>(32, std::max<int64_t>(8, om::ceil_div(F, tiles)));
+  if (M > 32) step = (step + 7) / 8 * 8;  // many rows: whole 16-byte stores matter more
+  g.b_step = g.b_box = (int)step;
   g.tiles_c = om::ceil_div(F, g.b_step);
   const CUtensorMap ta = om::gx_map(x2.data_ptr(), false, M, K, x2.stride(0), M <= 32 ? 32 : 128);
   const CUtensorMap tb = om::gx_map(w2.data_ptr(), false, 2 * F, K, w2.stride(0), g.b_box);
@@ -232,9 +219,10 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_swiglu_
   check_swiglu("swiglu_bwd", x, w);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t K = x.size(x.dim() - 1), F = w.size(0) / 2, M = x.numel() / K;
+  const int64_t Fp = (F + 7) / 8 * 8;
   TORCH_CHECK(gu.is_cuda() && gu.scalar_type() == at::kFloat && gu.dim() == 2 && gu.size(0) == M &&
-                  gu.size(1) == 2 * F && gu.is_contiguous(),
-              "swiglu_bwd: gu must be fp32 [rows, 2F] as swiglu saved it");
+                  gu.size(1) == 2 * Fp && gu.is_contiguous() && (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0,
+              "swiglu_bwd: gu must be the fp32 projections that swiglu saved");
   TORCH_CHECK(dh.is_cuda() && dh.numel() == M * F && (F == 0 || dh.size(-1) == F), "swiglu_bwd: dh must be [..., F]");
   c10::optional<torch::Tensor> dx, dw;
   if (need_dx) dx = torch::empty(x.sizes(), x.options());
@@ -249,12 +237,14 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_swiglu_
   const int64_t ld = (2 * F + 7) / 8 * 8;
   auto dgu = torch::empty({M, ld}, x.options());
   auto ptr = [](const torch::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); };
-  const bool v8 = F % 8 == 0 && (reinterpret_cast<uintptr_t>(gu.data_ptr()) & 15) == 0 && d2.stride(0) % 8 == 0 &&
-                  (reinterpret_cast<uintptr_t>(d2.data_ptr()) & 15) == 0;
-  const long long work = M * (v8 ? F / 8 : F);
-  const int blocks = (int)std::min<long long>((work + 255) / 256, (long long)om::num_sms() * 16);
-  auto grad = v8 ? om::swiglu_grad_kernel<8> : om::swiglu_grad_kernel<1>;
-  om::launch_dependent(grad, blocks, 256, 0, st, gu.data_ptr<float>(), (long long)(2 * F), ptr(d2),
+  const bool v8 = F % 8 == 0 && d2.stride(0) % 8 == 0 && (reinterpret_cast<uintptr_t>(d2.data_ptr()) & 15) == 0;
+  const int cols = (int)(v8 ? F / 8 : F);
+  int bx = 32;
+  while (bx < 256 && bx < cols) bx *= 2;
+  const dim3 block(bx, 256 / bx);
+  const dim3 blocks(om::ceil_div(cols, bx), (unsigned)std::min<int64_t>(om::ceil_div(M, block.y), 65535));
+  om::launch_dependent(v8 ? om::swiglu_grad_kernel<8> : om::swiglu_grad_kernel<1>, blocks, block, 0, st,
+                       (const float*)gu.data_ptr<float>(), (int)Fp, (const __nv_bfloat16*)ptr(d2),
                        (long long)d2.stride(0), ptr(dgu), (long long)ld, (long long)M, (int)F);
   auto product = [&](om::GxOperand a, om::GxOperand b, int64_t rows, int64_t cols, int64_t k, torch::Tensor& out) {
     const om::GxPlan p = om::gx_plan(rows, cols, k);

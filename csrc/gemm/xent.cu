@@ -6,8 +6,8 @@
 //   dz_j = gloss (exp(z_j - lse) - e / V - (1 - e) [j = t]),   dx = c dz W,  dW = c dz^T x
 //
 // Forward: the GEMM's epilogue reduces each 128 x 256 tile of logits to one (max, sum of
-// exponentials) pair a row, in base 2 and fp32, and picks z_t; a second kernel joins the pairs of
-// a row in tile order. What leaves the chip is M V / 32 bytes instead of 4 M V.
+// exponentials) pair a row and half tile, in base 2 and fp32, and picks z_t; a second kernel joins
+// the pairs of a row in a fixed order. What leaves the chip is M V / 16 bytes instead of 4 M V.
 //
 // Gradient: the vocabulary is walked in pieces. Each piece's logits are computed again, and the
 // epilogue turns them into dz (16 bits: its rounding is 2^-9 relative per entry and independent,
@@ -34,55 +34,54 @@ struct XentRows {
   int V;
 };
 
-// Fwd partials of row r and column tile tc: (max, sum 2^(z2 - max)) with z2 = z log2 e.
+// Fwd partials of row r and half of column tile tc: (max, sum 2^(z2 - max)) with z2 = z log2 e. The
+// logits are summed in segments of 1024: loss and lse stay in fp32, where the tensor cores' cutting
+// off shows (K = 5120: 8e-7 of lse in one piece; the segments are added with rounding).
 template <bool SMOOTH>
 struct EpiXentFwd {
   struct Args {
     XentRows x;
-    float2* part;   // [tiles_c][M]
-    float* sumz;    // [tiles_c][M] sums of z (SMOOTH)
+    float2* part;   // [2 tiles_c][M]
+    float* sumz;    // [2 tiles_c][M] sums of z (SMOOTH)
     float* zt;      // [M] z of the target, -inf if masked
   };
+  static constexpr int SEG = 16;
   static __device__ __forceinline__ long long row(const GemmX& g, const Args& e, int r) {
     return r < g.rows ? e.x.targets[r] : -1;
   }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const long long& target, const OutMaps&,
-                                              RowStage&, uint32_t tbase, int r, int tc, int) {
+  static __device__ __forceinline__ void finish(const GemmX& g, const Args& e, const long long& target,
+                                                float (&z)[BN / 2], int r, int tc, int half) {
     const bool row = r < g.rows;
-    const int t0 = tc * BN;
-    // the target's column within this tile, or a value no column has
-    const long long in = target - t0;
-    const int tcol = target >= 0 && in >= 0 && in < BN ? (int)in : -1;
     const float c2 = e.x.scale * XE_LOG2E;
     float m = -INFINITY, s = 0.f, zs = 0.f;
-#pragma unroll 1
-    for (int cc = 0; cc < BN / 32; ++cc) {
-      const int c0 = t0 + cc * 32;
-      if (c0 >= g.cols) break;
-      uint32_t v[32];
-      tmem_ld_32x32b_x32(tbase + cc * 32, v);
-      uint32_t bits = 0xffffffffu;
-      if (g.cols - c0 < 32) bits = (1u << (g.cols - c0)) - 1u;
-      if (e.x.keep != nullptr && row) bits &= (uint32_t)e.x.keep[r * e.x.ldk + (c0 >> 5)];
-      tc_wait_ld();
-      float f[32], mx = -INFINITY;
-      if (bits == 0xffffffffu) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * c2;
-      } else {
+    for (int i = 0; i < BN / 64; ++i) {
+      const int c0 = tc * BN + (2 * i + half) * 32;
+      uint32_t bits = g.cols - c0 >= 32 ? 0xffffffffu : g.cols > c0 ? (1u << (g.cols - c0)) - 1u : 0u;
+      if (e.x.keep != nullptr && row && bits) bits &= (uint32_t)e.x.keep[r * e.x.ldk + (c0 >> 5)];
+      float* f = z + i * 32;  // z2 in place; masked columns -inf
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? __uint_as_float(v[j]) * c2 : -INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < 32; ++j) mx = fmaxf(mx, f[j]);
+      for (int j = 0; j < 32; ++j) f[j] *= c2;
       if constexpr (SMOOTH) {
-        float a = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a += (bits >> j) & 1u ? __uint_as_float(v[j]) : 0.f;
-        zs += a;
+        for (int j = 0; j < 32; ++j) zs += (bits >> j) & 1u ? f[j] : 0.f;
       }
-      const float mn = fmaxf(m, mx);
+      const long long in = target - c0;
+      if (target >= 0 && in >= 0 && in < 32) {
+        const uint32_t hit = bits & (1u << (int)in);  // a mask, not an index: registers stay registers
+        float t = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t += (hit >> j) & 1u ? f[j] : 0.f;
+        e.zt[r] = hit ? t * XE_LN2 : -INFINITY;
+      }
+      if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = (bits >> j) & 1u ? f[j] : -INFINITY;
+      }
+      float mn = m;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) mn = fmaxf(mn, f[j]);
       const float ref = mn == -INFINITY ? 0.f : mn;  // nothing kept so far: every term is 2^-inf = 0
       float a0 = 0.f, a1 = 0.f;
 #pragma unroll
@@ -92,18 +91,11 @@ struct EpiXentFwd {
       }
       s = s * fast_exp2(m - ref) + (a0 + a1);
       m = mn;
-      if ((tcol >> 5) == cc) {  // tcol = -1 matches no chunk
-        const uint32_t hit = bits & (1u << (tcol & 31));  // a mask, not an index: registers stay registers
-        float z = 0.f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) z += (hit >> i) & 1u ? __uint_as_float(v[i]) : 0.f;
-        e.zt[r] = hit ? z * e.x.scale : -INFINITY;
-      }
     }
     if (row) {
-      const size_t at = (size_t)tc * g.rows + r;
+      const size_t at = (size_t)(2 * tc + half) * g.rows + r;
       e.part[at] = make_float2(m, s);
-      if constexpr (SMOOTH) e.sumz[at] = zs * e.x.scale;
+      if constexpr (SMOOTH) e.sumz[at] = zs * XE_LN2;
     }
   }
 };
@@ -167,6 +159,7 @@ struct EpiXentBwd {
     float smoothing;
     int v0;              // the piece's first column
   };
+  static constexpr int SEG = 0;
   struct Row {
     float gz, l2;  // c gloss (0: ignored), lse log2 e
     int tcol;      // the target's column in the piece, or -1
@@ -183,11 +176,11 @@ struct EpiXentBwd {
   }
   template <int BN>
   static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const Row& w, const OutMaps& o,
-                                              RowStage& st, uint32_t tbase, int r, int tc, int) {
+                                              const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
     const float c2 = e.x.scale * XE_LOG2E;
     const float base = e.smoothing / (float)e.x.V;
 #pragma unroll 1
-    for (int cc = 0; cc < BN / 64; ++cc) {
+    for (int cc = half; cc < BN / 64; cc += 2) {
       const int c64 = tc * BN + cc * 64;
       if (c64 >= g.cols || r - st.lane >= g.rows) break;
       uint8_t* b = st.begin();
@@ -321,7 +314,7 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
   if (M == 0) return {loss, lse};
   auto st = at::cuda::getCurrentCUDAStream().stream();
   const om::GemmX g = xent_gemm(in, in.V, status.data_ptr<int>());
-  const int64_t n = (int64_t)g.tiles_c * M;
+  const int64_t n = 2 * (int64_t)g.tiles_c * M;
   const bool smooth = smoothing != 0.0;
   auto ws = torch::empty({n * (smooth ? 3 : 2) + M}, f32);
   float* p = ws.data_ptr<float>();
@@ -336,7 +329,7 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
     run(om::EpiXentFwd<false>{});
   om::launch_dependent(om::xent_join_kernel, om::ceil_div(M, 32), 32 * om::XE_JOIN, 0, st, (const float2*)p,
                        (const float*)(smooth ? p + 2 * n + M : nullptr), (const float*)(p + 2 * n), in.rows, (int)M,
-                       g.tiles_c, (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
+                       2 * g.tiles_c, (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
   return {loss, lse};
 }
 

@@ -20,7 +20,7 @@
 
 namespace om {
 
-// V elements (1, or 16 bytes' worth) from / to memory as fp32
+// V elements (1, 2 or 8) from / to memory as fp32
 template <typename T, int V>
 struct Vec {
   uint32_t u[V * sizeof(T) / 4 > 0 ? V * sizeof(T) / 4 : 1];
@@ -31,7 +31,10 @@ struct Vec {
         const uint4 q = reinterpret_cast<const uint4*>(p)[i];
         u[4 * i] = q.x; u[4 * i + 1] = q.y; u[4 * i + 2] = q.z; u[4 * i + 3] = q.w;
       }
-    } else if constexpr (sizeof(T) == 2) {
+    } else if constexpr (V * sizeof(T) == 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      u[0] = q.x; u[1] = q.y;
+    } else if constexpr (V * sizeof(T) == 2) {
       u[0] = *reinterpret_cast<const unsigned short*>(p);
     } else {
       u[0] = *reinterpret_cast<const uint32_t*>(p);
@@ -57,6 +60,10 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
   } else if constexpr (sizeof(T) == 4 && V == 8) {
     reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else if constexpr (sizeof(T) == 2 && V == 2) {
+    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]);
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
   } else if constexpr (sizeof(T) == 2) {
     p[0] = __float2bfloat16_rn(f[0]);
   } else {
@@ -636,14 +643,14 @@ __global__ void __launch_bounds__(32 * NORM_JOIN) norm_join_kernel(const float* 
     out[c] = t;
 }
 
-// Threads of a row: 16 elements a thread with 16-byte accesses, single elements otherwise
-// (16 each from 512 columns on).
+// Threads of a row: 16 elements each where the row is long enough, with 16-byte accesses (vec 8), with
+// pairs (vec 2: an even row length off the 16-byte grid) or one by one.
 template <typename F>
-static void norm_shape(const char* op, int D, bool vec, F&& f) {
+static void norm_shape(const char* op, int D, int vec, F&& f) {
   using std::integral_constant;
 #define OM_NORM_CASE(G_, V_, P_) \
   return f(integral_constant<int, G_>{}, integral_constant<int, V_>{}, integral_constant<int, P_>{})
-  if (vec) {
+  if (vec == 8) {
     if (D <= 256) OM_NORM_CASE(32, 8, 1);
     if (D <= 512) OM_NORM_CASE(32, 8, 2);
     if (D <= 1024) OM_NORM_CASE(64, 8, 2);
@@ -651,10 +658,17 @@ static void norm_shape(const char* op, int D, bool vec, F&& f) {
     if (D <= 4096) OM_NORM_CASE(256, 8, 2);
     if (D <= 8192) OM_NORM_CASE(512, 8, 2);
     if (D <= 16384) OM_NORM_CASE(1024, 8, 2);
+  } else if (vec == 2) {
+    if (D <= 128) OM_NORM_CASE(32, 2, 2);
+    if (D <= 512) OM_NORM_CASE(32, 2, 8);
+    if (D <= 2048) OM_NORM_CASE(128, 2, 8);
+    if (D <= 8192) OM_NORM_CASE(512, 2, 8);
+    if (D <= 16384) OM_NORM_CASE(1024, 2, 8);
   } else {
     if (D <= 128) OM_NORM_CASE(32, 1, 4);
-    if (D <= 1024) OM_NORM_CASE(128, 1, 8);
-    if (D <= 4096) OM_NORM_CASE(512, 1, 8);
+    if (D <= 512) OM_NORM_CASE(32, 1, 16);
+    if (D <= 2048) OM_NORM_CASE(128, 1, 16);
+    if (D <= 8192) OM_NORM_CASE(512, 1, 16);
     if (D <= 16384) OM_NORM_CASE(1024, 1, 16);
   }
 #undef OM_NORM_CASE
@@ -703,8 +717,6 @@ struct Residents {
   }
 };
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 }  // namespace om
 
 namespace {
@@ -721,8 +733,13 @@ torch::Tensor norm_cols(const char* op, const char* name, const torch::Tensor& t
               " must be a CUDA [D] tensor of the weight's type");
   return t.contiguous();
 }
-bool norm_vec(const torch::Tensor& t) {
-  return (t.dim() == 1 || t.stride(0) % 8 == 0) && om::aligned16(t.data_ptr());
+// Elements that one access of every row of `t` can take: 8 (16-byte rows), 2 or 1
+int norm_vec(const torch::Tensor& t) {
+  const auto ok = [&](int v) {
+    return t.size(t.dim() - 1) % v == 0 && (t.dim() == 1 || t.stride(0) % v == 0) &&
+           reinterpret_cast<uintptr_t>(t.data_ptr()) % std::min<size_t>(16, v * t.element_size()) == 0;
+  };
+  return ok(8) ? 8 : ok(2) ? 2 : 1;
 }
 
 }  // namespace
@@ -742,18 +759,18 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
   const auto ty = x.scalar_type(), wt = w.scalar_type();
   const torch::Tensor x2 = norm_rows(op, "x", x, M, D, ty), w2 = norm_cols(op, "w", w, D, wt);
   torch::Tensor d2, b2, h;
-  bool vec = D % 8 == 0 && norm_vec(x2) && norm_vec(w2);
+  int vec = std::min(norm_vec(x2), norm_vec(w2));
   if (delta.has_value()) {
     d2 = norm_rows(op, "delta", *delta, M, D, ty);
     a.ldd = d2.stride(0);
     a.delta = d2.data_ptr();
-    vec = vec && norm_vec(d2);
+    vec = std::min(vec, norm_vec(d2));
   }
   if (b.has_value()) {
     TORCH_CHECK(layer, "norm_train: RMSNorm takes no bias");
     b2 = norm_cols(op, "b", *b, D, wt);
     a.b = b2.data_ptr();
-    vec = vec && norm_vec(b2);
+    vec = std::min(vec, norm_vec(b2));
   }
   auto y = torch::empty(x.sizes(), x.options());
   h = delta.has_value() ? torch::empty(x.sizes(), x.options()) : x;
@@ -823,12 +840,12 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
   const torch::Tensor h2 = norm_rows(op, "h", h, M, D, ty), y2 = norm_rows(op, "dy", dy.to(ty), M, D, ty);
   const torch::Tensor w2 = norm_cols(op, "w", w, D, wt);
   torch::Tensor d2;
-  bool vec = D % 8 == 0 && norm_vec(h2) && norm_vec(y2) && norm_vec(w2);
+  int vec = std::min({norm_vec(h2), norm_vec(y2), norm_vec(w2)});
   if (dh.has_value()) {
     d2 = norm_rows(op, "dh", dh->to(ty), M, D, ty);
     a.lddh = d2.stride(0);
     a.dh = d2.data_ptr();
-    vec = vec && norm_vec(d2);
+    vec = std::min(vec, norm_vec(d2));
   }
   TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * M,
               "norm_train_bwd: stats must be fp32 [M, 2]");

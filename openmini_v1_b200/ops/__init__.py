@@ -310,7 +310,8 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
 
 def swiglu(x, w, save=False):
     """silu(x Wg^T) * (x Wu^T) of x [..., K] and w [2F, K] (gate rows first) -> [..., F]. With
-    ``save`` also the projections, fp32 [rows, 2F], that :func:`swiglu_bwd` reads."""
+    ``save`` also the fp32 projections that :func:`swiglu_bwd` reads (on the GPU their rows and h's
+    are a multiple of 8 elements apart, so h of an odd F is a strided view)."""
     _same_device("swiglu", x, w)
     if w.dim() != 2 or w.shape[0] % 2 or w.shape[1] != x.shape[-1]:
         raise ValueError("swiglu: w must be [2F, K]")

@@ -6,10 +6,12 @@
 //   dS = P * (dO V^T - rowsum(dO * O))
 //   dQ = c dS K,   dK = c dS^T Q
 //
-// No gradient is summed by atomics (the same result on every run): one launch holds two kinds of
-// CTAs, the heavy ones first, and the others fill the SMs behind them.
-//   kv  one CTA per 128 keys of a KV head walks the 64-query tiles of its query heads: dK, dV
-//   q   one CTA per 128 queries of a head walks the 64-key tiles: dQ
+// No gradient is summed by atomics (the same result on every run). Two kinds of work items:
+//   kv  128 keys of a KV head walk the 64-query tiles of its query heads: dK, dV
+//   q   128 queries of a head walk the 64-key tiles: dQ
+// One CTA an SM stays and takes the next item off a counter, the heavy ones first; the next item's
+// rows are loaded and its first scores computed while the last one's results are written, because
+// setting up a CTA and filling its pipeline (about 5 us) is more than a short item's work.
 // Both keep their rows (keys, or queries) in the MMA's 128 lanes and compute S and dP of a
 // 64-column tile from shared memory; the softmax threads turn the tile into P and dS and write
 // them, as 16-bit pairs, over S and dP in tensor memory, from where they are the A operand of the
@@ -17,7 +19,7 @@
 // (S^T) needs no transposition. Rounding P and dS to 16 bits enters each gradient at 2^-8
 // relative per term at the most, independently; sums are fp32 in tensor memory.
 //
-// Tensor memory of a kv CTA: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512 columns, all
+// Tensor memory of a kv item: dV 128 + dK 128 + two stages of (S 64 + dP 64) = 512 columns, all
 // there are; this is what sets the 64-query tile. Eight softmax warps work on one tile, 32 columns
 // a thread, and two such groups take the tiles in turn: a tile's exponentials (512 cycles at the
 // SM's 16 a cycle) and its loads and stores of tensor memory have to fit beside the 1280 cycles of
@@ -29,9 +31,10 @@
 // Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared
 // memory before a product contracts over them, so that whatever padding holds (NaN too) adds 0.
 //
-// Work split: where all CTAs together would leave SMs idle, the query heads of a KV head are
-// divided among `nsplit` CTAs, which leave fp32 partials that a last kernel adds in order.
+// Work split: where the items would leave SMs idle, the query heads of a KV head are divided among
+// `nsplit` items, which leave fp32 partials that a last kernel adds in order.
 #include <c10/cuda/CUDAGuard.h>
+#include <type_traits>
 #include "../common/om_host.h"
 #include "../common/om_ptx.cuh"
 
@@ -63,8 +66,9 @@ struct AttnBwdArgs {
   int B, T, S, H, Hkv, G, hd;
   int Tp;               // T rounded up to 64
   int causal, off;      // key j visible to query i when j <= i + off
-  int nsplit, gper;     // kv CTAs of a KV head and key tile, and the query heads of one
-  int kv_blocks;        // the grid's first blocks
+  int nsplit, gper;     // kv items of a KV head and key tile, and the query heads of one
+  int kv_items, items;  // kv items come first
+  int* next;            // the next item
   float scale, scale_log2;
   int* status;
 };
@@ -84,11 +88,13 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
 __global__ void __launch_bounds__(256) attn_bwd_stat_kernel(const __nv_bfloat16* __restrict__ o,
                                                             const __nv_bfloat16* __restrict__ go,
                                                             const float* __restrict__ lse, const int* lens,
-                                                            float* __restrict__ stat, int T, int Tp, int H, int hd,
+                                                            float* __restrict__ stat, int* next, int T, int Tp, int H,
+                                                            int hd,
                                                             long long ob, long long ot, long long oh, long long gb,
                                                             long long gt, long long gh) {
   grid_wait();
   grid_release();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *next = 0;
   const int sub = threadIdx.x & 15, b = blockIdx.y;
   const unsigned n = (unsigned)Tp * H;  // below 2^31
   const int len = lens ? min(lens[b], T) : T;
@@ -220,14 +226,14 @@ __device__ __forceinline__ void write_acc(uint32_t tmem, OUT* dst, bool live, bo
   }
 }
 
-// Zeros for the 128 rows of a CTA that has no tile to walk.
-template <int D, bool KV>
-__device__ __forceinline__ void write_zero(const AttnBwdArgs& a, int b, int kvh, int head, int split, int row0) {
-  const int vecs = a.hd / 8, rows = min(128, (KV ? a.S : a.T) - row0);
+// Zeros for the 128 rows of an item that has no tile to walk; `t` of `n` threads.
+__device__ __forceinline__ void write_zero(const AttnBwdArgs& a, bool kv, int b, int kvh, int head, int split, int row0,
+                                           int t, int n) {
+  const int vecs = a.hd / 8, rows = min(128, (kv ? a.S : a.T) - row0);
   const uint4 z = make_uint4(0, 0, 0, 0);
-  for (int i = threadIdx.x; i < rows * vecs; i += blockDim.x) {
+  for (int i = t; i < rows * vecs; i += n) {
     const int row = row0 + i / vecs, c = i % vecs * 8;
-    if constexpr (KV) {
+    if (kv) {
       const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd + c;
       if (a.nsplit > 1) {
         const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
@@ -247,67 +253,78 @@ __device__ __forceinline__ void write_zero(const AttnBwdArgs& a, int b, int kvh,
   }
 }
 
-// ------------------------------------------------------------------ the CTA of either kind
-// KV: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
-// else: resident Q, dO; streamed K, V; accumulates dQ.
-template <int D, bool KV>
-__device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUtensorMap& tmG, const CUtensorMap& tmK,
-                                             const CUtensorMap& tmV, const AttnBwdArgs& a, int block, uint8_t* smem) {
-  using C = fa_bw::Cfg<D>;
-  constexpr int NS = fa_bw::NSTAGE;
-  constexpr int STAGE0 = KV ? 256 : 128;  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D), then the stages
-  uint64_t* fix_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-  uint64_t* full = fix_full + 1;    // [NS]
-  uint64_t* empty = full + NS;      // [NS]
-  uint64_t* land = empty + NS;      // a padded tile before its rows are cleared
-  uint64_t* s_full = land + 1;      // [2] S of a stage is there
-  uint64_t* dp_full = s_full + 2;   // [2] dP is
-  uint64_t* ds_full = dp_full + 2;  // [2] P and dS are
-  uint64_t* acc_full = ds_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // which rows, heads and tiles; the heaviest tiles come first: under a causal mask the first
-  // keys (kv) and the last queries (q)
-  int b, kvh, head = 0, split = 0, row0, first, ntile, total;
-  {
-    const int heads = KV ? a.Hkv * a.nsplit : a.H;
+// A work item: its rows, heads and tiles.
+struct Item {
+  bool kv;
+  int b, kvh, head, split, row0, first, ntile, total;
+  int nstream, nrow;  // valid rows of the streamed and of the resident operands
+  __device__ __forceinline__ Item(const AttnBwdArgs& a, int i) {
+    kv = i < a.kv_items;
+    if (!kv) i -= a.kv_items;
+    const int heads = kv ? a.Hkv * a.nsplit : a.H;
     const int per = a.B * heads;
-    int tile = block / per, rest = block % per;
+    const int tile = i / per, rest = i % per;
     b = rest / heads;
-    rest %= heads;
+    head = rest % heads;
+    split = 0;
     const int nk = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;
     const int nq = a.lens ? max(0, min(a.lens[b], a.T)) : a.T;
-    if constexpr (KV) {
-      split = rest % a.nsplit;
-      kvh = rest / a.nsplit;
+    if (kv) {  // the heaviest are the first keys, under a causal mask
+      split = head % a.nsplit;
+      kvh = head / a.nsplit;
       row0 = tile * 128;
       head = kvh * a.G + split * a.gper;
       first = a.causal ? max(0, row0 - a.off) / 64 : 0;
       ntile = row0 < nk ? max(0, (nq + 63) / 64 - first) : 0;
       total = ntile * max(0, min(a.G - split * a.gper, a.gper));
-    } else {
-      head = rest;
+      nstream = nq;
+      nrow = nk;
+    } else {  // and the last queries
       kvh = head / a.G;
       row0 = ((a.T + 127) / 128 - 1 - tile) * 128;
       const int last = min(nq, row0 + 128) - 1;
       const int kend = last < row0 ? 0 : (a.causal ? min(nk, last + a.off + 1) : nk);
       first = 0;
       total = ntile = kend > 0 ? (kend + 63) / 64 : 0;
+      nstream = nk;
+      nrow = nq;
     }
   }
-  const int len_b = a.lens ? max(0, min(a.lens[b], a.S)) : a.S;    // T == S with lens
-  const int nstream = KV ? (a.lens ? len_b : a.T) : len_b;         // valid rows of the streamed operands
-  const int nrow = KV ? len_b : (a.lens ? len_b : a.T);            // valid rows of the resident ones
-  const bool may_pad = a.lens != nullptr && nstream < a.S;         // beyond T the copies fill zeros themselves
+};
 
-  if (total == 0) {  // nothing but padding: zeros, without tensor memory
-    write_zero<D, KV>(a, b, kvh, head, split, row0);
-    return;
-  }
+// kv: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
+// q:  resident Q, dO; streamed K, V; accumulates dQ.
+// Counters run over all items of a CTA: `tile` numbers the streamed tiles (ring stage, S / dP
+// region and barrier phases go by it), `done` the items that had any.
+template <int D>
+__global__ void __launch_bounds__(fa_bw::THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const AttnBwdArgs a) {
+  using C = fa_bw::Cfg<D>;
+  constexpr int NS = fa_bw::NSTAGE;
+  constexpr int STAGE0 = 256;  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D), then S and dP
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* fix_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
+  uint64_t* fix_empty = fix_full + 1;  // the item's last scores are computed
+  uint64_t* full = fix_empty + 1;      // [NS]
+  uint64_t* empty = full + NS;         // [NS]
+  uint64_t* land = empty + NS;         // a padded tile before its rows are cleared
+  uint64_t* s_full = land + 1;         // [2] S of a tile is there
+  uint64_t* dp_full = s_full + 2;      // [2] dP is
+  uint64_t* ds_full = dp_full + 2;     // [2] P and dS are
+  uint64_t* acc_full = ds_full + 2;    // the item's sums are
+  uint64_t* acc_empty = acc_full + 1;  // and have been read
+  uint64_t* item_full = acc_empty + 1; // [2] the next item's number
+  uint64_t* item_empty = item_full + 2;  // [2]
+  int* items = reinterpret_cast<int*>(item_empty + 2);  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     mbar_init(fix_full, 1);
+    mbar_init(fix_empty, 1);
     for (int s = 0; s < NS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -317,197 +334,275 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
       mbar_init(&s_full[s], 1);
       mbar_init(&dp_full[s], 1);
       mbar_init(&ds_full[s], 256);
+      mbar_init(&item_full[s], 1);
+      mbar_init(&item_empty[s], 17);
     }
     mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 16);
     fence_barrier_init();
   }
   if (warp == 2) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_wait();
+  grid_release();
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer (the whole warp)
     bool ok = true;
-    int it = 0, landed = 0;
-    if (lane == 0) {
-      mbar_arrive_expect_tx(fix_full, C::FIX_BYTES);
-      for (int h = 0; h < C::H; ++h)
-        for (int r = 0; r < 2; ++r) {
-          const int off = h * C::BIG + r * C::SMALL;
-          tma_load_4d(smem + off, KV ? &tmK : &tmQ, fix_full, h * 64, KV ? kvh : head, row0 + r * 64, b);
-          tma_load_4d(smem + C::H * C::BIG + off, KV ? &tmV : &tmG, fix_full, h * 64, KV ? kvh : head, row0 + r * 64, b);
-        }
-    }
-    int tile = 0, hd = head;
-    for (; it < total; ++it) {
-      const int s = it % NS, x0 = (first + tile) * 64;
-      ok = mbar_wait(&empty[s], ((it / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY);
-      ok = __all_sync(0xffffffffu, ok);
+    int tile = 0, landed = 0, done = 0;
+    for (int k = 0; ok; ++k) {
+      int n = 0;
+      if (lane == 0) n = atomicAdd(a.next, 1);
+      n = __shfl_sync(0xffffffffu, n, 0);
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY));
       if (!ok) break;
-      uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
-      const bool pad = may_pad && nstream - x0 < 64;
-      uint64_t* bar = pad ? land : &full[s];
       if (lane == 0) {
-        mbar_arrive_expect_tx(bar, C::ST_BYTES + (KV ? C::STAT : 0));
-        for (int h = 0; h < C::H; ++h) {
-          tma_load_4d(st + h * C::SMALL, KV ? &tmQ : &tmK, bar, h * 64, KV ? hd : kvh, x0, b);
-          tma_load_4d(st + (C::H + h) * C::SMALL, KV ? &tmG : &tmV, bar, h * 64, KV ? hd : kvh, x0, b);
-        }
-        if constexpr (KV)
-          bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + (((size_t)b * a.H + hd) * a.Tp + x0) * 2, C::STAT, bar);
+        items[k & 1] = n < a.items ? n : -1;
+        mbar_arrive(&item_full[k & 1]);
+      }
+      if (n >= a.items) break;
+      const Item w(a, n);
+      if (w.total == 0) continue;
+      const CUtensorMap* r0 = w.kv ? &tmK : &tmQ;
+      const CUtensorMap* r1 = w.kv ? &tmV : &tmG;
+      const CUtensorMap* x0 = w.kv ? &tmQ : &tmK;
+      const CUtensorMap* x1 = w.kv ? &tmG : &tmV;
+      ok = __all_sync(0xffffffffu, mbar_wait(fix_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(fix_full, C::FIX_BYTES);
+        for (int h = 0; h < C::H; ++h)
+          for (int r = 0; r < 2; ++r) {
+            const int off = h * C::BIG + r * C::SMALL;
+            tma_load_4d(smem + off, r0, fix_full, h * 64, w.kv ? w.kvh : w.head, w.row0 + r * 64, w.b);
+            tma_load_4d(smem + C::H * C::BIG + off, r1, fix_full, h * 64, w.kv ? w.kvh : w.head, w.row0 + r * 64, w.b);
+          }
       }
       __syncwarp();
-      if (pad) {
-        ok = mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL);
-        ++landed;
-        ok = __all_sync(0xffffffffu, ok);
+      ++done;
+      const bool may_pad = a.lens != nullptr && w.nstream < a.S;  // beyond T the copies fill zeros themselves
+      int t = 0, hd = w.head;
+      for (int i = 0; i < w.total; ++i, ++tile) {
+        const int s = tile % NS, row = (w.first + t) * 64;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((tile / NS) & 1) ^ 1, a.status, OM_ERR_WAIT_EMPTY));
         if (!ok) break;
-        clear_rows<2 * C::H>(st, nstream - x0, lane);
-        fence_proxy_async_smem();
+        uint8_t* st = smem + C::FIX_BYTES + s * C::ST_BYTES;
+        const bool pad = may_pad && w.nstream - row < 64;
+        uint64_t* bar = pad ? land : &full[s];
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, C::ST_BYTES + (w.kv ? C::STAT : 0));
+          for (int h = 0; h < C::H; ++h) {
+            tma_load_4d(st + h * C::SMALL, x0, bar, h * 64, w.kv ? hd : w.kvh, row, w.b);
+            tma_load_4d(st + (C::H + h) * C::SMALL, x1, bar, h * 64, w.kv ? hd : w.kvh, row, w.b);
+          }
+          if (w.kv)
+            bulk_load(smem + C::STAT_OFF + s * C::STAT, a.stat + (((size_t)w.b * a.H + hd) * a.Tp + row) * 2, C::STAT,
+                      bar);
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
-      }
-      if (++tile == ntile) {
-        tile = 0;
-        ++hd;
+        if (pad) {
+          ok = __all_sync(0xffffffffu, mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL));
+          ++landed;
+          if (!ok) break;
+          clear_rows<2 * C::H>(st, w.nstream - row, lane);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+        if (++t == w.ntile) {
+          t = 0;
+          ++hd;
+        }
       }
     }
     if (!ok) {  // wait (bounded) for the loads that may still be in flight
-      for (int j = max(0, it - NS); j < it; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
-      mbar_wait(fix_full, 0, nullptr, 0);
+      for (int j = max(0, tile - NS); j < tile; ++j) mbar_wait(&full[j % NS], (j / NS) & 1, nullptr, 0);
+      if (done > 0) mbar_wait(fix_full, (done - 1) & 1, nullptr, 0);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one()) {
       constexpr uint32_t IDESC_S = idesc_bf16_f32(128, 64);
       constexpr uint32_t IDESC_A = idesc_bf16_f32_bmn(128, D);
-      const uint32_t r0 = smem_u32(smem), r1 = r0 + C::H * C::BIG;  // K, V or Q, dO
-      // S (which = 0) or dP (1) of tile i, from the resident rows and the tile's 64
-      auto scores = [&](int i, int which) {
-        const uint32_t x = smem_u32(smem + C::FIX_BYTES + (i % NS) * C::ST_BYTES) + which * C::H * C::SMALL;
-        const uint32_t r = which ? r1 : r0;
-        const uint32_t d = tmem + STAGE0 + tile_region(i, which);
+      // descriptors by their low words: this thread's instructions are what the tensor pipe waits for
+      const uint32_t r_lo = smem_desc_lo(smem_u32(smem), 16);                  // K, V or Q, dO
+      const uint32_t x_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), 16);   // streamed, K-major
+      const uint32_t m_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), C::SMALL);  // streamed, MN-major
+      // S (which = 0) or dP (1) of a tile, from the resident rows and the tile's 64
+      auto scores = [&](int tile, auto which_c) {
+        constexpr int which = decltype(which_c)::value;
+        const uint32_t x = x_lo + (tile % NS) * (C::ST_BYTES / 16);
+        const uint32_t d = tmem + STAGE0 + tile_region(tile, which);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          tc_mma_f16(d, smem_desc_sw128(r + (k >> 2) * C::BIG + (k & 3) * 32, 1024),
-                     smem_desc_sw128(x + (k >> 2) * C::SMALL + (k & 3) * 32, 1024), IDESC_S, k > 0);
-        tc_commit(which ? &dp_full[i & 1] : &s_full[i & 1]);
+          tc_mma_f16_lo(d, r_lo + (which * C::H * C::BIG + (k >> 2) * C::BIG + (k & 3) * 32) / 16,
+                        x + (which * C::H * C::SMALL + (k >> 2) * C::SMALL + (k & 3) * 32) / 16, IDESC_S, k > 0);
+        tc_commit(which ? &dp_full[tile & 1] : &s_full[tile & 1]);
       };
-      auto loaded = [&](int i) {
-        const bool there = mbar_poll(&full[i % NS], (i / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+      const std::integral_constant<int, 0> S{};
+      const std::integral_constant<int, 1> DP{};
+      auto loaded = [&](int tile) {
+        const bool there = mbar_poll(&full[tile % NS], (tile / NS) & 1, a.status, OM_ERR_WAIT_FULL);
         tc_fence_after();
         return there;
       };
-      bool ok = mbar_wait(fix_full, 0, a.status, OM_ERR_WAIT_FULL);
-      for (int i = 0; i < 2 && i < total && ok; ++i) {
-        ok = loaded(i);
+      int tile = 0, done = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        ok = mbar_poll(&item_full[k & 1], (k >> 1) & 1, a.status, OM_ERR_WAIT_FULL);
         if (!ok) break;
-        scores(i, 0);
-        scores(i, 1);
-      }
-      for (int i = 0; i < total && ok; ++i) {
-        ok = mbar_poll(&ds_full[i & 1], (i >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-        if (!ok) break;
-        tc_fence_after();
-        // dP of tile i has been read: its columns take the next S of this parity at once
-        if (i + 2 < total) {
-          ok = loaded(i + 2);
+        const int n = items[k & 1];
+        mbar_arrive(&item_empty[k & 1]);
+        if (n < 0) break;
+        const Item w(a, n);
+        if (w.total == 0) continue;
+        ok = mbar_poll(fix_full, done & 1, a.status, OM_ERR_WAIT_FULL);
+        for (int i = 0; i < 2 && i < w.total && ok; ++i) {
+          ok = loaded(tile + i);
           if (!ok) break;
-          scores(i + 2, 0);
+          scores(tile + i, S);
+          scores(tile + i, DP);
         }
-        const uint32_t x0 = smem_u32(smem + C::FIX_BYTES + (i % NS) * C::ST_BYTES), x1 = x0 + C::H * C::SMALL;
-        const uint32_t p = tmem + STAGE0 + tile_region(i, 0);
-        if constexpr (KV) {
+        if (ok && w.total <= 2) tc_commit(fix_empty);
+        for (int i = 0; i < w.total && ok; ++i, ++tile) {
+          ok = mbar_poll(&ds_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+          if (!ok) break;
+          tc_fence_after();
+          // dP of this tile has been read: its columns take the next S of this parity at once
+          if (i + 2 < w.total) {
+            ok = loaded(tile + 2);
+            if (!ok) break;
+            scores(tile + 2, S);
+          }
+          if (i == 0) {  // the sums of the item before have been read
+            ok = mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          const uint32_t x = m_lo + (tile % NS) * (C::ST_BYTES / 16);
+          const uint32_t p = tmem + STAGE0 + tile_region(tile, 0);
+          if (w.kv) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // dV += P^T dO, 16 queries a step
-            tc_mma_f16_ts(tmem, p + (k >> 1) * 32 + (k & 1) * 8, smem_desc_sw128_mn(x1 + k * 2048, C::SMALL, 1024),
-                          IDESC_A, i > 0 || k > 0);
+            for (int j = 0; j < 4; ++j)  // dV += P^T dO, 16 queries a step
+              tc_mma_f16_ts_lo(tmem, p + (j >> 1) * 32 + (j & 1) * 8, x + (C::H * C::SMALL + j * 2048) / 16, IDESC_A,
+                               j > 0 ? 1 : i);
+          }
+          const uint32_t d = tmem + (w.kv ? 128 : 0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)  // dK += dS^T Q, or dQ += dS K
+            tc_mma_f16_ts_lo(d, p + 16 + (j >> 1) * 32 + (j & 1) * 8, x + j * 2048 / 16, IDESC_A, j > 0 ? 1 : i);
+          tc_commit(&empty[tile % NS]);
+          // P and dS of this tile are read by the products just issued; the tensor pipe runs this
+          // thread's products in order, so the next dP may take their columns
+          if (i + 2 < w.total) {
+            scores(tile + 2, DP);
+            if (i + 3 == w.total) tc_commit(fix_empty);  // the item's last scores
+          }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // dK += dS^T Q, or dQ += dS K
-          tc_mma_f16_ts(tmem + (KV ? 128 : 0), p + 16 + (k >> 1) * 32 + (k & 1) * 8,
-                        smem_desc_sw128_mn(x0 + k * 2048, C::SMALL, 1024), IDESC_A, i > 0 || k > 0);
-        tc_commit(&empty[i % NS]);
-        // P and dS of tile i are read by the products just issued; the tensor pipe runs this
-        // thread's products in order, so the next dP may take their columns
-        if (i + 2 < total) scores(i + 2, 1);
+        if (ok) tc_commit(acc_full);
+        ++done;
       }
-      if (ok) tc_commit(acc_full);
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax and output
-    const int group = (warp - 4) >> 3;           // tiles group, group + 2, ...
+    const int group = (warp - 4) >> 3;           // tiles of one parity
     const int half = ((warp - 4) >> 2) & 1;      // columns 32 half .. of a tile
     const int t = (warp & 3) * 32 + lane;        // row == TMEM lane
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int row = row0 + t;
-    float2 own = make_float2(0.f, 0.f);
-    bool zero = false;
-    if constexpr (!KV) {
-      own.x = -INFINITY;
-      if (row < nrow) {
-        const float* p = a.stat + (((size_t)b * a.H + head) * a.Tp + (row & ~63)) * 2 + (row & 63);
-        own = make_float2(p[0], p[64]);
-      }
-      zero = own.x == -INFINITY;                 // padding, or no visible key: gradient 0
-    }
+    int tile = 0, done = 0;
     bool ok = true;
-    int tile = group % ntile;
-    for (int it = group; it < total; it += 2) {
-      const int x0 = (first + tile) * 64;
-      tile += 2;
-      while (tile >= ntile) tile -= ntile;
-      // whoever reads a tile's statistics waits for their copy as well
-      if constexpr (KV) ok = mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
-      ok = ok && mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-      ok = __all_sync(0xffffffffu, ok);
+    for (int k = 0; ok; ++k) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&item_full[k & 1], (k >> 1) & 1, a.status, OM_ERR_WAIT_FULL));
       if (!ok) break;
-      tc_fence_after();
-      const uint32_t s_at = lanes + STAGE0 + tile_region(it, 0) + half * 32;
-      const uint32_t dp_at = lanes + STAGE0 + tile_region(it, 1) + half * 32;
-      const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT) + half * 128;
-      const bool masked = KV ? row0 + 128 > nrow || (a.causal && row0 + 127 > x0 + a.off)
-                             : x0 + 64 > nstream || (a.causal && x0 + 63 > row0 + a.off);
-      const int lo = (!KV ? 0 : row >= nrow ? 64 : (a.causal ? row - a.off - x0 : 0)) - half * 32;
-      const int hi = (KV ? 64 : min(nstream - x0, a.causal ? row + a.off + 1 - x0 : 64)) - half * 32;
-      uint64_t p[16];
-      if (masked)
-        tile_p<KV, true>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
+      const int n = items[k & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[k & 1]);
+      if (n < 0) break;
+      const Item w(a, n);
+      if (w.total == 0) {
+        write_zero(a, w.kv, w.b, w.kvh, w.head, w.split, w.row0, threadIdx.x - 128, 512);
+        continue;
+      }
+      const int row = w.row0 + t;
+      float2 own = make_float2(0.f, 0.f);
+      bool zero = false;
+      if (!w.kv) {
+        own.x = -INFINITY;
+        if (row < w.nrow) {
+          const float* p = a.stat + (((size_t)w.b * a.H + w.head) * a.Tp + (row & ~63)) * 2 + (row & 63);
+          own = make_float2(p[0], p[64]);
+        }
+        zero = own.x == -INFINITY;               // padding, or no visible key: gradient 0
+      }
+      auto walk = [&](auto kv_c) {
+        constexpr bool KV = decltype(kv_c)::value;
+        const int skip = (group ^ tile) & 1;     // this group's first tile of the item
+        int q = skip % w.ntile;
+        for (int i = skip; i < w.total; i += 2) {
+          const int it = tile + i, x0 = (w.first + q) * 64;
+          q += 2;
+          while (q >= w.ntile) q -= w.ntile;
+          // whoever reads a tile's statistics waits for their copy as well
+          if constexpr (KV) ok = mbar_wait(&full[it % NS], (it / NS) & 1, a.status, OM_ERR_WAIT_FULL);
+          ok = ok && mbar_wait(&s_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t s_at = lanes + STAGE0 + tile_region(it, 0) + half * 32;
+          const uint32_t dp_at = lanes + STAGE0 + tile_region(it, 1) + half * 32;
+          const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT) + half * 128;
+          const bool masked = KV ? w.row0 + 128 > w.nrow || (a.causal && w.row0 + 127 > x0 + a.off)
+                                 : x0 + 64 > w.nstream || (a.causal && x0 + 63 > w.row0 + a.off);
+          const int lo = (!KV ? 0 : row >= w.nrow ? 64 : (a.causal ? row - a.off - x0 : 0)) - half * 32;
+          const int hi = (KV ? 64 : min(w.nstream - x0, a.causal ? row + a.off + 1 - x0 : 64)) - half * 32;
+          uint64_t p[16];
+          if (masked)
+            tile_p<KV, true>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
+          else
+            tile_p<KV, false>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
+          ok = __all_sync(0xffffffffu, mbar_wait(&dp_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM));
+          if (!ok) return;
+          tc_fence_after();
+          if (masked)
+            tile_ds<KV, true>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
+          else
+            tile_ds<KV, false>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
+          tc_fence_before();
+          mbar_arrive(&ds_full[it & 1]);
+        }
+      };
+      if (w.kv)
+        walk(std::true_type{});
       else
-        tile_p<KV, false>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
-      ok = mbar_wait(&dp_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-      ok = __all_sync(0xffffffffu, ok);
+        walk(std::false_type{});
       if (!ok) break;
-      tc_fence_after();
-      if (masked)
-        tile_ds<KV, true>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
-      else
-        tile_ds<KV, false>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
-      tc_fence_before();
-      mbar_arrive(&ds_full[it & 1]);
-    }
-    if (ok) ok = mbar_wait(acc_full, 0, a.status, OM_ERR_WAIT_ACCUM);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+      tile += w.total;
+      ok = __all_sync(0xffffffffu, mbar_wait(acc_full, done & 1, a.status, OM_ERR_WAIT_ACCUM));
+      if (!ok) break;
+      ++done;
       tc_fence_after();
       const int col0 = half * (D / 2);  // each half writes half of the columns
-      if constexpr (KV) {               // group 0 writes dV, group 1 dK
+      if (w.kv) {                       // group 0 writes dV, group 1 dK
         const bool live = row < a.S;
-        const size_t at = (((size_t)b * a.S + row) * a.Hkv + kvh) * a.hd + col0;
+        const size_t at = (((size_t)w.b * a.S + row) * a.Hkv + w.kvh) * a.hd + col0;
         const float f = group ? a.scale : 1.f;
         const uint32_t acc = lanes + group * 128 + col0;
         if (a.nsplit > 1) {
           const size_t plane = (size_t)a.B * a.S * a.Hkv * a.hd;
-          write_acc<D / 2>(acc, a.part + (split * 2 + group) * plane + at, live, zero, f, a.hd - col0);
+          write_acc<D / 2>(acc, a.part + (w.split * 2 + group) * plane + at, live, zero, f, a.hd - col0);
         } else {
           write_acc<D / 2>(acc, (group ? a.dk : a.dv) + at, live, zero, f, a.hd - col0);
         }
       } else if (group == 0) {
-        write_acc<D / 2>(lanes + col0, a.dq + (((size_t)b * a.T + row) * a.H + head) * a.hd + col0, row < a.T, zero,
+        write_acc<D / 2>(lanes + col0, a.dq + (((size_t)w.b * a.T + row) * a.H + w.head) * a.hd + col0, row < a.T, zero,
                          a.scale, a.hd - col0);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
     }
   }
 
@@ -517,21 +612,6 @@ __device__ __forceinline__ void attn_bwd_cta(const CUtensorMap& tmQ, const CUten
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-template <int D>
-__global__ void __launch_bounds__(fa_bw::THREADS, 1)
-    attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const AttnBwdArgs a) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  grid_wait();
-  grid_release();
-  if ((int)blockIdx.x < a.kv_blocks)
-    attn_bwd_cta<D, true>(tmQ, tmG, tmK, tmV, a, blockIdx.x, smem);
-  else
-    attn_bwd_cta<D, false>(tmQ, tmG, tmK, tmV, a, blockIdx.x - a.kv_blocks, smem);
 }
 
 // Adds the query-head splits' fp32 partials in split order.
@@ -583,9 +663,7 @@ static void attn_bwd_launch(const AttnBwdArgs& a, const CUtensorMap& q, const CU
     OM_CUDA_CHECK(cudaFuncSetAttribute(attn_bwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     attr_set[dev].store(true);
   }
-  const long long blocks = a.kv_blocks + (long long)((a.T + 127) / 128) * a.B * a.H;
-  TORCH_CHECK(blocks < (1ll << 31), "attention_bwd: too many tiles");
-  launch_dependent(attn_bwd_kernel<D>, (unsigned)blocks, fa_bw::THREADS, C::SMEM, st, q, g, k, v, a);
+  launch_dependent(attn_bwd_kernel<D>, std::min(a.items, num_sms()), fa_bw::THREADS, C::SMEM, st, q, g, k, v, a);
   if (a.nsplit > 1) {
     const long long n = (long long)a.B * a.S * a.Hkv * a.hd;
     const int jb = (int)std::min<long long>((2 * n + 1023) / 1024, (long long)num_sms() * 8);
@@ -663,26 +741,29 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   a.dk = ptr(dk);
   a.dv = ptr(dv);
   a.status = status.data_ptr<int>();
-  // A kv CTA with all query heads of its KV head walks up to G T / 64 tiles. The launch ends about
-  // when the longest CTA or the average SM does, so a CTA gets as many heads as fit into the
+  // A kv item with all query heads of its KV head walks up to G T / 64 tiles. The launch ends about
+  // when the longest item or the average SM does, so an item gets as many heads as fit into the
   // average (a q tile counts 0.75 of a kv tile), and all of them where that is a few tiles anyway
   // (a join costs more).
   const int64_t qt = (T + 63) / 64, kt = (S + 127) / 128;
   const double average = (double)B * H * qt * kt * (causal ? 0.5 : 1.0) * 1.75 / om::num_sms();
   a.gper = a.G * qt <= 16 ? a.G : (int)std::min<double>(a.G, std::max(1.0, average / qt));
   a.nsplit = (a.G + a.gper - 1) / a.gper;
-  TORCH_CHECK(kt * B * Hkv * a.nsplit < (1ll << 30), "attention_bwd: too many tiles");
-  a.kv_blocks = (int)(kt * B * Hkv * a.nsplit);
-  // scratch: the rows' statistics, then the split heads' partials
+  const int64_t kv_items = kt * B * Hkv * a.nsplit, q_items = (T + 127) / 128 * B * H;
+  TORCH_CHECK(kv_items + q_items < (1ll << 30), "attention_bwd: too many tiles");
+  a.kv_items = (int)kv_items;
+  a.items = (int)(kv_items + q_items);
+  // scratch: the rows' statistics, then the split heads' partials, then the item counter
   const int64_t stat_floats = B * H * a.Tp * 2, plane = B * S * Hkv * D;
-  auto ws = torch::empty({stat_floats + (a.nsplit > 1 ? 2 * a.nsplit * plane : 0)}, lse.options());
+  auto ws = torch::empty({stat_floats + (a.nsplit > 1 ? 2 * a.nsplit * plane : 0) + 1}, lse.options());
   float* stat = ws.data_ptr<float>();
   a.stat = stat;
   a.part = a.nsplit > 1 ? ws.data_ptr<float>() + stat_floats : nullptr;
+  a.next = reinterpret_cast<int*>(ws.data_ptr<float>() + ws.numel() - 1);
   const int64_t rows = (int64_t)a.Tp * H;
   const int blocks = (int)std::min<int64_t>((rows + 15) / 16, std::max<int64_t>(1, om::num_sms() * 16 / B));
   om::launch_dependent(om::attn_bwd_stat_kernel, dim3(blocks, (unsigned)B), 256, 0, st, ptr(out), ptr(dout),
-                       lse.data_ptr<float>(), a.lens, stat, a.T, a.Tp, a.H, a.hd, (long long)out.stride(0),
+                       lse.data_ptr<float>(), a.lens, stat, a.next, a.T, a.Tp, a.H, a.hd, (long long)out.stride(0),
                        (long long)out.stride(1), (long long)out.stride(2), (long long)dout.stride(0),
                        (long long)dout.stride(1), (long long)dout.stride(2));
   const CUtensorMap mq = om::map_bthd(q), mg = om::map_bthd(dout), mk = om::map_bthd(k), mv = om::map_bthd(v);

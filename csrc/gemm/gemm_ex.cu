@@ -9,10 +9,11 @@ namespace om {
 template <int SUB>
 __global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __restrict__ P, int splits, long long rows,
                                                              int cols, int ldacc, __nv_bfloat16* __restrict__ out,
-                                                             long long ldo, int vec) {
+                                                             long long ldo, int vec, Factor factor) {
   __shared__ float4 sh[SUB > 1 ? 256 : 1];
   grid_wait();
   grid_release();
+  const float mul = factor_of(factor);
   const int nv = ldacc >> 2, lanes = 256 / SUB, sub = threadIdx.x / lanes, lane = threadIdx.x % lanes;
   const long long plane = rows * ldacc, n = rows * nv;
   for (long long i0 = blockIdx.x * (long long)lanes; i0 < n; i0 += gridDim.x * (long long)lanes) {
@@ -40,6 +41,7 @@ __global__ void __launch_bounds__(256) planes_to_bf16_kernel(const float* __rest
       }
     }
     if (!live) continue;
+    a.x *= mul; a.y *= mul; a.z *= mul; a.w *= mul;
     __nv_bfloat16* o = out + r * ldo + c;
     if (vec && c + 4 <= cols) {
       uint2 w;
@@ -127,7 +129,8 @@ static void product(const GxPlan& p, GxOperand a, GxOperand b, const OutMaps& o,
 }
 
 void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
-                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st) {
+                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st,
+                Factor factor) {
   TORCH_CHECK(b.mn, "gx_product: B is MN-major");
   GemmX g{};
   g.rows = (int)rows;
@@ -143,7 +146,7 @@ void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t
   OutMaps o{};
   if (p.splits == 1 && first && last) {
     o.m[0] = gx_out(out, rows, cols, ldo);
-    product<EpiStore>(p, a, b, o, g, {}, K, st);
+    product<EpiStore>(p, a, b, o, g, {factor}, K, st);
     return;
   }
   const int ldacc = ceil_div(cols, 32) * 32;
@@ -156,7 +159,7 @@ void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t
     const int blocks = (int)std::min<long long>((work + lanes - 1) / lanes, (long long)num_sms() * 8);
     launch_dependent(many ? planes_to_bf16_kernel<8> : planes_to_bf16_kernel<1>, blocks, 256, 0, st, acc, p.splits,
                      (long long)rows, (int)cols, ldacc, out, (long long)ldo,
-                     (int)(ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0));
+                     (int)(ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0), factor);
   }
 }
 

@@ -516,13 +516,30 @@ __device__ __forceinline__ void store_row32(float* dst, const float (&f)[32], in
 
 struct NoRow {};
 
+// A factor of a whole product, applied in fp32 before its one rounding: mul times the mantissa (1 to
+// 2) of *ref, where there is one. An operand that carries a value common to all its rows divides it
+// out first, so that the value's rounding does not become a bias of every term.
+struct Factor {
+  const float* ref;
+  float mul;
+};
+__device__ __forceinline__ float mantissa_of(float v) {
+  const uint32_t u = __float_as_uint(v), e = (u >> 23) & 255u;
+  return e == 0u || e == 255u ? 1.f : __uint_as_float((u & 0x007fffffu) | 0x3f800000u);
+}
+__device__ __forceinline__ float factor_of(const Factor& f) {
+  return f.ref != nullptr ? f.mul * mantissa_of(*f.ref) : f.mul;
+}
+
 // bf16 rows through map 0, 64 columns a store.
 struct EpiStore {
-  struct Args {};
+  struct Args {
+    Factor factor;
+  };
   static constexpr int SEG = 0;
-  static __device__ __forceinline__ NoRow row(const GemmX&, const Args&, int) { return {}; }
+  static __device__ __forceinline__ float row(const GemmX&, const Args& e, int) { return factor_of(e.factor); }
   template <int BN>
-  static __device__ __forceinline__ void tile(const GemmX& g, const Args&, const NoRow&, const OutMaps& o,
+  static __device__ __forceinline__ void tile(const GemmX& g, const Args&, const float& factor, const OutMaps& o,
                                               const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
 #pragma unroll 1
     for (int cc = half; cc < BN / 64; cc += 2) {
@@ -536,7 +553,7 @@ struct EpiStore {
         tc_wait_ld();
         float f[32];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * factor;
         st.put(b, h, f);
       }
       st.end([&] { tma_store_2d(&o.m[0], b, c0, r - st.lane); });

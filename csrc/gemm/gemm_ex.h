@@ -87,6 +87,7 @@ struct GxPlan {
 GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K);
 int64_t gx_acc_floats(const GxPlan& p, int64_t rows, int64_t cols, bool pieces);
 void gx_product(const GxPlan& p, GxOperand a, GxOperand b, int64_t rows, int64_t cols, int64_t K,
-                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st);
+                __nv_bfloat16* out, int64_t ldo, float* acc, bool first, bool last, int* status, cudaStream_t st,
+                Factor factor = {nullptr, 1.f});
 
 }  // namespace om

@@ -10,10 +10,14 @@
 // the pairs of a row in a fixed order. What leaves the chip is M V / 16 bytes instead of 4 M V.
 //
 // Gradient: the vocabulary is walked in pieces. Each piece's logits are computed again, and the
-// epilogue turns them into dz (16 bits: its rounding is 2^-9 relative per entry and independent,
-// like that of a stored activation) in a workspace of one piece; dx takes the piece's product
+// epilogue turns them into dz (16 bits) in a workspace of one piece; dx takes the piece's product
 // into fp32 sums, dW's rows of the piece are finished at once. Four products instead of three is
 // the price of not keeping M V values.
+// What is rounded is dz without what all rows share: gloss / m ((p - e / V) / (1 - e) - [j = t]), m the
+// mantissa of the first row's gloss. Under a mean loss every target's entry is then within p_t of
+// -2^k and takes at most p_t from its rounding; with the common factor c (1 - e) m inside, all of
+// them would be off by the same amount of up to 2^-9, the whole of an output's own rounding again.
+// The factor is applied to the sums.
 //
 // What bounds it: the tensor cores (2 M K V flops a product). The epilogue's exponentials take
 // 2048 cycles a tile beside 8 K cycles of products, on other warps.
@@ -161,7 +165,7 @@ struct EpiXentBwd {
   };
   static constexpr int SEG = 0;
   struct Row {
-    float gz, l2;  // c gloss (0: ignored), lse log2 e
+    float gz, l2;  // gloss / m (0: ignored), lse log2 e
     int tcol;      // the target's column in the piece, or -1
   };
   static __device__ __forceinline__ Row row(const GemmX& g, const Args& e, int r) {
@@ -169,7 +173,7 @@ struct EpiXentBwd {
     if (r >= g.rows) return o;
     const long long t = e.x.targets[r];
     if (t < 0 || t >= e.x.V || t == e.x.ignore) return o;
-    o.gz = e.dloss[r] * e.x.scale;
+    o.gz = e.dloss[r] / mantissa_of(e.dloss[0]);
     o.l2 = e.lse[r] * XE_LOG2E;
     if (t >= e.v0 && t < e.v0 + (long long)g.cols) o.tcol = (int)(t - e.v0);
     return o;
@@ -178,7 +182,7 @@ struct EpiXentBwd {
   static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const Row& w, const OutMaps& o,
                                               const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
     const float c2 = e.x.scale * XE_LOG2E;
-    const float base = e.smoothing / (float)e.x.V;
+    const float inv = 1.f / (1.f - e.smoothing), base = inv * e.smoothing / (float)e.x.V;
 #pragma unroll 1
     for (int cc = half; cc < BN / 64; cc += 2) {
       const int c64 = tc * BN + cc * 64;
@@ -199,12 +203,12 @@ struct EpiXentBwd {
           for (int j = 0; j < 32; ++j) f[j] = 0.f;
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) f[j] = fast_exp2(__uint_as_float(v[j]) * c2 - w.l2) - base;
+          for (int j = 0; j < 32; ++j) f[j] = fmaf(fast_exp2(__uint_as_float(v[j]) * c2 - w.l2), inv, -base);
           // tcol = -1 matches no column; a mask, not an index: registers stay registers
           const uint32_t hit = (w.tcol >> 5) == (c0 >> 5) ? 1u << (w.tcol & 31) : 0u;
           if (hit) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] -= (hit >> j) & 1u ? 1.f - e.smoothing : 0.f;
+            for (int j = 0; j < 32; ++j) f[j] -= (hit >> j) & 1u ? 1.f : 0.f;
           }
           if (bits == 0xffffffffu) {
 #pragma unroll
@@ -270,34 +274,42 @@ XentIn check_xent(const char* op, const torch::Tensor& x, const torch::Tensor& w
   return in;
 }
 
-// The product x W^T of `cols` vocabulary rows from wv with either logits epilogue, on CTA pairs where
-// there are enough tiles.
-template <class Epi>
-void xent_logits(const XentIn& in, const void* wv, const om::OutMaps& o, om::GemmX g, const typename Epi::Args& e,
-                 cudaStream_t st) {
-  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, in.M, in.K, in.x.stride(0), 128);
-  const CUtensorMap tb = om::gx_map(wv, false, g.cols, in.K, in.w.stride(0), 128);
-  if (om::gx_pairs(in.M, g.cols, in.K)) {
-    g.tiles_r = om::ceil_div(in.M, 256);
-    om::gx_launch_pair<false, false, Epi>(ta, tb, o, g, e, st);
-  } else {
-    om::gx_launch<256, false, false, Epi>(ta, tb, o, g, e, st);
-  }
+// Column tile of the product x W^T: 256 on CTA pairs or single CTAs; narrower where that needs no more
+// waves of tiles (few rows and a small vocabulary: 910 x 1196 x 7336 on 40 tiles of 256 or 152 of 64).
+struct XentTile {
+  int bn, pair;
+};
+XentTile xent_tile(const XentIn& in, int64_t cols) {
+  if (om::gx_pairs(in.M, cols, in.K)) return {256, 1};
+  const int64_t tiles = (int64_t)om::ceil_div(in.M, 128) * om::ceil_div(cols, 256), sms = om::num_sms();
+  return {tiles * 4 <= sms ? 64 : tiles * 2 <= sms ? 128 : 256, 0};
 }
 
-om::GemmX xent_gemm(const XentIn& in, int64_t cols, int* status) {
+// The product with `cols` vocabulary rows from wv and either logits epilogue.
+template <class Epi>
+void xent_logits(const XentIn& in, const XentTile& t, const void* wv, int64_t cols, const om::OutMaps& o,
+                 const typename Epi::Args& e, int* status, cudaStream_t st) {
   om::GemmX g{};
   g.rows = (int)in.M;
   g.cols = (int)cols;
   g.num_kb = om::ceil_div(in.K, 64);
   g.splits = 1;
   g.kb_per_split = g.num_kb;
-  g.tiles_r = om::ceil_div(in.M, 128);
-  g.tiles_c = om::ceil_div(cols, 256);
-  g.b_step = 256;
-  g.b_second = g.b_box = 128;
+  g.tiles_r = om::ceil_div(in.M, t.pair ? 256 : 128);
+  g.tiles_c = om::ceil_div(cols, t.bn);
+  g.b_step = t.bn;
+  g.b_second = g.b_box = t.bn / 2;
   g.status = status;
-  return g;
+  const CUtensorMap ta = om::gx_map(in.x.data_ptr(), false, in.M, in.K, in.x.stride(0), 128);
+  const CUtensorMap tb = om::gx_map(wv, false, cols, in.K, in.w.stride(0), t.bn / 2);
+  if (t.pair)
+    om::gx_launch_pair<false, false, Epi>(ta, tb, o, g, e, st);
+  else if (t.bn == 64)
+    om::gx_launch<64, false, false, Epi>(ta, tb, o, g, e, st);
+  else if (t.bn == 128)
+    om::gx_launch<128, false, false, Epi>(ta, tb, o, g, e, st);
+  else
+    om::gx_launch<256, false, false, Epi>(ta, tb, o, g, e, st);
 }
 
 }  // namespace
@@ -313,15 +325,16 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
   const int64_t M = in.M;
   if (M == 0) return {loss, lse};
   auto st = at::cuda::getCurrentCUDAStream().stream();
-  const om::GemmX g = xent_gemm(in, in.V, status.data_ptr<int>());
-  const int64_t n = 2 * (int64_t)g.tiles_c * M;
+  const XentTile tile = xent_tile(in, in.V);
+  const int tiles = 2 * om::ceil_div(in.V, tile.bn);  // halves of column tiles
+  const int64_t n = (int64_t)tiles * M;
   const bool smooth = smoothing != 0.0;
   auto ws = torch::empty({n * (smooth ? 3 : 2) + M}, f32);
   float* p = ws.data_ptr<float>();
   auto run = [&](auto epi) {
     using E = decltype(epi);
     typename E::Args e{in.rows, reinterpret_cast<float2*>(p), smooth ? p + 2 * n + M : nullptr, p + 2 * n};
-    xent_logits<E>(in, in.w.data_ptr(), om::OutMaps{}, g, e, st);
+    xent_logits<E>(in, tile, in.w.data_ptr(), in.V, om::OutMaps{}, e, status.data_ptr<int>(), st);
   };
   if (smooth)
     run(om::EpiXentFwd<true>{});
@@ -329,7 +342,7 @@ std::pair<torch::Tensor, torch::Tensor> om_linear_xent(torch::Tensor x, torch::T
     run(om::EpiXentFwd<false>{});
   om::launch_dependent(om::xent_join_kernel, om::ceil_div(M, 32), 32 * om::XE_JOIN, 0, st, (const float2*)p,
                        (const float*)(smooth ? p + 2 * n + M : nullptr), (const float*)(p + 2 * n), in.rows, (int)M,
-                       2 * g.tiles_c, (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), g.status);
+                       tiles, (float)smoothing, loss.data_ptr<float>(), lse.data_ptr<float>(), status.data_ptr<int>());
   return {loss, lse};
 }
 
@@ -367,20 +380,20 @@ std::pair<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> om_linear_
   if (nx + nw) acc = torch::empty({nx + nw}, lse.options());
   float* ax = nx ? acc.data_ptr<float>() : nullptr;
   float* aw = nw ? acc.data_ptr<float>() + nx : nullptr;  // nx is a multiple of 32
+  const om::Factor factor{dloss.data_ptr<float>(), (float)(scale * (1.0 - smoothing))};
   for (int64_t v0 = 0; v0 < V; v0 += C) {
     const int64_t n = std::min(C, V - v0);
     const __nv_bfloat16* wv = ptr(in.w) + v0 * in.w.stride(0);
-    const om::GemmX g = xent_gemm(in, n, status.data_ptr<int>());
     const om::EpiXentBwd::Args e{in.rows, lse.data_ptr<float>(), dloss.data_ptr<float>(), (float)smoothing, (int)v0};
     om::OutMaps o{};
     o.m[0] = om::gx_out(ptr(dz), M, n, ld);
-    xent_logits<om::EpiXentBwd>(in, wv, o, g, e, st);
+    xent_logits<om::EpiXentBwd>(in, xent_tile(in, n), wv, n, o, e, status.data_ptr<int>(), st);
     if (need_dx)
       om::gx_product(px, {dz.data_ptr(), false, ld}, {wv, true, in.w.stride(0)}, M, K, n, ptr(*dx), K, ax, v0 == 0,
-                     v0 + n == V, g.status, st);
+                     v0 + n == V, status.data_ptr<int>(), st, factor);
     if (need_dw)
       om::gx_product(pw, {dz.data_ptr(), true, ld}, {in.x.data_ptr(), true, in.x.stride(0)}, n, K, M,
-                     ptr(*dw) + v0 * K, K, aw, true, true, g.status, st);
+                     ptr(*dw) + v0 * K, K, aw, true, true, status.data_ptr<int>(), st, factor);
   }
   return {dx, dw};
 }

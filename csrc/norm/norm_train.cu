@@ -20,7 +20,7 @@
 
 namespace om {
 
-// V elements (1, 2 or 8) from / to memory as fp32
+// V elements (1 or 8) from / to memory as fp32
 template <typename T, int V>
 struct Vec {
   uint32_t u[V * sizeof(T) / 4 > 0 ? V * sizeof(T) / 4 : 1];
@@ -31,9 +31,6 @@ struct Vec {
         const uint4 q = reinterpret_cast<const uint4*>(p)[i];
         u[4 * i] = q.x; u[4 * i + 1] = q.y; u[4 * i + 2] = q.z; u[4 * i + 3] = q.w;
       }
-    } else if constexpr (V * sizeof(T) == 8) {
-      const uint2 q = *reinterpret_cast<const uint2*>(p);
-      u[0] = q.x; u[1] = q.y;
     } else if constexpr (V * sizeof(T) == 2) {
       u[0] = *reinterpret_cast<const unsigned short*>(p);
     } else {
@@ -60,10 +57,6 @@ __device__ __forceinline__ void store_vec(T* p, const float* f) {
   } else if constexpr (sizeof(T) == 4 && V == 8) {
     reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else if constexpr (sizeof(T) == 2 && V == 2) {
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(f[0], f[1]);
-  } else if constexpr (V == 2) {
-    *reinterpret_cast<float2*>(p) = make_float2(f[0], f[1]);
   } else if constexpr (sizeof(T) == 2) {
     p[0] = __float2bfloat16_rn(f[0]);
   } else {
@@ -137,26 +130,42 @@ constexpr int norm_threads() { return G < 256 ? 256 : G; }
 
 // A ring of rows in shared memory, one per group of G threads: NA arrays a stage, filled by bulk
 // copies that the group's first thread starts. Only arrival is signalled: a stage is filled again
-// after a barrier of the group that follows its last read.
-template <typename T, int G, int NA>
+// after a barrier of the group that follows its last read. ODD: rows may start anywhere; the
+// 16-byte blocks that hold a row are copied whole, and it is read at its offset in them.
+template <typename T, int G, int NA, bool ODD = false>
 struct RowRing {
   uint8_t* base;      // this group's stages
   uint64_t* full;     // this group's barriers
   const T* src[NA];
   long long ld[NA];
   int stages;
-  uint32_t bytes;     // of a row
+  uint32_t bytes;     // of a row's place in a stage
+  uint32_t len;       // ODD: bytes of a row
   int s;              // the stage in turn and the phase of its barrier
   uint32_t phase;
+  __device__ __forceinline__ uint32_t off(int i, long long row) const {
+    return ODD ? (uint32_t)(reinterpret_cast<uintptr_t>(src[i] + row * ld[i]) & 15) : 0u;
+  }
   __device__ __forceinline__ void fill(int stage, long long row) const {  // one thread
-    mbar_arrive_expect_tx(&full[stage], NA * bytes);
+    uint32_t n[NA], all = 0;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      n[i] = ODD ? (src[i] != nullptr ? (off(i, row) + len + 15) & ~15u : 0u) : bytes;
+      all += n[i];
+    }
+    mbar_arrive_expect_tx(&full[stage], all);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-      bulk_load(base + (size_t)(stage * NA + i) * bytes, src[i] + row * ld[i], bytes, &full[stage]);
+      if (n[i])
+        bulk_load(base + (size_t)(stage * NA + i) * bytes,
+                  reinterpret_cast<const uint8_t*>(src[i] + row * ld[i]) - off(i, row), n[i], &full[stage]);
   }
   __device__ __forceinline__ bool wait(int* status) const { return mbar_wait(&full[s], phase, status, OM_ERR_WAIT_FULL); }
   __device__ __forceinline__ const T* row(int i) const {
     return reinterpret_cast<const T*>(base + (size_t)(s * NA + i) * bytes);
+  }
+  __device__ __forceinline__ const T* row_at(int i, long long r) const {  // ODD
+    return reinterpret_cast<const T*>(base + (size_t)(s * NA + i) * bytes + off(i, r));
   }
   __device__ __forceinline__ void next() {
     if (++s == stages) {
@@ -167,6 +176,8 @@ struct RowRing {
 };
 
 constexpr int RING_MAX = 8;  // stages
+// place of a row that may start anywhere in its first 16-byte block
+__host__ __device__ constexpr uint32_t odd_place(uint32_t len) { return (len + 30u) & ~15u; }
 
 struct NormFwd {
   const void *x, *delta, *w, *b;
@@ -615,6 +626,185 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
   write_partials<G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }
 
+// Rows that do not start on 16 bytes (an odd length, an offset view): the same ring, read element by
+// element, 16 a thread, in the order of the lanes, so that shared memory and the stores are whole
+// lines.
+template <typename T>
+__device__ __forceinline__ float elem(const T* p) {
+  if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
+  return *p;
+}
+
+template <typename T, typename W, bool LAYER, int G>
+__global__ void __launch_bounds__(norm_threads<G>()) norm_fwd_odd_kernel(const NormFwd a) {
+  constexpr int NT = norm_threads<G>(), RPB = NT / G, P = 16;
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float sh[2 * (NT / 32)];
+  __shared__ uint64_t bars[RPB * RING_MAX];
+  const int grp = threadIdx.x / G, lane = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
+  RowRing<T, G, 2, true> ring;
+  ring.stages = a.stages;
+  ring.s = 0;
+  ring.phase = 0;
+  ring.len = a.D * sizeof(T);
+  ring.bytes = odd_place(ring.len);
+  ring.base = ring_mem + (size_t)grp * a.stages * 2 * ring.bytes;
+  ring.full = bars + grp * RING_MAX;
+  ring.src[0] = static_cast<const T*>(a.x);
+  ring.ld[0] = a.ldx;
+  ring.src[1] = static_cast<const T*>(a.delta);
+  ring.ld[1] = a.ldd;
+  if (lane == 0) {
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+    fence_barrier_init();
+  }
+  grid_wait();
+  grid_release();
+  if (lane == 0) {
+    for (int k = 0; k < a.stages; ++k)
+      if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
+  }
+  __syncthreads();
+  int flip = 0;
+  for (long long base = row0; base < a.M; base += step) {
+    const long long row = base + grp;
+    const bool live = row < a.M && ring.wait(a.status);
+    const T* x = ring.row_at(0, row);
+    const T* d = ring.row_at(1, row);
+    float f[P], sum[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = lane + i * G;
+      f[i] = 0.f;
+      if (live && c < a.D) {
+        f[i] = elem(x + c);
+        if (a.delta) {
+          f[i] = round_to<T>(f[i] + elem(d + c));
+          store_vec<T, 1>(static_cast<T*>(a.h) + row * a.D + c, &f[i]);
+        }
+      }
+      sum[0] += LAYER ? f[i] : f[i] * f[i];
+    }
+    group_sum<G, 1>(sum, sh, flip);
+    if constexpr (G == 32) __syncwarp();
+    if (lane == 0 && row + a.stages * step < a.M) ring.fill(ring.s, row + a.stages * step);
+    ring.next();
+    float mu = 0.f;
+    if constexpr (LAYER) {
+      mu = sum[0] / a.D;
+      sum[0] = 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float t = lane + i * G < a.D ? f[i] - mu : 0.f;
+        sum[0] += t * t;
+      }
+      group_sum<G, 1>(sum, sh, flip);
+    }
+    if (!live) continue;
+    const float r = rsqrtf(sum[0] / a.D + a.eps);
+    if (lane == 0) *reinterpret_cast<float2*>(a.stats + 2 * row) = make_float2(mu, r);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = lane + i * G;
+      if (c >= a.D) continue;
+      float o = (f[i] - mu) * r * elem(static_cast<const W*>(a.w) + c);
+      if (LAYER && a.b) o += elem(static_cast<const W*>(a.b) + c);
+      store_vec<T, 1>(static_cast<T*>(a.y) + row * a.D + c, &o);
+    }
+  }
+}
+
+// The row is read from the ring twice, for the sums and for dx, instead of being held; its stage is
+// filled again after the next row's reduction, when every thread is past it.
+template <typename T, typename W, bool LAYER, int G>
+__global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_odd_kernel(const NormBwd a) {
+  constexpr int NT = norm_threads<G>(), RPB = NT / G, N = LAYER ? 2 : 1, P = 16;
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float sh[2 * N * (NT / 32)];
+  __shared__ uint64_t bars[RPB * RING_MAX];
+  const int grp = threadIdx.x / G, lane = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * RPB, row0 = (long long)blockIdx.x * RPB;
+  RowRing<T, G, 3, true> ring;
+  ring.stages = a.stages;
+  ring.s = 0;
+  ring.phase = 0;
+  ring.len = a.D * sizeof(T);
+  ring.bytes = odd_place(ring.len);
+  ring.base = ring_mem + (size_t)grp * a.stages * 3 * ring.bytes;
+  ring.full = bars + grp * RING_MAX;
+  ring.src[0] = static_cast<const T*>(a.h);
+  ring.ld[0] = a.ldh;
+  ring.src[1] = static_cast<const T*>(a.dy);
+  ring.ld[1] = a.ldy;
+  ring.src[2] = static_cast<const T*>(a.dh);
+  ring.ld[2] = a.lddh;
+  if (lane == 0) {
+    for (int i = 0; i < a.stages; ++i) mbar_init(&ring.full[i], 1);
+    fence_barrier_init();
+  }
+  grid_wait();
+  grid_release();
+  if (lane == 0) {
+    for (int k = 0; k < a.stages; ++k)
+      if (row0 + grp + k * step < a.M) ring.fill(k, row0 + grp + k * step);
+  }
+  float dw[P][1], db[LAYER ? P : 1][1], w[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int c = lane + i * G;
+    w[i] = c < a.D ? elem(static_cast<const W*>(a.w) + c) : 0.f;
+    dw[i][0] = 0.f;
+    if constexpr (LAYER) db[i][0] = 0.f;
+  }
+  __syncthreads();
+  int flip = 0;
+  for (long long base = row0; base < a.M; base += step) {
+    const long long row = base + grp;
+    const bool live = row < a.M && ring.wait(a.status);
+    float2 st = make_float2(0.f, 0.f);
+    if (live) st = *reinterpret_cast<const float2*>(a.stats + 2 * row);
+    const T* h = ring.row_at(0, row);
+    const T* y = ring.row_at(1, row);
+    const T* dh = ring.row_at(2, row);
+    float s[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int c = lane + i * G;
+      if (live && c < a.D) {
+        const float v = elem(y + c), n = (elem(h + c) - st.x) * st.y, g = v * w[i];
+        s[0] += g * n;
+        dw[i][0] += v * n;
+        if constexpr (LAYER) {
+          s[N - 1] += g;
+          db[i][0] += v;
+        }
+      }
+    }
+    group_sum<G, N>(s, sh, flip);
+    if constexpr (G == 32) __syncwarp();
+    if (lane == 0 && row >= row0 + grp + step && row + (a.stages - 1) * step < a.M)
+      ring.fill(ring.s == 0 ? a.stages - 1 : ring.s - 1, row + (a.stages - 1) * step);
+    if (live) {
+      const float c1 = s[0] / a.D, c2 = LAYER ? s[N - 1] / a.D : 0.f;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const int c = lane + i * G;
+        if (c >= a.D) continue;
+        const float n = (elem(h + c) - st.x) * st.y;
+        float o = st.y * (elem(y + c) * w[i] - n * c1 - c2);
+        if (a.dh) o += elem(dh + c);
+        store_vec<T, 1>(static_cast<T*>(a.dx) + row * a.D + c, &o);
+      }
+    }
+    ring.next();
+  }
+  __syncthreads();  // every copy has been waited for and read: the ring's memory is free
+  write_partials<G, 1, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
+}
+
 // dw (db) = sum over blocks, in a fixed order: 32 columns a block, each of 16 warps takes every
 // sixteenth partial row, joined in warp order.
 constexpr int NORM_JOIN = 16;
@@ -643,14 +833,13 @@ __global__ void __launch_bounds__(32 * NORM_JOIN) norm_join_kernel(const float* 
     out[c] = t;
 }
 
-// Threads of a row: 16 elements each where the row is long enough, with 16-byte accesses (vec 8), with
-// pairs (vec 2: an even row length off the 16-byte grid) or one by one.
+// Threads of a row: 16 elements each where the row is long enough, with 16-byte accesses or one by one.
 template <typename F>
-static void norm_shape(const char* op, int D, int vec, F&& f) {
+static void norm_shape(const char* op, int D, bool vec, F&& f) {
   using std::integral_constant;
 #define OM_NORM_CASE(G_, V_, P_) \
   return f(integral_constant<int, G_>{}, integral_constant<int, V_>{}, integral_constant<int, P_>{})
-  if (vec == 8) {
+  if (vec) {
     if (D <= 256) OM_NORM_CASE(32, 8, 1);
     if (D <= 512) OM_NORM_CASE(32, 8, 2);
     if (D <= 1024) OM_NORM_CASE(64, 8, 2);
@@ -658,14 +847,7 @@ static void norm_shape(const char* op, int D, int vec, F&& f) {
     if (D <= 4096) OM_NORM_CASE(256, 8, 2);
     if (D <= 8192) OM_NORM_CASE(512, 8, 2);
     if (D <= 16384) OM_NORM_CASE(1024, 8, 2);
-  } else if (vec == 2) {
-    if (D <= 128) OM_NORM_CASE(32, 2, 2);
-    if (D <= 512) OM_NORM_CASE(32, 2, 8);
-    if (D <= 2048) OM_NORM_CASE(128, 2, 8);
-    if (D <= 8192) OM_NORM_CASE(512, 2, 8);
-    if (D <= 16384) OM_NORM_CASE(1024, 2, 8);
   } else {
-    if (D <= 128) OM_NORM_CASE(32, 1, 4);
     if (D <= 512) OM_NORM_CASE(32, 1, 16);
     if (D <= 2048) OM_NORM_CASE(128, 1, 16);
     if (D <= 8192) OM_NORM_CASE(512, 1, 16);
@@ -733,13 +915,10 @@ torch::Tensor norm_cols(const char* op, const char* name, const torch::Tensor& t
               " must be a CUDA [D] tensor of the weight's type");
   return t.contiguous();
 }
-// Elements that one access of every row of `t` can take: 8 (16-byte rows), 2 or 1
-int norm_vec(const torch::Tensor& t) {
-  const auto ok = [&](int v) {
-    return t.size(t.dim() - 1) % v == 0 && (t.dim() == 1 || t.stride(0) % v == 0) &&
-           reinterpret_cast<uintptr_t>(t.data_ptr()) % std::min<size_t>(16, v * t.element_size()) == 0;
-  };
-  return ok(8) ? 8 : ok(2) ? 2 : 1;
+// Whether every row of `t` is whole 16-byte blocks
+bool norm_vec(const torch::Tensor& t) {
+  return t.size(t.dim() - 1) % 8 == 0 && (t.dim() == 1 || t.stride(0) % 8 == 0) &&
+         (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
 
 }  // namespace
@@ -759,18 +938,18 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
   const auto ty = x.scalar_type(), wt = w.scalar_type();
   const torch::Tensor x2 = norm_rows(op, "x", x, M, D, ty), w2 = norm_cols(op, "w", w, D, wt);
   torch::Tensor d2, b2, h;
-  int vec = std::min(norm_vec(x2), norm_vec(w2));
+  bool vec = norm_vec(x2) && norm_vec(w2);
   if (delta.has_value()) {
     d2 = norm_rows(op, "delta", *delta, M, D, ty);
     a.ldd = d2.stride(0);
     a.delta = d2.data_ptr();
-    vec = std::min(vec, norm_vec(d2));
+    vec = vec && norm_vec(d2);
   }
   if (b.has_value()) {
     TORCH_CHECK(layer, "norm_train: RMSNorm takes no bias");
     b2 = norm_cols(op, "b", *b, D, wt);
     a.b = b2.data_ptr();
-    vec = std::min(vec, norm_vec(b2));
+    vec = vec && norm_vec(b2);
   }
   auto y = torch::empty(x.sizes(), x.options());
   h = delta.has_value() ? torch::empty(x.sizes(), x.options()) : x;
@@ -816,6 +995,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> om_norm_train(torch::Ten
             go(om::norm_fwd_ring_kernel<T, W, false, false, g, p>, res[3]);
           return;
         }
+      } else {
+        const size_t stage = (size_t)(NT / g) * 2 * om::odd_place((uint32_t)(D * sizeof(T)));
+        a.stages = om::ring_stages(stage);
+        if (a.stages >= 2) {
+          static om::Residents res[2];
+          auto kernel = layer ? om::norm_fwd_odd_kernel<T, W, true, g> : om::norm_fwd_odd_kernel<T, W, false, g>;
+          const size_t smem = a.stages * stage;
+          const int grid = (int)std::min<long long>(blocks, om::num_sms() * res[layer].get(kernel, NT, smem));
+          om::launch_dependent(kernel, grid, NT, smem, st, a);
+          return;
+        }
       }
       om::launch_dependent(layer ? om::norm_fwd_kernel<T, W, true, g, v, p> : om::norm_fwd_kernel<T, W, false, g, v, p>,
                            (unsigned)blocks, NT, 0, st, a);
@@ -840,12 +1030,12 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
   const torch::Tensor h2 = norm_rows(op, "h", h, M, D, ty), y2 = norm_rows(op, "dy", dy.to(ty), M, D, ty);
   const torch::Tensor w2 = norm_cols(op, "w", w, D, wt);
   torch::Tensor d2;
-  int vec = std::min({norm_vec(h2), norm_vec(y2), norm_vec(w2)});
+  bool vec = norm_vec(h2) && norm_vec(y2) && norm_vec(w2);
   if (dh.has_value()) {
     d2 = norm_rows(op, "dh", dh->to(ty), M, D, ty);
     a.lddh = d2.stride(0);
     a.dh = d2.data_ptr();
-    vec = std::min(vec, norm_vec(d2));
+    vec = vec && norm_vec(d2);
   }
   TORCH_CHECK(stats.is_cuda() && stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * M,
               "norm_train_bwd: stats must be fp32 [M, 2]");
@@ -901,6 +1091,18 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
             go(om::norm_bwd_ring_kernel<T, W, false, true, g, p>, res[2], smem);
           else
             go(om::norm_bwd_ring_kernel<T, W, false, false, g, p>, res[3], smem);
+          return;
+        }
+      } else {
+        const size_t stage = (size_t)RPB * 3 * om::odd_place((uint32_t)(D * sizeof(T)));
+        a.stages = om::ring_stages(stage);
+        if (a.stages >= 2) {
+          const size_t smem = std::max(a.stages * stage, joined);
+          static om::Residents res[2];
+          if (layer)
+            go(om::norm_bwd_odd_kernel<T, W, true, g>, res[1], smem);
+          else
+            go(om::norm_bwd_odd_kernel<T, W, false, g>, res[0], smem);
           return;
         }
       }

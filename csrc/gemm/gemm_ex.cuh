@@ -115,11 +115,13 @@ __host__ __device__ constexpr uint32_t idesc_bf16_x(int M, int N, bool amn, bool
   return idesc_bf16_f32(M, N) | (amn ? 1u << 15 : 0u) | (bmn ? 1u << 16 : 0u);
 }
 
-// AR: rows of A that are loaded. The MMA reads 128; for a few tokens the rest is whatever follows in
-// shared memory, which ends in accumulator rows that are never read, and the room goes to stages.
+// AR: rows of A that are loaded, and the row tile. For a few tokens (32) the MMA has 64 rows, of which
+// the last 32 are whatever follows in shared memory; they end in accumulator rows that are never
+// read, and the room goes to stages. A 64-row accumulator has 16 rows in each quarter of the lanes.
 template <int BN, int AR = 128>
 struct GemmXCfg {
   static constexpr int BK = 64;
+  static constexpr int MM = AR <= 64 ? 64 : 128;  // rows of the MMA
   static constexpr int A_BYTES = AR * BK * 2;
   static constexpr int B_BYTES = BN * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
@@ -127,7 +129,7 @@ struct GemmXCfg {
   static constexpr int TMEM_COLS = BN <= 128 ? 2 * BN : 512;  // a power of two
   static constexpr int OUT_BYTES = 8 * 4096;  // eight epilogue warps; also what lies behind a short A
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 /*align slack*/ + 512;
-  static_assert((128 - AR) * BK * 2 <= B_BYTES + OUT_BYTES, "the MMA reads 128 rows of A");
+  static_assert((MM - AR) * BK * 2 <= B_BYTES + OUT_BYTES, "the MMA reads MM rows of A");
 };
 
 // Steps of one segment: the whole contraction (`kb1` is past its end) unless the Epi wants shorter ones.
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(GX_THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (elect_one()) {
-      constexpr uint32_t IDESC = idesc_bf16_x(128, BN, AMN, BMN);
+      constexpr uint32_t IDESC = idesc_bf16_x(C::MM, BN, AMN, BMN);
       int it = 0, local = 0;
       bool ok = true;
       for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(GX_THREADS, 1)
     for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
       int tr, tc, sp;
       gx_coords(g, u, tr, tc, sp);
-      const int r = tr * 128 + q * 32 + lane;
+      const int r = C::MM == 128 ? tr * 128 + q * 32 + lane : lane < 16 ? tr * 64 + q * 16 + lane : g.rows;
       const auto row = Epi::row(g, e, r);  // the row's own inputs, read while the products run
       if constexpr (Epi::SEG == 0) {
         const int acc = local & 1;

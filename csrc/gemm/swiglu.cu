@@ -36,7 +36,7 @@ struct EpiSwiglu {
   static __device__ __forceinline__ void tile(const GemmX& g, const Args& e, const NoRow&, const OutMaps& o,
                                               const RowStage& st, uint32_t tbase, int r, int tc, int, int half) {
     constexpr int HALF = BN / 2;
-    const int F = g.cols, r0 = r - st.lane;
+    const int F = g.cols, r0 = __shfl_sync(0xffffffffu, r, 0);
 #pragma unroll 1
     for (int cc = half; cc < HALF / 32; cc += 2) {
       const int c0 = tc * g.b_step + cc * 32;

@@ -67,10 +67,11 @@ void gx_launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const OutMaps&
 }
 
 // Whether a product goes to pairs: a 256 x 256 tile for every pair of SMs, rows that fill more than
-// one half of a tile, and a contraction of 512 or more, below which setting up the pair costs more
-// than it saves.
+// one half of a tile, and a contraction long enough for the setting up of a pair's tile (4096 rows,
+// gated projection of 8192 / cross entropy of 32000, us on pairs and on single CTAs: K = 256 46 and 37 /
+// 108 and 94; K = 512 58 and 56 / 120 and 109; K = 1024 89 and 102 / 175 and 190).
 inline bool gx_pairs(int64_t rows, int64_t cols, int64_t K) {
-  return rows > 128 && K >= 512 && (int64_t)ceil_div(rows, 256) * ceil_div(cols, 256) >= num_sms() / 2;
+  return rows > 128 && K >= 768 && (int64_t)ceil_div(rows, 256) * ceil_div(cols, 256) >= num_sms() / 2;
 }
 
 struct GxOperand {

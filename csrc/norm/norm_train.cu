@@ -367,27 +367,36 @@ struct NormBwd {
   void* dx;
   const float* stats;
   float* part;  // [blocks][1 or 2][D]: dw, db
+  void *dw, *db;  // of the weight's type: written straight by a single block
   long long M, ldy, ldh, lddh;
   int D;
   int stages;
   int* status;
 };
 
-// The block's row groups are added up in group order through shared memory (acc: [D]).
-template <int G, int V, int P, int N, int RPB>
+// The block's row groups are added up in group order through shared memory (acc: [D]); the sum goes to
+// the block's partial, or is the result if there is no other block.
+template <typename W, int G, int V, int P, int N, int RPB>
 __device__ __forceinline__ void write_partials(const NormBwd& a, const float (&dw)[P][V],
                                                const float (&db)[N == 2 ? P : 1][V], float* acc) {
   const int lane = threadIdx.x % G;
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    float* out = a.part + ((size_t)blockIdx.x * N + k) * a.D;
+    float* part = a.part + ((size_t)blockIdx.x * N + k) * a.D;
+    W* out = static_cast<W*>(k == 0 ? a.dw : a.db);
+    auto put = [&](int c, float v) {
+      if (gridDim.x > 1)
+        part[c] = v;
+      else if (out != nullptr)
+        store_vec<W, 1>(out + c, &v);
+    };
     if constexpr (RPB == 1) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         const int c = (lane + i * G) * V;
         if (c >= a.D) continue;
 #pragma unroll
-        for (int j = 0; j < V; ++j) out[c + j] = k == 0 ? dw[i][j] : db[N == 2 ? i : 0][j];
+        for (int j = 0; j < V; ++j) put(c + j, k == 0 ? dw[i][j] : db[N == 2 ? i : 0][j]);
       }
     } else {
       for (int grp = 0; grp < RPB; ++grp) {
@@ -405,7 +414,7 @@ __device__ __forceinline__ void write_partials(const NormBwd& a, const float (&d
               else if (grp < RPB - 1)
                 acc[c + j] += t;
               else
-                out[c + j] = acc[c + j] + t;
+                put(c + j, acc[c + j] + t);
             }
           }
         }
@@ -497,7 +506,7 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_kernel(const NormB
     }
   }
   extern __shared__ float acc[];  // [D] when RPB > 1
-  write_partials<G, V, P, N, RPB>(a, dw, db, acc);
+  write_partials<W, G, V, P, N, RPB>(a, dw, db, acc);
 }
 
 // The same with the rows in a ring.
@@ -623,7 +632,7 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_ring_kernel(const 
       }
     }
   __syncthreads();  // every copy has been waited for and read: the ring's memory is free
-  write_partials<G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
+  write_partials<W, G, V, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }
 
 // Rows that do not start on 16 bytes (an odd length, an offset view): the same ring, read element by
@@ -802,7 +811,7 @@ __global__ void __launch_bounds__(norm_threads<G>()) norm_bwd_odd_kernel(const N
     ring.next();
   }
   __syncthreads();  // every copy has been waited for and read: the ring's memory is free
-  write_partials<G, 1, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
+  write_partials<W, G, 1, P, N, RPB>(a, dw, db, reinterpret_cast<float*>(ring_mem));
 }
 
 // dw (db) = sum over blocks, in a fixed order: 32 columns a block, each of 16 warps takes every
@@ -1068,13 +1077,21 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
       constexpr int NT = om::norm_threads<g>(), RPB = NT / g;
       auto go = [&](auto kernel, om::Residents& res, size_t smem) {
         const long long most = (M + RPB - 1) / RPB;
-        const int blocks = (int)std::min<long long>(most, om::num_sms() * res.get(kernel, NT, smem));
-        auto part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());
-        a.part = part.data_ptr<float>();
+        int blocks = (int)std::min<long long>(most, om::num_sms() * res.get(kernel, NT, smem));
+        // Few rows: one block walks up to eight a group and writes dw itself, which takes less time
+        // than handing partials to a second kernel.
+        if (most <= 8) blocks = 1;
+        torch::Tensor part;
+        if (blocks > 1) {
+          part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());
+          a.part = part.data_ptr<float>();
+        }
+        a.dw = dw.data_ptr();
+        a.db = bias ? db->data_ptr() : nullptr;
         om::launch_dependent(kernel, blocks, NT, smem, st, a);
-        om::launch_dependent(om::norm_join_kernel<W>, dim3((a.D + 31) / 32, bias ? 2 : 1), 32 * om::NORM_JOIN, 0, st,
-                             (const float*)a.part, blocks, n, a.D, reinterpret_cast<W*>(dw.data_ptr()),
-                             bias ? reinterpret_cast<W*>(db->data_ptr()) : (W*)nullptr);
+        if (blocks > 1)
+          om::launch_dependent(om::norm_join_kernel<W>, dim3((a.D + 31) / 32, bias ? 2 : 1), 32 * om::NORM_JOIN, 0, st,
+                               (const float*)a.part, blocks, n, a.D, static_cast<W*>(a.dw), static_cast<W*>(a.db));
       };
       const size_t joined = RPB > 1 ? (size_t)a.D * sizeof(float) : 0;
       if constexpr (v == 8) {

@@ -28,6 +28,7 @@ import torch
 import torch.distributed as dist
 
 from ..engine.request import SamplingParams
+from .. import ops
 from ..models.policy import Policy, token_logprobs
 from .grpo import GRPOConfig, group_relative_advantage, grpo_loss
 from .replay import KeepRouting, KeepSamplingMask, unpack_words
@@ -159,6 +160,8 @@ class GRPOTrainer:
         if self.reducer is not None:
             self.reducer.finish()
         gn = torch.nn.utils.clip_grad_norm_(self.policy.parameters(), self.cfg.max_grad_norm)
+        if dev.type == "cuda":  # nothing is learnt from a step in which a kernel reported an error
+            ops.check_status(dev)
         self.opt.step()
         self.policy.export_to(self.engine.model)
         self.step_idx += 1

@@ -22,6 +22,8 @@ from dataclasses import dataclass, field
 import torch
 import torch.distributed as dist
 
+from .. import ops
+from ..models.policy import Policy
 from .checkpoint import CheckpointManager
 from .ddp import GradReducer
 from .loss import DynamicLossScaler, causal_lm_loss, perplexity
@@ -116,7 +118,7 @@ class Trainer:
     def _loss(self, batch):
         ids = batch["input_ids"].to(self.device)
         labels = batch["labels"].to(self.device)
-        if ids.is_cuda and hasattr(self.model, "loss"):  # no logits in memory
+        if ids.is_cuda and isinstance(self.model, Policy):  # no logits in memory
             return self.model.loss(ids, labels, self.cfg.label_smoothing_factor)
         logits = self.model(ids)
         return causal_lm_loss(logits, labels, self.cfg.label_smoothing_factor)
@@ -192,6 +194,8 @@ class Trainer:
                 self.scaler.scale_loss(loss / acc).backward()
                 st.micro_step = i + 1
                 st.last_loss = float(loss.detach())
+                if loss.is_cuda:  # a label outside the vocabulary, a wait that gave up: stop before the step
+                    ops.check_status(loss.device)
                 if not last:
                     continue
                 info = self._optimizer_step()

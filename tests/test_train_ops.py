@@ -687,3 +687,27 @@ def test_trainer_step_on_gpu_uses_no_logits():
     losses = [r["loss"] for r in st.history if "loss" in r]
     assert losses[-1] < losses[0] and all(math.isfinite(v) for v in losses)
     ops.check_status()
+
+
+@pytest.mark.gpu
+def test_trainer_stops_at_a_label_outside_the_vocabulary():
+    import tempfile
+
+    from openmini_v1_b200.train.trainer import Trainer, TrainingConfig
+    p = small_policy("cuda")
+    before = p.lm_head.detach().clone()
+    ids = torch.randint(0, 520, (2, 32), generator=gen("cpu", 4))
+    labels = ids.clone()
+    labels[1, 7] = 520
+
+    class Loader(list):
+        def set_epoch(self, e):
+            pass
+
+    with tempfile.TemporaryDirectory() as d:
+        tr = Trainer(p, TrainingConfig(num_train_epochs=1, output_dir=d, save_steps=0),
+                     Loader([{"input_ids": ids, "labels": labels}]))
+        with pytest.raises(RuntimeError, match="status"):
+            tr.train()
+    assert torch.equal(before, p.lm_head.detach())
+    ops.check_status()

@@ -79,8 +79,9 @@ GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
     }
   }
   const int64_t tiles = tr * ceil_div(cols, p.bn);
-  // a split has to be worth its fp32 plane (written and read once): 8 steps of 64 at least
-  int s = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
+  // a split has to be worth its fp32 plane (written and read once) and a second launch: 8 steps of 64
+  // at least, of 32 and more in all
+  int s = kb < 32 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
   const int per = ceil_div(kb, s);
   p.splits = ceil_div(kb, per);
   return p;

@@ -30,7 +30,7 @@
 //
 // What bounds it: the tensor cores, 1280 + 1024 of their cycles for a pair of tiles at head_dim 128
 // (kv + q), at the clock that the power limit leaves. Measured (B200, back to back): 1 x 8192, 40 / 8
-// heads of 128, causal 2.27 ms, 760 TFLOP/s of the five products, 1060 of the seven; 4 x <= 1499 padded,
+// heads of 128, causal 2.28 ms, 753 TFLOP/s of the five products, 1060 of the seven; 4 x <= 1499 padded,
 // 16 / 4 heads 121 us; head_dim 64, 1 x 8192, 32 / 8 heads 1.25 ms, where the exponentials bound it.
 //
 // Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared

@@ -14,7 +14,7 @@
 //
 // What bounds it: the tensor cores for M of a few hundred and more; the weight's bytes below
 // (2 F K * 2 bytes for a single token). Measured (B200, back to back): 4096 x 4096 -> 11008, forward and
-// gradient 1.85 ms, its three products at 1270 TFLOP/s; one token, 8192 -> 28672 184 us (5.1 TB/s).
+// gradient 1.85 to 1.90 ms, its three products at 1230 to 1270 TFLOP/s; one token, 8192 -> 28672 185 us (5.1 TB/s).
 #include <c10/cuda/CUDAGuard.h>
 #include "gemm_ex.h"
 

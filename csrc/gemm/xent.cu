@@ -17,12 +17,13 @@
 // mantissa of the first row's gloss. Under a mean loss every target's entry is then within p_t of
 // -2^k and takes at most p_t from its rounding; with the common factor c (1 - e) m inside, all of
 // them would be off by the same amount of up to 2^-9, the whole of an output's own rounding again.
-// The factor is applied to the sums.
+// The factor is applied to the sums. Weights that differ by row keep the rounding of their own target's
+// entry (up to 2^-9 of the row's dx): the weight has to be inside dz, over whose rows dW sums.
 //
 // What bounds it: the tensor cores (2 M K V flops a product). The epilogue's exponentials take
 // 2048 cycles a tile beside 8 K cycles of products, on other warps. Measured (B200, back to back): 4096 x
-// 5120 -> 152064, forward and gradient 18.8 ms, its four products at 1360 TFLOP/s (the library GEMM's
-// sustained rate is 1395); forward alone of 4000 x 2048 -> 32000 with a keep mask 390 us, 1340 TFLOP/s.
+// 5120 -> 152064, forward and gradient 18.8 to 19.2 ms, its four products at 1330 to 1360 TFLOP/s (the library GEMM's
+// sustained rate is 1395); forward alone of 4000 x 2048 -> 32000 with a keep mask 397 us, 1320 TFLOP/s.
 #include <c10/cuda/CUDAGuard.h>
 #include "gemm_ex.h"
 

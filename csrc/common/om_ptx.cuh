@@ -1,7 +1,7 @@
 // Inline-PTX building blocks for sm_100a kernels: mbarriers with bounded waits,
-// TMA tile loads (no cluster multicast anywhere in this tree), tcgen05 TMEM
-// allocation / MMA / commit / load, and the shared-memory + instruction
-// descriptors that tcgen05.mma consumes.
+// TMA tile loads (none of them multicast: what goes to both CTAs of a pair is a barrier
+// arrive of tcgen05.commit), tcgen05 TMEM allocation / MMA / commit / load, and the
+// shared-memory + instruction descriptors that tcgen05.mma consumes.
 //
 // Every wait in this file is bounded: after OM_WAIT_LIMIT_NS of wall time on
 // the device global timer it records an error code in the caller's status word
@@ -18,7 +18,10 @@
 
 namespace om {
 
-// Status codes written to the kernel's status word (first error wins).
+// Codes of the kernel's status word. Its low byte is the first wait that gave up (1 to 4), or
+// OM_ERR_BOUNDS if there was none; with both, OM_ERR_BOUNDS is the second byte. Waits stop early
+// only when another wait has given up: a bad index in the data is reported and changes nothing in
+// the kernels that come after it.
 enum : int {
   OM_OK = 0,
   OM_ERR_WAIT_FULL = 1,      // consumer gave up waiting for a filled stage
@@ -35,7 +38,19 @@ __device__ __forceinline__ uint64_t globaltimer() {
 }
 
 __device__ __forceinline__ void record_error(int* status, int code) {
-  if (status) atomicCAS(status, 0, code);
+  if (!status) return;
+  const int old = atomicCAS(status, 0, code);
+  if (old == 0 || old == code) return;
+  if (code == OM_ERR_BOUNDS) {
+    if (old < 256) atomicCAS(status, old, old | OM_ERR_BOUNDS << 8);
+  } else if (old == OM_ERR_BOUNDS) {
+    atomicCAS(status, old, code | OM_ERR_BOUNDS << 8);
+  }
+}
+// Whether a wait has given up somewhere on this device since the status word was last cleared.
+__device__ __forceinline__ bool wait_failed(const int* status) {
+  const int code = *(const volatile int*)status & 255;
+  return code != OM_OK && code != OM_ERR_BOUNDS;
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -101,7 +116,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
         record_error(status, code);
         return false;
       }
-      if (status && *(volatile int*)status != 0) return false;  // someone else already failed
+      if (status && wait_failed(status)) return false;  // someone else already gave up
     }
   }
 }
@@ -131,7 +146,7 @@ __device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, int* s
         record_error(status, code);
         return false;
       }
-      if (status && *(volatile int*)status != 0) return false;
+      if (status && wait_failed(status)) return false;
     }
   }
 }
@@ -149,7 +164,7 @@ __device__ __forceinline__ bool mbar_wait_sleep(uint64_t* bar, uint32_t parity, 
         record_error(status, code);
         return false;
       }
-      if (status && *(volatile int*)status != 0) return false;
+      if (status && wait_failed(status)) return false;
     }
   }
 }

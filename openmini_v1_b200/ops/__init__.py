@@ -24,8 +24,10 @@ __all__ = [
 
 class DeviceContext:
     """Per-device scratch owned by the op layer: a status word that kernels set
-    on a bounded-wait timeout or a bounds violation, and growable fp32
-    workspaces for split-K GEMM partials and split-KV attention partials."""
+    on a bounded-wait timeout (after which other waits stop early, so later
+    results may be incomplete) or a bounds violation (which touches no other
+    call), and growable fp32 workspaces for split-K GEMM partials and split-KV
+    attention partials."""
 
     def __init__(self, device: torch.device):
         self.device = device
@@ -73,6 +75,16 @@ def ctx(device) -> DeviceContext:
     return c
 
 
+def status_text(v: int) -> str:
+    """What a device status word says."""
+    waits = {1: "a wait for a filled stage", 2: "a wait for a free stage", 3: "a wait for an accumulator",
+             4: "a wait for a peer"}
+    said = [f"{waits[v & 255]} gave up"] if v & 255 in waits else []
+    if 5 in (v & 255, v >> 8):
+        said.append("an index in the data was out of range")
+    return "; ".join(said)
+
+
 def check_status(device=None):
     """Raise if any kernel on ``device`` recorded an error (timeout / bounds)."""
     if device is None:
@@ -81,7 +93,7 @@ def check_status(device=None):
     v = int(c.status.item())
     if v != 0:
         c.status.zero_()
-        raise RuntimeError(f"device kernel reported error status {v} on {device}")
+        raise RuntimeError(f"device kernel reported error status {v} ({status_text(v)}) on {device}")
 
 
 # Split-K scratch: sized for the largest decode GEMM partial (splits x M x N fp32).

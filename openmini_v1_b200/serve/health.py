@@ -75,7 +75,7 @@ class HealthChecker:
             st = int(ops.ctx(torch.device("cuda", torch.cuda.current_device())).status.item())
             c.details["kernel_status"] = st
             if st != 0:
-                c.status, c.message = "unhealthy", f"a device wait gave up (status {st})"
+                c.status, c.message = "unhealthy", f"{ops.status_text(st)} (status {st})"
         except Exception as e:  # health must answer even when the device does not
             c.status, c.message = "unhealthy", repr(e)
         return c

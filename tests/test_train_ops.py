@@ -711,3 +711,38 @@ def test_trainer_stops_at_a_label_outside_the_vocabulary():
             tr.train()
     assert torch.equal(before, p.lm_head.detach())
     ops.check_status()
+
+
+# ----------------------------------------------------------------------------- errors in the data
+def test_status_text():
+    """A status word's low byte is the first wait that gave up or 5, its second byte 5 beside a wait."""
+    assert ops.status_text(5) == "an index in the data was out of range"
+    assert ops.status_text(1) == "a wait for a filled stage gave up"
+    assert ops.status_text(3 | 5 << 8) == "a wait for an accumulator gave up; an index in the data was out of range"
+
+
+@pytest.mark.gpu
+def test_targets_outside_the_vocabulary_leave_other_results_alone():
+    """They count as ignored, the status says so, and neither the gradient of the same call nor later calls
+    (products of several waves of tiles, with long waits) stop early."""
+    ops.check_status()
+    g = gen("cuda", 0)
+    x, w, dl = randn(g, 2049, 1024), randn(g, 4100, 1024, std=1 / 32), randn(g, 2049, dtype=F32)
+    wf, dh = randn(g, 4400, 1024, std=1 / 32), randn(g, 2049, 2200)
+    t = torch.randint(0, 4100, (2049,), generator=g, device="cuda")
+    t[::97] = -100
+    bad = t.clone()
+    bad[::97] = 4100
+    bad[97] = -7
+
+    def all_of(t):
+        loss, lse = ops.linear_xent(x, w, t)
+        h, gu = ops.swiglu(x, wf, save=True)
+        return [loss, lse, *ops.linear_xent_bwd(x, w, t, lse, dl), h, *ops.swiglu_bwd(x, wf, gu, dh)]
+
+    want, got = all_of(t), all_of(bad)
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    ops.check_status()

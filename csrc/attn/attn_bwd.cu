@@ -29,9 +29,9 @@
 // (and of no fp32 dQ in memory).
 //
 // What bounds it: the tensor cores, 1280 + 1024 of their cycles for a pair of tiles at head_dim 128
-// (kv + q), at the clock that the power limit leaves. Measured (B200, back to back): 1 x 8192, 40 / 8
-// heads of 128, causal 2.28 ms, 753 TFLOP/s of the five products, 1060 of the seven; 4 x <= 1499 padded,
-// 16 / 4 heads 121 us; head_dim 64, 1 x 8192, 32 / 8 heads 1.25 ms, where the exponentials bound it.
+// (kv + q) and the waits of a kv item's dP for its columns, at the clock that the power limit leaves. Measured (B200, back to back): 1 x 8192, 40 / 8
+// heads of 128, causal 2.42 ms, 709 TFLOP/s of the five products, 993 of the seven; 4 x <= 1499 padded,
+// 16 / 4 heads 127 us; head_dim 64, 1 x 8192, 32 / 8 heads 1.32 ms, where the exponentials bound it.
 //
 // Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared
 // memory before a product contracts over them, so that whatever padding holds (NaN too) adds 0.
@@ -136,11 +136,27 @@ __device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
   }
 }
 
-// Where tile i keeps its S (which = 0) and dP (1): four regions of 64 columns, two for each parity
-// of i. P and dS are written over S, so the region of dP is free once dS is there; the next tile
-// of the parity puts its S into it, before P and dS are used up, and its dP over P and dS after.
-__device__ __forceinline__ uint32_t tile_region(int i, int which) {
-  return (uint32_t)((i & 1) * 128 + (((i >> 1) ^ which) & 1) * 64);
+// Where tile i keeps its S (which = 0) and dP (1), from tensor memory's start: regions of 64 columns,
+// each parity of i has its own. P and dS are written over S, so the region of dP is free once dS is
+// there and the next tile of the parity puts its S into it. That tile's dP takes
+//   2 regions: the place of P and dS, once the products that read them are complete;
+//   3 regions: the third one, which the products of the tile before those left long ago.
+// kv items at head_dim over 64 have 2, because dV and dK take half of the columns; q items have 128
+// more from the second sum they do not need, and narrow heads leave the upper halves of both sums.
+// (1 x 8192, 40 / 8 heads of 128: 2.50 ms with 2 for all, 2.42 ms with 3 for q items.)
+template <int D>
+constexpr bool three_regions(bool kv) {
+  return D <= 64 || !kv;
+}
+template <int D>
+__device__ __forceinline__ uint32_t tile_region(int i, int which, bool three) {
+  const int odd = i & 1;
+  int slot = ((i >> 1) ^ which) & 1;
+  if (three) {
+    slot = ((i >> 1) + which) % 3;
+    if (slot == 2) return D <= 64 ? 64 + odd * 128 : 128 + odd * 64;
+  }
+  return 256 + odd * 128 + slot * 64;
 }
 
 // A thread's 32 columns of S -> P, kept in fp32 pairs; COLQ: also written in 16 bits over the
@@ -297,6 +313,22 @@ struct Item {
   }
 };
 
+// Bounded wait for the first of two phases: 1 or 2, 0 when neither came.
+__device__ __forceinline__ int poll_either(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* status, int code) {
+  const uint64_t t0 = globaltimer();
+  for (uint32_t spins = 1;; ++spins) {
+    if (mbar_test_wait(a, pa)) return 1;
+    if (mbar_test_wait(b, pb)) return 2;
+    if ((spins & 1023u) == 0) {
+      if (globaltimer() - t0 > OM_WAIT_LIMIT_NS) {
+        record_error(status, code);
+        return 0;
+      }
+      if (wait_failed(status)) return 0;
+    }
+  }
+}
+
 // kv: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
 // q:  resident Q, dO; streamed K, V; accumulates dQ.
 // Counters run over all items of a CTA: `tile` numbers the streamed tiles (ring stage, S / dP
@@ -308,7 +340,7 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
                     const AttnBwdArgs a) {
   using C = fa_bw::Cfg<D>;
   constexpr int NS = fa_bw::NSTAGE;
-  constexpr int STAGE0 = 256;  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D), then S and dP
+  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D); S and dP in tile_region
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* fix_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
@@ -437,10 +469,11 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
       const uint32_t x_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), 16);   // streamed, K-major
       const uint32_t m_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), C::SMALL);  // streamed, MN-major
       // S (which = 0) or dP (1) of a tile, from the resident rows and the tile's 64
+      bool three = D <= 64;
       auto scores = [&](int tile, auto which_c) {
         constexpr int which = decltype(which_c)::value;
         const uint32_t x = x_lo + (tile % NS) * (C::ST_BYTES / 16);
-        const uint32_t d = tmem + STAGE0 + tile_region(tile, which);
+        const uint32_t d = tmem + tile_region<D>(tile, which, three);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           tc_mma_f16_lo(d, r_lo + (which * C::H * C::BIG + (k >> 2) * C::BIG + (k & 3) * 32) / 16,
@@ -454,6 +487,13 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         tc_fence_after();
         return there;
       };
+      // The products that read P and dS of a tile are complete. Products of one shape into one accumulator
+      // run in order by themselves; a dP over the P and dS that other products read has to wait.
+      auto used = [&](int tile) {
+        const bool so = mbar_poll(&empty[tile % NS], (tile / NS) & 1, a.status, OM_ERR_WAIT_ACCUM);
+        tc_fence_after();
+        return so;
+      };
       int tile = 0, done = 0;
       bool ok = true;
       for (int k = 0; ok; ++k) {
@@ -465,15 +505,36 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         const Item w(a, n);
         if (w.total == 0) continue;
         ok = mbar_poll(fix_full, done & 1, a.status, OM_ERR_WAIT_FULL);
+        if (ok && three != three_regions<D>(w.kv)) {  // once a CTA: the columns change hands
+          three = !three;
+          ok = (tile == 0 || used(tile - 1)) && mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM);
+          tc_fence_after();
+        }
         for (int i = 0; i < 2 && i < w.total && ok; ++i) {
           ok = loaded(tile + i);
-          if (!ok) break;
-          scores(tile + i, S);
-          scores(tile + i, DP);
+          if (ok) scores(tile + i, S);
+        }
+        for (int i = 0; i < 2 && i < w.total && ok; ++i) {  // over P and dS of the item before
+          const int last = tile + i - (three ? 4 : 2);
+          ok = last < 0 || used(last);
+          if (ok) scores(tile + i, DP);
         }
         if (ok && w.total <= 2) tc_commit(fix_empty);
+        bool owed = false;  // dP of the next tile is still to be issued
         for (int i = 0; i < w.total && ok; ++i, ++tile) {
-          ok = mbar_poll(&ds_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+          auto pay = [&](int t, int last) {
+            tc_fence_after();
+            scores(t, DP);
+            owed = false;
+            if (last == w.total) tc_commit(fix_empty);  // the item's last scores
+          };
+          if (owed && !three) {  // this tile's dS or the columns of the next one's dP, whichever comes first
+            const int first = poll_either(&empty[(tile - 1) % NS], ((tile - 1) / NS) & 1, &ds_full[tile & 1],
+                                          (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+            ok = first != 0;
+            if (first == 1) pay(tile + 1, i + 2);
+          }
+          ok = ok && mbar_poll(&ds_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
           if (!ok) break;
           tc_fence_after();
           // dP of this tile has been read: its columns take the next S of this parity at once
@@ -482,13 +543,18 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
             if (!ok) break;
             scores(tile + 2, S);
           }
+          if (owed) {
+            ok = used(tile - 1);
+            if (!ok) break;
+            pay(tile + 1, i + 2);
+          }
           if (i == 0) {  // the sums of the item before have been read
             ok = mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM);
             if (!ok) break;
             tc_fence_after();
           }
           const uint32_t x = m_lo + (tile % NS) * (C::ST_BYTES / 16);
-          const uint32_t p = tmem + STAGE0 + tile_region(tile, 0);
+          const uint32_t p = tmem + tile_region<D>(tile, 0, three);
           if (w.kv) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // dV += P^T dO, 16 queries a step
@@ -500,11 +566,10 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
           for (int j = 0; j < 4; ++j)  // dK += dS^T Q, or dQ += dS K
             tc_mma_f16_ts_lo(d, p + 16 + (j >> 1) * 32 + (j & 1) * 8, x + j * 2048 / 16, IDESC_A, j > 0 ? 1 : i);
           tc_commit(&empty[tile % NS]);
-          // P and dS of this tile are read by the products just issued; the tensor pipe runs this
-          // thread's products in order, so the next dP may take their columns
-          if (i + 2 < w.total) {
-            scores(tile + 2, DP);
-            if (i + 3 == w.total) tc_commit(fix_empty);  // the item's last scores
+          owed = i + 2 < w.total;
+          if (owed && three) {
+            ok = tile < 2 || used(tile - 2);
+            if (ok) pay(tile + 2, i + 3);
           }
         }
         if (ok) tc_commit(acc_full);
@@ -556,8 +621,9 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           tc_fence_after();
-          const uint32_t s_at = lanes + STAGE0 + tile_region(it, 0) + half * 32;
-          const uint32_t dp_at = lanes + STAGE0 + tile_region(it, 1) + half * 32;
+          constexpr bool three = three_regions<D>(KV);
+          const uint32_t s_at = lanes + tile_region<D>(it, 0, three) + half * 32;
+          const uint32_t dp_at = lanes + tile_region<D>(it, 1, three) + half * 32;
           const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT) + half * 128;
           const bool masked = KV ? w.row0 + 128 > w.nrow || (a.causal && w.row0 + 127 > x0 + a.off)
                                  : x0 + 64 > w.nstream || (a.causal && x0 + 63 > w.row0 + a.off);
@@ -749,8 +815,8 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   // A kv item with all query heads of its KV head walks up to G T / 64 tiles. The launch ends about
   // when the longest item or the average SM does, so an item gets as many heads as fit into the
   // average (a q tile counts 0.75 of a kv tile), and all of them where that is a few tiles anyway
-  // (a join costs more). Split and not: 1 x 2048, 16 / 4 heads of 128 92 and 125 us; 1 x 4096, 16 / 2
-  // heads 232 and 449; with 16 tiles 24.7 and 25.4, with 8 tiles 25.0 and 20.7.
+  // (a join costs more). Split and not, 16 / 4 heads of 128: 1 x 2048 97 and 138 us; 1 x 512 (32 tiles) 26.8
+  // and 43.5; 1 x 256 (16 tiles) 27.6 and 26.8; 1 x 128 23.6 and 19.7. 1 x 4096, 16 / 2 heads 250 and 508.
   const int64_t qt = (T + 63) / 64, kt = (S + 127) / 128;
   const double average = (double)B * H * qt * kt * (causal ? 0.5 : 1.0) * 1.75 / om::num_sms();
   a.gper = a.G * qt <= 16 ? a.G : (int)std::min<double>(a.G, std::max(1.0, average / qt));

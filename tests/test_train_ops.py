@@ -746,3 +746,16 @@ def test_targets_outside_the_vocabulary_leave_other_results_alone():
     for a, b in zip(want, got):
         assert torch.equal(a, b)
     ops.check_status()
+
+
+# ----------------------------------------------------------------------------- paths that need large grids
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [
+    (6, 300, 300, 16, 4, 128, True, [300, 0, 129, 1, 64, 257]), (3, 700, 700, 12, 2, 64, True, None),
+    (2, 520, 777, 16, 16, 96, True, None), (4, 390, 390, 16, 8, 128, False, [390, 0, 65, 389]),
+    (2, 900, 500, 8, 4, 64, True, None)], ids=str)
+def test_attention_bwd_several_items_a_cta(shape):
+    """More work items than SMs (up to three each), full, ragged and empty ones in turn: the resident rows, the
+    accumulators and the tiles' places in tensor memory are handed from item to item."""
+    check_attention(attention_case("cuda", *shape), shape[6])
+    ops.check_status()

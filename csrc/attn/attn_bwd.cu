@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
   uint64_t* acc_empty = acc_full + 1;  // and have been read
   uint64_t* item_full = acc_empty + 1; // [2] the next item's number
   uint64_t* item_empty = item_full + 2;  // [2]
-  int* items = reinterpret_cast<int*>(item_empty + 2);  // [2]
+  uint64_t* drained = item_empty + 2;
+  int* items = reinterpret_cast<int*>(drained + 1);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(items + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -374,6 +375,7 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
       mbar_init(&item_full[s], 1);
       mbar_init(&item_empty[s], 17);
     }
+    mbar_init(drained, 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 16);
     fence_barrier_init();
@@ -443,7 +445,10 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         if (pad) {
           ok = __all_sync(0xffffffffu, mbar_wait(land, landed & 1, a.status, OM_ERR_WAIT_FULL));
           ++landed;
-          if (!ok) break;
+          if (!ok) {
+            mbar_wait(land, (landed - 1) & 1, nullptr, 0);
+            break;
+          }
           clear_rows<2 * C::H>(st, w.nstream - row, lane);
           fence_proxy_async_smem();
           __syncwarp();
@@ -574,6 +579,10 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         }
         if (ok) tc_commit(acc_full);
         ++done;
+      }
+      if (!ok) {  // wait (bounded) for the products that may still be running
+        tc_commit(drained);
+        mbar_wait(drained, 0, nullptr, 0);
       }
     }
   } else if (warp >= 4) {

@@ -462,12 +462,12 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t d_tmem, uint64_t a_desc
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrive on the barrier at this offset in both CTAs once this thread's MMAs so far are done.
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+// Arrive on the barrier at this offset in the CTAs of `mask` (both) once this thread's MMAs so far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar, uint16_t mask = 3) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
           smem_u32(bar)),
-      "h"((uint16_t)3)
+      "h"(mask)
       : "memory");
 }
 

@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(GX_THREADS, 1)
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = g.tiles_r * g.tiles_c * g.splits;
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(GX_THREADS, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 256);
     }
+    mbar_init(drained, 1);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -243,6 +245,10 @@ __global__ void __launch_bounds__(GX_THREADS, 1)
           }
           if (ok) tc_commit(&tfull[acc]);
         }
+      }
+      if (!ok) {  // wait (bounded) for the products that may still be running
+        tc_commit(drained);
+        mbar_wait(drained, 0, nullptr, 0);
       }
     }
   } else if (warp >= 4) {
@@ -328,7 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GX_THREADS, 1)
   uint64_t* empty = full + C::STAGES;
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + 2;  // the leader's count both CTAs' epilogue warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
@@ -344,6 +351,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GX_THREADS, 1)
       mbar_init(&tfull[a], 1);
       mbar_init(&tempty[a], 16);
     }
+    mbar_init(drained, 1);
     fence_barrier_init();
   }
   if (warp == 0 && lane == 0) {
@@ -433,6 +441,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GX_THREADS, 1)
           }
           if (ok) tc_commit_pair(&tfull[acc]);
         }
+      }
+      if (!ok) {  // wait (bounded) for the products that may still be running
+        tc_commit_pair(drained, 1);
+        mbar_wait(drained, 0, nullptr, 0);
       }
     }
   } else if (warp >= 4) {

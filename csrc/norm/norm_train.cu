@@ -163,7 +163,13 @@ struct RowRing {
         bulk_load(base + (size_t)(stage * NA + i) * bytes,
                   reinterpret_cast<const uint8_t*>(src[i] + row * ld[i]) - off(i, row), n[i], &full[stage]);
   }
-  __device__ __forceinline__ bool wait(int* status) const { return mbar_wait(&full[s], phase, status, OM_ERR_WAIT_FULL); }
+  // Not stopped by another wait that gave up: a group's copies depend on nobody, and leaving early would
+  // leave them in flight.
+  __device__ __forceinline__ bool wait(int* status) const {
+    if (mbar_wait(&full[s], phase, nullptr, 0)) return true;
+    record_error(status, OM_ERR_WAIT_FULL);
+    return false;
+  }
   __device__ __forceinline__ const T* row(int i) const {
     return reinterpret_cast<const T*>(base + (size_t)(s * NA + i) * bytes);
   }

@@ -135,7 +135,9 @@ void check_swiglu(const char* op, const torch::Tensor& x, const torch::Tensor& w
   const int64_t K = x.size(-1);
   TORCH_CHECK(w.dim() == 2 && w.size(0) % 2 == 0 && w.size(1) == K, op, ": w must be [2F, K]");
   TORCH_CHECK(K > 0 && K % 8 == 0, op, ": K must be a positive multiple of 8");
-  TORCH_CHECK(x.numel() / K < (1ll << 31) && w.size(0) < (1ll << 31) && K < (1ll << 30), op, ": too large");
+  // a tile may reach 255 rows past the last one, whose index is 32 bits
+  TORCH_CHECK(x.numel() / K < (1ll << 31) - 256 && w.size(0) < (1ll << 31) - 256 && K < (1ll << 30), op,
+              ": too large");
 }
 
 }  // namespace

@@ -748,6 +748,19 @@ def test_targets_outside_the_vocabulary_leave_other_results_alone():
     ops.check_status()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2 ** 31 - 256, 2 ** 31 - 1])
+def test_swiglu_refuses_rows_whose_tiles_pass_32_bits(rows):
+    """The last row tile's index must not wrap; refused before anything of that size is allocated."""
+    x = torch.zeros(1, 8, dtype=B16, device="cuda").expand(rows, 8)
+    w = torch.zeros(16, 8, dtype=B16, device="cuda")
+    before = torch.cuda.memory_allocated()
+    for call in (lambda: ops.swiglu(x, w), lambda: ops.swiglu_bwd(x, w, x, x)):
+        with pytest.raises(RuntimeError, match="too large"):
+            call()
+    assert torch.cuda.memory_allocated() == before
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -803,7 +803,7 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   auto dq = torch::empty({B, T, H, D}, q.options());
   auto dk = torch::empty({B, S, Hkv, D}, q.options());
   auto dv = torch::empty({B, S, Hkv, D}, q.options());
-  if (B == 0 || T == 0 || S == 0) {
+  if (B == 0 || T == 0 || S == 0 || H == 0) {
     dq.zero_();
     dk.zero_();
     dv.zero_();

@@ -319,7 +319,7 @@ def attention_bwd(q, k, v, out, lse, dout, scale, causal=True, lens=None):
     ds = (p * (dp - delta)).masked_fill(~vis, 0.0)
     dq = torch.einsum("bhqk,bkhd->bqhd", ds, kf) * scale
     dk = torch.einsum("bhqk,bqhd->bkhd", ds, qf) * scale
-    if G > 1:
+    if G != 1:
         dk = dk.view(B, S, Hkv, G, D).sum(3)
         dv = dv.view(B, S, Hkv, G, D).sum(3)
     return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)

@@ -761,6 +761,17 @@ def test_swiglu_refuses_rows_whose_tiles_pass_32_bits(rows):
     assert torch.cuda.memory_allocated() == before
 
 
+@on_devices
+@pytest.mark.parametrize("B,T,S,H,Hkv", [(0, 3, 3, 2, 1), (2, 0, 5, 2, 1), (2, 5, 0, 2, 2), (1, 4, 4, 0, 1)])
+def test_attention_bwd_of_nothing(dev, B, T, S, H, Hkv):
+    """No sequence, query, key or query head: empty results, and zeros for the keys nobody reads."""
+    q, k = (torch.ones(B, n, h, 64, dtype=B16, device=dev) for n, h in ((T, H), (S, Hkv)))
+    lse = torch.zeros(B, T, H, device=dev)
+    got = ops.attention_bwd(q, k, k, q, lse, q, 1.0, causal=False)
+    for g, like in zip(got, (q, k, k)):
+        assert g.shape == like.shape and not g.any()
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(32 * XE_JOIN) xent_join_kernel(const float2* _
     m = mn;
     z += sz[w][lane];
   }
-  const float l = m == -INFINITY ? -INFINITY : (m + log2f(s)) * XE_LN2;
+  const float l = s == 0.f ? -INFINITY : (m + log2f(s)) * XE_LN2;  // no column: -inf; a NaN logit: NaN
   lse[r] = l;
   float out = 0.f;
   if (t >= 0 && t < x.V && t != x.ignore) {

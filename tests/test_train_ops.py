@@ -772,6 +772,20 @@ def test_attention_bwd_of_nothing(dev, B, T, S, H, Hkv):
         assert g.shape == like.shape and not g.any()
 
 
+@on_devices
+def test_linear_xent_of_nan_rows(dev):
+    """A row of NaN logits has a NaN lse; -inf is the lse of a row without a column alone."""
+    g = gen(dev, 1)
+    x, w = randn(g, 5, 64), randn(g, 300, 64)
+    x[1] = float("nan")
+    t = torch.tensor([0, 1, 2, -100, 4], device=dev)
+    loss, lse = ops.linear_xent(x, w, t)
+    dx, dw = ops.linear_xent_bwd(x, w, t, lse, torch.ones(5, device=dev))
+    ok = torch.tensor([True, False, True, True, True])
+    for v in (loss, lse, dx.float().sum(-1)):
+        assert torch.equal(torch.isfinite(v).cpu(), ok) and bool(torch.isnan(v[1]))
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -52,7 +52,7 @@ class _Norm(torch.autograd.Function):
         y, h, stats = ops.norm_train(x, w, b, eps, kind=kind, delta=delta)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(h, w, stats)
-        ctx.kind, ctx.bias, ctx.summed = kind, b is not None, delta is not None
+        ctx.kind, ctx.bias, ctx.summed, ctx.eps = kind, b is not None, delta is not None, eps
         return (y, h) if delta is not None else y
 
     @staticmethod
@@ -60,8 +60,26 @@ class _Norm(torch.autograd.Function):
         h, w, stats = ctx.saved_tensors
         if gy is None:
             gy = torch.zeros_like(h)
-        dx, dw, db = ops.norm_train_bwd(gy, h, w, stats, kind=ctx.kind, bias=ctx.bias, dh=gh)
-        return dx, dx if ctx.summed else None, dw, db, None, None
+        if torch.is_grad_enabled():
+            dx, dw, db = _norm_grad(gy, h, w, ctx.eps, ctx.kind, gh)
+        else:
+            dx, dw, db = ops.norm_train_bwd(gy, h, w, stats, kind=ctx.kind, bias=ctx.bias, dh=gh)
+        return dx, dx if ctx.summed else None, dw, db if ctx.bias else None, None, None
+
+
+def _norm_grad(gy, h, w, eps, kind, gh):
+    """(dx, dw, db) of a norm in plain operations on h, w and gy, for create_graph=True: a function
+    of all three that differentiates on."""
+    hf, g = h.float(), gy.float()
+    d = hf - hf.mean(-1, keepdim=True) if kind == "layer" else hf
+    r = torch.rsqrt(d.pow(2).mean(-1, keepdim=True) + eps)
+    n, a = d * r, g * w.float()
+    dx = a - n * (a * n).mean(-1, keepdim=True)
+    if kind == "layer":
+        dx = dx - a.mean(-1, keepdim=True)
+    dx = dx * r if gh is None else dx * r + gh.float()
+    over_rows = lambda t: t.reshape(-1, t.shape[-1]).sum(0).to(w.dtype)  # noqa: E731
+    return dx.to(h.dtype), over_rows(g * n), over_rows(g)
 
 
 def _norm_native(x, w):

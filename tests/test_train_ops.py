@@ -786,6 +786,36 @@ def test_linear_xent_of_nan_rows(dev):
         assert torch.equal(torch.isfinite(v).cpu(), ok) and bool(torch.isnan(v[1]))
 
 
+def _norm_forms():
+    from openmini_v1_b200.ops import autograd as ag
+    rms = lambda x, w: x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-5) * w  # noqa: E731
+
+    def layer(x, w, b):
+        d = x - x.mean(-1, keepdim=True)
+        return d * torch.rsqrt(d.pow(2).mean(-1, keepdim=True) + 1e-5) * w + b
+
+    return {"rms": (lambda x, y, w: ag.rmsnorm(x, w, 1e-5), lambda x, y, w: rms(x, w)),
+            "add": (lambda x, y, w: sum(ag.add_rmsnorm(x, y, w, 1e-5)), lambda x, y, w: rms(x + y, w) + x + y),
+            "layer": (lambda x, y, w: ag.layernorm(x, w, y[0], 1e-5), lambda x, y, w: layer(x, w, y[0]))}
+
+
+@on_devices
+@pytest.mark.parametrize("form,shape", [("rms", (6, 48)), ("add", (6, 48)), ("layer", (6, 48)), ("rms", (48,))])
+def test_norms_differentiate_twice(dev, form, shape):
+    """A gradient taken with create_graph=True differentiates on: f(x) = sum norm(x)^3, then |grad f|^2."""
+    got, want = _norm_forms()[form]
+    g = gen(dev, 2)
+    inputs = [randn(g, *shape, dtype=F32), randn(g, *shape, dtype=F32), randn(g, 48, dtype=F32)]
+    out = []
+    for f, dt in ((got, F32), (want, torch.float64)):
+        a = [t.to(dt).requires_grad_(True) for t in inputs]
+        used = [t for t, name in zip(a, "xyw") if not (form == "rms" and name == "y")]
+        first = torch.autograd.grad((f(*a) ** 3).sum(), used, create_graph=True)
+        out.append([*first, *torch.autograd.grad(sum((v ** 2).sum() for v in first), used)])
+    for a, b in zip(*out):
+        torch.testing.assert_close(a.double(), b, rtol=2e-4, atol=2e-4 * float(b.abs().max()))
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -43,6 +43,35 @@ def linear(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     return y.reshape(*shp[:-1], w.shape[0])
 
 
+class _FirstOnly(torch.autograd.Function):
+    """A gradient as it is, tied to what it was computed from: differentiating it raises."""
+
+    @staticmethod
+    def forward(ctx, op, grad, *of):
+        ctx.op = op
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.op} has first derivatives only: a gradient taken with create_graph=True cannot be "
+                           "differentiated through it")
+
+
+def _first_only(op):
+    """Marks the backward of a Function whose gradients have no graph. (Without a mark their second
+    derivatives would be left out of a sum in silence.)"""
+    def mark(fn):
+        def backward(ctx, *grads):
+            with torch.no_grad():
+                out = fn(ctx, *grads)
+            if not torch.is_grad_enabled():
+                return out
+            of = [t for t in (*ctx.saved_tensors, *grads) if t is not None]
+            return tuple(None if g is None else _FirstOnly.apply(op, g, *of) for g in out)
+        return backward
+    return mark
+
+
 class _Norm(torch.autograd.Function):
     """y = norm(x (+ delta)) w (+ b) on the native kernels (``ops.norm_train``); with delta the sum
     h comes back too, and its gradient joins dx in the same pass."""
@@ -120,6 +149,7 @@ class _SwiGLU(torch.autograd.Function):
         return h
 
     @staticmethod
+    @_first_only("swiglu")
     def backward(ctx, gh):
         x, w, gu = ctx.saved_tensors
         return ops.swiglu_bwd(x, w, gu, gh, ctx.needs_input_grad[0], ctx.needs_input_grad[1])
@@ -146,6 +176,7 @@ class _LinearXent(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @_first_only("linear_xent")
     def backward(ctx, gl):
         x, w, targets, lse, keep = ctx.saved_tensors
         dx, dw = ops.linear_xent_bwd(x, w, targets, lse, gl, *ctx.args, keep=keep, need_dx=ctx.needs_input_grad[0],
@@ -214,6 +245,7 @@ class _Attention(torch.autograd.Function):
         return out.to(q.dtype)
 
     @staticmethod
+    @_first_only("attention")
     def backward(ctx, go):
         q, k, v, out, lse, lens = ctx.saved_tensors
         dq, dk, dv = ops.attention_bwd(q, k, v, out, lse, go, ctx.scale, causal=True, lens=lens)

@@ -816,6 +816,26 @@ def test_norms_differentiate_twice(dev, form, shape):
         torch.testing.assert_close(a.double(), b, rtol=2e-4, atol=2e-4 * float(b.abs().max()))
 
 
+@on_devices
+def test_second_derivatives_of_the_fused_products_are_refused(dev):
+    """swiglu, linear_xent and attention have first derivatives only, and say so, also beside a path
+    that has more (on the CPU the first two are plain operations)."""
+    from openmini_v1_b200.ops import autograd as ag
+    g = gen(dev, 2)
+    x, w = randn(g, 8, 64).requires_grad_(True), randn(g, 48, 64).requires_grad_(True)
+    q = randn(g, 1, 16, 2, 64).requires_grad_(True)
+    t = torch.randint(0, 48, (8,), generator=g, device=dev)
+    forms = [(lambda: ag.attention(q, q, q, 0.1), q)]
+    if dev == "cuda":
+        forms += [(lambda: ag.swiglu(x, w), x), (lambda: ag.linear_xent(x, w, t), x)]
+    for f, v in forms:
+        want, = torch.autograd.grad(f().float().sum(), v)
+        first, = torch.autograd.grad(f().float().sum() + v.float().pow(3).sum(), v, create_graph=True)
+        torch.testing.assert_close(first.float(), want.float() + 3 * v.detach().float().pow(2), atol=0.1, rtol=2e-2)
+        with pytest.raises(RuntimeError, match="first derivatives only"):
+            torch.autograd.grad(first.float().pow(2).sum(), v)
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

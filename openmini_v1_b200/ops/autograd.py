@@ -7,6 +7,7 @@ x @ w^T form on transposed copies); on the CPU it is the fp32 torch statement.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import ops
 
@@ -111,9 +112,15 @@ def _norm_grad(gy, h, w, eps, kind, gh):
     return dx.to(h.dtype), over_rows(g * n), over_rows(g)
 
 
-def _norm_native(x, w):
-    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32) and w.dtype in (x.dtype, torch.float32)
-            and x.shape[-1] <= 16384)
+def _norm_native(x, w, delta=None, b=None):
+    """Whether the kernels take this norm. The plain statement takes the rest: other types, gains and
+    deltas that broadcast, and what torch.func or a forward-mode dual has to see through."""
+    return (x.is_cuda and x.dim() > 0 and x.dtype in (torch.bfloat16, torch.float32)
+            and w.dtype in (x.dtype, torch.float32) and w.shape == x.shape[-1:] and 0 < x.shape[-1] <= 16384
+            and (delta is None or (delta.shape == x.shape and delta.dtype == x.dtype))
+            and (b is None or (b.shape == w.shape and b.dtype == w.dtype))
+            and not torch._C._are_functorch_transforms_active()
+            and all(t is None or unpack_dual(t).tangent is None for t in (x, w, delta, b)))
 
 
 def rmsnorm(x, w, eps):
@@ -125,7 +132,7 @@ def rmsnorm(x, w, eps):
 
 def add_rmsnorm(x, delta, w, eps):
     """(rmsnorm(h), h) with h = x + delta: the residual add and the norm that follows it."""
-    if _norm_native(x, w):
+    if _norm_native(x, w, delta):
         return _Norm.apply(x, delta, w, None, eps, "rms")
     h = x + delta
     return rmsnorm(h, w, eps), h
@@ -133,7 +140,7 @@ def add_rmsnorm(x, delta, w, eps):
 
 def layernorm(x, w, b, eps):
     """LayerNorm with gain and (optional) bias over the last dimension."""
-    if _norm_native(x, w):
+    if _norm_native(x, w, b=b):
         return _Norm.apply(x, None, w, b, eps, "layer")
     xf = x.float()
     mu = xf.mean(-1, keepdim=True)

@@ -836,6 +836,32 @@ def test_second_derivatives_of_the_fused_products_are_refused(dev):
             torch.autograd.grad(first.float().pow(2).sum(), v)
 
 
+@on_devices
+def test_rmsnorm_under_transforms_and_with_other_gains(dev):
+    """vmap, jvp and forward-mode duals go through ag.rmsnorm, and a gain need not be a vector of the row's length."""
+    import torch.autograd.forward_ad as fw
+
+    from openmini_v1_b200.ops import autograd as ag
+    g = gen(dev, 4)
+    x, v, w = randn(g, 3, 5, 48, dtype=F32), randn(g, 3, 5, 48, dtype=F32), randn(g, 48, dtype=F32)
+    plain = lambda x, w: x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-5) * w  # noqa: E731
+    f = lambda x: ag.rmsnorm(x, w, 1e-5)  # noqa: E731
+    torch.testing.assert_close(torch.func.vmap(f)(x), plain(x, w))
+    y, dy = torch.func.jvp(f, (x,), (v,))
+    wy, wdy = torch.func.jvp(lambda x: plain(x, w), (x,), (v,))
+    torch.testing.assert_close(y, wy)
+    torch.testing.assert_close(dy, wdy)
+    with fw.dual_level():
+        torch.testing.assert_close(fw.unpack_dual(f(fw.make_dual(x, v))).tangent, wdy)
+    torch.testing.assert_close(torch.func.grad(lambda x: f(x).pow(3).sum())(x),
+                               torch.func.grad(lambda x: plain(x, w).pow(3).sum())(x), rtol=1e-4, atol=1e-4)
+    for gain in (w[None], w[:1], torch.tensor(0.5, device=dev), randn(g, 5, 48, dtype=F32)):
+        torch.testing.assert_close(ag.rmsnorm(x, gain, 1e-5), plain(x, gain))
+    torch.testing.assert_close(ag.layernorm(x, w[None], None, 1e-5),
+                               torch.nn.functional.layer_norm(x, (48,)) * w, rtol=1e-4, atol=1e-4)
+    torch.testing.assert_close(ag.add_rmsnorm(x, v[:1], w, 1e-5)[0], plain(x + v[:1], w))
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .. import ops
 from ..ops import autograd as ag
 from ..ops import reference as ref
 from .config import ModelConfig
@@ -103,12 +104,17 @@ class Policy(nn.Module):
         """ids [B, T] -> logits [B, T, V] (fp32)."""
         return ag.linear(self.hidden(ids, forced_routing, record_routing), self._w(self.lm_head)).float()
 
-    def loss(self, ids: torch.Tensor, labels: torch.Tensor, label_smoothing: float = 0.0) -> torch.Tensor:
+    def loss(self, ids: torch.Tensor, labels: torch.Tensor, label_smoothing: float = 0.0,
+             check: bool = True) -> torch.Tensor:
         """Mean next-token cross entropy (``train.loss.causal_lm_loss`` of the logits) without the
-        logits: position t predicts labels[t + 1], labels of -100 do not count."""
+        logits: position t predicts labels[t + 1], labels of -100 do not count. Any other label
+        outside the vocabulary raises, as does any error that a kernel reported before; a caller that
+        looks at the device status itself (``ops.check_status``) leaves that out with ``check``."""
         tgt = torch.full_like(labels, -100)
         tgt[:, :-1] = labels[:, 1:]
         rows = ag.linear_xent(self.hidden(ids), self._w(self.lm_head), tgt, smoothing=label_smoothing)
+        if check and rows.is_cuda:
+            ops.check_status(rows.device)
         return rows.sum() / (tgt != -100).sum().clamp(min=1)
 
     def logprobs(self, hidden: torch.Tensor, targets: torch.Tensor, temperature: float = 1.0, keep=None):

@@ -119,7 +119,7 @@ class Trainer:
         ids = batch["input_ids"].to(self.device)
         labels = batch["labels"].to(self.device)
         if ids.is_cuda and isinstance(self.model, Policy):  # no logits in memory
-            return self.model.loss(ids, labels, self.cfg.label_smoothing_factor)
+            return self.model.loss(ids, labels, self.cfg.label_smoothing_factor, check=False)  # the callers check
         logits = self.model(ids)
         return causal_lm_loss(logits, labels, self.cfg.label_smoothing_factor)
 
@@ -147,6 +147,8 @@ class Trainer:
             tot += float(self._loss(batch))
             n += 1
         self.model.train()
+        if self.device.type == "cuda":  # a label outside the vocabulary has counted as a loss of 0
+            ops.check_status(self.device)
         t = torch.tensor([tot, float(n)], device=self.device)
         if dist.is_initialized() and self.reducer.world > 1:
             dist.all_reduce(t, group=self.reducer.group)

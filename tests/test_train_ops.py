@@ -862,6 +862,29 @@ def test_rmsnorm_under_transforms_and_with_other_gains(dev):
     torch.testing.assert_close(ag.add_rmsnorm(x, v[:1], w, 1e-5)[0], plain(x + v[:1], w))
 
 
+@pytest.mark.gpu
+def test_a_label_outside_the_vocabulary_has_no_loss():
+    """Neither Policy.loss nor an evaluation returns a number for it."""
+    import tempfile
+
+    from openmini_v1_b200.train.trainer import Trainer, TrainingConfig
+    p = small_policy("cuda")
+    ids = torch.randint(0, 520, (2, 32), generator=gen("cpu", 4))
+    labels = ids.clone()
+    labels[1, 7] = 520
+    with pytest.raises(RuntimeError, match="out of range"):
+        p.loss(ids.cuda(), labels.cuda())
+    ops.check_status()
+    good = {"input_ids": ids, "labels": ids}
+    with tempfile.TemporaryDirectory() as d:
+        tr = Trainer(p, TrainingConfig(num_train_epochs=1, output_dir=d, save_steps=0), [good],
+                     eval_loader=[good, {"input_ids": ids, "labels": labels}, good])
+        with pytest.raises(RuntimeError, match="out of range"):
+            tr.evaluate()
+        tr.eval_loader = [good]
+        assert math.isfinite(tr.evaluate())
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -10,6 +10,7 @@ from __future__ import annotations
 import threading
 
 import torch
+import torch.distributed as dist
 
 from .. import _native
 from . import reference as ref
@@ -85,15 +86,22 @@ def status_text(v: int) -> str:
     return "; ".join(said)
 
 
-def check_status(device=None):
-    """Raise if any kernel on ``device`` recorded an error (timeout / bounds)."""
+def check_status(device=None, across=False, group=None):
+    """Raise if any kernel on ``device`` recorded an error (timeout / bounds). With ``across`` the
+    ranks of ``group`` (None: all) call this together, and all of them raise if one has an error."""
     if device is None:
         device = torch.device("cuda", torch.cuda.current_device())
     c = ctx(device)
+    if across:
+        worst = c.status.clone()
+        dist.all_reduce(worst, op=dist.ReduceOp.MAX, group=group)
+        worst = int(worst.item())
     v = int(c.status.item())
     if v != 0:
         c.status.zero_()
         raise RuntimeError(f"device kernel reported error status {v} ({status_text(v)}) on {device}")
+    if across and worst != 0:
+        raise RuntimeError(f"device kernel of another rank reported error status {worst} ({status_text(worst)})")
 
 
 # Split-K scratch: sized for the largest decode GEMM partial (splits x M x N fp32).

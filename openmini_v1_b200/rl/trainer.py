@@ -160,8 +160,8 @@ class GRPOTrainer:
         if self.reducer is not None:
             self.reducer.finish()
         gn = torch.nn.utils.clip_grad_norm_(self.policy.parameters(), self.cfg.max_grad_norm)
-        if dev.type == "cuda":  # nothing is learnt from a step in which a kernel reported an error
-            ops.check_status(dev)
+        # nothing is learnt from a step in which a kernel of any rank reported an error
+        ops.check_status(dev, across=self.reducer is not None, group=self.dp_group)
         self.opt.step()
         self.policy.export_to(self.engine.model)
         self.step_idx += 1

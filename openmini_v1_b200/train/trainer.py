@@ -123,8 +123,18 @@ class Trainer:
         logits = self.model(ids)
         return causal_lm_loss(logits, labels, self.cfg.label_smoothing_factor)
 
+    def _check(self):
+        """Stop before a step in which a kernel of any rank reported an error: nothing is learnt from it."""
+        try:
+            ops.check_status(self.device, across=self.reducer.world > 1, group=self.reducer.group)
+        except RuntimeError:
+            self.opt.zero_grad(set_to_none=True)
+            raise
+
     def _optimizer_step(self) -> dict:
         self.reducer.finish()
+        if self.reducer.world > 1:
+            self._check()
         params = [p for p in self.model.parameters() if p.grad is not None]
         ok = self.scaler.unscale_and_check(params)
         gn = float(torch.nn.utils.clip_grad_norm_(params, self.cfg.max_grad_norm)) if params else 0.0
@@ -147,8 +157,8 @@ class Trainer:
             tot += float(self._loss(batch))
             n += 1
         self.model.train()
-        if self.device.type == "cuda":  # a label outside the vocabulary has counted as a loss of 0
-            ops.check_status(self.device)
+        # on the GPU a label outside the vocabulary has counted as a loss of 0
+        ops.check_status(self.device, across=self.reducer.world > 1, group=self.reducer.group)
         t = torch.tensor([tot, float(n)], device=self.device)
         if dist.is_initialized() and self.reducer.world > 1:
             dist.all_reduce(t, group=self.reducer.group)
@@ -196,8 +206,8 @@ class Trainer:
                 self.scaler.scale_loss(loss / acc).backward()
                 st.micro_step = i + 1
                 st.last_loss = float(loss.detach())
-                if loss.is_cuda:  # a label outside the vocabulary, a wait that gave up: stop before the step
-                    ops.check_status(loss.device)
+                if self.reducer.world == 1:  # a label outside the vocabulary, a wait that gave up; with more
+                    self._check()            # ranks all look together, once their gradients are summed
                 if not last:
                     continue
                 info = self._optimizer_step()

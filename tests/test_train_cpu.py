@@ -6,6 +6,7 @@ import os
 import socket
 import struct
 
+import pytest
 import torch
 import torch.multiprocessing as mp
 
@@ -114,6 +115,63 @@ def _dp_worker(rank, world, port, q):
         q.put((rank, g))
     finally:
         dist.destroy_process_group()
+
+
+def _error_worker(rank, port, q, where, out):
+    """Three batches on each of two ranks; in the second one rank 1's status word reports an error."""
+    import torch.distributed as dist
+    from openmini_v1_b200 import ops
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        torch.manual_seed(0)
+        m = Policy(_cfg(), seed=1)
+        seen, plain = [], m.forward
+
+        def forward(*a, **k):
+            seen.append(1)
+            if rank == 1 and len(seen) == 3:  # micro-batch 1 of step 2, or of the evaluation's two batches
+                ops.ctx(torch.device("cpu")).status.fill_(5)
+            return plain(*a, **k)
+
+        m.forward = forward
+        ids = torch.randint(0, 259, (2, 9), generator=torch.Generator().manual_seed(rank))
+
+        class Loader(list):
+            def set_epoch(self, e):
+                pass
+
+        batches = Loader([{"input_ids": ids, "labels": ids}] * 6)
+        tr = Trainer(m, TrainingConfig(num_train_epochs=1, output_dir=out, save_steps=0, logging_steps=1,
+                                       gradient_accumulation_steps=2), batches, eval_loader=batches)
+        told = None
+        try:
+            tr.evaluate() if where == "evaluate" else tr.train()
+        except RuntimeError as e:
+            told = str(e)
+        q.put((rank, told, tr.state.global_step, torch.cat([p.detach().reshape(-1) for p in m.parameters()]).numpy().copy()))
+        dist.barrier()
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("where", ["train", "evaluate"])
+def test_an_error_on_one_rank_stops_every_rank(where, tmp_path):
+    """Both ranks raise, before the step whose gradients the error has spoilt, and hold the same weights."""
+    port = _free_port()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_error_worker, args=(r, port, q, where, str(tmp_path))) for r in range(2)]
+    for p in ps:
+        p.start()
+    res = sorted((q.get(timeout=240) for _ in range(2)), key=lambda r: r[0])
+    for p in ps:
+        p.join(60)
+        assert p.exitcode == 0
+    (_, a, sa, wa), (_, b, sb, wb) = res
+    assert a is not None and "another rank" in a and "out of range" in b
+    assert sa == sb == (1 if where == "train" else 0)
+    assert (wa == wb).all()
 
 
 def test_dp_grad_average():

@@ -163,6 +163,14 @@ class Policy(nn.Module):
                 M["down"] = L.down.detach().to(dt).to(model.device).contiguous()
 
 
+def logits_free(model) -> bool:
+    """Whether ``loss`` and ``logprobs`` on the hidden states are what calling the model would give: a
+    Policy whose class has its own ``forward``, or that has hooks, has to be called."""
+    return (isinstance(model, Policy) and type(model).forward is Policy.forward
+            and not (model._forward_hooks or model._forward_pre_hooks or model._backward_hooks
+                     or model._backward_pre_hooks))
+
+
 def _rope(x, pos, inv_f, mode):
     ang = pos.float()[:, None] * inv_f[None, :]
     c, s = torch.cos(ang)[None, :, None, :], torch.sin(ang)[None, :, None, :]

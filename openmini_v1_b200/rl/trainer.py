@@ -29,7 +29,7 @@ import torch.distributed as dist
 
 from ..engine.request import SamplingParams
 from .. import ops
-from ..models.policy import Policy, token_logprobs
+from ..models.policy import Policy, logits_free, token_logprobs
 from .grpo import GRPOConfig, group_relative_advantage, grpo_loss
 from .replay import KeepRouting, KeepSamplingMask, unpack_words
 
@@ -106,7 +106,7 @@ class GRPOTrainer:
                         for i, r in enumerate(per):
                             rows[i, :r[layer].shape[0]] = r[layer]
                         routing[layer] = rows.view(len(grp) * T, k)
-            if dev.type == "cuda" and hasattr(model, "logprobs"):
+            if dev.type == "cuda" and logits_free(model):
                 out += self._logp_rows(model, grp, seqs, ids.to(dev), routing)
                 continue
             logits = model(ids.to(dev), forced_routing=routing)

@@ -23,7 +23,7 @@ import torch
 import torch.distributed as dist
 
 from .. import ops
-from ..models.policy import Policy
+from ..models.policy import logits_free
 from .checkpoint import CheckpointManager
 from .ddp import GradReducer
 from .loss import DynamicLossScaler, causal_lm_loss, perplexity
@@ -118,7 +118,7 @@ class Trainer:
     def _loss(self, batch):
         ids = batch["input_ids"].to(self.device)
         labels = batch["labels"].to(self.device)
-        if ids.is_cuda and isinstance(self.model, Policy):  # no logits in memory
+        if ids.is_cuda and logits_free(self.model):  # no logits in memory
             return self.model.loss(ids, labels, self.cfg.label_smoothing_factor, check=False)  # the callers check
         logits = self.model(ids)
         return causal_lm_loss(logits, labels, self.cfg.label_smoothing_factor)

@@ -885,6 +885,92 @@ def test_a_label_outside_the_vocabulary_has_no_loss():
         assert math.isfinite(tr.evaluate())
 
 
+@pytest.mark.gpu
+def test_trainer_runs_the_models_own_forward():
+    """A subclass's forward and forward hooks decide the loss on the GPU as they do on the CPU."""
+    import tempfile
+
+    from openmini_v1_b200.models.policy import Policy
+    from openmini_v1_b200.train.loss import causal_lm_loss
+    from openmini_v1_b200.train.trainer import Trainer, TrainingConfig
+
+    class Sharp(Policy):
+        def forward(self, *a, **k):
+            return super().forward(*a, **k) * 3.0
+
+    base = small_policy("cuda")
+    ids = torch.randint(0, 520, (2, 32), generator=gen("cpu", 4))
+    batch = {"input_ids": ids, "labels": ids}
+    want = float(causal_lm_loss(base(ids.cuda()) * 3.0, ids.cuda()))
+    sharp = Sharp(base.cfg, device="cuda", seed=5)
+    hooked = small_policy("cuda")
+    hooked.register_forward_hook(lambda m, a, out: out * 3.0)
+    for m in (sharp, hooked):
+        with tempfile.TemporaryDirectory() as d:
+            tr = Trainer(m, TrainingConfig(num_train_epochs=1, output_dir=d, save_steps=0), [batch])
+            assert abs(float(tr._loss(batch)) - want) < 1e-3 * want
+    plain = float(causal_lm_loss(base(ids.cuda()), ids.cuda()))
+    assert abs(plain - want) > 1e-3 * want
+
+
+def grpo_case(cls=None):
+    """A trainer without its engine, samples of unequal lengths, kept sets for some of them."""
+    from openmini_v1_b200.models.policy import Policy
+    from openmini_v1_b200.rl.replay import EnforceMode, KeepRouting, KeepSamplingMask
+    from openmini_v1_b200.rl.trainer import GRPOTrainer
+    pol = small_policy("cuda", moe=True) if cls is None else cls(small_policy("cpu").cfg, device="cuda", seed=5)
+    tr = GRPOTrainer.__new__(GRPOTrainer)
+    tr.policy, tr.temperature, tr.train_batch = pol, 0.8, 3
+    tr.keep_routing, tr.keep_mask = KeepRouting(100, EnforceMode.NONE), KeepSamplingMask(100)
+    g = gen("cpu", 6)
+    samples = []
+    for i, (n, c) in enumerate([(4, 9), (17, 1), (3, 30), (40, 12), (5, 5)]):
+        toks = torch.randint(0, 520, (n + c,), generator=g).tolist()
+        samples.append({"key": f"s{i}", "prompt": toks[:n], "completion": toks[n:]})
+        if i % 2 == 0:
+            mask = torch.rand(c, 520, generator=g) < 0.3
+            mask[torch.arange(c), torch.tensor(toks[n:])] = True
+            tr.keep_mask.save(f"s{i}", words_of(mask))
+    return tr, pol, samples
+
+
+def grpo_case(cls=None):
+    """A trainer without its engine, samples of unequal lengths, kept sets for some of them."""
+    from openmini_v1_b200.models.policy import Policy
+    from openmini_v1_b200.rl.replay import EnforceMode, KeepRouting, KeepSamplingMask
+    from openmini_v1_b200.rl.trainer import GRPOTrainer
+    pol = small_policy("cuda", moe=True) if cls is None else cls(small_policy("cpu").cfg, device="cuda", seed=5)
+    tr = GRPOTrainer.__new__(GRPOTrainer)
+    tr.policy, tr.temperature, tr.train_batch = pol, 0.8, 3
+    tr.keep_routing, tr.keep_mask = KeepRouting(100, EnforceMode.NONE), KeepSamplingMask(100)
+    g = gen("cpu", 6)
+    samples = []
+    for i, (n, c) in enumerate([(4, 9), (17, 1), (3, 30), (40, 12), (5, 5)]):
+        toks = torch.randint(0, 520, (n + c,), generator=g).tolist()
+        samples.append({"key": f"s{i}", "prompt": toks[:n], "completion": toks[n:]})
+        if i % 2 == 0:
+            mask = torch.rand(c, 520, generator=g) < 0.3
+            mask[torch.arange(c), torch.tensor(toks[n:])] = True
+            tr.keep_mask.save(f"s{i}", words_of(mask))
+    return tr, pol, samples
+
+
+@pytest.mark.gpu
+def test_grpo_runs_the_models_own_forward():
+    from openmini_v1_b200.models.policy import Policy
+
+    class Sharp(Policy):
+        def forward(self, *a, **k):
+            return super().forward(*a, **k) * 3.0
+
+    tr, pol, samples = grpo_case(Sharp)
+    tr.keep_mask.clear()
+    got = tr._batch_logp(pol, samples[:1])[0]
+    ids = torch.tensor(samples[0]["prompt"] + samples[0]["completion"], device="cuda")
+    want = torch.log_softmax(pol(ids[None, :-1])[0, 3:] / 0.8, -1).gather(-1, ids[4:, None])[:, 0]
+    torch.testing.assert_close(got, want, atol=2e-2, rtol=2e-2)
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

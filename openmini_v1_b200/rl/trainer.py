@@ -133,7 +133,7 @@ class GRPOTrainer:
             if any(x is not None for x in items):
                 words.append(item[0][:n[i]].to(dev) if item is not None else
                              torch.full((n[i], (V + 31) // 32), -1, dtype=torch.int32, device=dev))
-        tgt = torch.tensor([t for s in grp for t in s["completion"]], device=dev)
+        tgt = torch.tensor([t for s in grp for t in s["completion"]], dtype=torch.long, device=dev)
         logp = model.logprobs(torch.cat(rows), tgt, self.temperature, torch.cat(words) if words else None)
         return list(logp.split(n))
 

@@ -971,6 +971,15 @@ def test_grpo_runs_the_models_own_forward():
     torch.testing.assert_close(got, want, atol=2e-2, rtol=2e-2)
 
 
+@pytest.mark.gpu
+def test_grpo_batch_of_empty_completions():
+    tr, pol, samples = grpo_case()
+    for s in samples:
+        s["completion"] = []
+    rows = tr._batch_logp(pol, samples)
+    assert [tuple(r.shape) for r in rows] == [(0,)] * 5
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

@@ -212,14 +212,14 @@ def _attend_batch(q, k, v, scale):
     out as a paged cache (16-token blocks), heads narrower than 128 filled up with zeros.
     (out [B, T, H, D], lse fp32 [B, T, H])."""
     B, T, H, D = q.shape
-    Hkv, dev = k.shape[2], q.device
-    nb = (T + 15) // 16
+    S, Hkv, dev = k.shape[1], k.shape[2], q.device
+    nb, off = (S + 15) // 16, S - T
     fill = lambda x, t: torch.nn.functional.pad(x, (0, 128 - D, 0, 0, 0, t)) if t or D < 128 else x  # noqa: E731
 
     def paged(x):
-        return fill(x, nb * 16 - T).reshape(B * nb, 16, Hkv, 128).transpose(1, 2).contiguous()
+        return fill(x, nb * 16 - S).reshape(B * nb, 16, Hkv, 128).transpose(1, 2).contiguous()
 
-    tiles = [(b * T + t, min(128, T - t), b, min(T, t + 128)) for t in range((T - 1) // 128 * 128, -1, -128)
+    tiles = [(b * T + t, min(128, T - t), b, off + min(T, t + 128)) for t in range((T - 1) // 128 * 128, -1, -128)
              for b in range(B)]   # longest first
     ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
     out = torch.empty(B * T, H * 128, dtype=q.dtype, device=dev)
@@ -227,13 +227,13 @@ def _attend_batch(q, k, v, scale):
     ops.flash_prefill(fill(q, 0).reshape(B * T, H * 128), paged(k), paged(v),
                       torch.arange(B * nb, dtype=torch.int32, device=dev).view(B, nb),
                       torch.arange(B, dtype=torch.int32, device=dev).repeat_interleave(T),
-                      torch.arange(1, T + 1, dtype=torch.int32, device=dev).repeat(B), ints(tiles), H, scale, out=out,
-                      lse=lse)
+                      torch.arange(off + 1, S + 1, dtype=torch.int32, device=dev).repeat(B), ints(tiles), H, scale,
+                      out=out, lse=lse)
     return out.view(B, T, H, 128)[..., :D], lse.view(B, T, H)
 
 
 class _Attention(torch.autograd.Function):
-    """Causal attention of q [B, T, H, D] over k, v [B, T, Hkv, D].
+    """Causal attention of q [B, T, H, D] over k, v [B, S, Hkv, D].
 
     Forward: the repo's attention (on CUDA one launch of the tcgen05 FlashAttention kernel, on the
     CPU the fp32 statement per sequence), which also returns the natural-log sum of exponentials L
@@ -260,8 +260,13 @@ class _Attention(torch.autograd.Function):
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, lens=None) -> torch.Tensor:
-    """Differentiable causal attention, q [B, T, H, D], k / v [B, T, Hkv, D] -> [B, T, H, D].
+    """Differentiable causal attention, q [B, T, H, D], k / v [B, S, Hkv, D] -> [B, T, H, D]: the
+    queries are the last T of S >= T tokens.
 
-    ``lens`` int32 [B]: valid tokens of right-padded sequences. Their rows do not depend on it (a
-    causal row sees no padding); the gradient leaves the padding out, in work and in value."""
+    ``lens`` int32 [B]: valid tokens of right-padded sequences (T == S). Their rows do not depend on it
+    (a causal row sees no padding); the gradient leaves the padding out, in work and in value."""
+    if lens is not None and k.shape[1] != q.shape[1]:
+        raise ValueError("attention: lens needs as many queries as keys")
+    if q.is_cuda and (k.shape[1] < q.shape[1] or v.shape != k.shape):
+        raise ValueError("attention: k and v [B, S, Hkv, D] need at least as many keys as q has queries")
     return _Attention.apply(q, k, v, scale, lens)

@@ -980,6 +980,33 @@ def test_grpo_batch_of_empty_completions():
     assert [tuple(r.shape) for r in rows] == [(0,)] * 5
 
 
+@on_devices
+@pytest.mark.parametrize("T,S,D", [(1, 5, 64), (5, 21, 128), (40, 173, 48), (129, 300, 128)])
+def test_attention_over_a_prefix(dev, T, S, D):
+    """Queries that are the last T of S tokens: keys up to their own."""
+    from openmini_v1_b200.ops import autograd as ag
+    c = attention_case(dev, 2, T, S, 4, 2, D, True, None)
+    q, k, v = (c[n].clone().requires_grad_(True) for n in "qkv")
+    out = ag.attention(q, k, v, c["scale"])
+    o6 = attention64(c["q"].double(), c["k"].double(), c["v"].double(), c["scale"], visible(2, T, S, True, None, dev))[0]
+    assert float((out.double() - o6).abs().max()) < 4 * U * float(c["v"].abs().max())
+    out.backward(c["do"])
+    for got, want, tol in zip((q.grad, k.grad, v.grad), c["want"], c["tol"]):
+        # the forward's own 16-bit out enters through rowsum(dO O)
+        assert float((got.double() - want).norm()) < 4 * U * float(want.norm()) + float(tol.norm())
+
+
+@on_devices
+def test_attention_refuses_what_it_cannot_mean(dev):
+    from openmini_v1_b200.ops import autograd as ag
+    q, k = randn(gen(dev, 1), 1, 5, 2, 64), randn(gen(dev, 2), 1, 3, 2, 64)
+    if dev == "cuda":
+        with pytest.raises(ValueError, match="keys"):
+            ag.attention(q, k, k, 0.1)
+    with pytest.raises(ValueError, match="lens"):
+        ag.attention(k, q, q, 0.1, torch.tensor([3], dtype=torch.int32, device=dev))
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [

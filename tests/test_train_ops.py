@@ -1007,6 +1007,31 @@ def test_attention_refuses_what_it_cannot_mean(dev):
         ag.attention(k, q, q, 0.1, torch.tensor([3], dtype=torch.int32, device=dev))
 
 
+@pytest.mark.gpu
+def test_grpo_log_probabilities_are_those_of_the_logits():
+    """Hidden rows and kept words (samples without any: all ones) against masked logits, with gradients."""
+    tr, pol, samples = grpo_case()
+
+    class Logits:  # no logprobs: the logits' path
+        def __call__(self, ids, forced_routing=None):
+            return pol(ids, forced_routing=forced_routing)
+
+    out = []
+    for model in (pol, Logits()):
+        pol.zero_grad()
+        rows = tr._batch_logp(model, samples)
+        assert [len(r) for r in rows] == [9, 1, 30, 12, 5]
+        w = torch.linspace(-1, 1, 57, device="cuda")
+        (torch.cat(rows) * w).sum().backward()
+        out.append((torch.cat(rows).detach(), {n: p.grad.clone() for n, p in pol.named_parameters() if p.grad is not None}))
+    ops.check_status()
+    (a, ga), (b, gb) = out
+    # the logits' path rounds logits of size up to 4 / 0.8 to 16 bits, in log p twice
+    assert float((a - b).abs().max()) < 2 * 2.0 ** -9 * 5 + 1e-3
+    for n in gb:
+        assert float((ga[n] - gb[n]).norm()) < 0.05 * float(gb[n].norm()) + 1e-6, n
+
+
 # ----------------------------------------------------------------------------- paths that need large grids
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [
@@ -1017,4 +1042,44 @@ def test_attention_bwd_several_items_a_cta(shape):
     """More work items than SMs (up to three each), full, ragged and empty ones in turn: the resident rows, the
     accumulators and the tiles' places in tensor memory are handed from item to item."""
     check_attention(attention_case("cuda", *shape), shape[6])
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,F", [(2300, 2056, 1100), (2305, 776, 1101)])
+def test_swiglu_on_cta_pairs(M, K, F):
+    """Contractions long enough for the CTA-pair GEMM: in all three products / in the forward one, odd F."""
+    x, w, dh, want, tol = swiglu_case("cuda", M, K, F)
+    h, gu = ops.swiglu(x, w, save=True)
+    assert torch.equal(ops.swiglu(x, w), h)
+    for name, g, a, t in zip(("h", "dx", "dw"), (h, *ops.swiglu_bwd(x, w, gu, dh)), want, tol):
+        close(g, a, t, name)
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [dict(M=4100, K=1280, V=33001), dict(M=1000, K=1024, V=150001, scale=1.2),
+                               dict(M=1000, K=1024, V=140000, keep=0.3)], ids=str)
+def test_linear_xent_in_pieces_of_large_products(c):
+    """Pieces of the vocabulary whose sums for dx run on CTA pairs / as split contractions."""
+    check_xent(xent_case("cuda", **c))
+    ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [
+    (70001, 256, "rms", True, B16, B16), (20011, 1000, "layer", False, B16, B16), (20011, 1024, "layer", True, B16, F32),
+    (9001, 2048, "rms", False, B16, B16), (5003, 4096, "rms", True, B16, B16), (3001, 8192, "layer", False, F32, F32),
+    (30011, 301, "layer", True, B16, F32), (30011, 301, "rms", False, F32, F32), (8009, 1031, "layer", False, B16, B16),
+    (2503, 4097, "rms", True, B16, B16)], ids=str)
+def test_norm_rows_refill_their_ring(c):
+    """More rows than all groups' rings hold at once: every stage is filled again and its phase turns."""
+    M, D, kind, delta, xt, wt = c
+    x, w, b, d, dy, dh, h, want, tol = norm_case("cuda", M, D, kind, delta, xt, wt)
+    y, hh, stats = ops.norm_train(x, w, b, 1e-5, kind=kind, delta=d)
+    assert torch.equal(hh, h)
+    for name, g, a, t in zip(("y", "dx", "dw", "db"),
+                             (y, *ops.norm_train_bwd(dy, hh, w, stats, kind=kind, bias=b is not None, dh=dh)), want, tol):
+        if a is not None:
+            close(g, a, t, name)
     ops.check_status()

@@ -1087,9 +1087,14 @@ std::tuple<torch::Tensor, torch::Tensor, c10::optional<torch::Tensor>> om_norm_t
       auto go = [&](auto kernel, om::Residents& res, size_t smem) {
         const long long most = (M + RPB - 1) / RPB;
         int blocks = (int)std::min<long long>(most, om::num_sms() * res.get(kernel, NT, smem));
-        // Few rows: one block walks up to eight a group and writes dw itself, which takes less time
-        // than handing partials to a second kernel.
-        if (most <= 8) blocks = 1;
+        // Few rows: one block walks them and writes dw itself. That saves a launch, 3 us of the caller's time, and
+        // costs the GPU a turn's time for each: 0.5 to 0.9 us, but 2 to 3 us where rows are read element by
+        // element or have more than 8192 elements. Forward and gradient, one block and several, us by the
+        // caller's clock and the GPU's alone: rows of 256 (eight a turn) in 8 turns 14.3 and 17.6, 11.1 and 8.4;
+        // in 16 turns 16.4 and 17.5, 15.8 and 8.6; 8192: 8 rows 14.6 and 17.7, 13.0 and 9.6, 16 rows 21.0 and
+        // 17.8, 20.5 and 9.9; 16384: 2 rows 15.4 and 18.0, 14.6 and 17.3, 4 rows 20.1 and 18.1, 19.0 and 17.6;
+        // 4097: 2 rows 14.5 and 17.6, 12.1 and 10.5, 4 rows 19.1 and 17.8, 18.1 and 10.7.
+        if (most <= (v == 8 && a.D <= 8192 ? 8 : 2)) blocks = 1;
         torch::Tensor part;
         if (blocks > 1) {
           part = torch::empty({(int64_t)blocks * n * a.D}, stats.options());

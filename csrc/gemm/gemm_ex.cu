@@ -79,11 +79,15 @@ GxPlan gx_plan(int64_t rows, int64_t cols, int64_t K) {
     }
   }
   const int64_t tiles = tr * ceil_div(cols, p.bn);
-  // a split has to be worth its fp32 plane (written and read once) and a second launch: 8 steps of 64
-  // at least, of 32 and more in all
-  int s = kb < 32 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
-  const int per = ceil_div(kb, s);
-  p.splits = ceil_div(kb, per);
+  // Split over K where that saves more steps than its fp32 planes (written and read once) and a second launch
+  // take: at least 8 steps of 64 a split, and 16 saved in all and 2 more for each MB of planes. Split and not, us:
+  // 688 x 256 x 1024 9.2 and 8.1, x 1536 9.9 and 9.9, x 2048 10.6 and 11.7, x 4096 12.1 and 18.9; 2048 x 512 (8.4 MB)
+  // x 2048 14.2 and 12.5, x 4096 21.4 and 20.9, x 8192 41.7 and 46.9; 1024 x 512 x 2048 12.1 and 11.5, x 4096 14.9
+  // and 17.3; 688 x 1024 x 2048 11.9 and 12.1, x 4096 15.2 and 19.1.
+  const int s = (int)std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kb / 8));
+  const int per = ceil_div(kb, s), splits = ceil_div(kb, per);
+  const double plane_mb = (double)rows * cols * 4e-6;
+  if (splits > 1 && kb - per >= 16 + 2 * splits * plane_mb) p.splits = splits;
   return p;
 }
 

@@ -277,15 +277,17 @@ XentIn check_xent(const char* op, const torch::Tensor& x, const torch::Tensor& w
   return in;
 }
 
-// Column tile of the product x W^T: 256 on CTA pairs or single CTAs; narrower where that needs no more
-// waves of tiles (few rows and a small vocabulary: 910 x 1196 x 7336 on 40 tiles of 256 or 152 of 64).
+// Column tile of the product x W^T: 256 on CTA pairs or single CTAs; half of that while its tiles are at most half
+// of the SMs, and 64 for the fewest. Forward with 64, 128 and 256 columns, us: 8 tiles of 256 (127 x 2048 -> 2048)
+// 11.4, 11.4, 15.9 (its gradient 17.0, 17.4, 22.7); 24 (500 x 1024 -> 1500) 8.7, 8.9, 11.9; 36 (128 x 2048 -> 9000)
+// 13.4, 12.4, 17.1; 72 (300 x 2048 -> 6000) 20.6, 13.5, 17.3; 118 (60 x 1024 -> 30000) 31.3, 22.0, 17.2.
 struct XentTile {
   int bn, pair;
 };
 XentTile xent_tile(const XentIn& in, int64_t cols) {
   if (om::gx_pairs(in.M, cols, in.K)) return {256, 1};
   const int64_t tiles = (int64_t)om::ceil_div(in.M, 128) * om::ceil_div(cols, 256), sms = om::num_sms();
-  return {tiles * 4 <= sms ? 64 : tiles * 2 <= sms ? 128 : 256, 0};
+  return {tiles * 6 <= sms ? 64 : tiles * 2 <= sms ? 128 : 256, 0};
 }
 
 // The product with `cols` vocabulary rows from wv and either logits epilogue.

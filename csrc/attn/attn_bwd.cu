@@ -28,10 +28,11 @@
 // Seven products instead of the five of a single loop is the price of the fixed summation order
 // (and of no fp32 dQ in memory).
 //
-// What bounds it: the tensor cores, 1280 + 1024 of their cycles for a pair of tiles at head_dim 128
-// (kv + q) and the waits of a kv item's dP for its columns, at the clock that the power limit leaves. Measured (B200, back to back): 1 x 8192, 40 / 8
-// heads of 128, causal 2.42 ms, 709 TFLOP/s of the five products, 993 of the seven; 4 x <= 1499 padded,
-// 16 / 4 heads 127 us; head_dim 64, 1 x 8192, 32 / 8 heads 1.32 ms, where the exponentials bound it.
+// What bounds it: the tensor cores take 1280 + 1024 cycles for a pair of tiles at head_dim 128 (kv + q) and are
+// busy for half of the time; the rest is a tile's way through S, P, dP and dS, two tiles at once.
+// Measured (B200, back to back): 1 x 8192, 40 / 8 heads of 128, causal 2.35 ms, 731 TFLOP/s of the five
+// products, 1023 of the seven; 4 x <= 1499 padded, 16 / 4 heads 122 us; head_dim 64, 1 x 8192, 32 / 8 heads
+// 1.27 ms, where the exponentials bound it.
 //
 // Padded batches: rows of Q, dO (or K) at and beyond a sequence's length are cleared in shared
 // memory before a product contracts over them, so that whatever padding holds (NaN too) adds 0.
@@ -136,31 +137,18 @@ __device__ __forceinline__ void clear_rows(uint8_t* p, int from, int lane) {
   }
 }
 
-// Where tile i keeps its S (which = 0) and dP (1), from tensor memory's start: regions of 64 columns,
-// each parity of i has its own. P and dS are written over S, so the region of dP is free once dS is
-// there and the next tile of the parity puts its S into it. That tile's dP takes
-//   2 regions: the place of P and dS, once the products that read them are complete;
-//   3 regions: the third one, which the products of the tile before those left long ago.
-// kv items at head_dim over 64 have 2, because dV and dK take half of the columns; q items have 128
-// more from the second sum they do not need, and narrow heads leave the upper halves of both sums.
-// (1 x 8192, 40 / 8 heads of 128: 2.50 ms with 2 for all, 2.42 ms with 3 for q items.)
-template <int D>
-constexpr bool three_regions(bool kv) {
-  return D <= 64 || !kv;
-}
-template <int D>
-__device__ __forceinline__ uint32_t tile_region(int i, int which, bool three) {
-  const int odd = i & 1;
-  int slot = ((i >> 1) ^ which) & 1;
-  if (three) {
-    slot = ((i >> 1) + which) % 3;
-    if (slot == 2) return D <= 64 ? 64 + odd * 128 : 128 + odd * 64;
-  }
-  return 256 + odd * 128 + slot * 64;
+// Where tile i keeps its S (which = 0) and dP (1): 64 columns each, for both parities of i. P is written
+// over S and dS over dP; the tile after the next takes both places, each when the products that read
+// it are complete. (Products of one shape into one accumulator run in order by themselves, others have
+// to be waited for.) The issue order dV(t), dP(t + 1), dK(t), S(t + 2) has two products between each and
+// the one whose end it waits for: 1 x 8192, 40 / 8 heads of 128 2.35 ms; dK, S, dP in one go 2.40; P and dS
+// both over S, so that dP waits for both products, 2.45; S as soon as dV is complete 2.66.
+__device__ __forceinline__ uint32_t tile_region(int i, int which) {
+  return (uint32_t)((i & 1) * 128 + which * 64);
 }
 
 // A thread's 32 columns of S -> P, kept in fp32 pairs; COLQ: also written in 16 bits over the
-// first 16 of these columns (the caller waits for the store). COLQ: columns are queries (S^T),
+// first 16 of these columns. COLQ: columns are queries (S^T),
 // their -lse come from shared memory; else the thread's row has one. MASK: column j is visible
 // when lo <= j < hi; selected, not multiplied: what lies under a mask may be anything.
 template <bool COLQ, bool MASK>
@@ -189,12 +177,15 @@ __device__ __forceinline__ void tile_p(uint32_t s_at, uint32_t stat, float own, 
       if constexpr (COLQ) pk[e / 2] = pack_bf16x2(p0, p1);
     }
   }
-  if constexpr (COLQ) tmem_st_32x32b_x16(s_at, pk);
+  if constexpr (COLQ) {
+    tmem_st_32x32b_x16(s_at, pk);
+    tc_wait_st();
+  }
 }
 
-// dS = P (dP - delta) of the same columns, in 16 bits to ds_at. stat / own: -delta.
+// dS = P (dP - delta) of the same columns, in 16 bits over the first 16 of them. stat / own: -delta.
 template <bool COLQ, bool MASK>
-__device__ __forceinline__ void tile_ds(uint32_t dp_at, uint32_t ds_at, uint32_t stat, float own, int lo, int hi,
+__device__ __forceinline__ void tile_ds(uint32_t dp_at, uint32_t stat, float own, int lo, int hi,
                                         const uint64_t (&p)[16]) {
   uint32_t dv[32];
   tmem_ld_32x32b_x32(dp_at, dv);
@@ -217,7 +208,7 @@ __device__ __forceinline__ void tile_ds(uint32_t dp_at, uint32_t ds_at, uint32_t
       dk[e / 2] = pack_bf16x2(d.x, d.y);
     }
   }
-  tmem_st_32x32b_x16(ds_at, dk);
+  tmem_st_32x32b_x16(dp_at, dk);
   tc_wait_st();
 }
 
@@ -313,22 +304,6 @@ struct Item {
   }
 };
 
-// Bounded wait for the first of two phases: 1 or 2, 0 when neither came.
-__device__ __forceinline__ int poll_either(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, int* status, int code) {
-  const uint64_t t0 = globaltimer();
-  for (uint32_t spins = 1;; ++spins) {
-    if (mbar_test_wait(a, pa)) return 1;
-    if (mbar_test_wait(b, pb)) return 2;
-    if ((spins & 1023u) == 0) {
-      if (globaltimer() - t0 > OM_WAIT_LIMIT_NS) {
-        record_error(status, code);
-        return 0;
-      }
-      if (wait_failed(status)) return 0;
-    }
-  }
-}
-
 // kv: resident K, V; streamed Q, dO (and their stats); accumulates dV, dK.
 // q:  resident Q, dO; streamed K, V; accumulates dQ.
 // Counters run over all items of a CTA: `tile` numbers the streamed tiles (ring stage, S / dP
@@ -340,7 +315,7 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
                     const AttnBwdArgs a) {
   using C = fa_bw::Cfg<D>;
   constexpr int NS = fa_bw::NSTAGE;
-  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D); S and dP in tile_region
+  constexpr int STAGE0 = 256;  // tensor memory: dV [0, D), dK [128, 128 + D) / dQ [0, D), then S and dP
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* fix_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
@@ -350,7 +325,9 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
   uint64_t* land = empty + NS;         // a padded tile before its rows are cleared
   uint64_t* s_full = land + 1;         // [2] S of a tile is there
   uint64_t* dp_full = s_full + 2;      // [2] dP is
-  uint64_t* ds_full = dp_full + 2;     // [2] P and dS are
+  uint64_t* p_full = dp_full + 2;      // [2] P is (q items: S has been read)
+  uint64_t* p_used = p_full + 2;       // [2] the products that read P are complete
+  uint64_t* ds_full = p_used + 2;      // [2] dS is there
   uint64_t* acc_full = ds_full + 2;    // the item's sums are
   uint64_t* acc_empty = acc_full + 1;  // and have been read
   uint64_t* item_full = acc_empty + 1; // [2] the next item's number
@@ -371,6 +348,8 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&dp_full[s], 1);
+      mbar_init(&p_full[s], 256);
+      mbar_init(&p_used[s], 1);
       mbar_init(&ds_full[s], 256);
       mbar_init(&item_full[s], 1);
       mbar_init(&item_empty[s], 17);
@@ -474,11 +453,10 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
       const uint32_t x_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), 16);   // streamed, K-major
       const uint32_t m_lo = smem_desc_lo(smem_u32(smem + C::FIX_BYTES), C::SMALL);  // streamed, MN-major
       // S (which = 0) or dP (1) of a tile, from the resident rows and the tile's 64
-      bool three = D <= 64;
       auto scores = [&](int tile, auto which_c) {
         constexpr int which = decltype(which_c)::value;
         const uint32_t x = x_lo + (tile % NS) * (C::ST_BYTES / 16);
-        const uint32_t d = tmem + tile_region<D>(tile, which, three);
+        const uint32_t d = tmem + STAGE0 + tile_region(tile, which);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
           tc_mma_f16_lo(d, r_lo + (which * C::H * C::BIG + (k >> 2) * C::BIG + (k & 3) * 32) / 16,
@@ -492,12 +470,23 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         tc_fence_after();
         return there;
       };
-      // The products that read P and dS of a tile are complete. Products of one shape into one accumulator
-      // run in order by themselves; a dP over the P and dS that other products read has to wait.
-      auto used = [&](int tile) {
+      auto p_gone = [&](int tile) {  // the products that read P of a tile are complete
+        const bool so = mbar_poll(&p_used[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+        tc_fence_after();
+        return so;
+      };
+      auto ds_gone = [&](int tile) {  // those that read its dS are
         const bool so = mbar_poll(&empty[tile % NS], (tile / NS) & 1, a.status, OM_ERR_WAIT_ACCUM);
         tc_fence_after();
         return so;
+      };
+      // S and dP of a tile in the place of the tile two before
+      auto both = [&](int tile) {
+        if (!loaded(tile) || !(tile < 2 || p_gone(tile - 2))) return false;
+        scores(tile, S);
+        if (!(tile < 2 || ds_gone(tile - 2))) return false;
+        scores(tile, DP);
+        return true;
       };
       int tile = 0, done = 0;
       bool ok = true;
@@ -510,71 +499,41 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
         const Item w(a, n);
         if (w.total == 0) continue;
         ok = mbar_poll(fix_full, done & 1, a.status, OM_ERR_WAIT_FULL);
-        if (ok && three != three_regions<D>(w.kv)) {  // once a CTA: the columns change hands
-          three = !three;
-          ok = (tile == 0 || used(tile - 1)) && mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM);
-          tc_fence_after();
-        }
-        for (int i = 0; i < 2 && i < w.total && ok; ++i) {
-          ok = loaded(tile + i);
-          if (ok) scores(tile + i, S);
-        }
-        for (int i = 0; i < 2 && i < w.total && ok; ++i) {  // over P and dS of the item before
-          const int last = tile + i - (three ? 4 : 2);
-          ok = last < 0 || used(last);
-          if (ok) scores(tile + i, DP);
-        }
+        for (int i = 0; i < 2 && i < w.total && ok; ++i) ok = both(tile + i);
         if (ok && w.total <= 2) tc_commit(fix_empty);
-        bool owed = false;  // dP of the next tile is still to be issued
         for (int i = 0; i < w.total && ok; ++i, ++tile) {
-          auto pay = [&](int t, int last) {
-            tc_fence_after();
-            scores(t, DP);
-            owed = false;
-            if (last == w.total) tc_commit(fix_empty);  // the item's last scores
-          };
-          if (owed && !three) {  // this tile's dS or the columns of the next one's dP, whichever comes first
-            const int first = poll_either(&empty[(tile - 1) % NS], ((tile - 1) / NS) & 1, &ds_full[tile & 1],
-                                          (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
-            ok = first != 0;
-            if (first == 1) pay(tile + 1, i + 2);
-          }
-          ok = ok && mbar_poll(&ds_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+          const uint32_t x = m_lo + (tile % NS) * (C::ST_BYTES / 16);
+          const uint32_t p = tmem + STAGE0 + tile_region(tile, 0), ds = tmem + STAGE0 + tile_region(tile, 1);
+          ok = mbar_poll(&p_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM) &&
+               // the sums of the item before have been read
+               (i > 0 || mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM));
           if (!ok) break;
           tc_fence_after();
-          // dP of this tile has been read: its columns take the next S of this parity at once
-          if (i + 2 < w.total) {
-            ok = loaded(tile + 2);
-            if (!ok) break;
-            scores(tile + 2, S);
-          }
-          if (owed) {
-            ok = used(tile - 1);
-            if (!ok) break;
-            pay(tile + 1, i + 2);
-          }
-          if (i == 0) {  // the sums of the item before have been read
-            ok = mbar_poll(acc_empty, (done & 1) ^ 1, a.status, OM_ERR_WAIT_ACCUM);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          const uint32_t x = m_lo + (tile % NS) * (C::ST_BYTES / 16);
-          const uint32_t p = tmem + tile_region<D>(tile, 0, three);
           if (w.kv) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // dV += P^T dO, 16 queries a step
               tc_mma_f16_ts_lo(tmem, p + (j >> 1) * 32 + (j & 1) * 8, x + (C::H * C::SMALL + j * 2048) / 16, IDESC_A,
                                j > 0 ? 1 : i);
           }
+          tc_commit(&p_used[tile & 1]);
+          if (i > 0 && i + 1 < w.total) {
+            ok = ds_gone(tile - 1);
+            if (!ok) break;
+            scores(tile + 1, DP);
+            if (i + 2 == w.total) tc_commit(fix_empty);  // the item's last scores
+          }
+          ok = mbar_poll(&ds_full[tile & 1], (tile >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM);
+          if (!ok) break;
+          tc_fence_after();
           const uint32_t d = tmem + (w.kv ? 128 : 0);
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // dK += dS^T Q, or dQ += dS K
-            tc_mma_f16_ts_lo(d, p + 16 + (j >> 1) * 32 + (j & 1) * 8, x + j * 2048 / 16, IDESC_A, j > 0 ? 1 : i);
+            tc_mma_f16_ts_lo(d, ds + (j >> 1) * 32 + (j & 1) * 8, x + j * 2048 / 16, IDESC_A, j > 0 ? 1 : i);
           tc_commit(&empty[tile % NS]);
-          owed = i + 2 < w.total;
-          if (owed && three) {
-            ok = tile < 2 || used(tile - 2);
-            if (ok) pay(tile + 2, i + 3);
+          if (i + 2 < w.total) {
+            ok = loaded(tile + 2) && p_gone(tile);
+            if (!ok) break;
+            scores(tile + 2, S);
           }
         }
         if (ok) tc_commit(acc_full);
@@ -630,9 +589,8 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) return;
           tc_fence_after();
-          constexpr bool three = three_regions<D>(KV);
-          const uint32_t s_at = lanes + tile_region<D>(it, 0, three) + half * 32;
-          const uint32_t dp_at = lanes + tile_region<D>(it, 1, three) + half * 32;
+          const uint32_t s_at = lanes + STAGE0 + tile_region(it, 0) + half * 32;
+          const uint32_t dp_at = lanes + STAGE0 + tile_region(it, 1) + half * 32;
           const uint32_t stat = smem_u32(smem + C::STAT_OFF + (it % NS) * C::STAT) + half * 128;
           const bool masked = KV ? w.row0 + 128 > w.nrow || (a.causal && w.row0 + 127 > x0 + a.off)
                                  : x0 + 64 > w.nstream || (a.causal && x0 + 63 > w.row0 + a.off);
@@ -643,13 +601,15 @@ __global__ void __launch_bounds__(fa_bw::THREADS, 1)
             tile_p<KV, true>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
           else
             tile_p<KV, false>(s_at, stat, own.x, a.scale_log2, lo, hi, p);
+          tc_fence_before();
+          mbar_arrive(&p_full[it & 1]);
           ok = __all_sync(0xffffffffu, mbar_wait(&dp_full[it & 1], (it >> 1) & 1, a.status, OM_ERR_WAIT_ACCUM));
           if (!ok) return;
           tc_fence_after();
           if (masked)
-            tile_ds<KV, true>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
+            tile_ds<KV, true>(dp_at, stat + 256, own.y, lo, hi, p);
           else
-            tile_ds<KV, false>(dp_at, s_at + 16, stat + 256, own.y, lo, hi, p);
+            tile_ds<KV, false>(dp_at, stat + 256, own.y, lo, hi, p);
           tc_fence_before();
           mbar_arrive(&ds_full[it & 1]);
         }
@@ -824,11 +784,11 @@ std::vector<torch::Tensor> om_attention_bwd(torch::Tensor q, torch::Tensor k, to
   // A kv item with all query heads of its KV head walks up to G T / 64 tiles. The launch ends about
   // when the longest item or the average SM does, so an item gets as many heads as fit into the
   // average (a q tile counts 0.75 of a kv tile), and all of them where that is a few tiles anyway
-  // (a join costs more). Split and not, 16 / 4 heads of 128: 1 x 2048 97 and 138 us; 1 x 512 (32 tiles) 26.8
-  // and 43.5; 1 x 256 (16 tiles) 27.6 and 26.8; 1 x 128 23.6 and 19.7. 1 x 4096, 16 / 2 heads 250 and 508.
+  // (a join costs more). Split and not, 16 / 4 heads of 128: 1 x 2048 92 and 123 us; 1 x 512 (32 tiles) 25.6
+  // and 39.2; 1 x 256 (16 tiles) 23.5 and 24.5; 1 x 128 23.3 and 19.7. 1 x 4096, 16 / 2 heads 236 and 449.
   const int64_t qt = (T + 63) / 64, kt = (S + 127) / 128;
   const double average = (double)B * H * qt * kt * (causal ? 0.5 : 1.0) * 1.75 / om::num_sms();
-  a.gper = a.G * qt <= 16 ? a.G : (int)std::min<double>(a.G, std::max(1.0, average / qt));
+  a.gper = a.G * qt < 16 ? a.G : (int)std::min<double>(a.G, std::max(1.0, average / qt));
   a.nsplit = (a.G + a.gper - 1) / a.gper;
   const int64_t kv_items = kt * B * Hkv * a.nsplit, q_items = (T + 127) / 128 * B * H;
   TORCH_CHECK(kv_items + q_items < (1ll << 30), "attention_bwd: too many tiles");

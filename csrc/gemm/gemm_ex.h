@@ -16,9 +16,6 @@ inline CUtensorMap gx_map(const void* p, bool mn, uint64_t rows, uint64_t K, uin
 }
 
 // Output maps of RowStage: boxes of 32 rows x 128 bytes. Rows start on 16 bytes.
-inline bool gx_storable(const void* p, int64_t ld, int bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * bytes % 16 == 0;
-}
 inline CUtensorMap gx_out(__nv_bfloat16* p, uint64_t rows, uint64_t cols, uint64_t ld) {
   return make_tmap_2d(p, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, cols, rows, ld, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B);
 }

@@ -228,7 +228,8 @@ struct EpiXentBwd {
   }
 };
 
-// Columns of one piece: dz of a piece stays within 256 MiB, in whole 256-column tiles.
+// Columns of one piece, in whole 256-column tiles: dz of a piece stays within 256 MiB, or takes 4096 M bytes
+// where that is more (from 65536 rows on): narrower pieces would be launches of few tiles.
 static int64_t piece_columns(int64_t M, int64_t V) {
   const int64_t cap = std::max<int64_t>(2048, (256ll << 20) / (2 * M) / 256 * 256);
   const int64_t n = (V + cap - 1) / cap;

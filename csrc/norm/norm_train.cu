@@ -10,13 +10,15 @@
 // cost no second read, and every group of threads walks rows grid-strided with the weights (and
 // its columns' dw and db) in registers. Rows come into a ring in shared memory by bulk copies,
 // several rows ahead: registers alone could hold one row ahead, which left the memory idle during
-// the reductions. Rows that do not start on 16 bytes, or of which two do not fit into shared
-// memory, are read straight into registers.
+// the reductions. Rows that do not start on 16 bytes take a ring of their own, from which they are
+// read element by element; rows of which two stages do not fit into shared memory (the longest fp32
+// ones) are read straight into registers.
 // The partial dw, db of the blocks are joined in a fixed order by a second kernel: fp32, no atomics,
 // the same result on every run.
 // Measured (B200): 8192 x 4096 bf16 with residual, forward 40 us (5.3 TB/s to and from memory), gradient
-// 44 us (5.6 TB/s); 19600 x 1024 LayerNorm with fp32 gain 21 and 30 us, bound by issue slots: a 2 KB row
-// has two warps' worth of work and two (three) reductions.
+// 44 us (5.6 TB/s); 19600 x 1024 LayerNorm with fp32 gain 21 and 30 us (3.8 and 4.0 TB/s): a 2 KB row is the
+// work of two warps, which meet at a barrier for each of its two sums (one in the gradient), and the
+// issue slots are half used.
 #include <c10/cuda/CUDAGuard.h>
 #include "../common/om_host.h"
 #include "../common/om_ptx.cuh"
